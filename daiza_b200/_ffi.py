@@ -74,6 +74,14 @@ SIGNATURES = {
     "dz_gqa_decode_host_async": [_P, _I, _I, _P, _P, _P, _P, _P, _P],
     "dz_gdn_decode_host_async": [_P, _I, _I, _P, _P, _P, _P, _P, _P, _P],
     "dz_gqa_decode_noalloc": [_P, _I, _I, _P, _P, _P, _P, _P, _P],
+    "dz_cache_create_q4": [_P, _I, _P, _I],
+    "dz_set_rope_axes": [_P, _P, _I],
+    "dz_qk_mrope": [_P, _I, _I64, _P, _P, _P, _P, _P, _P],
+    "dz_qk_mrope_bf16": [_P, _I, _I64, _P, _P, _P, _P, _P, _P],
+    "dz_gqa_decode_q4": [_P, _I, _I, _P, _P, _P, _P, _P, _P, _P],
+    "dz_kv_rows_q4": [_P, _I, _I, _P, _P, _P, _P, _P, _P],
+    "dz_kv_weights_q4": [_P, _I, _I, _P, _P, _P],
+    "dz_kv_set_weights_q4": [_P, _I, _I, _P, _P, _P],
     "dz_last_launch_count": [_P],
     "dz_device_error": [_P, C.POINTER(C.c_int32)],
 }

@@ -44,6 +44,8 @@ void free_cache(dz_ctx* ctx) {
     for (auto& L : ctx->layers) {
         L.d_kv = nullptr;
         L.h_kv.clear();
+        L.d_q4 = nullptr;
+        L.h_q4.clear();
         L.len.clear();
         L.d_ssm = nullptr;
         L.h_ssm.clear();
@@ -53,17 +55,12 @@ void free_cache(dz_ctx* ctx) {
     ctx->rope_n = 0;
     ctx->q_buf = ctx->part_o = ctx->part_ml = nullptr;
     ctx->part_items = 0;
+    ctx->q4 = ctx->q4_track = false;
+    ctx->q4_frag = nullptr;
+    ctx->q4_qs = ctx->q4_sc = nullptr;
     ctx->n_seqs = 0;
     ctx->caps.clear();
     for (auto& sn : ctx->snaps) sn.valid = false;
-}
-
-// A KV length of (layer, seq) went down to new_len (truncate, reset, import,
-// fill): snapshots of seq keep the lowest length seen, so a restore can tell
-// whether rows under its saved length may have been rewritten.
-void kv_lowered(dz_ctx* ctx, int layer, int seq, int64_t new_len) {
-    for (auto& sn : ctx->snaps)
-        if (sn.valid && sn.seq == seq && sn.kv_low[layer] > new_len) sn.kv_low[layer] = new_len;
 }
 
 dz_status dev_alloc(dz_ctx* ctx, void** p, size_t bytes, bool zero) {
@@ -130,6 +127,11 @@ dz_status ensure_stage(dz_ctx* ctx, size_t bytes) {
     return DZ_OK;
 }
 
+// The f32 entry points' answer to a context whose KV caches are held in 4 bits.
+dz_status f32_only(dz_ctx* ctx, const char* instead) {
+    return fail(ctx, DZ_ESTATE, "the KV caches are held in 4 bits: %s", instead);
+}
+
 dz_status check_seqs(dz_ctx* ctx, int B, const int32_t* seq_ids) {
     if (B <= 0 || !seq_ids) return fail(ctx, DZ_EINVAL, "B must be positive and seq_ids non-null");
     if (ctx->n_seqs == 0) return fail(ctx, DZ_ESTATE, "no cache: call dz_cache_create first");
@@ -146,6 +148,14 @@ dz_status check_seqs(dz_ctx* ctx, int B, const int32_t* seq_ids) {
 }  // namespace
 
 namespace dz {
+// A KV length of (layer, seq) went down to new_len (truncate, reset, import,
+// fill): snapshots of seq keep the lowest length seen, so a restore can tell
+// whether rows under its saved length may have been rewritten.
+void kv_lowered(dz_ctx* ctx, int layer, int seq, int64_t new_len) {
+    for (auto& sn : ctx->snaps)
+        if (sn.valid && sn.seq == seq && sn.kv_low[layer] > new_len) sn.kv_low[layer] = new_len;
+}
+
 cudaError_t ensure_prefill_scratch(dz_ctx* ctx, size_t bytes) {
     if (ctx->pf_bytes >= bytes) return cudaSuccess;
     if (ctx->pf) cudaFree(ctx->pf);
@@ -209,6 +219,8 @@ dz_status dz_ctx_create(int device, const dz_config* cfg, dz_ctx** out) {
     if (cfg) ctx->cfg = *cfg; else dz_config_default(&ctx->cfg);
     dz_status st = check_config(ctx, ctx->cfg);
     if (st != DZ_OK) { delete ctx; return st; }
+    const int32_t sections[3] = {11, 11, 10};   // config.rs:47-74
+    rope_axes_set(ctx->axes, sections, false, ctx->cfg.rope_freq_base);
     int ndev = 0;
     if (cudaGetDeviceCount(&ndev) != cudaSuccess || device < 0 || device >= ndev) {
         cudaGetLastError();
@@ -253,6 +265,8 @@ dz_status dz_ctx_destroy(dz_ctx* ctx) {
         free_q1_maps(ctx);
         if (ctx->mlp) cudaFree(ctx->mlp);
         if (ctx->d_err) cudaFree(ctx->d_err);
+        if (ctx->q4_scratch) cudaFree(ctx->q4_scratch);
+        for (void* p : ctx->q4_retired) cudaFree(p);
         if (ctx->snap_mem) cudaFree(ctx->snap_mem);
         for (auto& e : ctx->pf_ev)
             if (e) cudaEventDestroy(e);
@@ -327,7 +341,8 @@ dz_status dz_layer_set_ssm_params(dz_ctx* ctx, int layer, const float* conv1d_t,
     return DZ_OK;
 }
 
-dz_status dz_cache_create(dz_ctx* ctx, int n_seqs, const int64_t* max_len) {
+// q4: full-attention layers hold K and V in 4 bits; track: with accumulated attention weights
+static dz_status cache_create(dz_ctx* ctx, int n_seqs, const int64_t* max_len, bool q4, bool track) {
     if (!ctx || n_seqs <= 0 || !max_len) return fail(ctx, DZ_EINVAL, "n_seqs must be positive, max_len non-null");
     int64_t max_cap = 0;
     for (int s = 0; s < n_seqs; ++s) {
@@ -343,7 +358,37 @@ dz_status dz_cache_create(dz_ctx* ctx, int n_seqs, const int64_t* max_len) {
     dz_status st;
     // KV slabs: one allocation per full-attention layer, sequences back to back
     for (auto& L : ctx->layers) {
-        if (L.is_attn) {
+        if (L.is_attn && q4) {
+            // zeroed: unwritten positions of a tile must hold finite scales (q4.cuh)
+            std::vector<Q4Slot> slots(n_seqs);
+            size_t bytes = 0, weights = 0;
+            for (int s = 0; s < n_seqs; ++s) {
+                slots[s].cap = max_len[s];
+                bytes += (size_t)kvc * slots[s].n_tiles() * Q4_TILE_BYTES;
+                weights += (size_t)kvc * max_len[s];
+            }
+            void *slab, *wslab = nullptr, *tab;
+            if ((st = dev_alloc(ctx, &slab, bytes, true)) != DZ_OK ||
+                (track && (st = dev_alloc(ctx, &wslab, weights * sizeof(float), true)) != DZ_OK) ||
+                (st = dev_alloc(ctx, &tab, n_seqs * sizeof(Q4Slot), false)) != DZ_OK) {
+                free_cache(ctx);
+                return st;
+            }
+            uint8_t* p = static_cast<uint8_t*>(slab);
+            float* w = static_cast<float*>(wslab);
+            for (int s = 0; s < n_seqs; ++s) {
+                slots[s].tiles = p;
+                slots[s].wts = w;
+                p += (size_t)kvc * slots[s].n_tiles() * Q4_TILE_BYTES;
+                if (w) w += (size_t)kvc * max_len[s];
+            }
+            L.d_q4 = static_cast<Q4Slot*>(tab);
+            DZ_CUDA(cudaMemcpy(L.d_q4, slots.data(), n_seqs * sizeof(Q4Slot), cudaMemcpyHostToDevice));
+            L.h_q4 = slots;
+            L.h_kv.resize(n_seqs);
+            for (int s = 0; s < n_seqs; ++s) L.h_kv[s] = KvSlot{nullptr, nullptr, max_len[s]};
+            L.len.assign(n_seqs, 0);
+        } else if (L.is_attn) {
             size_t total = 0;
             for (int s = 0; s < n_seqs; ++s) total += (size_t)2 * kvc * max_len[s] * HD;
             void* slab;
@@ -380,8 +425,8 @@ dz_status dz_cache_create(dz_ctx* ctx, int n_seqs, const int64_t* max_len) {
             L.head.assign(n_seqs, 0);
         }
     }
-    // RoPE table for positions [0, max_cap)
-    {
+    // RoPE table for positions [0, max_cap); 4-bit caches turn by angles computed in the kernels
+    if (!q4) {
         std::vector<float> tab((size_t)max_cap * 2 * ROPE);
         rope_rows(0, max_cap, ROPE, ctx->cfg.rope_freq_base, tab.data());
         void* d;
@@ -415,11 +460,45 @@ dz_status dz_cache_create(dz_ctx* ctx, int n_seqs, const int64_t* max_len) {
             return st;
         }
         ctx->part_ml = static_cast<float*>(d);
+        if (q4) {
+            if ((st = dev_alloc(ctx, &d, (size_t)nb * kvc * 16 * 32 * 4 * sizeof(uint32_t), false)) != DZ_OK) {
+                free_cache(ctx);
+                return st;
+            }
+            ctx->q4_frag = static_cast<uint32_t*>(d);
+            if ((st = dev_alloc(ctx, &d, (size_t)nb * kvc * 8 * sizeof(float), false)) != DZ_OK) {
+                free_cache(ctx);
+                return st;
+            }
+            ctx->q4_qs = static_cast<float*>(d);
+            if (track) {
+                const size_t tiles = (size_t)(sum_n / Q4_TILE) + nb;
+                if ((st = dev_alloc(ctx, &d, tiles * kvc * GRP * Q4_TILE * sizeof(float), false)) != DZ_OK) {
+                    free_cache(ctx);
+                    return st;
+                }
+                ctx->q4_sc = static_cast<float*>(d);
+            }
+        }
     }
     ctx->n_seqs = n_seqs;
+    ctx->q4 = q4;
+    ctx->q4_track = track;
     ctx->caps.assign(max_len, max_len + n_seqs);
     DZ_CUDA(cudaDeviceSynchronize());
     return DZ_OK;
+}
+
+dz_status dz_cache_create(dz_ctx* ctx, int n_seqs, const int64_t* max_len) {
+    return cache_create(ctx, n_seqs, max_len, false, false);
+}
+
+dz_status dz_cache_create_q4(dz_ctx* ctx, int n_seqs, const int64_t* max_len, int track_weights) {
+    try {
+        return cache_create(ctx, n_seqs, max_len, true, track_weights != 0);
+    } catch (const std::bad_alloc&) {
+        return fail(ctx, DZ_ENOMEM, "dz_cache_create_q4: out of host memory");
+    }
 }
 
 dz_status dz_kv_len(const dz_ctx* ctx, int layer, int seq, int64_t* out_len) {
@@ -468,6 +547,7 @@ dz_status dz_kv_export(dz_ctx* ctx, int layer, int seq, float* k_flat, float* v_
     const int kvc = ctx->cfg.kv_head_count;
     const int64_t n = L.len[seq];
     if (n == 0) return DZ_OK;
+    if (ctx->q4) return q4_export(ctx, layer, seq, k_flat, v_flat);
     // device [kvh][cap][256] -> host [len][kvh][256]: one 2-D copy per head
     for (int h = 0; h < kvc; ++h) {
         DZ_CUDA(cudaMemcpy2D(k_flat + (size_t)h * HD, (size_t)kvc * HD * 4, L.h_kv[seq].k + (size_t)h * L.h_kv[seq].cap * HD,
@@ -488,6 +568,13 @@ dz_status dz_kv_import(dz_ctx* ctx, int layer, int seq, const float* k_flat, con
     DeviceGuard g(ctx->device);
     if (!g.ok) return fail(ctx, DZ_ECUDA, "cudaSetDevice(%d) failed", ctx->device);
     const int kvc = ctx->cfg.kv_head_count;
+    if (ctx->q4) {
+        const dz_status st = q4_import(ctx, layer, seq, k_flat, v_flat, len);
+        if (st != DZ_OK) return st;
+        L.len[seq] = len;
+        kv_lowered(ctx, layer, seq, 0);
+        return DZ_OK;
+    }
     for (int h = 0; h < kvc && len > 0; ++h) {
         DZ_CUDA(cudaMemcpy2D(L.h_kv[seq].k + (size_t)h * L.h_kv[seq].cap * HD, HD * 4, k_flat + (size_t)h * HD,
                              (size_t)kvc * HD * 4, HD * 4, len, cudaMemcpyDefault));
@@ -532,6 +619,7 @@ dz_status dz_ssm_import(dz_ctx* ctx, int layer, int seq, const float* state, con
 dz_status dz_kv_fill_pattern(dz_ctx* ctx, int layer, int seq, int64_t len, int byte_value) {
     if (!layer_ok(ctx, layer) || !ctx->layers[layer].is_attn || seq < 0 || seq >= ctx->n_seqs || len < 0)
         return fail(ctx, DZ_EINVAL, "bad fill arguments");
+    if (ctx->q4) return f32_only(ctx, "dz_kv_import fills them");
     LayerState& L = ctx->layers[layer];
     if (len > L.h_kv[seq].cap) return fail(ctx, DZ_ESTATE, "fill of %lld rows exceeds capacity", (long long)len);
     DeviceGuard g(ctx->device);
@@ -822,6 +910,7 @@ static dz_status gqa_decode_check(dz_ctx* ctx, int layer, int B, const int32_t* 
     if (!L.params_set) return fail(ctx, DZ_ESTATE, "layer %d has no parameters", layer);
     dz_status st = check_seqs(ctx, B, seq_ids);
     if (st != DZ_OK) return st;
+    if (ctx->q4) return f32_only(ctx, "use dz_gqa_decode_q4");
     if (pos)
         for (int b = 0; b < B; ++b)
             if (pos[b] < 0 || pos[b] >= ctx->rope_n)
@@ -1046,6 +1135,7 @@ static dz_status gqa_prefill_common(dz_ctx* ctx, int layer, int seq, int64_t T, 
     if (seq < 0 || seq >= ctx->n_seqs) return fail(ctx, DZ_EINVAL, "bad seq %d", seq);
     if (T <= 0) return fail(ctx, DZ_EINVAL, "T must be positive");
     if (!out) return fail(ctx, DZ_EINVAL, "null tensor");
+    if (ctx->q4) return f32_only(ctx, "use dz_gqa_prefill_q4");
     if (L.len[seq] + T > L.h_kv[seq].cap)
         return fail(ctx, DZ_ESTATE, "prefill of %lld tokens overflows KV cache (len %lld, cap %lld)", (long long)T,
                     (long long)L.len[seq], (long long)L.h_kv[seq].cap);

@@ -35,6 +35,26 @@ struct GqaDecodeDesc {
     int32_t cum[MAXB + 1];     // prefix sum of chunks(b) = ceil((len+1)/chunk)
 };
 
+// One sequence's 4-bit KV cache for one full-attention layer (format: q4.cuh):
+//   tiles [kv_head_count][ceil(cap / 16)][4352 bytes]
+//   wts   [kv_head_count][cap] f32 accumulated attention weights (tracked caches)
+constexpr int Q4_TILE = 16, Q4_TILE_BYTES = 4352;
+struct Q4Slot {
+    uint8_t* tiles;
+    float* wts;
+    int64_t cap;
+    __host__ __device__ int64_t n_tiles() const { return (cap + Q4_TILE - 1) / Q4_TILE; }
+    __host__ __device__ uint8_t* tile(int kvh, int64_t t) const { return tiles + (kvh * n_tiles() + t) * Q4_TILE_BYTES; }
+};
+// The three rotary positions (time, height, width) of each batch row of a decode launch.
+struct Q4Pos { int32_t p[MAXB][3]; };
+// Rotary axes: which of a token's three positions turns pair i, and the pair's frequency
+// base^(-2i/64) in half turns.
+struct RopeAxes {
+    uint8_t axis[ROPE / 2];
+    double turn[ROPE / 2];
+};
+
 struct GdnDecodeDesc {
     int B;
     int32_t sid[MAXB];
@@ -52,6 +72,8 @@ struct LayerState {
     float* norm_w = nullptr;   // [128]
     KvSlot* d_kv = nullptr;    // [n_seqs]
     std::vector<KvSlot> h_kv;
+    Q4Slot* d_q4 = nullptr;    // [n_seqs], caches held in 4 bits (h_kv then has the capacities only)
+    std::vector<Q4Slot> h_q4;
     std::vector<int64_t> len;  // host-authoritative KvCache::len
     SsmSlot* d_ssm = nullptr;  // [n_seqs]
     std::vector<SsmSlot> h_ssm;
@@ -118,6 +140,17 @@ struct dz_ctx {
         cudaEvent_t landed = nullptr, done = nullptr;
     } hs[2];                     // 0: gated GQA, 1: Gated DeltaNet
     cudaEvent_t pf_ev[dz::PF_MAX_SEGMENTS + 1] = {};
+    // 4-bit KV caches (dz_cache_create_q4): the decode kernels' q operand and its scales,
+    // the scores of tracked caches, and scratch of prompts and evictions.  A buffer that is
+    // outgrown stays allocated until the context goes: a captured graph may hold it.
+    bool q4 = false, q4_track = false;
+    dz::RopeAxes axes{};
+    uint32_t* q4_frag = nullptr;  // [min(n_seqs, MAXB)][kvc][16][32][4]
+    float* q4_qs = nullptr;       // [min(n_seqs, MAXB)][kvc][8]
+    float* q4_sc = nullptr;       // [tiles of one launch][kvc][6][16]
+    void* q4_scratch = nullptr;
+    size_t q4_scratch_bytes = 0;
+    std::vector<void*> q4_retired;
     // sequence snapshots: slots of snap_slot_floats floats each (sized by the config)
     float* snap_mem = nullptr;
     size_t snap_slot_floats = 0;
@@ -257,6 +290,19 @@ cudaError_t launch_q1_gemv(dz_ctx* ctx, int n_mats, const uint8_t* const* w, con
 // block tail (block_tail.cu): RMSNorm rows and SwiGLU, stream-ordered
 cudaError_t launch_rmsnorm_rows(const float* x, const float* w, float eps, int T, int n, float* out, cudaStream_t st);
 cudaError_t launch_swiglu(float* gate, const float* up, int64_t n, cudaStream_t st);
+// merge of the split-K partials, normalisation and gate (gqa_decode.cu)
+cudaError_t launch_gqa_combine(dz_ctx* ctx, const GqaDecodeDesc& d, const float* q_gate, float* out, cudaStream_t st,
+                               const float* part_o, const float* part_ml);
+// 4-bit KV caches (q4_*.cu)
+cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, const GqaDecodeDesc& d, const Q4Pos& pos, const float* q_gate,
+                             const float* k, const float* v, float* out, cudaStream_t st, int* n_launch);
+dz_status q4_import(dz_ctx* ctx, int layer, int seq, const float* k, const float* v, int64_t len);
+dz_status q4_export(dz_ctx* ctx, int layer, int seq, float* k, float* v);
+// grows ctx->q4_scratch to at least `bytes` (the old buffer is kept: see above)
+cudaError_t ensure_q4_scratch(dz_ctx* ctx, size_t bytes);
+void rope_axes_set(RopeAxes& a, const int32_t sections[3], bool interleaved, double base);
+// a KV length went down: snapshots remember the lowest (dz_attn.cu)
+void kv_lowered(dz_ctx* ctx, int layer, int seq, int64_t new_len);
 // grows ctx->q1 to at least `bytes`
 cudaError_t ensure_q1_scratch(dz_ctx* ctx, size_t bytes);
 // grows ctx->gdn_rec to at least `bytes`

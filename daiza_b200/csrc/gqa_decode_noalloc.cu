@@ -116,6 +116,7 @@ extern "C" dz_status dz_gqa_decode_noalloc(dz_ctx* ctx, int layer, int B, const 
     if (!L.params_set) return set_err(ctx, DZ_ESTATE, "layer has no parameters");
     if (!q_gate || !k || !v || !out || !seq_ids) return set_err(ctx, DZ_EINVAL, "null pointer argument");
     if (ctx->n_seqs == 0) return set_err(ctx, DZ_ESTATE, "no cache: call dz_cache_create first");
+    if (ctx->q4) return set_err(ctx, DZ_ESTATE, "the KV caches are held in 4 bits: use dz_gqa_decode_q4");
     if (B <= 0 || B > NOALLOC_MAX_SEQS)
         return set_err(ctx, DZ_EINVAL, "dz_gqa_decode_noalloc: B=" + std::to_string(B) +
                                            " outside 1.." + std::to_string(NOALLOC_MAX_SEQS) +

@@ -1,0 +1,212 @@
+// q4.cuh -- the 4-bit KV cache: row format, tile layout and the device functions
+// that write rows into tiles and read them back.
+//
+// A row is one position of one kv head, K or V: 256 values in 8 groups of 32.
+//   t = max|x| / 7 of the group; s = t rounded to 4 significant bits (nearest
+//   even, grid 2^-17 below 2^-14), at most 896; code = clamp(rint(x / s), -7, 7);
+//   the held value is code * s.  NaN is held as 0, infinities saturate, a group
+//   whose s rounds to 0 is held as 0.
+// Rounding the scale to the nearest (not up) loses nothing: t / s <= 17/16, so the
+// largest |x| / s is 7.44 and still lands within half a step of code 7.
+// s is a positive f16 whose low 7 bits are zero, so 8 bits of it are stored
+// (f16 bits >> 7).  code * s has at most 3 + 4 significant bits: exact in f16, so
+// the matrix instructions multiply the held values themselves, with no second
+// rounding and no scale in an epilogue.  896 is the largest s for which 72 * s,
+// the constant of the unpacking below, is still an f16.
+//
+// Where a value next to a border falls must not depend on rounding in the
+// arithmetic before it: K's norm and rotation run in f64 on the way here, and the
+// code is decided from the exact remainder x - code * s.
+//
+// Tile: 16 positions of one kv head, 4352 bytes (K codes 2048, V codes 2048, K
+// scales 128, V scales 128), in the register order of mma.m16n8k16, so that a warp
+// reads a tile with 16-byte loads and no shuffles.  With r = lane / 4, c = lane % 4:
+//   K codes  [pos / 8][i 0..1][lane (r = pos % 8)][4 words]: word w = 4 i + j holds
+//            dims 64 c + 8 w .. + 7 of that position, dim e at bit (e & 1) * 16 + (e >> 1) * 4
+//   V codes  [i 0..3][lane][4 words]: word m = 4 i + j holds dims 32 r + 2 m (A) and
+//            32 r + 2 m + 1 (B) at positions 2c, 2c+1, 2c+8, 2c+9: position 2c + u + 8 w
+//            at bit u * 16 + w * 4, dim B 8 bits above dim A
+//   K scales [lane][4]: (pos r, group 2c), (r, 2c+1), (r + 8, 2c), (r + 8, 2c+1)
+//   V scales [lane][4]: group r at positions 2c, 2c+1, 2c+8, 2c+9
+// Codes are stored as code + 8.  Unwritten positions hold finite scales always
+// (the cache starts zeroed), since a masked probability of 0 still multiplies V.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "dz_internal.h"
+
+namespace dz {
+namespace q4 {
+
+constexpr float SCALE_MAX = 896.0f;
+constexpr int OFF_V = 2048, OFF_KS = 4096, OFF_VS = 4224;
+static_assert(OFF_VS + 128 == Q4_TILE_BYTES, "tile layout");
+static_assert(Q4_TILE_BYTES % 16 == 0, "tiles move by bulk copies");
+
+// ---- scales ------------------------------------------------------------------------
+// s (as stored byte) from the group's largest magnitude.  t's significand is cut to 4
+// bits in integer arithmetic; below 2^-14 the grid is 2^-17.
+__device__ __forceinline__ uint32_t scale_byte(double amax) {
+    const double t = fmin(amax / 7.0, (double)SCALE_MAX);
+    if (t < 6.103515625e-05)                                   // 2^-14: f16 subnormals
+        return (uint32_t)__double2int_rn(t * 131072.0);        // 0..8 (8 = the smallest normal)
+    const long long b = __double_as_longlong(t);
+    const long long odd = (b >> 49) & 1;                       // keep 3 fraction bits of 52, nearest even
+    const long long r = (b + ((1ll << 48) - 1) + odd) >> 49;   // exponent and 3 fraction bits
+    return (uint32_t)(r - ((1023 - 15) << 3));                 // rebias to f16: exponent << 3 | fraction
+}
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+    return __half2float(__ushort_as_half((unsigned short)(byte << 7)));
+}
+// code + 8 of x: the nearest whole multiple of s (ties to even), decided exactly.
+// inv = 1 / s (0 if s is 0), an approximation that the remainder corrects.
+__device__ __forceinline__ uint32_t code8(double x, double s, float inv) {
+    float kf = rintf(fminf(fmaxf((float)x * inv, -7.0f), 7.0f));
+    const double d = fma((double)-kf, s, x), h = 0.5 * s;      // exact where it is near a border
+    const bool odd = ((int)kf) & 1;
+    if (d > h || (d == h && odd)) kf += 1.0f;
+    else if (d < -h || (d == -h && odd)) kf -= 1.0f;
+    kf = fminf(fmaxf(kf, -7.0f), 7.0f);
+    return s > 0.0 ? (uint32_t)((int)kf + 8) : 8u;
+}
+__device__ __forceinline__ double not_nan(double x) { return x == x ? x : 0.0; }
+
+// two scale bytes (bits 0..7 and 16..23) -> an f16 pair
+__device__ __forceinline__ uint32_t scale_pair(uint32_t bytes) { return bytes << 7; }
+
+// ---- unpacking ---------------------------------------------------------------------
+__device__ __forceinline__ uint32_t hfma2_u(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t hmul2_u(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+constexpr uint32_t NEG72 = 0xD480D480u;                        // f16 pair of -72
+// Nibbles n at bits 4..7 and 20..23 of x -> the f16 pair (n - 8) * s.  Under the
+// exponent of 64 those bits have weights 8, 4, 2, 1: 64 + n.  (64 + n) s - 72 s in
+// one fused operation is exact; c = -72 s.
+__device__ __forceinline__ uint32_t unpack(uint32_t x, uint32_t s, uint32_t c) {
+    return hfma2_u((x & 0x00F000F0u) | 0x54005400u, s, c);
+}
+
+// ---- rotary positions ----------------------------------------------------------------
+// Angle of pair i at position p in half turns, reduced to [-1, 1]: p * base^(-2i/64) / pi.
+// In f64: at p = 10^6 an f32 angle is off by 0.03.
+__device__ __forceinline__ double rope_half_turns(int p, double turn) {
+    const double u = (double)p * turn;
+    return u - 2.0 * rint(0.5 * u);
+}
+// (cos, sin) of pair i at a token's three positions
+__device__ __forceinline__ double2 rope_cs(const RopeAxes& a, int i, int t, int h, int w) {
+    const int ax = a.axis[i];
+    double s, c;
+    sincospi(rope_half_turns(ax == 0 ? t : (ax == 1 ? h : w), a.turn[i]), &s, &c);
+    return make_double2(c, s);
+}
+
+// ---- a row in registers ----------------------------------------------------------------
+// Lane l holds dims 8 l .. 8 l + 7 of a row (a group of 32 = 4 lanes).
+
+// RMS norm, weight and rotation (attention.rs:92-113, with the reference's '+' sign for
+// both halves, math/rope.rs:205-210), in f64 for rows that are quantised and in f32 for
+// the others.  cs: (cos, sin) of the 32 pairs.  The partner of dim i < 32 is i + 32:
+// lane ^ 4.
+__device__ __forceinline__ double inv_sqrt(double x) { return 1.0 / sqrt(x); }
+__device__ __forceinline__ float inv_sqrt(float x) { return 1.0f / sqrtf(x); }
+template <typename F, typename C>
+__device__ __forceinline__ void norm_rotate(F (&x)[8], const float* __restrict__ w, const C* cs, float eps, int lane) {
+    F ss = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const F inv = inv_sqrt(ss / (F)HD + (F)eps);
+    const float4 w0 = reinterpret_cast<const float4*>(w)[2 * lane], w1 = reinterpret_cast<const float4*>(w)[2 * lane + 1];
+    const float wv[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * (F)wv[e];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const F p = __shfl_xor_sync(0xffffffffu, x[e], 4);
+        if (lane < 8) {
+            const C c = cs[8 * (lane & 3) + e];
+            x[e] = x[e] * (F)c.x + p * (F)c.y;
+        }
+    }
+}
+
+// Quantise the row: the stored scale byte of this lane's group and the 8 codes + 8.
+__device__ __forceinline__ uint32_t quantise(double (&x)[8], uint32_t (&code)[8]) {
+    double a = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        x[e] = not_nan(x[e]);
+        a = fmax(a, fabs(x[e]));
+    }
+    a = fmax(a, __shfl_xor_sync(0xffffffffu, a, 1));
+    a = fmax(a, __shfl_xor_sync(0xffffffffu, a, 2));
+    const uint32_t sb = scale_byte(a);
+    const float s = scale_value(sb), inv = s > 0.0f ? 1.0f / s : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) code[e] = code8(x[e], (double)s, inv);
+    return sb;
+}
+
+// Writes K's codes and scale of position p (0..15) of a tile.  Lane l's 8 dims are one
+// word: c = l / 8, word l % 8.
+__device__ __forceinline__ void put_k(uint8_t* tile, int p, int lane, const uint32_t (&code)[8], uint32_t sb) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w |= code[e] << ((e & 1) * 16 + (e >> 1) * 4);
+    const int c = lane >> 3, ws = lane & 7, n = p & 7;
+    *reinterpret_cast<uint32_t*>(tile + ((p >> 3) * 2 + (ws >> 2)) * 512 + (n * 4 + c) * 16 + (ws & 3) * 4) = w;
+    const int g = lane >> 2;
+    if ((lane & 3) == 0) tile[OFF_KS + (n * 4 + (g >> 1)) * 4 + (p >> 3) * 2 + (g & 1)] = (uint8_t)sb;
+}
+// The four V words of lane l's dims at column c: group r = l / 4, words 4 (l % 4) .. + 3.
+__device__ __forceinline__ uint4* v_words(uint8_t* tile, int lane, int c) {
+    return reinterpret_cast<uint4*>(tile + OFF_V + (lane & 3) * 512 + ((lane >> 2) * 4 + c) * 16);
+}
+// The same words with position p's nibbles replaced by the codes.
+__device__ __forceinline__ void merge_v(uint4& w, int p, const uint32_t (&code)[8]) {
+    const int sh = (p & 1) * 16 + (p >> 3) * 4;
+    const uint32_t keep = ~(0x0F0Fu << sh);
+    w.x = (w.x & keep) | ((code[0] | code[1] << 8) << sh);
+    w.y = (w.y & keep) | ((code[2] | code[3] << 8) << sh);
+    w.z = (w.z & keep) | ((code[4] | code[5] << 8) << sh);
+    w.w = (w.w & keep) | ((code[6] | code[7] << 8) << sh);
+}
+__device__ __forceinline__ void put_v_scale(uint8_t* tile, int p, int lane, uint32_t sb) {
+    if ((lane & 3) == 0)
+        tile[OFF_VS + ((lane >> 2) * 4 + ((p & 7) >> 1)) * 4 + (p & 1) + (p >> 3) * 2] = (uint8_t)sb;
+}
+
+// Reads lane l's 8 dims of K or V at position p of a tile as f16 pairs.
+__device__ __forceinline__ void get_k(const uint8_t* tile, int p, int lane, uint32_t (&h)[4]) {
+    const int c = lane >> 3, ws = lane & 7, n = p & 7, g = lane >> 2;
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + ((p >> 3) * 2 + (ws >> 2)) * 512 + (n * 4 + c) * 16 +
+                                                          (ws & 3) * 4);
+    const uint32_t b = tile[OFF_KS + (n * 4 + (g >> 1)) * 4 + (p >> 3) * 2 + (g & 1)];
+    const uint32_t s = scale_pair(b | b << 16), k = hmul2_u(s, NEG72);
+    h[0] = unpack(w << 4, s, k);
+    h[1] = unpack(w, s, k);
+    h[2] = unpack(w >> 4, s, k);
+    h[3] = unpack(w >> 8, s, k);
+}
+__device__ __forceinline__ void get_v(const uint8_t* tile, int p, int lane, uint32_t (&h)[4]) {
+    const int c = (p & 7) >> 1;
+    const uint4 w = *reinterpret_cast<const uint4*>(tile + OFF_V + (lane & 3) * 512 + ((lane >> 2) * 4 + c) * 16);
+    const uint32_t b = tile[OFF_VS + ((lane >> 2) * 4 + c) * 4 + (p & 1) + (p >> 3) * 2];
+    const uint32_t s = scale_pair(b | b << 16), k = hmul2_u(s, NEG72);
+    const int sh = (p & 1) * 16 + (p >> 3) * 4;
+    const uint32_t x[4] = {w.x >> sh, w.y >> sh, w.z >> sh, w.w >> sh};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = unpack((x[i] & 0xFu) << 4 | (x[i] & 0xF00u) << 12, s, k);
+}
+
+}  // namespace q4
+}  // namespace dz

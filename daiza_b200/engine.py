@@ -44,6 +44,25 @@ def _stream(stream):
     return C.c_void_p(s.cuda_stream)
 
 
+def _tensor(name, t, dtype, numel):
+    """Pointer of a contiguous CUDA tensor that a 4-bit cache call reads or writes; DZ_EINVAL otherwise."""
+    if not (t.is_cuda and t.dtype == dtype and t.is_contiguous() and t.numel() == numel):
+        raise _ffi.DzError(_ffi.DZ_EINVAL, f"{name} must be a contiguous CUDA {dtype} tensor of {numel} values, got "
+                                           f"{tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
+    return _ptr(t)
+
+
+def _ids(seq_ids):
+    return np.ascontiguousarray(np.atleast_1d(seq_ids), np.int32)
+
+
+def _per_seq(name, values, ids):
+    a = np.ascontiguousarray(np.atleast_1d(values), np.int64)
+    if a.shape != ids.shape:
+        raise _ffi.DzError(_ffi.DZ_EINVAL, f"{name} needs one number per sequence ({len(ids)}), got {a.shape}")
+    return a
+
+
 def default_config(n_layers=64, full_attention_interval=4, kv_heads=None, v_heads=None, qtile_split=None):
     """Config::default (config.rs:47-74) with an optional head slice and
     GQA-prefill query-tile split (index, count)."""
@@ -258,6 +277,74 @@ class Context:
         assert ps.shape == ids.shape
         self._chk(self.lib.dz_gqa_decode_at(self.h, layer, len(ids), _np_ptr(ids), _np_ptr(ps), _ptr(q_gate), _ptr(k),
                                             _ptr(v), _ptr(out), _stream(stream)))
+
+    # ---- KV caches held in 4 bits -------------------------------------------
+    def cache_create_q4(self, max_len, track=False):
+        """cache_create with K and V held in 4 bits; track: accumulate attention weights."""
+        ml = np.ascontiguousarray(np.atleast_1d(max_len), np.int64)
+        self._chk(self.lib.dz_cache_create_q4(self.h, len(ml), _np_ptr(ml), int(bool(track))))
+        self.n_seqs = len(ml)
+
+    def set_rope_axes(self, sections=(11, 11, 10), interleaved=False):
+        """Which of a token's (time, height, width) positions turns each of the 32 rotary pairs."""
+        s = np.ascontiguousarray(sections, np.int32)
+        if s.shape != (3,):
+            raise _ffi.DzError(_ffi.DZ_EINVAL, f"sections has three numbers, got {s.shape}")
+        self._chk(self.lib.dz_set_rope_axes(self.h, _np_ptr(s), int(bool(interleaved))))
+
+    def qk_mrope(self, layer, pos, q_gate, k, q_out, k_out, stream=None):
+        """QK-RMSNorm, rotation by pos [T][3] (int32) and q's 1/16; q_gate [T][6*kvc][512] and k [T][kvc][256] f32 or
+        bf16, q_out [T][6*kvc][256] and k_out [T][kvc][256] of the same type."""
+        import torch
+        T = k.numel() // (self.kvc * HD)
+        dt = torch.bfloat16 if k.dtype == torch.bfloat16 else torch.float32
+        fn = self.lib.dz_qk_mrope_bf16 if dt == torch.bfloat16 else self.lib.dz_qk_mrope
+        self._chk(fn(self.h, layer, T, _tensor("pos", pos, torch.int32, 3 * T),
+                     _tensor("q_gate", q_gate, dt, T * self.nq * QG_ROW), _tensor("k", k, dt, T * self.kvc * HD),
+                     _tensor("q_out", q_out, dt, T * self.nq * HD), _tensor("k_out", k_out, dt, T * self.kvc * HD),
+                     _stream(stream)))
+
+    def gqa_decode_q4(self, layer, seq_ids, q_gate, k, v, out, stream=None, pos=None):
+        """gqa_decode on 4-bit caches; pos: [B][3] rotary positions (host), default the cache lengths."""
+        import torch
+        ids, f = _ids(seq_ids), torch.float32
+        B, p3 = len(ids), None
+        if pos is not None:
+            p3 = np.ascontiguousarray(pos, np.int32)
+            if p3.shape != (B, 3):
+                raise _ffi.DzError(_ffi.DZ_EINVAL, f"pos is [{B}][3], got {p3.shape}")
+        self._chk(self.lib.dz_gqa_decode_q4(
+            self.h, layer, B, _np_ptr(ids), None if p3 is None else _np_ptr(p3),
+            _tensor("q_gate", q_gate, f, B * self.nq * QG_ROW), _tensor("k", k, f, B * self.kvc * HD),
+            _tensor("v", v, f, B * self.kvc * HD), _tensor("out", out, f, B * self.nq * HD), _stream(stream)))
+
+    def kv_rows_q4(self, layer, seq_ids, first, count, k, v, stream=None):
+        """Held rows [first, first + count) of each sequence as f32 [sum count][kvc][256]."""
+        import torch
+        ids = _ids(seq_ids)
+        a, n = _per_seq("first", first, ids), _per_seq("count", count, ids)
+        total = int(np.maximum(n, 0).sum()) * self.kvc * HD
+        self._chk(self.lib.dz_kv_rows_q4(self.h, layer, len(ids), _np_ptr(ids), _np_ptr(a), _np_ptr(n),
+                                         _tensor("k", k, torch.float32, total), _tensor("v", v, torch.float32, total),
+                                         _stream(stream)))
+
+    def _weights_numel(self, layer, ids):
+        return self.kvc * sum(self.kv_len(layer, int(s)) for s in ids)
+
+    def kv_weights_q4(self, layer, seq_ids, out, stream=None):
+        """Accumulated attention weights, sequence by sequence [kvc][length]."""
+        import torch
+        ids = _ids(seq_ids)
+        self._chk(self.lib.dz_kv_weights_q4(
+            self.h, layer, len(ids), _np_ptr(ids),
+            _tensor("out", out, torch.float32, self._weights_numel(layer, ids)), _stream(stream)))
+
+    def kv_set_weights_q4(self, layer, seq_ids, weights, stream=None):
+        import torch
+        ids = _ids(seq_ids)
+        self._chk(self.lib.dz_kv_set_weights_q4(
+            self.h, layer, len(ids), _np_ptr(ids),
+            _tensor("weights", weights, torch.float32, self._weights_numel(layer, ids)), _stream(stream)))
 
     def gdn_decode(self, layer, seq_ids, qkv, alpha, beta, z, y, stream=None):
         ids = np.ascontiguousarray(np.atleast_1d(seq_ids), np.int32)

@@ -244,6 +244,68 @@ dz_status dz_rmsnorm_rows(dz_ctx* ctx, int T, int n, const float* x, const float
 dz_status dz_block_mlp(dz_ctx* ctx, int T, int hidden, int d_ff, float* h, const float* post_norm_w,
                        const void* w_gate, const void* w_up, const void* w_down, void* stream);
 
+/* ---- KV caches held in 4 bits ------------------------------------------------ */
+/* dz_cache_create_q4 is dz_cache_create with the K and V of every full-attention
+ * layer held in 4 bits: 272 bytes per (position, kv head) instead of 2048.  A row
+ * of 256 values is 8 groups of 32; a group's scale s is max|x| / 7 rounded to 4
+ * significant bits (nearest even; grid 2^-17 below 2^-14; at most 896), each value
+ * the multiple of s nearest to it (ties to even) within 7 s.  NaN is held as 0,
+ * infinities as 7 * 896 with their sign.  K is normalised, rotated and quantised in
+ * f64, so the held codes do not depend on rounding on the way.  Attention works on
+ * the held values, the new token's own row included.
+ * With track_weights, the caches also accumulate attention weights (below).
+ *
+ * The length, truncate, reset, snapshot, import, export and session calls work on
+ * these caches as on f32 ones: import (and session load) quantises, export (and
+ * session save) gives the held values; importing those again gives the same rows.
+ * Snapshots do not hold the accumulated weights.  The f32 compute calls
+ * (dz_gqa_decode*, dz_gqa_prefill*, dz_kv_fill_pattern) refuse them (DZ_ESTATE), as
+ * the calls below refuse f32 caches.  dz_rope_table is empty: rotary angles are
+ * computed in f64 from the positions, at any position.
+ * The calls below use scratch of the context: calls that overlap on the GPU (two
+ * streams, two replayed graphs) race, so order them. */
+dz_status dz_cache_create_q4(dz_ctx* ctx, int n_seqs, const int64_t* max_len, int track_weights);
+
+/* Rotary positions with three axes (time, height, width): which axis turns each of
+ * the 32 rotary pairs.  sections (host [3]) sum to 32.  Contiguous: the first
+ * sections[0] pairs turn by time, the next sections[1] by height, the rest by
+ * width.  Interleaved: t h w t h w ..., time where height or width has used up its
+ * pairs (at most 11 and 10).  Default {11, 11, 10}, contiguous
+ * (Daiza-engine/src/model/config.rs:47-74).  Text has the same position on every
+ * axis.  Pair i at position p turns by p * base^(-2i/64), taken in f64, with the
+ * sign convention of dz_gqa_decode. */
+dz_status dz_set_rope_axes(dz_ctx* ctx, const int32_t* sections, int interleaved);
+/* QK-RMSNorm, rotation by pos (device int32 [T][3]) and q's 1/16 as a pass of its
+ * own: q_out [T][6*kvc][256] from the q halves of q_gate [T][6*kvc][512], k_out
+ * [T][kvc][256] from k.  f32, or bf16 in and out (computed in f32, rounded once).
+ * All 16-byte aligned; k_out may be k, otherwise no overlap. */
+dz_status dz_qk_mrope(dz_ctx* ctx, int layer, int64_t T, const int32_t* pos, const float* q_gate, const float* k,
+                      float* q_out, float* k_out, void* stream);
+dz_status dz_qk_mrope_bf16(dz_ctx* ctx, int layer, int64_t T, const int32_t* pos, const uint16_t* q_gate,
+                           const uint16_t* k, uint16_t* q_out, uint16_t* k_out, void* stream);
+
+/* dz_gqa_decode on 4-bit caches.  pos: host int32 [B][3], the new tokens' rotary
+ * positions (>= 0), or NULL for the cache length on every axis; after an eviction
+ * the caller gives them, since slots are no longer positions.  q_gate, k and v
+ * 16-byte aligned. */
+dz_status dz_gqa_decode_q4(dz_ctx* ctx, int layer, int B, const int32_t* seq_ids, const int32_t* pos,
+                           const float* q_gate, const float* k, const float* v, float* out, void* stream);
+
+/* Held rows as f32: rows [first[b], first[b] + count[b]) of each sequence (host
+ * arrays), one sequence behind the other: device k, v [sum count][kvc][256],
+ * 16-byte aligned.  Stream-ordered. */
+dz_status dz_kv_rows_q4(dz_ctx* ctx, int layer, int B, const int32_t* seq_ids, const int64_t* first,
+                        const int64_t* count, float* k, float* v, void* stream);
+
+/* Accumulated attention weights (caches made with track_weights): every decode call
+ * adds to each position of each kv head the softmax probabilities that the head's 6
+ * q heads give it; a new position starts with those of its own token, an imported
+ * one with 0.  Device f32, sequence b's [kvc][length] behind those before it: read
+ * them, or set them (to restore them with a snapshot, or to fade them). */
+dz_status dz_kv_weights_q4(dz_ctx* ctx, int layer, int B, const int32_t* seq_ids, float* out, void* stream);
+dz_status dz_kv_set_weights_q4(dz_ctx* ctx, int layer, int B, const int32_t* seq_ids, const float* weights,
+                               void* stream);
+
 /* ---- DZSS session files -------------------------------------------------- */
 /* Save / restore one sequence's caches in the reference's session format v1
  * (Daiza-runtime/src/session_persist.rs:1-36, save_to_disk :76-140,

@@ -1,0 +1,98 @@
+"""4-bit KV cache, what needs no GPU: properties of the row format (oracle/q4_ref.py) and
+refusals that come before any device work."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from oracle import q4_ref as R
+
+
+def rows(seed, n=64, spread=3.0):
+    r = np.random.default_rng(seed)
+    return r.standard_normal((n, 256)) * np.exp(spread * r.standard_normal((n, 1)))
+
+
+def test_held_values_are_f16_with_few_bits():
+    """code * scale is exact in f16, and 72 * scale (the unpacking's constant) is one too."""
+    _, s = R.codes(np.concatenate([rows(1), rows(2) * 1e4, rows(3) * 1e-6]))
+    held = R.hold(rows(1))
+    assert np.array_equal(held, held.astype(np.float16).astype(np.float64))
+    for k in (1, 7, 72):
+        assert np.array_equal(k * s, (k * s).astype(np.float16).astype(np.float64))
+    assert np.all((s.astype(np.float16).view(np.uint16) & 127) == 0)     # 8 bits hold it
+
+
+def test_error_is_half_a_step_and_holding_again_changes_nothing():
+    x = rows(4, spread=1.0)                          # nothing near the largest held value
+    c, s = R.codes(x)
+    held = R.hold(x)
+    normal = np.repeat(s, 32, -1) >= 2.0 ** -14
+    assert np.all((np.abs(x - held) <= np.repeat(s, 32, -1) / 2)[normal])
+    assert np.abs(c).max() == 7
+    for v in (held, R.hold(1e-6 * x), R.hold(1e5 * x)):
+        assert np.array_equal(R.hold(v), v)
+
+
+def test_ties_zeros_and_what_is_not_finite():
+    x = np.zeros((3, 256))
+    x[0, :4] = [7.0, 0.5, 1.5, -2.5]                 # scale 1: ties go to the even code
+    x[1, :3] = [np.nan, np.inf, -np.inf]
+    x[2, 0] = 2.0 ** -30                             # below half the smallest scale
+    assert R.hold(x)[0, :4].tolist() == [7.0, 0.0, 2.0, -2.0]
+    assert R.hold(x)[1, :3].tolist() == [0.0, 7 * 896.0, -7 * 896.0]
+    assert not R.hold(x)[2].any()
+
+
+def test_axes_of_the_rotary_pairs():
+    assert np.bincount(R.axes()).tolist() == [11, 11, 10]
+    assert np.bincount(R.axes(interleaved=True)).tolist() == [11, 11, 10]
+    assert R.axes(interleaved=True)[:6].tolist() == [0, 1, 2, 0, 1, 2]
+    assert R.axes((16, 8, 8), True)[24:].tolist() == [0, 0, 0, 0, 0, 0, 0, 0]
+
+
+def test_prompt_is_its_tokens_one_by_one():
+    r = np.random.default_rng(5)
+    qg, k, v = r.standard_normal((5, 6, 512)), r.standard_normal((5, 1, 256)), r.standard_normal((5, 1, 256))
+    qn, kn = 1 + 0.1 * r.standard_normal((2, 256))
+    whole, steps = R.Cache(1), R.Cache(1)
+    a = whole.extend(qg, k, v, qn, kn)
+    b = np.concatenate([steps.extend(qg[t:t + 1], k[t:t + 1], v[t:t + 1], qn, kn) for t in range(5)])
+    assert np.array_equal(a, b) and np.array_equal(whole.w, steps.w)
+    assert np.allclose(whole.w.sum(), 5 * 6)
+
+
+def test_eviction_keeps_the_recent_and_the_heaviest():
+    c = R.Cache(1, np.ones((6, 1, 256)), np.ones((6, 1, 256)))
+    c.w = np.array([[0.5, 0.0, 0.5, 2.0, 0.5, 0.0]])
+    assert c.evict(4, 1).tolist() == [[0, 2, 3, 5]]          # of three equal weights the first two
+    assert c.w.tolist() == [[0.5, 0.5, 2.0, 0.0]]
+    assert c.evict(9, 1).tolist() == [[0, 1, 2, 3]]
+
+
+def test_null_contexts_are_refused():
+    from daiza_b200 import _ffi
+    lib, none = _ffi.lib(), None
+    sections = (C.c_int32 * 3)(11, 11, 10)
+    one = (C.c_int64 * 1)(4)
+    ids = (C.c_int32 * 1)(0)
+    assert lib.dz_cache_create_q4(none, 1, one, 0) == _ffi.DZ_EINVAL
+    assert lib.dz_set_rope_axes(none, sections, 0) == _ffi.DZ_EINVAL
+    assert lib.dz_qk_mrope(none, 0, 1, none, none, none, none, none, none) == _ffi.DZ_EINVAL
+    assert lib.dz_qk_mrope_bf16(none, 0, 1, none, none, none, none, none, none) == _ffi.DZ_EINVAL
+    assert lib.dz_gqa_decode_q4(none, 0, 1, ids, none, none, none, none, none, none) == _ffi.DZ_EINVAL
+    assert lib.dz_kv_rows_q4(none, 0, 1, ids, one, one, none, none, none) == _ffi.DZ_EINVAL
+    assert lib.dz_kv_weights_q4(none, 0, 1, ids, none, none) == _ffi.DZ_EINVAL
+    assert lib.dz_kv_set_weights_q4(none, 0, 1, ids, none, none) == _ffi.DZ_EINVAL
+
+
+def test_host_tensors_wrong_types_and_sizes_are_refused():
+    torch = pytest.importorskip("torch")
+    from daiza_b200 import engine
+    from daiza_b200._ffi import DZ_EINVAL, DzError
+    for bad in (torch.zeros(4), torch.zeros(4, dtype=torch.bfloat16)):
+        with pytest.raises(DzError) as e:
+            engine._tensor("x", bad, torch.float32, 4)
+        assert e.value.status == DZ_EINVAL
+    with pytest.raises(DzError):
+        engine._per_seq("count", [1, 2], engine._ids([0]))
