@@ -57,7 +57,7 @@ void free_cache(dz_ctx* ctx) {
     ctx->part_items = 0;
     ctx->q4 = ctx->q4_track = false;
     ctx->q4_frag = nullptr;
-    ctx->q4_qs = ctx->q4_sc = nullptr;
+    ctx->q4_sc = nullptr;
     ctx->n_seqs = 0;
     ctx->caps.clear();
     for (auto& sn : ctx->snaps) sn.valid = false;
@@ -461,16 +461,11 @@ static dz_status cache_create(dz_ctx* ctx, int n_seqs, const int64_t* max_len, b
         }
         ctx->part_ml = static_cast<float*>(d);
         if (q4) {
-            if ((st = dev_alloc(ctx, &d, (size_t)nb * kvc * 16 * 32 * 4 * sizeof(uint32_t), false)) != DZ_OK) {
+            if ((st = dev_alloc(ctx, &d, (size_t)nb * kvc * Q4_FRAG_WORDS * sizeof(uint32_t), false)) != DZ_OK) {
                 free_cache(ctx);
                 return st;
             }
             ctx->q4_frag = static_cast<uint32_t*>(d);
-            if ((st = dev_alloc(ctx, &d, (size_t)nb * kvc * 8 * sizeof(float), false)) != DZ_OK) {
-                free_cache(ctx);
-                return st;
-            }
-            ctx->q4_qs = static_cast<float*>(d);
             if (track) {
                 const size_t tiles = (size_t)(sum_n / Q4_TILE) + nb;
                 if ((st = dev_alloc(ctx, &d, tiles * kvc * GRP * Q4_TILE * sizeof(float), false)) != DZ_OK) {

@@ -46,6 +46,19 @@ struct Q4Slot {
     __host__ __device__ int64_t n_tiles() const { return (cap + Q4_TILE - 1) / Q4_TILE; }
     __host__ __device__ uint8_t* tile(int kvh, int64_t t) const { return tiles + (kvh * n_tiles() + t) * Q4_TILE_BYTES; }
 };
+// Rows (sequence, kv head) and tiles of one decode launch over 4-bit caches; cum[b] = tiles of the sequences before b, one kv head.
+struct Q4Rows {
+    int B, kvc;
+    int32_t sid[MAXB], len[MAXB];                // slot of sequence b, its length before this token
+    int32_t cum[MAXB + 1];
+    __host__ __device__ int64_t tiles() const { return (int64_t)cum[B] * kvc; }
+    __host__ __device__ int row_tiles(int b) const { return cum[b + 1] - cum[b]; }
+    __host__ __device__ int64_t row_start(int row) const {
+        const int b = row / kvc;
+        return (int64_t)cum[b] * kvc + (int64_t)(row - b * kvc) * row_tiles(b);
+    }
+};
+constexpr int Q4_FRAG_WORDS = 16 * 32 * 4 + 16;   // q as matrix operand, one row (q4_decode.cu)
 // The three rotary positions (time, height, width) of each batch row of a decode launch.
 struct Q4Pos { int32_t p[MAXB][3]; };
 // Rotary axes: which of a token's three positions turns pair i, and the pair's frequency
@@ -140,14 +153,12 @@ struct dz_ctx {
         cudaEvent_t landed = nullptr, done = nullptr;
     } hs[2];                     // 0: gated GQA, 1: Gated DeltaNet
     cudaEvent_t pf_ev[dz::PF_MAX_SEGMENTS + 1] = {};
-    // 4-bit KV caches (dz_cache_create_q4): the decode kernels' q operand and its scales,
-    // the scores of tracked caches, and scratch of prompts and evictions.  A buffer that is
+    // 4-bit KV caches (dz_cache_create_q4): the decode kernels' q operand, the scores of tracked caches, and scratch of prompts and evictions.  A buffer that is
     // outgrown stays allocated until the context goes: a captured graph may hold it.
     bool q4 = false, q4_track = false;
     dz::RopeAxes axes{};
-    uint32_t* q4_frag = nullptr;  // [min(n_seqs, MAXB)][kvc][16][32][4]
-    float* q4_qs = nullptr;       // [min(n_seqs, MAXB)][kvc][8]
-    float* q4_sc = nullptr;       // [tiles of one launch][kvc][6][16]
+    uint32_t* q4_frag = nullptr;  // [min(n_seqs, MAXB)][kvc][Q4_FRAG_WORDS]
+    float* q4_sc = nullptr;       // [tiles of one launch, all kv heads][6][16]
     void* q4_scratch = nullptr;
     size_t q4_scratch_bytes = 0;
     std::vector<void*> q4_retired;
@@ -290,12 +301,10 @@ cudaError_t launch_q1_gemv(dz_ctx* ctx, int n_mats, const uint8_t* const* w, con
 // block tail (block_tail.cu): RMSNorm rows and SwiGLU, stream-ordered
 cudaError_t launch_rmsnorm_rows(const float* x, const float* w, float eps, int T, int n, float* out, cudaStream_t st);
 cudaError_t launch_swiglu(float* gate, const float* up, int64_t n, cudaStream_t st);
-// merge of the split-K partials, normalisation and gate (gqa_decode.cu)
-cudaError_t launch_gqa_combine(dz_ctx* ctx, const GqaDecodeDesc& d, const float* q_gate, float* out, cudaStream_t st,
-                               const float* part_o, const float* part_ml);
 // 4-bit KV caches (q4_*.cu)
-cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, const GqaDecodeDesc& d, const Q4Pos& pos, const float* q_gate,
+cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, const Q4Rows& d, const Q4Pos& pos, const float* q_gate,
                              const float* k, const float* v, float* out, cudaStream_t st, int* n_launch);
+int q4_decode_runs(int n_sm);   // most partials of a launch, beside one per row
 dz_status q4_import(dz_ctx* ctx, int layer, int seq, const float* k, const float* v, int64_t len);
 dz_status q4_export(dz_ctx* ctx, int layer, int seq, float* k, float* v);
 // grows ctx->q4_scratch to at least `bytes` (the old buffer is kept: see above)

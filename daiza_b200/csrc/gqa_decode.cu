@@ -435,25 +435,6 @@ __global__ void __launch_bounds__(32 * CMB_MAX_GROUPS) gqa_combine_kernel(GqaDec
     }
 }
 
-// the combine grid as a programmatic dependent of the split grid before it
-cudaError_t launch_gqa_combine(dz_ctx* ctx, const GqaDecodeDesc& d, const float* q_gate, float* out, cudaStream_t st,
-                               const float* part_o, const float* part_ml) {
-    const int kvc = ctx->cfg.kv_head_count;
-    int max_nc = 0;
-    for (int b = 0; b < d.B; ++b) max_nc = std::max(max_nc, d.cum[b + 1] - d.cum[b]);
-    const int groups = max_nc > 256 / 2 ? 32 : (max_nc > 64 ? 16 : 8);
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t lc{};
-    lc.gridDim = dim3(GRP * kvc, d.B);
-    lc.blockDim = dim3(32 * groups);
-    lc.stream = st;
-    lc.attrs = at;
-    lc.numAttrs = 1;
-    return cudaLaunchKernelEx(&lc, gqa_combine_kernel, d, kvc, part_o, part_ml, q_gate, out);
-}
-
 // prep as a programmatic dependent of whatever came before in the stream (it
 // waits for that grid before anything else), then the split grid as a
 // programmatic dependent of prep (old K/V tiles stream in while prep finishes)
@@ -464,6 +445,8 @@ cudaError_t launch_gqa_decode_scratch(dz_ctx* ctx, int layer, const GqaDecodeDes
     const LayerState& L = ctx->layers[layer];
     const int kvc = ctx->cfg.kv_head_count;
     const int items = d.cum[d.B] * kvc;
+    int max_nc = 0;
+    for (int b = 0; b < d.B; ++b) max_nc = std::max(max_nc, d.cum[b + 1] - d.cum[b]);
     cudaError_t e = cudaFuncSetAttribute(gqa_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)sizeof(SplitSmem));
     if (e != cudaSuccess) return e;
@@ -492,7 +475,11 @@ cudaError_t launch_gqa_decode_scratch(dz_ctx* ctx, int layer, const GqaDecodeDes
     e = cudaLaunchKernelEx(&lc, gqa_split_kernel, d, kvc, (const KvSlot*)L.d_kv, (const float*)q_buf, part_o,
                            part_ml, ctx->d_err, items);
     if (e != cudaSuccess) return e;
-    e = launch_gqa_combine(ctx, d, q_gate, out, st, part_o, part_ml);
+    const int groups = max_nc > 256 / 2 ? 32 : (max_nc > 64 ? 16 : 8);
+    lc.gridDim = dim3(GRP * kvc, d.B);
+    lc.blockDim = dim3(32 * groups);
+    lc.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&lc, gqa_combine_kernel, d, kvc, (const float*)part_o, (const float*)part_ml, q_gate, out);
     if (e != cudaSuccess) return e;
     *n_launch += 3;
     return cudaGetLastError();

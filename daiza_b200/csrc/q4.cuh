@@ -85,12 +85,33 @@ __device__ __forceinline__ uint32_t hmul2_u(uint32_t a, uint32_t b) {
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
+// (x & mask) | magic in one operation (written in C++ it becomes two: one immediate each)
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t magic) {
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "r"(mask), "r"(magic));
+    return d;
+}
 constexpr uint32_t NEG72 = 0xD480D480u;                        // f16 pair of -72
 // Nibbles n at bits 4..7 and 20..23 of x -> the f16 pair (n - 8) * s.  Under the
 // exponent of 64 those bits have weights 8, 4, 2, 1: 64 + n.  (64 + n) s - 72 s in
 // one fused operation is exact; c = -72 s.
 __device__ __forceinline__ uint32_t unpack(uint32_t x, uint32_t s, uint32_t c) {
-    return hfma2_u((x & 0x00F000F0u) | 0x54005400u, s, c);
+    return hfma2_u(and_or(x, 0x00F000F0u, 0x54005400u), s, c);
+}
+
+// The matrix loops unpack a word's four pairs from w and w >> 8 alone: nibbles at bits
+// 0..3 and 16..19 under the exponent of 1024 (weights 8 4 2 1: 1024 + n), nibbles at bits
+// 4..7 and 20..23 under that of 64.  -1032 s would leave f16 at s = 64, so these work with
+// s / 16 and give value / 16, still exact (s / 16 is a multiple of 2^-21, f16's grid 2^-24).
+struct Scale16 { uint32_t s, c_lo, c_hi; };                    // f16 pairs: s / 16, -1032 s / 16, -72 s / 16
+__device__ __forceinline__ Scale16 scale16(uint32_t pair) {    // pair: scale_pair()
+    return {hmul2_u(pair, 0x2C002C00u), hmul2_u(pair, 0xD408D408u), hmul2_u(pair, 0xC480C480u)};
+}
+__device__ __forceinline__ uint32_t unpack_lo(uint32_t x, const Scale16& k) {
+    return hfma2_u(and_or(x, 0x000F000Fu, 0x64006400u), k.s, k.c_lo);
+}
+__device__ __forceinline__ uint32_t unpack_hi(uint32_t x, const Scale16& k) {
+    return hfma2_u(and_or(x, 0x00F000F0u, 0x54005400u), k.s, k.c_hi);
 }
 
 // ---- rotary positions ----------------------------------------------------------------

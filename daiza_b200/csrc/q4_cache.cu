@@ -407,26 +407,20 @@ dz_status dz_gqa_decode_q4(dz_ctx* ctx, int layer, int B, const int32_t* seq_ids
         const int kvc = ctx->cfg.kv_head_count, nq = GRP * kvc;
         int launches = 0;
         for (int b0 = 0; b0 < B; b0 += MAXB) {
-            GqaDecodeDesc d;
+            Q4Rows d;
             Q4Pos p3;
             d.B = std::min(MAXB, B - b0);
-            int64_t n[MAXB];
-            for (int b = 0; b < d.B; ++b) n[b] = L.len[seq_ids[b0 + b]] + 1;
-            const int64_t chunk = decode_chunk_balanced(ctx->n_sm, kvc, n, d.B, ctx->part_items);
-            d.chunk = (int)chunk;
+            d.kvc = kvc;
             d.cum[0] = 0;
-            int32_t tiles = 0;
             for (int b = 0; b < d.B; ++b) {
                 d.sid[b] = seq_ids[b0 + b];
-                d.len[b] = (int32_t)(n[b] - 1);
-                d.pos[b] = tiles;                 // first of the sequence's tiles in the score scratch
-                tiles += (int32_t)((n[b] + Q4_TILE - 1) / Q4_TILE);
+                d.len[b] = (int32_t)L.len[d.sid[b]];
                 for (int i = 0; i < 3; ++i) p3.p[b][i] = pos ? pos[3 * (b0 + b) + i] : d.len[b];
-                d.cum[b + 1] = d.cum[b] + (int32_t)((n[b] + chunk - 1) / chunk);
+                d.cum[b + 1] = d.cum[b] + (int32_t)(((int64_t)d.len[b] + Q4_TILE) / Q4_TILE);
             }
-            if ((int64_t)d.cum[d.B] * kvc > ctx->part_items)   // cannot happen under decode_items_bound
-                return fail(ctx, DZ_ESTATE, "%lld split-K items exceed the scratch (%lld)",
-                            (long long)d.cum[d.B] * kvc, (long long)ctx->part_items);
+            if (q4_decode_runs(ctx->n_sm) + d.B * kvc > ctx->part_items)   // cannot happen under decode_items_bound
+                return fail(ctx, DZ_ESTATE, "the partials of %d sequences exceed the scratch (%lld)", d.B,
+                            (long long)ctx->part_items);
             Q4_CUDA(launch_q4_decode(ctx, layer, d, p3, q_gate + (size_t)b0 * nq * QG_ROW, k + (size_t)b0 * kvc * HD,
                                      v + (size_t)b0 * kvc * HD, out + (size_t)b0 * nq * HD,
                                      static_cast<cudaStream_t>(stream), &launches));

@@ -4,9 +4,9 @@
 // held in 4 bits and rotary positions of three axes.  Stream-ordered kernels:
 //   1. q4_prep     : per sequence and head -- deinterleave [Q_h | gate_h], QK-RMSNorm,
 //                    rotation; q as matrix operand, K and V quantised into slot len.
-//   2. q4_split    : per (sequence, chunk, kv head), one warp each: scores, online
-//                    softmax, P V over the chunk's tiles; unnormalised partials out.
-//   3. gqa_combine : (gqa_decode.cu) merge, normalise, gate.
+//   2. q4_split    : scores, online softmax and P V over the cached tiles, cut evenly
+//                    over the SMs; unnormalised partials out.
+//   3. q4_combine  : per (sequence, q head) -- merge, normalise, gate.
 //   4. q4_weights  : tracked caches -- the new attention weights are added.
 #include <algorithm>
 #include <cstddef>
@@ -18,22 +18,25 @@ namespace q4 {
 
 // ---------------------------------------------------------------------------
 // 1. prep: grid (B, ceil((nq + kvc) / 8)), one head per warp.
-//    q is scaled by log2(e) / 16 (scores in log2 units) and by a power of two that
+//    q is scaled by log2(e) (scores in log2 units; the 1/16 comes with K's unpacking,
+//    which gives K / 16) and by a power of two that
 //    puts the head's largest magnitude into [2^11, 2^12), then split into f16 hi + lo
 //    (22 bits; f16 subnormals start 2^25 below), in the register order of the A
 //    operand of mma.m16n8k16: rows 0..7 are the hi parts of the group's heads (6 and 7
 //    empty), rows 8..15 the lo parts, so one product of K gives both.
 //      q_frag [b][kvh][step 16][lane][hi 0,1 | lo 0,1 | hi 2,3 | lo 2,3]
 //    where step s, lane (r, c) covers dims 64 c + 4 s .. + 3 of head r.
+//    and behind the 16 steps the heads' factors back (f32 [8], 0 for the empty heads).
 // ---------------------------------------------------------------------------
-constexpr int FRAG_WORDS = 16 * 32 * 4;       // words of q_frag per (sequence, kv head)
+using Rows = Q4Rows;
+constexpr int FRAG_WORDS = Q4_FRAG_WORDS, FRAG_SCALES = 16 * 32 * 4;
 
-__global__ void __launch_bounds__(256) q4_prep_kernel(GqaDecodeDesc d, Q4Pos pos, RopeAxes axes, int kvc,
-                                                      const Q4Slot* __restrict__ slots,
+__global__ void __launch_bounds__(256) q4_prep_kernel(const __grid_constant__ Rows d, const __grid_constant__ Q4Pos pos,
+                                                      RopeAxes axes, const Q4Slot* __restrict__ slots,
                                                       const float* __restrict__ q_norm, const float* __restrict__ k_norm,
                                                       const float* __restrict__ q_gate, const float* __restrict__ k_in,
                                                       const float* __restrict__ v_in, uint32_t* __restrict__ q_frag,
-                                                      float* __restrict__ q_scale, float eps) {
+                                                      float eps) {
     __shared__ double2 cs[ROPE / 2];
     const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 0) cs[lane] = rope_cs(axes, lane, pos.p[b][0], pos.p[b][1], pos.p[b][2]);
@@ -42,7 +45,7 @@ __global__ void __launch_bounds__(256) q4_prep_kernel(GqaDecodeDesc d, Q4Pos pos
     // before the split grid may start streaming old tiles.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-    const int nq = GRP * kvc;
+    const int kvc = d.kvc, nq = GRP * kvc;
     const int task = blockIdx.y * 8 + warp;
     if (task >= nq + kvc) return;
     if (task < nq) {
@@ -53,7 +56,7 @@ __global__ void __launch_bounds__(256) q4_prep_kernel(GqaDecodeDesc d, Q4Pos pos
         float amax = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            x[e] *= 0.0625f * LOG2E;
+            x[e] *= LOG2E;
             amax = fmaxf(amax, fabsf(x[e]));
         }
         amax = warp_max(amax);
@@ -74,15 +77,14 @@ __global__ void __launch_bounds__(256) q4_prep_kernel(GqaDecodeDesc d, Q4Pos pos
         const int at = (lane & 7) * 64 + r * 4 + (lane >> 3);  // steps 2 w and 2 w + 1 of word w = lane % 8, c = lane / 8
         dst[at] = make_uint4(hi[0], lo[0], hi[1], lo[1]);
         dst[at + 32] = make_uint4(hi[2], lo[2], hi[3], lo[3]);
-        if (lane == 0)
-            q_scale[(b * kvc + kvh) * 8 + r] = __uint_as_float((uint32_t)(254 - field) << 23);
+        if (lane == 0) reinterpret_cast<uint32_t*>(dst)[FRAG_SCALES + r] = (uint32_t)(254 - field) << 23;
     } else {
         const int kvh = task - nq, slot_pos = d.len[b];
         uint4* dst = reinterpret_cast<uint4*>(q_frag + (size_t)(b * kvc + kvh) * FRAG_WORDS);
 #pragma unroll
         for (int i = 0; i < 4; ++i)                            // the operand's empty rows: heads 6 and 7
             dst[(4 * i + (lane >> 3)) * 32 + 24 + (lane & 7)] = make_uint4(0u, 0u, 0u, 0u);
-        if (lane < 2) q_scale[(b * kvc + kvh) * 8 + 6 + lane] = 0.0f;
+        if (lane < 2) reinterpret_cast<uint32_t*>(dst)[FRAG_SCALES + 6 + lane] = 0u;
         uint8_t* tile = slots[d.sid[b]].tile(kvh, slot_pos >> 4);
         const int p = slot_pos & 15;
         const size_t at = ((size_t)b * kvc + kvh) * HD + 8 * lane;
@@ -104,49 +106,73 @@ __global__ void __launch_bounds__(256) q4_prep_kernel(GqaDecodeDesc d, Q4Pos pos
 }
 
 // ---------------------------------------------------------------------------
-// 2. split-K attention, one warp per (sequence, chunk, kv head).
-//    A tile (16 positions, 4352 bytes) is one bulk copy into the warp's own ring.
-//    Scores: S = Q K^T, A = q (hi rows, lo rows), B = the 8 positions of a K word row,
-//    16 steps of 16 dims; thread (r, c) gets head r at positions 2c, 2c+1 (hi sum and
-//    lo sum, added).  That is the B operand's own layout, so P needs no shuffle:
-//    O^T += V^T P^T, A = V's dims x 16 positions, B = P (hi, then lo), 16 tiles of 16
-//    dims accumulated in 64 registers.
+// 2. attention over the tiles, the whole batch cut into equal runs of tiles, a warp each.
+//    Rows are (sequence, kv head) in order; their tiles are numbered through, and run c
+//    of R takes tiles [W c / R, W (c + 1) / R): every warp reads the same number of bytes
+//    however ragged the batch is, and no warp waits for another.  A run covers parts of
+//    one or more rows; each part (segment) gives one unnormalised partial, at index
+//    c + row (unique: both only grow along the runs).
+//    A tile (16 positions, 4352 bytes) is one bulk copy into the warp's own ring,
+//    requested across segment ends; q of the segment is another.
+//    Scores: S = Q K^T, A = q (hi rows, lo rows), B = the 8 positions of a K word row, 16
+//    steps of 16 dims; thread (r, c) gets head r at positions 2c, 2c+1 (hi sum and lo sum,
+//    added).  That is the B operand's own layout, so P needs no shuffle: O^T += V^T P^T,
+//    A = V's dims x 16 positions, B = P (hi, then lo), 16 tiles of 16 dims accumulated in
+//    64 registers.
 // ---------------------------------------------------------------------------
-constexpr int Q4_STAGES = 4;
-constexpr int Q4_WARPS = GQA_SPLIT_WARPS;
-constexpr float P_LOG2 = 12.0f;               // p is scaled by 2^12: its f16 lo part keeps 11 bits down to 2^-11
+constexpr int STAGES = 2, WARPS = 12;
+// p is taken against a maximum that may be stale by P_SLACK and is scaled by 2^P_LOG2: at
+// most 2^15, and its f16 lo part keeps its bits down to 2^-21 of the maximum.
+constexpr float P_LOG2 = 8.0f, P_SLACK = 7.0f;
 
-struct alignas(128) Q4Ring {
-    uint8_t tile[Q4_STAGES][Q4_TILE_BYTES];
-    uint64_t full[Q4_STAGES];
+struct alignas(128) Ring {
+    uint8_t tile[STAGES][Q4_TILE_BYTES];
+    uint32_t q[FRAG_WORDS];
+    uint64_t full[STAGES], q_full;
 };
-static_assert(sizeof(Q4Ring) % 128 == 0 && Q4_TILE_BYTES % 128 == 0, "bulk copies need 16-byte alignment");
-struct Q4Smem { Q4Ring w[Q4_WARPS]; };
+static_assert(Q4_TILE_BYTES % 128 == 0 && sizeof(Ring) % 128 == 0 && FRAG_WORDS % 4 == 0,
+              "bulk copies need 16-byte alignment");
 
-struct Q4Item { int b, kvh, p0, p1, ntiles; const uint8_t* base; };
+// W c overflows nothing: W is below 2^36 tiles, c below 2^12 runs
+__host__ __device__ inline int64_t run_start(int64_t W, int c, int R) { return W * c / R; }
+// the run that holds a tile
+__device__ __forceinline__ int run_of(int64_t tile, int64_t W, int R) {
+    int c = (int)(tile * R / W);
+    while (run_start(W, c + 1, R) <= tile) ++c;
+    while (run_start(W, c, R) > tile) --c;
+    return c;
+}
 
-__device__ __forceinline__ Q4Item q4_item(const GqaDecodeDesc& d, int kvc, const Q4Slot* __restrict__ slots, int item) {
-    Q4Item it;
-    const int chunk_idx = item / kvc;
-    it.kvh = item - chunk_idx * kvc;
-    int lo = 0, hi = d.B - 1;                    // last b with cum[b] <= chunk_idx
+// The part of a row that a run covers: tiles [t0, t1) of the row.
+struct Segment { int b, row, t0, t1; const uint8_t* base; };
+
+__device__ __forceinline__ Segment segment_at(const Rows& d, const Q4Slot* __restrict__ slots, int64_t tile, int64_t end) {
+    Segment s;
+    int lo = 0, hi = d.B - 1;                    // last b whose rows start at or before the tile
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (d.cum[mid] <= chunk_idx) lo = mid; else hi = mid - 1;
+        if ((int64_t)d.cum[mid] * d.kvc <= tile) lo = mid; else hi = mid - 1;
     }
-    it.b = lo;
-    it.p0 = (chunk_idx - d.cum[lo]) * d.chunk;   // a multiple of 16
-    it.p1 = min(d.len[lo] + 1, it.p0 + d.chunk);
-    it.ntiles = (it.p1 - it.p0 + Q4_TILE - 1) / Q4_TILE;
-    it.base = slots[d.sid[lo]].tile(it.kvh, it.p0 >> 4);
-    return it;
+    s.b = lo;
+    const int n = d.row_tiles(lo);
+    int64_t in = tile - (int64_t)d.cum[lo] * d.kvc;
+    int kvh = 0;
+    while (in >= n) {
+        in -= n;
+        ++kvh;
+    }
+    s.row = lo * d.kvc + kvh;
+    s.t0 = (int)in;
+    s.t1 = (int)min((int64_t)n, s.t0 + (end - tile));
+    s.base = slots[d.sid[lo]].tile(kvh, 0);
+    return s;
 }
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ float ex2f(float x) {
     float y;
@@ -154,24 +180,132 @@ __device__ __forceinline__ float ex2f(float x) {
     return y;
 }
 
+// One warp's running softmax over the tiles that it takes of a segment.
+struct State {
+    float o[16][4];                              // O^T / 16: tile m, dims 32 r + 2 m, + 1, heads 2c, 2c + 1
+    float m, l;                                  // head r; l is this thread's share
+};
+
 template <bool TRACK>
-__global__ void __launch_bounds__(32 * Q4_WARPS, 1)
-    q4_split_kernel(GqaDecodeDesc d, int kvc, const Q4Slot* __restrict__ slots, const uint32_t* __restrict__ q_frag,
-                    const float* __restrict__ q_scale, float* __restrict__ part_o, float* __restrict__ part_ml,
-                    float* __restrict__ scores, int* err, int n_items) {
+__device__ __forceinline__ void attend_tile(State& st, const uint8_t* tile, const uint32_t* q, float qs, int valid,
+                                            float* __restrict__ scores, int lane) {
+    const int r = lane >> 2, c = lane & 3;
+    // ---- scores of 2 x 8 positions
+    float x[4];
+    {
+        const uint32_t kb = *reinterpret_cast<const uint32_t*>(tile + OFF_KS + lane * 4);
+        float s0[2][4] = {}, s1[2][4] = {};      // two sums per 8 positions: four independent chains
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint32_t ws[2][4];
+            Scale16 sc[2];
+#pragma unroll
+            for (int n8 = 0; n8 < 2; ++n8) {
+                const uint4 w4 = *reinterpret_cast<const uint4*>(tile + (n8 * 2 + i) * 512 + lane * 16);
+                ws[n8][0] = w4.x; ws[n8][1] = w4.y; ws[n8][2] = w4.z; ws[n8][3] = w4.w;
+                // the group's scale byte in both halves
+                sc[n8] = scale16(scale_pair(__byte_perm(kb, 0u, 0x4040 + 0x0101 * (n8 * 2 + i))));
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const uint4 qa = reinterpret_cast<const uint4*>(q)[(8 * i + 2 * u) * 32 + lane];
+                const uint4 qb = reinterpret_cast<const uint4*>(q)[(8 * i + 2 * u + 1) * 32 + lane];
+#pragma unroll
+                for (int n8 = 0; n8 < 2; ++n8) {
+                    const uint32_t w = ws[n8][u], w8 = w >> 8;
+                    mma(s0[n8], qa.x, qa.y, qa.z, qa.w, unpack_lo(w, sc[n8]), unpack_hi(w, sc[n8]));
+                    mma(s1[n8], qb.x, qb.y, qb.z, qb.w, unpack_lo(w8, sc[n8]), unpack_hi(w8, sc[n8]));
+                }
+            }
+        }
+#pragma unroll
+        for (int n8 = 0; n8 < 2; ++n8) {
+            x[2 * n8] = ((s0[n8][0] + s1[n8][0]) + (s0[n8][2] + s1[n8][2])) * qs;
+            x[2 * n8 + 1] = ((s0[n8][1] + s1[n8][1]) + (s0[n8][3] + s1[n8][3])) * qs;
+        }
+    }
+    if (TRACK) {
+        if (r < GRP) {                           // [tile][head][16]
+            *reinterpret_cast<float2*>(scores + r * Q4_TILE + 2 * c) = make_float2(x[0], x[1]);
+            *reinterpret_cast<float2*>(scores + r * Q4_TILE + 2 * c + 8) = make_float2(x[2], x[3]);
+        }
+    }
+    if (valid < Q4_TILE) {                       // the row's last tile
+        if (2 * c >= valid) x[0] = -INFINITY;
+        if (2 * c + 1 >= valid) x[1] = -INFINITY;
+        if (2 * c + 8 >= valid) x[2] = -INFINITY;
+        if (2 * c + 9 >= valid) x[3] = -INFINITY;
+    }
+    // ---- online softmax
+    float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    // rescale only when some head's maximum has outgrown what f16 holds of 2^P_LOG2 p
+    if (__any_sync(0xffffffffu, mx > st.m + P_SLACK)) {
+        const float m_new = fmaxf(st.m, mx), a = ex2f(st.m - m_new);
+        st.l *= a;
+        st.m = m_new;
+        const float a0 = __shfl_sync(0xffffffffu, a, 8 * c), a1 = __shfl_sync(0xffffffffu, a, 8 * c + 4);
+#pragma unroll
+        for (int m = 0; m < 16; ++m) {
+            st.o[m][0] *= a0;
+            st.o[m][1] *= a1;
+            st.o[m][2] *= a0;
+            st.o[m][3] *= a1;
+        }
+    }
+    const float off = P_LOG2 - st.m;
+    uint32_t ph[2], pl[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float p0 = ex2f(x[2 * i] + off), p1 = ex2f(x[2 * i + 1] + off);
+        st.l += p0 + p1;
+        const __half2 h = __floats2half2_rn(p0, p1);
+        const __half2 l = __floats2half2_rn(p0 - __low2float(h), p1 - __high2float(h));
+        ph[i] = *reinterpret_cast<const uint32_t*>(&h);
+        pl[i] = *reinterpret_cast<const uint32_t*>(&l);
+    }
+    // ---- O^T += V^T P^T
+    const uint32_t vb = *reinterpret_cast<const uint32_t*>(tile + OFF_VS + lane * 4);
+    const Scale16 sa = scale16(scale_pair(__byte_perm(vb, 0u, 0x4140)));
+    const Scale16 sb = scale16(scale_pair(__byte_perm(vb, 0u, 0x4342)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint4 w4 = *reinterpret_cast<const uint4*>(tile + OFF_V + i * 512 + lane * 16);
+        const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const uint32_t w = ws[u], w8 = w >> 8;
+            const uint32_t a0 = unpack_lo(w, sa), a2 = unpack_hi(w, sb);
+            const uint32_t a1 = unpack_lo(w8, sa), a3 = unpack_hi(w8, sb);
+            mma(st.o[4 * i + u], a0, a1, a2, a3, ph[0], ph[1]);
+            mma(st.o[4 * i + u], a0, a1, a2, a3, pl[0], pl[1]);
+        }
+    }
+}
+
+template <bool TRACK>
+__global__ void __launch_bounds__(32 * WARPS, 1)
+    q4_split_kernel(const __grid_constant__ Rows d, int R, const Q4Slot* __restrict__ slots,
+                    const uint32_t* __restrict__ q_frag, float* __restrict__ part_o, float* __restrict__ part_ml,
+                    float* __restrict__ scores, int* err) {
     extern __shared__ __align__(128) unsigned char smem_raw[];
-    Q4Ring& R = reinterpret_cast<Q4Smem*>(smem_raw)->w[threadIdx.x >> 5];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-    const int gw = blockIdx.x * Q4_WARPS + warp, nw = gridDim.x * Q4_WARPS;
+    Ring& ring = reinterpret_cast<Ring*>(smem_raw)[warp];
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int run = warp * gridDim.x + blockIdx.x;   // few runs: spread over the SMs first
+    if (run >= R) return;
+    const int64_t W = d.tiles(), run0 = run_start(W, run, R), run1 = run_start(W, run + 1, R);
     if (lane == 0) {
-        for (int s = 0; s < Q4_STAGES; ++s) mbar_init(&R.full[s], 1);
+        for (int s = 0; s < STAGES; ++s) mbar_init(&ring.full[s], 1);
+        mbar_init(&ring.q_full, 1);
         fence_mbar_init();
     }
     __syncwarp();
-    asm volatile("griddepcontrol.launch_dependents;");
-    int p_item = gw, p_tile = 0;
-    Q4Item pinfo{};
-    if (p_item < n_items) pinfo = q4_item(d, kvc, slots, p_item);
+    // producer: the next tile to request
+    int64_t p_end = run0;                        // end of the producer's segment
+    Segment ps{};
+    int p_t = 0;
     // the tile that holds slot len is written by q4_prep: requested after the grid-dependency wait
     bool dep_done = false;
     auto wait_prep = [&]() {
@@ -181,180 +315,160 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 1)
         }
     };
     auto produce = [&](int stage) {
-        if (p_item >= n_items) return;
-        if (pinfo.p0 + (p_tile + 1) * Q4_TILE > d.len[pinfo.b]) wait_prep();
+        if (p_t == ps.t1) {
+            if (p_end == run1) return;
+            ps = segment_at(d, slots, p_end, run1);
+            p_end += ps.t1 - ps.t0;
+            p_t = ps.t0;
+        }
+        if (p_t == d.row_tiles(ps.b) - 1) wait_prep();
         if (lane == 0) {
-            mbar_arrive_expect_tx(&R.full[stage], Q4_TILE_BYTES);
-            bulk_g2s(R.tile[stage], pinfo.base + (size_t)p_tile * Q4_TILE_BYTES, Q4_TILE_BYTES, &R.full[stage]);
+            mbar_arrive_expect_tx(&ring.full[stage], Q4_TILE_BYTES);
+            bulk_g2s(ring.tile[stage], ps.base + (size_t)p_t * Q4_TILE_BYTES, Q4_TILE_BYTES, &ring.full[stage]);
         }
-        if (++p_tile == pinfo.ntiles) {
-            p_item += nw;
-            p_tile = 0;
-            if (p_item < n_items) pinfo = q4_item(d, kvc, slots, p_item);
-        }
+        ++p_t;
     };
-    for (int s = 0; s < Q4_STAGES; ++s) produce(s);
+    for (int s = 0; s < STAGES; ++s) produce(s);
     wait_prep();                                 // q_frag
 
-    int j = 0;
-    for (int item = gw; item < n_items; item += nw) {
-        const Q4Item it = q4_item(d, kvc, slots, item);
-        uint4 q[16];
-        {
-            const uint4* src = reinterpret_cast<const uint4*>(q_frag + (size_t)(it.b * kvc + it.kvh) * FRAG_WORDS) + lane;
-#pragma unroll
-            for (int s = 0; s < 16; ++s) q[s] = src[s * 32];
+    int stage = 0;
+    uint32_t phase = 0, q_phase = 0;
+    for (int64_t at = run0; at < run1; q_phase ^= 1u) {
+        const Segment sg = segment_at(d, slots, at, run1);
+        if (lane == 0) {
+            mbar_arrive_expect_tx(&ring.q_full, FRAG_WORDS * 4);
+            bulk_g2s(ring.q, q_frag + (size_t)sg.row * FRAG_WORDS, FRAG_WORDS * 4, &ring.q_full);
         }
-        const float qs = q_scale[(it.b * kvc + it.kvh) * 8 + r];
-        float o[16][4];
+        if (!mbar_wait(&ring.q_full, q_phase, err)) return;
+        const float qs = __uint_as_float(ring.q[FRAG_SCALES + r]);
+        const int n = d.len[sg.b] + 1;
+        State st;
 #pragma unroll
         for (int m = 0; m < 16; ++m)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[m][e] = 0.0f;
-        float m_run = -INFINITY, l_run = 0.0f;   // head r; l is this thread's share
-
-        for (int t = 0; t < it.ntiles; ++t, ++j) {
-            const int stage = j % Q4_STAGES;
-            if (!mbar_wait(&R.full[stage], (uint32_t)((j / Q4_STAGES) & 1), err)) return;
-            const uint8_t* tile = R.tile[stage];
-            // ---- scores of 2 x 8 positions
-            float x[4];
-            {
-                const uint32_t kb = *reinterpret_cast<const uint32_t*>(tile + OFF_KS + lane * 4);
-#pragma unroll
-                for (int n8 = 0; n8 < 2; ++n8) {
-                    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint4 w4 = *reinterpret_cast<const uint4*>(tile + (n8 * 2 + i) * 512 + lane * 16);
-                        // the group's scale byte in both halves
-                        const uint32_t sc = scale_pair(__byte_perm(kb, 0u, 0x4040 + 0x0101 * (n8 * 2 + i)));
-                        const uint32_t cc = hmul2_u(sc, NEG72);
-                        const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            const uint32_t w = ws[u];
-                            const uint4 qa = q[8 * i + 2 * u], qb = q[8 * i + 2 * u + 1];
-                            mma(s0, qa.x, qa.y, qa.z, qa.w, unpack(w << 4, sc, cc), unpack(w, sc, cc));
-                            mma(s1, qb.x, qb.y, qb.z, qb.w, unpack(w >> 4, sc, cc), unpack(w >> 8, sc, cc));
-                        }
-                    }
-                    x[2 * n8] = ((s0[0] + s1[0]) + (s0[2] + s1[2])) * qs;
-                    x[2 * n8 + 1] = ((s0[1] + s1[1]) + (s0[3] + s1[3])) * qs;
-                }
-            }
-            const int pos = it.p0 + t * Q4_TILE + 2 * c;
-            if (TRACK) {
-                if (r < GRP) {
-                    // [tile of the launch][kvh][head][16]; tiles of sequence b start at tile_cum
-                    float* sc = scores + (((size_t)d.pos[it.b] + ((it.p0 >> 4) + t)) * kvc + it.kvh) * (GRP * Q4_TILE) +
-                                r * Q4_TILE + 2 * c;
-                    *reinterpret_cast<float2*>(sc) = make_float2(x[0], x[1]);
-                    *reinterpret_cast<float2*>(sc + 8) = make_float2(x[2], x[3]);
-                }
-            }
-            if (t == it.ntiles - 1) {
-                if (pos >= it.p1) x[0] = -INFINITY;
-                if (pos + 1 >= it.p1) x[1] = -INFINITY;
-                if (pos + 8 >= it.p1) x[2] = -INFINITY;
-                if (pos + 9 >= it.p1) x[3] = -INFINITY;
-            }
-            // ---- online softmax
-            float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float m_new = fmaxf(m_run, mx);
-            if (__any_sync(0xffffffffu, m_new > m_run)) {
-                const float a = ex2f(m_run - m_new);
-                l_run *= a;
-                const float a0 = __shfl_sync(0xffffffffu, a, 8 * c), a1 = __shfl_sync(0xffffffffu, a, 8 * c + 4);
-#pragma unroll
-                for (int m = 0; m < 16; ++m) {
-                    o[m][0] *= a0;
-                    o[m][1] *= a1;
-                    o[m][2] *= a0;
-                    o[m][3] *= a1;
-                }
-                m_run = m_new;
-            }
-            const float off = P_LOG2 - m_run;
-            float p[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                p[e] = ex2f(x[e] + off);
-                l_run += p[e];
-            }
-            uint32_t ph[2], pl[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const __half2 h = __floats2half2_rn(p[2 * i], p[2 * i + 1]);
-                const __half2 l = __floats2half2_rn(p[2 * i] - __low2float(h), p[2 * i + 1] - __high2float(h));
-                ph[i] = *reinterpret_cast<const uint32_t*>(&h);
-                pl[i] = *reinterpret_cast<const uint32_t*>(&l);
-            }
-            // ---- O^T += V^T P^T
-            {
-                const uint32_t vb = *reinterpret_cast<const uint32_t*>(tile + OFF_VS + lane * 4);
-                const uint32_t sa = scale_pair(__byte_perm(vb, 0u, 0x4140)), sb = scale_pair(__byte_perm(vb, 0u, 0x4342));
-                const uint32_t ca = hmul2_u(sa, NEG72), cb = hmul2_u(sb, NEG72);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint4 w4 = *reinterpret_cast<const uint4*>(tile + OFF_V + i * 512 + lane * 16);
-                    const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const uint32_t w = ws[u];
-                        const uint32_t a0 = unpack(w << 4, sa, ca), a2 = unpack(w, sb, cb);
-                        const uint32_t a1 = unpack(w >> 4, sa, ca), a3 = unpack(w >> 8, sb, cb);
-                        mma(o[4 * i + u], a0, a1, a2, a3, ph[0], ph[1]);
-                        mma(o[4 * i + u], a0, a1, a2, a3, pl[0], pl[1]);
-                    }
-                }
-            }
+            for (int e = 0; e < 4; ++e) st.o[m][e] = 0.0f;
+        st.m = -INFINITY;
+        st.l = 0.0f;
+        for (int t = sg.t0; t < sg.t1; ++t, ++at) {
+            if (!mbar_wait(&ring.full[stage], phase, err)) return;
+            attend_tile<TRACK>(st, ring.tile[stage], ring.q, qs, n - t * Q4_TILE,
+                               TRACK ? scores + (size_t)at * (GRP * Q4_TILE) : nullptr, lane);
             __syncwarp();
             produce(stage);
-        }
-        // ---- partials: thread (r, c) holds dims 32 r .. + 31 of heads 2c, 2c + 1
-        l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
-        l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
-        if (c < GRP / 2) {
-            float* po = part_o + ((size_t)item * GRP + 2 * c) * HD + 32 * r;
-#pragma unroll
-            for (int m = 0; m < 16; m += 2) {
-                *reinterpret_cast<float4*>(po + 2 * m) = make_float4(o[m][0], o[m][2], o[m + 1][0], o[m + 1][2]);
-                *reinterpret_cast<float4*>(po + HD + 2 * m) = make_float4(o[m][1], o[m][3], o[m + 1][1], o[m + 1][3]);
+            if (++stage == STAGES) {
+                stage = 0;
+                phase ^= 1u;
             }
         }
-        if (c == 0 && r < GRP) {
-            part_ml[((size_t)item * GRP + r) * 2 + 0] = m_run - P_LOG2;
-            part_ml[((size_t)item * GRP + r) * 2 + 1] = l_run;
+        // ---- the segment's partial: thread (r, c) holds dims 32 r .. + 31 of heads 2c, 2c + 1
+        st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
+        st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
+        const size_t part = (size_t)run + sg.row;
+        if (c < GRP / 2) {
+            float* po = part_o + (part * GRP + 2 * c) * HD + 32 * r;
+#pragma unroll
+            for (int m = 0; m < 16; m += 2) {    // V came as V / 16
+                *reinterpret_cast<float4*>(po + 2 * m) =
+                    make_float4(16.0f * st.o[m][0], 16.0f * st.o[m][2], 16.0f * st.o[m + 1][0], 16.0f * st.o[m + 1][2]);
+                *reinterpret_cast<float4*>(po + HD + 2 * m) =
+                    make_float4(16.0f * st.o[m][1], 16.0f * st.o[m][3], 16.0f * st.o[m + 1][1], 16.0f * st.o[m + 1][3]);
+            }
         }
+        if (c == 0 && r < GRP)
+            reinterpret_cast<float2*>(part_ml)[part * GRP + r] = make_float2(st.m - P_LOG2, st.l);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// 3. combine: merge a row's partials, divide, gate.  Grid (6 kvc, B, 4 quarters of the
+//    dims), 16 groups of 16 threads that take partials in turn, 4 dims a thread.
+// ---------------------------------------------------------------------------
+constexpr int MAX_RUNS = 2048;                   // warps of the split grid (148 SMs: 1776)
+constexpr int CMB_DIMS = 64;
+
+__global__ void __launch_bounds__(256) q4_combine_kernel(const __grid_constant__ Rows d, int R,
+                                                         const float* __restrict__ part_o,
+                                                         const float* __restrict__ part_ml,
+                                                         const float* __restrict__ q_gate, float* __restrict__ out) {
+    __shared__ float wgt[MAX_RUNS];
+    __shared__ float red[2][8];
+    __shared__ float4 acc[16][CMB_DIMS / 4];
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int nq = GRP * d.kvc, qh = blockIdx.x, b = blockIdx.y, d0 = blockIdx.z * CMB_DIMS, tid = threadIdx.x;
+    const int kvh = qh / GRP, h = qh - kvh * GRP, row = b * d.kvc + kvh;
+    const int warp = tid >> 5, lane = tid & 31;
+    const float gate = tid < CMB_DIMS ? q_gate[((size_t)b * nq + qh) * QG_ROW + HD + d0 + tid] : 0.0f;
+    const int64_t W = d.tiles(), start = d.row_start(row);
+    const int c0 = run_of(start, W, R), nc = run_of(start + d.row_tiles(b) - 1, W, R) - c0 + 1;
+    const size_t part0 = (size_t)c0 + row;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const float2* ml = reinterpret_cast<const float2*>(part_ml) + part0 * GRP + h;
+    float m = -INFINITY;
+    for (int i = tid; i < nc; i += 256) m = fmaxf(m, ml[(size_t)i * GRP].x);
+    m = warp_max(m);
+    if (lane == 0) red[0][warp] = m;
+    __syncthreads();
+    float M = red[0][0];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) M = fmaxf(M, red[0][w]);
+    float l = 0.0f;
+    for (int i = tid; i < nc; i += 256) {
+        const float2 v = ml[(size_t)i * GRP];
+        const float w = exp2f(v.x - M);
+        wgt[i] = w;
+        l += v.y * w;
+    }
+    l = warp_sum(l);
+    if (lane == 0) red[1][warp] = l;
+    __syncthreads();
+    const int g = tid >> 4, e = tid & 15;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = g; i < nc; i += 16) {
+        const float4 v = reinterpret_cast<const float4*>(part_o + ((part0 + i) * GRP + h) * HD + d0)[e];
+        const float w = wgt[i];
+        a.x = fmaf(v.x, w, a.x);
+        a.y = fmaf(v.y, w, a.y);
+        a.z = fmaf(v.z, w, a.z);
+        a.w = fmaf(v.w, w, a.w);
+    }
+    acc[g][e] = a;
+    __syncthreads();
+    if (tid < CMB_DIMS) {
+        float L = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) L += red[1][w];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o += reinterpret_cast<const float*>(acc[k])[tid];
+        out[((size_t)b * nq + qh) * HD + d0 + tid] = o * (1.0f / L) * sigmoidf_acc(gate);
     }
 }
 
 // ---------------------------------------------------------------------------
 // 4. tracked caches: weight of position j of a kv head += sum over its 6 q heads of
-//    exp2(score - M) / L, with M and L merged from the chunks' (m, l).  The new
+//    exp2(score - M) / L, with M and L merged from the partials' (m, l).  The new
 //    position's weight starts here.  Grid (ceil(longest / 1024), kvc, B).
 // ---------------------------------------------------------------------------
 constexpr int WT_SPAN = 1024;
 
-__global__ void __launch_bounds__(256) q4_weights_kernel(GqaDecodeDesc d, int kvc, const Q4Slot* __restrict__ slots,
+__global__ void __launch_bounds__(256) q4_weights_kernel(const __grid_constant__ Rows d, int R,
+                                                         const Q4Slot* __restrict__ slots,
                                                          const float* __restrict__ part_ml,
                                                          const float* __restrict__ scores) {
     __shared__ float M[GRP], L[GRP];
     const int b = blockIdx.z, kvh = blockIdx.y, n = d.len[b] + 1, j0 = blockIdx.x * WT_SPAN;
     if (j0 >= n) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = b * d.kvc + kvh;
+    const int64_t W = d.tiles(), start = d.row_start(row);
     if (warp < GRP) {
-        const int c0 = d.cum[b], nc = d.cum[b + 1] - c0;
-        const float2* ml = reinterpret_cast<const float2*>(part_ml) + ((size_t)c0 * kvc + kvh) * GRP + warp;
+        const int c0 = run_of(start, W, R), nc = run_of(start + d.row_tiles(b) - 1, W, R) - c0 + 1;
+        const float2* ml = reinterpret_cast<const float2*>(part_ml) + ((size_t)c0 + row) * GRP + warp;
         float m = -INFINITY;
-        for (int i = lane; i < nc; i += 32) m = fmaxf(m, ml[(size_t)i * kvc * GRP].x);
+        for (int i = lane; i < nc; i += 32) m = fmaxf(m, ml[(size_t)i * GRP].x);
         m = warp_max(m);
         float l = 0.0f;
         for (int i = lane; i < nc; i += 32) {
-            const float2 v = ml[(size_t)i * kvc * GRP];
+            const float2 v = ml[(size_t)i * GRP];
             l += v.y * exp2f(v.x - m);
         }
         l = warp_sum(l);
@@ -367,7 +481,7 @@ __global__ void __launch_bounds__(256) q4_weights_kernel(GqaDecodeDesc d, int kv
     const Q4Slot slot = slots[d.sid[b]];
     float* wts = slot.wts + (size_t)kvh * slot.cap;
     for (int j = j0 + threadIdx.x; j < min(n, j0 + WT_SPAN); j += 256) {
-        const float* sc = scores + (((size_t)d.pos[b] + (j >> 4)) * kvc + kvh) * (GRP * Q4_TILE) + (j & 15);
+        const float* sc = scores + (size_t)(start + (j >> 4)) * (GRP * Q4_TILE) + (j & 15);
         float w = 0.0f;
 #pragma unroll
         for (int h = 0; h < GRP; ++h) w += ex2f(sc[h * Q4_TILE] - M[h]) * L[h];
@@ -377,14 +491,17 @@ __global__ void __launch_bounds__(256) q4_weights_kernel(GqaDecodeDesc d, int kv
 
 }  // namespace q4
 
-cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, const GqaDecodeDesc& d, const Q4Pos& pos, const float* q_gate,
+int q4_decode_runs(int n_sm) { return std::min(q4::WARPS * n_sm, q4::MAX_RUNS); }
+
+cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, const Q4Rows& d, const Q4Pos& pos, const float* q_gate,
                              const float* k, const float* v, float* out, cudaStream_t st, int* n_launch) {
     using namespace q4;
     const LayerState& L = ctx->layers[layer];
-    const int kvc = ctx->cfg.kv_head_count;
-    const int items = d.cum[d.B] * kvc;
+    const int kvc = d.kvc;
+    const int R = (int)std::min<int64_t>(d.tiles(), q4_decode_runs(ctx->n_sm));
+    const int smem = WARPS * (int)sizeof(Ring);
     auto split = ctx->q4_track ? q4_split_kernel<true> : q4_split_kernel<false>;
-    cudaError_t e = cudaFuncSetAttribute(split, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Q4Smem));
+    cudaError_t e = cudaFuncSetAttribute(split, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -395,22 +512,27 @@ cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, const GqaDecodeDesc& d, con
     lc.stream = st;
     lc.attrs = at;
     lc.numAttrs = 1;
-    e = cudaLaunchKernelEx(&lc, q4_prep_kernel, d, pos, ctx->axes, kvc, (const Q4Slot*)L.d_q4, (const float*)L.q_norm,
-                           (const float*)L.k_norm, q_gate, k, v, ctx->q4_frag, ctx->q4_qs, ctx->cfg.rms_eps);
+    e = cudaLaunchKernelEx(&lc, q4_prep_kernel, d, pos, ctx->axes, (const Q4Slot*)L.d_q4, (const float*)L.q_norm,
+                           (const float*)L.k_norm, q_gate, k, v, ctx->q4_frag, ctx->cfg.rms_eps);
     if (e != cudaSuccess) return e;
-    lc.gridDim = dim3(std::min((items + Q4_WARPS - 1) / Q4_WARPS, ctx->n_sm));
-    lc.blockDim = dim3(32 * Q4_WARPS);
-    lc.dynamicSmemBytes = sizeof(Q4Smem);
-    e = cudaLaunchKernelEx(&lc, split, d, kvc, (const Q4Slot*)L.d_q4, (const uint32_t*)ctx->q4_frag,
-                           (const float*)ctx->q4_qs, ctx->part_o, ctx->part_ml, ctx->q4_sc, ctx->d_err, items);
+    lc.gridDim = dim3(std::min(R, ctx->n_sm));
+    lc.blockDim = dim3(32 * WARPS);
+    lc.dynamicSmemBytes = smem;
+    e = cudaLaunchKernelEx(&lc, split, d, R, (const Q4Slot*)L.d_q4, (const uint32_t*)ctx->q4_frag, ctx->part_o,
+                           ctx->part_ml, ctx->q4_sc, ctx->d_err);
     if (e != cudaSuccess) return e;
-    if ((e = launch_gqa_combine(ctx, d, q_gate, out, st, ctx->part_o, ctx->part_ml)) != cudaSuccess) return e;
+    lc.gridDim = dim3(GRP * kvc, d.B, HD / CMB_DIMS);
+    lc.blockDim = dim3(256);
+    lc.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&lc, q4_combine_kernel, d, R, (const float*)ctx->part_o, (const float*)ctx->part_ml, q_gate,
+                           out);
+    if (e != cudaSuccess) return e;
     *n_launch += 3;
     if (ctx->q4_track) {
         int longest = 0;
         for (int b = 0; b < d.B; ++b) longest = std::max(longest, d.len[b] + 1);
         q4_weights_kernel<<<dim3((longest + WT_SPAN - 1) / WT_SPAN, kvc, d.B), 256, 0, st>>>(
-            d, kvc, (const Q4Slot*)L.d_q4, ctx->part_ml, ctx->q4_sc);
+            d, R, (const Q4Slot*)L.d_q4, ctx->part_ml, ctx->q4_sc);
         *n_launch += 1;
     }
     return cudaGetLastError();
