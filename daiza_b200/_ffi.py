@@ -79,6 +79,8 @@ SIGNATURES = {
     "dz_qk_mrope": [_P, _I, _I64, _P, _P, _P, _P, _P, _P],
     "dz_qk_mrope_bf16": [_P, _I, _I64, _P, _P, _P, _P, _P, _P],
     "dz_gqa_decode_q4": [_P, _I, _I, _P, _P, _P, _P, _P, _P, _P],
+    "dz_gqa_prefill_q4": [_P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P],
+    "dz_gqa_prefill_q4_bf16": [_P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P],
     "dz_kv_rows_q4": [_P, _I, _I, _P, _P, _P, _P, _P, _P],
     "dz_kv_weights_q4": [_P, _I, _I, _P, _P, _P],
     "dz_kv_set_weights_q4": [_P, _I, _I, _P, _P, _P],

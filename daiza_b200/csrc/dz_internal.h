@@ -304,6 +304,13 @@ cudaError_t launch_swiglu(float* gate, const float* up, int64_t n, cudaStream_t 
 // 4-bit KV caches (q4_*.cu)
 cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, const Q4Rows& d, const Q4Pos& pos, const float* q_gate,
                              const float* k, const float* v, float* out, cudaStream_t st, int* n_launch);
+// prompts: lens[i] new tokens of each sequence, packed; f32 or bf16 (uint16_t) tensors
+cudaError_t launch_q4_prefill(dz_ctx* ctx, int layer, int n, const int32_t* seq_ids, const int64_t* lens,
+                              const int32_t* pos, const float* q_gate, const float* k, const float* v, float* out,
+                              cudaStream_t st, int* n_launch);
+cudaError_t launch_q4_prefill(dz_ctx* ctx, int layer, int n, const int32_t* seq_ids, const int64_t* lens,
+                              const int32_t* pos, const uint16_t* q_gate, const uint16_t* k, const uint16_t* v,
+                              uint16_t* out, cudaStream_t st, int* n_launch);
 int q4_decode_runs(int n_sm);   // most partials of a launch, beside one per row
 dz_status q4_import(dz_ctx* ctx, int layer, int seq, const float* k, const float* v, int64_t len);
 dz_status q4_export(dz_ctx* ctx, int layer, int seq, float* k, float* v);

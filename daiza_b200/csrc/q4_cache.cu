@@ -431,6 +431,53 @@ dz_status dz_gqa_decode_q4(dz_ctx* ctx, int layer, int B, const int32_t* seq_ids
     });
 }
 
+}  // extern "C"
+
+template <typename T>
+static dz_status gqa_prefill(dz_ctx* ctx, int layer, int n_seqs, const int32_t* seq_ids, const int64_t* T_new,
+                             const int32_t* pos, const T* q_gate, const T* k, const T* v, T* out, void* stream) {
+    return guarded(ctx, [&]() -> dz_status {
+        dz_status st = check_layer(ctx, layer, true);
+        if (st != DZ_OK || (st = check_seqs(ctx, n_seqs, seq_ids, "seq_ids")) != DZ_OK) return st;
+        if (!T_new) return fail(ctx, DZ_EINVAL, "null T");
+        const LayerState& L = ctx->layers[layer];
+        int64_t total = 0;
+        for (int i = 0; i < n_seqs; ++i) {
+            const int64_t len = L.len[seq_ids[i]], cap = L.h_q4[seq_ids[i]].cap;
+            if (T_new[i] < 0) return fail(ctx, DZ_EINVAL, "T[%d]=%lld is negative", i, (long long)T_new[i]);
+            if (T_new[i] > cap - len)
+                return fail(ctx, DZ_ESTATE, "prefill of %lld tokens overflows the KV cache of seq %d (len %lld, cap %lld)",
+                            (long long)T_new[i], seq_ids[i], (long long)len, (long long)cap);
+            total += T_new[i];
+        }
+        if (total < 1 || total > INT32_MAX) return fail(ctx, DZ_EINVAL, "%lld tokens outside 1..2^31-1", (long long)total);
+        if (!q_gate || !k || !v || !out) return fail(ctx, DZ_EINVAL, "null tensor");
+        if (!aligned16(q_gate) || !aligned16(k) || !aligned16(v) || !aligned16(out))
+            return fail(ctx, DZ_EINVAL, "q_gate, k, v and out must be 16-byte aligned");
+        DeviceGuard g(ctx->device);
+        if (!g.ok) return fail(ctx, DZ_ECUDA, "cudaSetDevice(%d) failed", ctx->device);
+        int launches = 0;
+        Q4_CUDA(launch_q4_prefill(ctx, layer, n_seqs, seq_ids, T_new, pos, q_gate, k, v, out,
+                                  static_cast<cudaStream_t>(stream), &launches));
+        ctx->last_launches = launches;
+        return DZ_OK;
+    });
+}
+
+extern "C" {
+
+dz_status dz_gqa_prefill_q4(dz_ctx* ctx, int layer, int n_seqs, const int32_t* seq_ids, const int64_t* T,
+                            const int32_t* pos, const float* q_gate, const float* k, const float* v, float* out,
+                            void* stream) {
+    return gqa_prefill(ctx, layer, n_seqs, seq_ids, T, pos, q_gate, k, v, out, stream);
+}
+
+dz_status dz_gqa_prefill_q4_bf16(dz_ctx* ctx, int layer, int n_seqs, const int32_t* seq_ids, const int64_t* T,
+                                 const int32_t* pos, const uint16_t* q_gate, const uint16_t* k, const uint16_t* v,
+                                 uint16_t* out, void* stream) {
+    return gqa_prefill(ctx, layer, n_seqs, seq_ids, T, pos, q_gate, k, v, out, stream);
+}
+
 dz_status dz_kv_rows_q4(dz_ctx* ctx, int layer, int B, const int32_t* seq_ids, const int64_t* first,
                         const int64_t* count, float* k, float* v, void* stream) {
     return guarded(ctx, [&]() -> dz_status {

@@ -318,6 +318,21 @@ class Context:
             _tensor("q_gate", q_gate, f, B * self.nq * QG_ROW), _tensor("k", k, f, B * self.kvc * HD),
             _tensor("v", v, f, B * self.kvc * HD), _tensor("out", out, f, B * self.nq * HD), _stream(stream)))
 
+    def gqa_prefill_q4(self, layer, seq_ids, lens, q_gate, k, v, out, stream=None, pos=None):
+        """lens[i] new tokens of each sequence, packed: q_gate [sum][6*kvc][512], k and v [sum][kvc][256], out
+        [sum][6*kvc*256], all f32 or all bf16; pos: int32 CUDA tensor [sum][3], default the cache slots."""
+        import torch
+        ids = _ids(seq_ids)
+        n = _per_seq("lens", lens, ids)
+        T = int(np.maximum(n, 0).sum())
+        dt = torch.bfloat16 if k.dtype == torch.bfloat16 else torch.float32
+        fn = self.lib.dz_gqa_prefill_q4_bf16 if dt == torch.bfloat16 else self.lib.dz_gqa_prefill_q4
+        self._chk(fn(self.h, layer, len(ids), _np_ptr(ids), _np_ptr(n),
+                     None if pos is None else _tensor("pos", pos, torch.int32, 3 * T),
+                     _tensor("q_gate", q_gate, dt, T * self.nq * QG_ROW), _tensor("k", k, dt, T * self.kvc * HD),
+                     _tensor("v", v, dt, T * self.kvc * HD), _tensor("out", out, dt, T * self.nq * HD),
+                     _stream(stream)))
+
     def kv_rows_q4(self, layer, seq_ids, first, count, k, v, stream=None):
         """Held rows [first, first + count) of each sequence as f32 [sum count][kvc][256]."""
         import torch

@@ -291,6 +291,23 @@ dz_status dz_qk_mrope_bf16(dz_ctx* ctx, int layer, int64_t T, const int32_t* pos
 dz_status dz_gqa_decode_q4(dz_ctx* ctx, int layer, int B, const int32_t* seq_ids, const int32_t* pos,
                            const float* q_gate, const float* k, const float* v, float* out, void* stream);
 
+/* Prompts of one or several sequences into 4-bit caches: T[i] new tokens (host [n_seqs],
+ * >= 0, at least one in all) of sequence seq_ids[i], packed one sequence behind the
+ * other, rows as in dz_gqa_prefill.  pos: device int32 [sum T][3], the tokens' rotary
+ * positions, or NULL for the cache slot on every axis.  Causal within each sequence,
+ * over its cached rows and the new ones as held: the result is that of one
+ * dz_gqa_decode_q4 per token, except that queries and probabilities are rounded to f16
+ * for the matrix products (K and V are exact there).  f32 in and out, or bf16 in and out.
+ * All tensors 16-byte aligned.  Tracked caches: new rows start with weight 0; prompts
+ * add no weights.  Scratch grows with the largest prompt (about 14 KB per new token and
+ * 4 KB per key, 2 GB at a time); make one such call before capturing a graph. */
+dz_status dz_gqa_prefill_q4(dz_ctx* ctx, int layer, int n_seqs, const int32_t* seq_ids, const int64_t* T,
+                            const int32_t* pos, const float* q_gate, const float* k, const float* v, float* out,
+                            void* stream);
+dz_status dz_gqa_prefill_q4_bf16(dz_ctx* ctx, int layer, int n_seqs, const int32_t* seq_ids, const int64_t* T,
+                                 const int32_t* pos, const uint16_t* q_gate, const uint16_t* k, const uint16_t* v,
+                                 uint16_t* out, void* stream);
+
 /* Held rows as f32: rows [first[b], first[b] + count[b]) of each sequence (host
  * arrays), one sequence behind the other: device k, v [sum count][kvc][256],
  * 16-byte aligned.  Stream-ordered. */
