@@ -82,6 +82,7 @@ SIGNATURES = {
     "dz_gqa_prefill_q4": [_P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P],
     "dz_gqa_prefill_q4_bf16": [_P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P],
     "dz_kv_rows_q4": [_P, _I, _I, _P, _P, _P, _P, _P, _P],
+    "dz_kv_evict_q4": [_P, _I, _I, _P, _P, _P, _P, _P, _P],
     "dz_kv_weights_q4": [_P, _I, _I, _P, _P, _P],
     "dz_kv_set_weights_q4": [_P, _I, _I, _P, _P, _P],
     "dz_last_launch_count": [_P],

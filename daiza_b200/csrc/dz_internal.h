@@ -311,6 +311,9 @@ cudaError_t launch_q4_prefill(dz_ctx* ctx, int layer, int n, const int32_t* seq_
 cudaError_t launch_q4_prefill(dz_ctx* ctx, int layer, int n, const int32_t* seq_ids, const int64_t* lens,
                               const int32_t* pos, const uint16_t* q_gate, const uint16_t* k, const uint16_t* v,
                               uint16_t* out, cudaStream_t st, int* n_launch);
+// eviction: src[b]'s heaviest and last entries into dst[b]; kept: device index list or null
+cudaError_t launch_q4_evict(dz_ctx* ctx, int layer, int B, const int32_t* src, const int32_t* dst, const int64_t* keep,
+                            const int64_t* recent, int32_t* kept, cudaStream_t st, int* n_launch);
 int q4_decode_runs(int n_sm);   // most partials of a launch, beside one per row
 dz_status q4_import(dz_ctx* ctx, int layer, int seq, const float* k, const float* v, int64_t len);
 dz_status q4_export(dz_ctx* ctx, int layer, int seq, float* k, float* v);

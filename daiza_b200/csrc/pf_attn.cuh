@@ -21,7 +21,7 @@ constexpr int BM = 128;        // query rows per CTA
 constexpr int BN = 128;        // keys per block (S = Q K^T runs as M128 x N128 products)
 constexpr int NK = 5;          // K ring: slots of one 64-dim box of a key block (128 x 64 bf16, 16 KB)
 constexpr int NV = 4;          // V ring: slots of 32 keys x 256 dims (4 boxes of 32 x 64 bf16, 16 KB)
-constexpr int NTHREADS = 320;  // warps 0-7 softmax, warp 8 TMA, warp 9 MMA
+constexpr int NTHREADS = 352;  // warps 0-7 softmax, warp 8 TMA of Q and K, warp 9 MMA, warp 10 TMA of V
 // TMEM columns: S buffers [0,128) and [128,256) (f32); P of a block (bf16 pairs)
 // overwrites the first 64 columns of its own S buffer; O accumulator [256,512)
 __host__ __device__ constexpr uint32_t S_COL(int st) { return 128u * (uint32_t)st; }
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(pf::NTHREADS, 1) pf_attn_kernel(const __grid_c
     bool ok = true;
 
     if (warp == 8) {
-        // ---------------- TMA producers: lane 0 = Q and K boxes, lane 1 = V slots ----------------
+        // ---------------- TMA producer of Q and K boxes ----------------
         if (lane == 0) {
             mbar_arrive_expect_tx(&sm.q_full, BM * HD * 2);
             for (int b = 0; b < 4; ++b) tma_load_3d(&sm.q[b][0][0], &tm_q, 64 * b, (int)tl.row, qh, &sm.q_full);
@@ -200,7 +200,11 @@ __global__ void __launch_bounds__(pf::NTHREADS, 1) pf_attn_kernel(const __grid_c
                 mbar_arrive_expect_tx(&sm.k_full[slot], BN * 64 * 2);
                 tma_load_3d(&sm.k[slot][0][0], &tm_k, 64 * b, (int)tl.key + j * BN, kvh, &sm.k_full[slot]);
             }
-        } else if (lane == 1) {
+        }
+    } else if (warp == 10) {
+        // ---------------- TMA producer of V slots: a warp of its own, since a lane that waits for
+        // K's slots would hold back the V loads of another lane of its warp ----------------
+        if (lane == 0) {
             for (int idx = 0; idx < 4 * nblk && ok; ++idx) {
                 const int slot = idx % NV, j = idx >> 2, kg = idx & 3;
                 if (idx >= NV && !wait_or_flag(&sm.v_empty[slot], ((idx / NV) - 1) & 1, err, ok)) break;

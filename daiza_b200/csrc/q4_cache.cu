@@ -570,4 +570,48 @@ dz_status dz_kv_set_weights_q4(dz_ctx* ctx, int layer, int B, const int32_t* seq
     return weights_copy(ctx, layer, B, seq_ids, nullptr, weights, stream);
 }
 
+dz_status dz_kv_evict_q4(dz_ctx* ctx, int layer, int B, const int32_t* seq_ids, const int32_t* into,
+                         const int64_t* keep, const int64_t* recent, int32_t* kept, void* stream) {
+    return guarded(ctx, [&]() -> dz_status {
+        dz_status st = check_layer(ctx, layer, false);
+        if (st != DZ_OK || (st = check_seqs(ctx, B, seq_ids, "seq_ids")) != DZ_OK ||
+            (into && (st = check_seqs(ctx, B, into, "into")) != DZ_OK) || (st = check_tracked(ctx)) != DZ_OK)
+            return st;
+        if (!keep || !recent) return fail(ctx, DZ_EINVAL, "null argument");
+        LayerState& L = ctx->layers[layer];
+        const int32_t* dst = into ? into : seq_ids;
+        std::vector<int> source_of(ctx->n_seqs, -1);
+        for (int b = 0; b < B; ++b) source_of[seq_ids[b]] = b;
+        int64_t total = 0;
+        for (int b = 0; b < B; ++b) {
+            const int64_t n = L.len[seq_ids[b]], k = std::min(keep[b], n);
+            if (keep[b] < 1 || recent[b] < 0 || recent[b] > keep[b])
+                return fail(ctx, DZ_EINVAL, "keep[%d]=%lld, recent[%d]=%lld: need keep >= 1 and 0 <= recent <= keep", b,
+                            (long long)keep[b], b, (long long)recent[b]);
+            if (source_of[dst[b]] >= 0 && source_of[dst[b]] != b)
+                return fail(ctx, DZ_EINVAL, "into[%d]=%d is a source of the same call", b, dst[b]);
+            if (k > L.h_q4[dst[b]].cap)
+                return fail(ctx, DZ_ESTATE, "%lld kept rows exceed the capacity %lld of seq %d", (long long)k,
+                            (long long)L.h_q4[dst[b]].cap, dst[b]);
+            total += k;
+        }
+        if (total * ctx->cfg.kv_head_count > INT32_MAX)
+            return fail(ctx, DZ_EINVAL, "%lld kept rows exceed 2^31-1 indices per call", (long long)total);
+        DeviceGuard g(ctx->device);
+        if (!g.ok) return fail(ctx, DZ_ECUDA, "cudaSetDevice(%d) failed", ctx->device);
+        int launches = 0;
+        Q4_CUDA(launch_q4_evict(ctx, layer, B, seq_ids, dst, keep, recent, kept, static_cast<cudaStream_t>(stream),
+                                &launches));
+        std::vector<int64_t> n(B);
+        for (int b = 0; b < B; ++b) n[b] = std::min(keep[b], L.len[seq_ids[b]]);
+        for (int b = 0; b < B; ++b) {
+            if (dst[b] == seq_ids[b] && n[b] == L.len[dst[b]]) continue;   // nothing moved
+            L.len[dst[b]] = n[b];
+            kv_lowered(ctx, layer, dst[b], 0);                             // rows rewritten from 0
+        }
+        ctx->last_launches = launches;
+        return DZ_OK;
+    });
+}
+
 }  // extern "C"

@@ -1,0 +1,325 @@
+// q4_evict.cu -- eviction from 4-bit KV caches by accumulated attention weight.
+//
+// Of each kv head of a sequence the last `recent` entries stay, and of the others the
+// heaviest, `keep` in all, in their order; equal weights: the earlier entry stays.
+//
+// One kernel, a cluster of CTAs per (sequence, kv head):
+//   1. the weight of the last entry that stays: radix selection over the weights as ordered
+//      32-bit keys, 11 + 11 + 10 bits, histograms per CTA, summed over the cluster through
+//      distributed shared memory;
+//   2. the indices that stay: each CTA counts its stretch of entries, prefix sums over the
+//      cluster, then writes its part of the list in order;
+//   3. the rows move, 16 positions a warp at a time: a round of destination tiles is built
+//      in shared memory from its sources, and written once every CTA of the cluster has
+//      read its own.  An entry only moves towards the front, so the sources of a later
+//      round lie behind everything that an earlier one writes: source and destination may
+//      be the same sequence.
+// Bound by latency (selection) for few sequences, by the rows' bytes for many.
+#include <algorithm>
+
+#include "q4.cuh"
+
+namespace dz {
+namespace q4 {
+
+constexpr int EV_CTAS = 8, EV_THREADS = 512, EV_WARPS = EV_THREADS / 32;
+constexpr int EV_TILES = 2;                      // tiles that a warp builds in a round
+constexpr int EV_PER = 4;                        // consecutive entries of a thread in step 2
+
+struct Evict {
+    int B, kvc;
+    int32_t src[MAXB], dst[MAXB], len[MAXB];
+    int32_t keep[MAXB], recent[MAXB];            // entries that stay (<= len), of which the last ones
+    int64_t out[MAXB];                           // first index of the sequence in the list
+};
+
+struct EvictSmem {
+    uint8_t tile[EV_WARPS * EV_TILES][Q4_TILE_BYTES];
+    float wts[EV_WARPS * EV_TILES][Q4_TILE];
+    uint32_t hist[3][2048];
+    uint32_t scan[EV_WARPS], scan2[EV_WARPS];
+    uint32_t found[2];                           // bin, entries above it
+    uint32_t count[2];                           // this CTA's entries above the threshold, and at it
+};
+
+// Weights in order as unsigned keys; NaN lowest, -0 as 0.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+    const uint32_t b = __float_as_uint(w + 0.0f);
+    if (w != w) return 0u;
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// a word of the same shared-memory place in CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t peer_word(const uint32_t* p, uint32_t rank) {
+    uint32_t a, v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+
+// Exclusive prefix sums of x over the block's threads, and their total.
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* warp_sums, uint32_t& total) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t v = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += y;
+    }
+    if (lane == 31) warp_sums[warp] = v;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < EV_WARPS; ++w) {
+        if (w < warp) before += warp_sums[w];
+        all += warp_sums[w];
+    }
+    __syncthreads();
+    total = all;
+    return before + v - x;
+}
+
+// A warp builds the tile of 16 entries whose sources are src[0 .. n) (n <= 16; the rest
+// becomes zeros) in shared memory, codes, scales and weights.
+__device__ __forceinline__ void build_tile(uint8_t* out, float* wts_out, const Q4Slot& slot, int kvh,
+                                           const int32_t* __restrict__ src, int n, int lane) {
+    const int32_t mine = lane < n ? src[lane] : -1;            // source of destination position `lane`
+    if (lane < Q4_TILE) wts_out[lane] = mine >= 0 ? slot.wts[(size_t)kvh * slot.cap + mine] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {                              // K codes: 8 pieces of 16 bytes a position
+        const int id = k * 32 + lane, p = id >> 3, i = (id >> 2) & 1, c = id & 3;
+        const int32_t s = __shfl_sync(0xffffffffu, mine, p);
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (s >= 0)
+            w = *reinterpret_cast<const uint4*>(slot.tile(kvh, s >> 4) + (((s >> 3) & 1) * 2 + i) * 512 +
+                                                ((s & 7) * 4 + c) * 16);
+        *reinterpret_cast<uint4*>(out + ((p >> 3) * 2 + i) * 512 + ((p & 7) * 4 + c) * 16) = w;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {                              // K scales: two groups at a time
+        const int id = k * 32 + lane, p = id >> 2, c = id & 3;
+        const int32_t s = __shfl_sync(0xffffffffu, mine, p);
+        uint16_t v = 0;
+        if (s >= 0)
+            v = *reinterpret_cast<const uint16_t*>(slot.tile(kvh, s >> 4) + OFF_KS + ((s & 7) * 4 + c) * 4 +
+                                                   ((s >> 3) & 1) * 2);
+        *reinterpret_cast<uint16_t*>(out + OFF_KS + ((p & 7) * 4 + c) * 4 + (p >> 3) * 2) = v;
+    }
+    // V: lane (r, c) has the words of positions 2c, 2c + 1, 2c + 8, 2c + 9
+    const int r = lane >> 2, c = lane & 3;
+    uint4 w[4] = {};
+    uint32_t scales = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int u = q & 1, hi = q >> 1;
+        const int32_t s = __shfl_sync(0xffffffffu, mine, 2 * c + u + 8 * hi);
+        if (s < 0) continue;
+        const uint8_t* tile = slot.tile(kvh, s >> 4);
+        const int from = r * 4 + ((s & 7) >> 1), sh = (s & 1) * 16 + ((s >> 3) & 1) * 4, to = u * 16 + hi * 4;
+        scales |= (uint32_t)tile[OFF_VS + from * 4 + (s & 1) + ((s >> 3) & 1) * 2] << (8 * q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4 x = *reinterpret_cast<const uint4*>(tile + OFF_V + i * 512 + from * 16);
+            w[i].x |= ((x.x >> sh) & 0x0F0Fu) << to;
+            w[i].y |= ((x.y >> sh) & 0x0F0Fu) << to;
+            w[i].z |= ((x.z >> sh) & 0x0F0Fu) << to;
+            w[i].w |= ((x.w >> sh) & 0x0F0Fu) << to;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(out + OFF_V + i * 512 + lane * 16) = w[i];
+    *reinterpret_cast<uint32_t*>(out + OFF_VS + lane * 4) = scales;
+}
+
+__global__ void __cluster_dims__(EV_CTAS, 1, 1) __launch_bounds__(EV_THREADS, 1)
+    q4_evict_kernel(const __grid_constant__ Evict d, const Q4Slot* __restrict__ slots, int32_t* list,
+                    int32_t* __restrict__ kept) {
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    EvictSmem& sm = *reinterpret_cast<EvictSmem*>(smem_raw);
+    const int rank = blockIdx.x % EV_CTAS, pair = blockIdx.x / EV_CTAS, b = pair / d.kvc, kvh = pair - b * d.kvc;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const Q4Slot src = slots[d.src[b]], dst = slots[d.dst[b]];
+    const int n = d.len[b], keep = d.keep[b], recent = d.recent[b];
+    const int old = n - recent, need = keep - recent;          // `need` of the first `old` entries stay
+    const float* wts = src.wts + (size_t)kvh * src.cap;
+    list += d.out[b] * d.kvc + (int64_t)kvh * keep;
+    if (kept) kept += d.out[b] * d.kvc + (int64_t)kvh * keep;
+    const int per = ((old + EV_CTAS - 1) / EV_CTAS + EV_PER - 1) / EV_PER * EV_PER;
+    const int lo = min(old, rank * per), hi = min(old, lo + per);
+
+    // ---- 1. threshold: entries with a larger key stay, and the first `ties` with this key
+    uint32_t threshold = 0, ties = 0;
+    const bool select = need > 0 && need < old;                // the same for the whole cluster
+    if (select) {
+        for (int i = tid; i < 3 * 2048; i += EV_THREADS) (&sm.hist[0][0])[i] = 0;
+        __syncthreads();
+        uint32_t prefix = 0, left = (uint32_t)need;            // key bits found so far; entries still to find below them
+#pragma unroll
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048;
+            for (int j = lo + tid; j < hi; j += EV_THREADS) {
+                const uint32_t k = weight_key(wts[j]);
+                const bool in = pass == 0 || (k >> (pass == 1 ? 21 : 10)) == prefix;
+                if (in) atomicAdd(&sm.hist[pass][(k >> shift) & (bins - 1)], 1u);
+            }
+            cluster_sync();
+            // this thread's 4 bins, from the highest bin down, over the cluster
+            uint32_t c[4] = {}, sum = 0;
+            const int top = bins - 1 - 4 * tid;
+            if (top >= 0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    for (int q = 0; q < EV_CTAS; ++q) c[i] += peer_word(&sm.hist[pass][top - i], q);
+                    sum += c[i];
+                }
+            }
+            uint32_t total, above = block_scan(sum, sm.scan, total);
+            if (top >= 0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (above < left && left <= above + c[i]) {
+                        sm.found[0] = (uint32_t)(top - i);
+                        sm.found[1] = above;
+                    }
+                    above += c[i];
+                }
+            }
+            __syncthreads();
+            prefix = prefix << (pass == 2 ? 10 : 11) | sm.found[0];
+            left -= sm.found[1];
+            __syncthreads();
+        }
+        threshold = prefix;
+        ties = left;
+    }
+
+    // ---- 2. the list of entries that stay
+    if (select) {
+        uint32_t gt = 0, eq = 0;
+        for (int j = lo + tid; j < hi; j += EV_THREADS) {
+            const uint32_t k = weight_key(wts[j]);
+            gt += k > threshold;
+            eq += k == threshold;
+        }
+        uint32_t all_gt, all_eq;
+        block_scan(gt, sm.scan, all_gt);
+        block_scan(eq, sm.scan2, all_eq);
+        if (tid == 0) {
+            sm.count[0] = all_gt;
+            sm.count[1] = all_eq;
+        }
+        cluster_sync();
+        uint32_t gt_before = 0, eq_before = 0;
+        for (int q = 0; q < rank; ++q) {
+            gt_before += peer_word(&sm.count[0], q);
+            eq_before += peer_word(&sm.count[1], q);
+        }
+        uint32_t at = gt_before + min(eq_before, ties);
+        for (int j0 = lo; j0 < hi; j0 += EV_PER * EV_THREADS) {
+            uint32_t g = 0, e = 0;
+            uint32_t is[EV_PER];
+            const int first = j0 + EV_PER * tid;
+#pragma unroll
+            for (int i = 0; i < EV_PER; ++i) {
+                const int j = first + i;
+                const uint32_t k = j < hi ? weight_key(wts[j]) : 0u;
+                is[i] = j >= hi ? 0u : (k > threshold ? 1u : (k == threshold ? 2u : 0u));
+                e += is[i] == 2u;
+            }
+            uint32_t chunk_eq, eq_at = block_scan(e, sm.scan, chunk_eq) + eq_before;
+#pragma unroll
+            for (int i = 0; i < EV_PER; ++i) {
+                if (is[i] == 2u && eq_at++ >= ties) is[i] = 0u;
+                g += is[i] != 0u;
+            }
+            uint32_t chunk, to = block_scan(g, sm.scan2, chunk) + at;
+#pragma unroll
+            for (int i = 0; i < EV_PER; ++i)
+                if (is[i]) {
+                    list[to] = first + i;
+                    if (kept) kept[to] = first + i;
+                    ++to;
+                }
+            eq_before += chunk_eq;
+            at += chunk;
+        }
+    } else if (need > 0) {                                     // nothing leaves
+        for (int j = lo + tid; j < hi; j += EV_THREADS) {
+            list[j] = j;
+            if (kept) kept[j] = j;
+        }
+    }
+    for (int j = rank * EV_THREADS + tid; j < recent; j += EV_CTAS * EV_THREADS) {
+        list[need + j] = old + j;
+        if (kept) kept[need + j] = old + j;
+    }
+    cluster_sync();                                            // the list; and no CTA leaves while another reads its words
+
+    // ---- 3. the rows move
+    if (d.src[b] == d.dst[b] && keep == n) return;             // nothing leaves: already in place (the whole cluster)
+    const int tiles = (keep + Q4_TILE - 1) / Q4_TILE;
+    constexpr int ROUND = EV_CTAS * EV_WARPS * EV_TILES;
+    for (int t0 = 0; t0 < tiles; t0 += ROUND) {
+        const int w0 = (warp * EV_CTAS + rank) * EV_TILES;     // few tiles: spread over the CTAs first
+#pragma unroll 1
+        for (int k = 0; k < EV_TILES; ++k) {
+            const int t = t0 + w0 + k;
+            if (t < tiles)
+                build_tile(sm.tile[warp * EV_TILES + k], sm.wts[warp * EV_TILES + k], src, kvh, list + (int64_t)t * Q4_TILE,
+                           min(Q4_TILE, keep - t * Q4_TILE), lane);
+        }
+        cluster_sync();                                        // every source of this round has been read
+#pragma unroll 1
+        for (int k = 0; k < EV_TILES; ++k) {
+            const int t = t0 + w0 + k;
+            if (t < tiles) {
+                const uint4* from = reinterpret_cast<const uint4*>(sm.tile[warp * EV_TILES + k]);
+                uint4* to = reinterpret_cast<uint4*>(dst.tile(kvh, t));
+                for (int i = lane; i < Q4_TILE_BYTES / 16; i += 32) to[i] = from[i];
+                const int j = t * Q4_TILE + lane;
+                if (lane < Q4_TILE && j < keep) dst.wts[(size_t)kvh * dst.cap + j] = sm.wts[warp * EV_TILES + k][lane];
+            }
+        }
+        __syncwarp();                                          // the warp's staging tiles are free again
+    }
+}
+
+}  // namespace q4
+
+cudaError_t launch_q4_evict(dz_ctx* ctx, int layer, int B, const int32_t* src, const int32_t* dst, const int64_t* keep,
+                            const int64_t* recent, int32_t* kept, cudaStream_t st, int* n_launch) {
+    const LayerState& L = ctx->layers[layer];
+    const int kvc = ctx->cfg.kv_head_count;
+    cudaError_t e = cudaFuncSetAttribute(q4::q4_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)sizeof(q4::EvictSmem));
+    if (e != cudaSuccess) return e;
+    int64_t rows = 0;
+    for (int b = 0; b < B; ++b) rows += std::min<int64_t>(keep[b], L.len[src[b]]);
+    if ((e = ensure_q4_scratch(ctx, std::max<int64_t>(rows, 1) * kvc * sizeof(int32_t))) != cudaSuccess) return e;
+    int64_t at = 0;
+    for (int b0 = 0; b0 < B; b0 += MAXB) {
+        q4::Evict d;
+        d.B = std::min(MAXB, B - b0);
+        d.kvc = kvc;
+        for (int b = 0; b < d.B; ++b) {
+            const int64_t n = L.len[src[b0 + b]], k = std::min(keep[b0 + b], n);
+            d.src[b] = src[b0 + b];
+            d.dst[b] = dst[b0 + b];
+            d.len[b] = (int32_t)n;
+            d.keep[b] = (int32_t)k;
+            d.recent[b] = (int32_t)std::min(recent[b0 + b], k);
+            d.out[b] = at;
+            at += k;
+        }
+        q4::q4_evict_kernel<<<d.B * kvc * q4::EV_CTAS, q4::EV_THREADS, sizeof(q4::EvictSmem), st>>>(
+            d, L.d_q4, static_cast<int32_t*>(ctx->q4_scratch), kept);
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        *n_launch += 1;
+    }
+    return cudaSuccess;
+}
+
+}  // namespace dz

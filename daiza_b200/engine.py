@@ -361,6 +361,22 @@ class Context:
             self.h, layer, len(ids), _np_ptr(ids),
             _tensor("weights", weights, torch.float32, self._weights_numel(layer, ids)), _stream(stream)))
 
+    def kv_evict_q4(self, layer, seq_ids, keep, recent, kept=None, into=None, stream=None):
+        """Keeps the last recent[b] and the heaviest other entries, keep[b] in all, per kv head; in place, or into the
+        sequences `into`.  kept: int32 CUDA tensor, per sequence [kvc][min(keep, length)], their former rows."""
+        import torch
+        ids = _ids(seq_ids)
+        k, r = _per_seq("keep", keep, ids), _per_seq("recent", recent, ids)
+        to = None if into is None else _ids(into)
+        if to is not None and to.shape != ids.shape:
+            raise _ffi.DzError(_ffi.DZ_EINVAL, f"into needs one sequence per source ({len(ids)}), got {to.shape}")
+        out = None
+        if kept is not None:
+            n = sum(max(0, min(int(a), self.kv_len(layer, int(s)))) for a, s in zip(k, ids))
+            out = _tensor("kept", kept, torch.int32, n * self.kvc)
+        self._chk(self.lib.dz_kv_evict_q4(self.h, layer, len(ids), _np_ptr(ids), None if to is None else _np_ptr(to),
+                                          _np_ptr(k), _np_ptr(r), out, _stream(stream)))
+
     def gdn_decode(self, layer, seq_ids, qkv, alpha, beta, z, y, stream=None):
         ids = np.ascontiguousarray(np.atleast_1d(seq_ids), np.int32)
         self._chk(self.lib.dz_gdn_decode(self.h, layer, len(ids), _np_ptr(ids), _ptr(qkv), _ptr(alpha), _ptr(beta),

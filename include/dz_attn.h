@@ -323,6 +323,20 @@ dz_status dz_kv_weights_q4(dz_ctx* ctx, int layer, int B, const int32_t* seq_ids
 dz_status dz_kv_set_weights_q4(dz_ctx* ctx, int layer, int B, const int32_t* seq_ids, const float* weights,
                                void* stream);
 
+/* Eviction by accumulated weight (tracked caches): of each kv head of sequence
+ * seq_ids[b] the last recent[b] entries stay and the heaviest of the others, keep[b]
+ * in all (host arrays, keep >= 1, 0 <= recent <= keep), in their order; of equal
+ * weights the earlier entry stays, a NaN counts as the lightest.  Every kv head keeps
+ * its own entries; a sequence of at most keep[b] stays as it is.  The kept rows, with
+ * their weights, become rows 0.. of the same sequence, or of sequence into[b] (host
+ * [B], distinct, or NULL), whose content they replace; the source then stays as it
+ * was.  kept: device int32, per sequence [kvc][min(keep, length)] one behind the other,
+ * the kept entries' former rows, or NULL.  Lengths are per layer: the calls after it
+ * give the rotary positions (pos), since slots are no longer positions.
+ * Stream-ordered; snapshots of a rewritten sequence are no longer restored. */
+dz_status dz_kv_evict_q4(dz_ctx* ctx, int layer, int B, const int32_t* seq_ids, const int32_t* into,
+                         const int64_t* keep, const int64_t* recent, int32_t* kept, void* stream);
+
 /* ---- DZSS session files -------------------------------------------------- */
 /* Save / restore one sequence's caches in the reference's session format v1
  * (Daiza-runtime/src/session_persist.rs:1-36, save_to_disk :76-140,
