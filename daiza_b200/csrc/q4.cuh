@@ -31,6 +31,7 @@
 // Codes are stored as code + 8.  Unwritten positions hold finite scales always
 // (the cache starts zeroed), since a masked probability of 0 still multiplies V.
 #pragma once
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "dz_internal.h"
@@ -160,6 +161,74 @@ __device__ __forceinline__ void norm_rotate(F (&x)[8], const float* __restrict__
     }
 }
 
+// Rows that are not quantised: lane l holds two runs of 4 dims, at split_dim(l, 0) and
+// split_dim(l, 1), such that a rotary pair (i, i + 32) lies in one lane (lanes 0..7).
+__device__ __forceinline__ int split_dim(int lane, int run) {
+    return lane < 8 ? 4 * lane + 32 * run : 8 * lane + 4 * run;
+}
+// RMS norm, weight (w: this lane's 8) and rotation in f32; cs: (cos, sin) of pairs
+// 4 l .. 4 l + 3 in lanes 0..7.
+__device__ __forceinline__ void norm_rotate_split(float (&x)[8], const float (&w)[8], const float2 (&cs)[4], float eps,
+                                                  int lane) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+    const float v = fmaf(warp_sum(ss), 1.0f / (float)HD, eps), g = rsqrtf(v);
+    const float inv = fmaf(fmaf(-v * g, g, 1.0f), 0.5f * g, g);   // one Newton step: to the last bit or so
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = (x[e] * inv) * w[e];
+    if (lane < 8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float a = x[e], b = x[e + 4];
+            x[e] = fmaf(a, cs[e].x, b * cs[e].y);
+            x[e + 4] = fmaf(b, cs[e].x, a * cs[e].y);
+        }
+    }
+}
+// The (cos, sin) that norm_rotate_split wants, from a lane's own pair (lane = pair).
+__device__ __forceinline__ void spread_pairs(float2 own, float2 (&cs)[4], int lane) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        cs[e].x = __shfl_sync(0xffffffffu, own.x, (4 * lane + e) & 31);
+        cs[e].y = __shfl_sync(0xffffffffu, own.y, (4 * lane + e) & 31);
+    }
+}
+// (cos, sin) of pair i at a token's three positions in f32, the angle reduced in f64
+__device__ __forceinline__ float2 rope_cs_f32(const RopeAxes& a, int i, int t, int h, int w) {
+    const int ax = a.axis[i];
+    float s, c;
+    sincospif((float)rope_half_turns(ax == 0 ? t : (ax == 1 ? h : w), a.turn[i]), &s, &c);
+    return make_float2(c, s);
+}
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ uint2 load4(const __nv_bfloat16* p) { return *reinterpret_cast<const uint2*>(p); }
+__device__ __forceinline__ float4 as_f32(float4 x) { return x; }
+__device__ __forceinline__ float4 as_f32(uint2 u) {
+    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
+                       __uint_as_float(u.y & 0xFFFF0000u));
+}
+// A lane's 8 dims of a row as they lie in memory: several rows can be in flight.
+template <typename T>
+struct SplitRow {
+    decltype(load4((const T*)nullptr)) a, b;
+    __device__ __forceinline__ void load(const T* row, int lane) {
+        a = load4(row + split_dim(lane, 0));
+        b = load4(row + split_dim(lane, 1));
+    }
+    __device__ __forceinline__ void values(float (&x)[8]) const {
+        const float4 u = as_f32(a), v = as_f32(b);
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+        x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+    }
+};
+template <typename T>
+__device__ __forceinline__ void load_split(const T* row, int lane, float (&x)[8]) {
+    SplitRow<T> r;
+    r.load(row, lane);
+    r.values(x);
+}
+
 // Quantise the row: the stored scale byte of this lane's group and the 8 codes + 8.
 __device__ __forceinline__ uint32_t quantise(double (&x)[8], uint32_t (&code)[8]) {
     double a = 0.0;
@@ -205,6 +274,32 @@ __device__ __forceinline__ void put_v_scale(uint8_t* tile, int p, int lane, uint
     if ((lane & 3) == 0)
         tile[OFF_VS + ((lane >> 2) * 4 + ((p & 7) >> 1)) * 4 + (p & 1) + (p >> 3) * 2] = (uint8_t)sb;
 }
+
+// V codes of several positions of one tile, from the warps of a block of 512 threads (a
+// word holds four positions): gathered in shared memory, then merged into the tile.
+struct TileMerge {
+    uint32_t code[512], mask[512];
+    __device__ __forceinline__ void begin() {
+        code[threadIdx.x] = mask[threadIdx.x] = 0u;
+        __syncthreads();
+    }
+    // position p's codes, by one warp
+    __device__ __forceinline__ void add(int p, int lane, const uint32_t (&c)[8]) {
+        const int at = (lane & 3) * 128 + ((lane >> 2) * 4 + ((p & 7) >> 1)) * 4, sh = (p & 1) * 16 + (p >> 3) * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            atomicOr(&code[at + i], (c[2 * i] | c[2 * i + 1] << 8) << sh);
+            atomicOr(&mask[at + i], 0x0F0Fu << sh);
+        }
+    }
+    __device__ __forceinline__ void end(uint8_t* tile) {
+        __syncthreads();
+        uint32_t* w = reinterpret_cast<uint32_t*>(tile + OFF_V) + threadIdx.x;
+        const uint32_t m = mask[threadIdx.x];
+        if (m == 0xFFFFFFFFu) *w = code[threadIdx.x];
+        else if (m) *w = (*w & ~m) | code[threadIdx.x];
+    }
+};
 
 // Reads lane l's 8 dims of K or V at position p of a tile as f16 pairs.
 __device__ __forceinline__ void get_k(const uint8_t* tile, int p, int lane, uint32_t (&h)[4]) {

@@ -4,7 +4,6 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
-#include <cuda_bf16.h>
 #include <new>
 
 #include "q4.cuh"
@@ -83,24 +82,18 @@ __global__ void __launch_bounds__(256) q4_rows_kernel(Ranges d, int kvc, const Q
     put(v + at);
 }
 
-// one warp per (tile, kv head): rows [16 t, min(16 t + 16, len)) from f32 [row][kvc][256],
-// the tile's other positions as they are.  k and v start at row `row0` (a multiple of 16).
-__global__ void __launch_bounds__(256) q4_import_kernel(Q4Slot slot, int kvc, int64_t row0, int64_t len,
+// One block per (tile, kv head), a warp per position: rows [row0, len) from f32
+// [row][kvc][256], the tile's other positions as they are.  k and v start at row `row0`
+// (a multiple of 16).
+__global__ void __launch_bounds__(512) q4_import_kernel(Q4Slot slot, int kvc, int64_t row0, int64_t len,
                                                         const float* __restrict__ k, const float* __restrict__ v) {
-    const int64_t n_tiles = (len - row0 + Q4_TILE - 1) / Q4_TILE;
-    const int64_t task = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (task >= n_tiles * kvc) return;
-    const int64_t t = task / kvc;
-    const int kvh = (int)(task - t * kvc);
+    __shared__ TileMerge merge;
+    const int64_t t = blockIdx.x / kvc;
+    const int kvh = (int)(blockIdx.x - t * kvc), p = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint8_t* tile = slot.tile(kvh, (row0 >> 4) + t);
-    uint4 w[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) w[c] = *v_words(tile, lane, c);
-#pragma unroll
-    for (int p = 0; p < Q4_TILE; ++p) {
-        const int64_t row = t * Q4_TILE + p;
-        if (row0 + row >= len) break;
+    merge.begin();
+    const int64_t row = t * Q4_TILE + p;
+    if (row0 + row < len) {
         const size_t at = ((size_t)row * kvc + kvh) * HD + 8 * lane;
         double x[8], y[8];
 #pragma unroll
@@ -112,11 +105,10 @@ __global__ void __launch_bounds__(256) q4_import_kernel(Q4Slot slot, int kvc, in
         uint32_t sb = quantise(x, code);
         put_k(tile, p, lane, code, sb);
         sb = quantise(y, code);
-        merge_v(w[(p & 7) >> 1], p, code);
+        merge.add(p, lane, code);
         put_v_scale(tile, p, lane, sb);
     }
-#pragma unroll
-    for (int c = 0; c < 4; ++c) *v_words(tile, lane, c) = w[c];
+    merge.end(tile);
 }
 
 // ---- accumulated weights ---------------------------------------------------------------
@@ -145,63 +137,59 @@ __global__ void __launch_bounds__(256) q4_weights_clear_kernel(Q4Slot slot, int 
 // QK-RMSNorm, rotation and q's 1/16 for T tokens.  HBM bound: q's halves of q_gate and k
 // read once, q and k written once.  The angle is reduced in f64, sine and cosine taken
 // in f32.
-__device__ __forceinline__ float2 rope_cs_f32(const RopeAxes& a, int i, const int32_t* __restrict__ pos) {
-    float s, c;
-    sincospif((float)rope_half_turns(pos[a.axis[i]], a.turn[i]), &s, &c);
-    return make_float2(c, s);
+__device__ __forceinline__ void store_split(float* row, int lane, const float (&x)[8]) {
+    *reinterpret_cast<float4*>(row + split_dim(lane, 0)) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(row + split_dim(lane, 1)) = make_float4(x[4], x[5], x[6], x[7]);
 }
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-    }
-}
-__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-}
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
+__device__ __forceinline__ void store_split(__nv_bfloat16* row, int lane, const float (&x)[8]) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const __nv_bfloat162 t = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
         w[i] = *reinterpret_cast<const uint32_t*>(&t);
     }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint2*>(row + split_dim(lane, 0)) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(row + split_dim(lane, 1)) = make_uint2(w[2], w[3]);
 }
 
-// one warp per (token, head)
+// A warp per token and share of its heads: grid (ceil(T / 8), shares).  Several rows are
+// in flight per warp: reading one at a time held the pass at 4.3 TB/s.
+constexpr int MROPE_ROWS = 7;
 template <typename T>
-__global__ void __launch_bounds__(256) qk_mrope_kernel(RopeAxes axes, int kvc, int64_t n_tokens,
+__global__ void __launch_bounds__(256) qk_mrope_kernel(const __grid_constant__ RopeAxes axes, int kvc, int64_t n_tokens,
                                                        const int32_t* __restrict__ pos, const T* __restrict__ q_gate,
                                                        const T* __restrict__ k, const float* __restrict__ q_norm,
                                                        const float* __restrict__ k_norm, T* __restrict__ q_out,
                                                        T* __restrict__ k_out, float eps) {
-    __shared__ float2 cs[ROPE / 2];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nq = GRP * kvc;
-    const int64_t t = blockIdx.x;
-    if (warp == 0) cs[lane] = rope_cs_f32(axes, lane, pos + 3 * t);
-    __syncthreads();
-    for (int task = blockIdx.y * 8 + warp; task < nq + kvc; task += gridDim.y * 8) {
-        const bool is_q = task < nq;
-        const T* src = is_q ? q_gate + (t * nq + task) * QG_ROW : k + (t * kvc + (task - nq)) * HD;
-        T* dst = is_q ? q_out + (t * nq + task) * HD : k_out + (t * kvc + (task - nq)) * HD;
-        float x[8];
-        load8(src + 8 * lane, x);
-        norm_rotate(x, is_q ? q_norm : k_norm, cs, eps, lane);
-        if (is_q) {
+    const int lane = threadIdx.x & 31, nq = GRP * kvc;
+    const int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (t >= n_tokens) return;
+    float2 cs[4];
+    spread_pairs(rope_cs_f32(axes, lane, pos[3 * t], pos[3 * t + 1], pos[3 * t + 2]), cs, lane);
+    float wq[8], wk[8];
+    load_split(q_norm, lane, wq);
+    load_split(k_norm, lane, wk);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] *= 0.0625f;
+    for (int e = 0; e < 8; ++e) wq[e] *= 0.0625f;
+    const int heads = nq + kvc, share = (heads + gridDim.y - 1) / gridDim.y;
+    const int h1 = min(heads, ((int)blockIdx.y + 1) * share);
+    for (int h0 = blockIdx.y * share; h0 < h1; h0 += MROPE_ROWS) {
+        SplitRow<T> in[MROPE_ROWS];
+#pragma unroll
+        for (int i = 0; i < MROPE_ROWS; ++i) {
+            const int h = h0 + i;
+            if (h < h1) in[i].load(h < nq ? q_gate + (t * nq + h) * QG_ROW : k + (t * kvc + (h - nq)) * HD, lane);
         }
-        store8(dst + 8 * lane, x);
+#pragma unroll
+        for (int i = 0; i < MROPE_ROWS; ++i) {
+            const int h = h0 + i;
+            if (h >= h1) break;
+            float x[8];
+            in[i].values(x);
+            if (h < nq) norm_rotate_split(x, wq, cs, eps, lane);
+            else norm_rotate_split(x, wk, cs, eps, lane);
+            store_split(h < nq ? q_out + (t * nq + h) * HD : k_out + (t * kvc + (h - nq)) * HD, lane, x);
+        }
     }
 }
 
@@ -288,8 +276,8 @@ dz_status q4_import(dz_ctx* ctx, int layer, int seq, const float* k, const float
         float* dv = dk + n * row;
         Q4_CUDA(cudaMemcpy(dk, k + r0 * row, n * row * sizeof(float), cudaMemcpyDefault));
         Q4_CUDA(cudaMemcpy(dv, v + r0 * row, n * row * sizeof(float), cudaMemcpyDefault));
-        const int64_t tasks = (n + Q4_TILE - 1) / Q4_TILE * kvc;
-        q4::q4_import_kernel<<<(unsigned)((tasks + 7) / 8), 256>>>(L.h_q4[seq], kvc, r0, r0 + n, dk, dv);
+        const int64_t blocks = (n + Q4_TILE - 1) / Q4_TILE * kvc;
+        q4::q4_import_kernel<<<(unsigned)blocks, 512>>>(L.h_q4[seq], kvc, r0, r0 + n, dk, dv);
         Q4_CUDA(cudaGetLastError());
     }
     if (ctx->q4_track && len > 0) {
@@ -365,7 +353,10 @@ static dz_status qk_mrope(dz_ctx* ctx, int layer, int64_t n, const int32_t* pos,
         if (!g.ok) return fail(ctx, DZ_ECUDA, "cudaSetDevice(%d) failed", ctx->device);
         const LayerState& L = ctx->layers[layer];
         const int kvc = ctx->cfg.kv_head_count;
-        q4::qk_mrope_kernel<T><<<dim3((unsigned)n, (GRP * kvc + kvc + 7) / 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        // few tokens: a warp per head, so that their latencies overlap
+        const int heads = GRP * kvc + kvc;
+        const int shares = n * 4 <= 64 * ctx->n_sm ? (n * heads <= 64 * ctx->n_sm ? heads : 4) : 1;
+        q4::qk_mrope_kernel<T><<<dim3((unsigned)((n + 7) / 8), shares), 256, 0, static_cast<cudaStream_t>(stream)>>>(
             ctx->axes, kvc, n, pos, q_gate, k, L.q_norm, L.k_norm, q_out, k_out, ctx->cfg.rms_eps);
         Q4_CUDA(cudaGetLastError());
         ctx->last_launches = 1;

@@ -112,26 +112,24 @@ __global__ void __launch_bounds__(256) q4_prep_kernel(const __grid_constant__ Ro
 //    however ragged the batch is, and no warp waits for another.  A run covers parts of
 //    one or more rows; each part (segment) gives one unnormalised partial, at index
 //    c + row (unique: both only grow along the runs).
-//    A tile (16 positions, 4352 bytes) is one bulk copy into the warp's own ring,
-//    requested across segment ends; q of the segment is another.
-//    Scores: S = Q K^T, A = q (hi rows, lo rows), B = the 8 positions of a K word row, 16
+//    Tiles come in pairs (32 positions, 8704 bytes): one bulk copy into the warp's own
+//    ring, requested across segment ends.
+//    Scores: S = Q K^T, A = q (hi rows, lo rows; in registers), B = the 8 positions of a K word row, 16
 //    steps of 16 dims; thread (r, c) gets head r at positions 2c, 2c+1 (hi sum and lo sum,
 //    added).  That is the B operand's own layout, so P needs no shuffle: O^T += V^T P^T,
 //    A = V's dims x 16 positions, B = P (hi, then lo), 16 tiles of 16 dims accumulated in
 //    64 registers.
 // ---------------------------------------------------------------------------
-constexpr int STAGES = 2, WARPS = 12;
+constexpr int STAGES = 3, WARPS = 8;
 // p is taken against a maximum that may be stale by P_SLACK and is scaled by 2^P_LOG2: at
 // most 2^15, and its f16 lo part keeps its bits down to 2^-21 of the maximum.
 constexpr float P_LOG2 = 8.0f, P_SLACK = 7.0f;
 
 struct alignas(128) Ring {
-    uint8_t tile[STAGES][Q4_TILE_BYTES];
-    uint32_t q[FRAG_WORDS];
-    uint64_t full[STAGES], q_full;
+    uint8_t pair[STAGES][2 * Q4_TILE_BYTES];
+    uint64_t full[STAGES];
 };
-static_assert(Q4_TILE_BYTES % 128 == 0 && sizeof(Ring) % 128 == 0 && FRAG_WORDS % 4 == 0,
-              "bulk copies need 16-byte alignment");
+static_assert(Q4_TILE_BYTES % 128 == 0 && sizeof(Ring) % 128 == 0, "bulk copies need 16-byte alignment");
 
 // W c overflows nothing: W is below 2^36 tiles, c below 2^12 runs
 __host__ __device__ inline int64_t run_start(int64_t W, int c, int R) { return W * c / R; }
@@ -174,6 +172,30 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// the same from 0
+__device__ __forceinline__ void mma0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                     uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// f32 pairs: a += (x, y), a *= s
+__device__ __forceinline__ void add2(uint64_t& a, float x, float y) {
+    asm("{.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tadd.rn.f32x2 %0, %0, t;}" : "+l"(a) : "f"(x), "f"(y));
+}
+__device__ __forceinline__ void mul2(uint64_t& a, uint64_t s) {
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a) : "l"(s));
+}
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+    return d;
+}
+__device__ __forceinline__ float2 halves(uint64_t a) {
+    float2 d;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(a));
+    return d;
+}
 __device__ __forceinline__ float ex2f(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -182,62 +204,73 @@ __device__ __forceinline__ float ex2f(float x) {
 
 // One warp's running softmax over the tiles that it takes of a segment.
 struct State {
-    float o[16][4];                              // O^T / 16: tile m, dims 32 r + 2 m, + 1, heads 2c, 2c + 1
+    uint64_t o[16][2];                           // O^T / 16: tile m, dims 32 r + 2 m, + 1: pair of heads 2c, 2c + 1
     float m, l;                                  // head r; l is this thread's share
 };
 
-template <bool TRACK>
-__device__ __forceinline__ void attend_tile(State& st, const uint8_t* tile, const uint32_t* q, float qs, int valid,
-                                            float* __restrict__ scores, int lane) {
+// NT tiles (1 or 2).  valid: positions of them that exist.
+template <int NT, bool TRACK>
+__device__ __forceinline__ void attend(State& st, const uint8_t* tiles, const uint4 (&q)[16], float qs, int valid,
+                                       float* __restrict__ scores, int lane) {
     const int r = lane >> 2, c = lane & 3;
-    // ---- scores of 2 x 8 positions
-    float x[4];
+    // ---- scores of NT x 2 x 8 positions: x[n][0], x[n][1] = head r at positions 8 n + 2 c, + 1
+    float x[2 * NT][2];
     {
-        const uint32_t kb = *reinterpret_cast<const uint32_t*>(tile + OFF_KS + lane * 4);
-        float s0[2][4] = {}, s1[2][4] = {};      // two sums per 8 positions: four independent chains
+        float s[2 * NT][4] = {};                 // hi and lo sums
+        uint32_t kb[NT];
+#pragma unroll
+        for (int k = 0; k < NT; ++k)
+            kb[k] = *reinterpret_cast<const uint32_t*>(tiles + k * Q4_TILE_BYTES + OFF_KS + lane * 4);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            uint32_t ws[2][4];
-            Scale16 sc[2];
+            uint32_t ws[2 * NT][4];
+            Scale16 sc[2 * NT];
 #pragma unroll
-            for (int n8 = 0; n8 < 2; ++n8) {
-                const uint4 w4 = *reinterpret_cast<const uint4*>(tile + (n8 * 2 + i) * 512 + lane * 16);
-                ws[n8][0] = w4.x; ws[n8][1] = w4.y; ws[n8][2] = w4.z; ws[n8][3] = w4.w;
+            for (int n = 0; n < 2 * NT; ++n) {
+                const uint4 w4 = *reinterpret_cast<const uint4*>(tiles + (n >> 1) * Q4_TILE_BYTES + ((n & 1) * 2 + i) * 512 +
+                                                                 lane * 16);
+                ws[n][0] = w4.x; ws[n][1] = w4.y; ws[n][2] = w4.z; ws[n][3] = w4.w;
                 // the group's scale byte in both halves
-                sc[n8] = scale16(scale_pair(__byte_perm(kb, 0u, 0x4040 + 0x0101 * (n8 * 2 + i))));
+                sc[n] = scale16(scale_pair(__byte_perm(kb[n >> 1], 0u, 0x4040 + 0x0101 * ((n & 1) * 2 + i))));
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const uint4 qa = reinterpret_cast<const uint4*>(q)[(8 * i + 2 * u) * 32 + lane];
-                const uint4 qb = reinterpret_cast<const uint4*>(q)[(8 * i + 2 * u + 1) * 32 + lane];
+                const uint4 qa = q[8 * i + 2 * u], qb = q[8 * i + 2 * u + 1];
 #pragma unroll
-                for (int n8 = 0; n8 < 2; ++n8) {
-                    const uint32_t w = ws[n8][u], w8 = w >> 8;
-                    mma(s0[n8], qa.x, qa.y, qa.z, qa.w, unpack_lo(w, sc[n8]), unpack_hi(w, sc[n8]));
-                    mma(s1[n8], qb.x, qb.y, qb.z, qb.w, unpack_lo(w8, sc[n8]), unpack_hi(w8, sc[n8]));
+                for (int n = 0; n < 2 * NT; ++n)
+                    mma(s[n], qa.x, qa.y, qa.z, qa.w, unpack_lo(ws[n][u], sc[n]), unpack_hi(ws[n][u], sc[n]));
+#pragma unroll
+                for (int n = 0; n < 2 * NT; ++n) {
+                    const uint32_t w8 = ws[n][u] >> 8;
+                    mma(s[n], qb.x, qb.y, qb.z, qb.w, unpack_lo(w8, sc[n]), unpack_hi(w8, sc[n]));
                 }
             }
         }
 #pragma unroll
-        for (int n8 = 0; n8 < 2; ++n8) {
-            x[2 * n8] = ((s0[n8][0] + s1[n8][0]) + (s0[n8][2] + s1[n8][2])) * qs;
-            x[2 * n8 + 1] = ((s0[n8][1] + s1[n8][1]) + (s0[n8][3] + s1[n8][3])) * qs;
+        for (int n = 0; n < 2 * NT; ++n) {
+            x[n][0] = (s[n][0] + s[n][2]) * qs;
+            x[n][1] = (s[n][1] + s[n][3]) * qs;
         }
     }
     if (TRACK) {
         if (r < GRP) {                           // [tile][head][16]
-            *reinterpret_cast<float2*>(scores + r * Q4_TILE + 2 * c) = make_float2(x[0], x[1]);
-            *reinterpret_cast<float2*>(scores + r * Q4_TILE + 2 * c + 8) = make_float2(x[2], x[3]);
+#pragma unroll
+            for (int n = 0; n < 2 * NT; ++n)
+                *reinterpret_cast<float2*>(scores + ((n >> 1) * GRP + r) * Q4_TILE + 2 * c + 8 * (n & 1)) =
+                    make_float2(x[n][0], x[n][1]);
         }
     }
-    if (valid < Q4_TILE) {                       // the row's last tile
-        if (2 * c >= valid) x[0] = -INFINITY;
-        if (2 * c + 1 >= valid) x[1] = -INFINITY;
-        if (2 * c + 8 >= valid) x[2] = -INFINITY;
-        if (2 * c + 9 >= valid) x[3] = -INFINITY;
+    if (valid < NT * Q4_TILE) {                  // the row's last tile
+#pragma unroll
+        for (int n = 0; n < 2 * NT; ++n) {
+            if (8 * n + 2 * c >= valid) x[n][0] = -INFINITY;
+            if (8 * n + 2 * c + 1 >= valid) x[n][1] = -INFINITY;
+        }
     }
     // ---- online softmax
-    float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    float mx = fmaxf(x[0][0], x[0][1]);
+#pragma unroll
+    for (int n = 1; n < 2 * NT; ++n) mx = fmaxf(mx, fmaxf(x[n][0], x[n][1]));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     // rescale only when some head's maximum has outgrown what f16 holds of 2^P_LOG2 p
@@ -246,40 +279,55 @@ __device__ __forceinline__ void attend_tile(State& st, const uint8_t* tile, cons
         st.l *= a;
         st.m = m_new;
         const float a0 = __shfl_sync(0xffffffffu, a, 8 * c), a1 = __shfl_sync(0xffffffffu, a, 8 * c + 4);
+        const uint64_t aa = pair_of(a0, a1);
 #pragma unroll
         for (int m = 0; m < 16; ++m) {
-            st.o[m][0] *= a0;
-            st.o[m][1] *= a1;
-            st.o[m][2] *= a0;
-            st.o[m][3] *= a1;
+            mul2(st.o[m][0], aa);
+            mul2(st.o[m][1], aa);
         }
     }
     const float off = P_LOG2 - st.m;
-    uint32_t ph[2], pl[2];
+    uint32_t ph[2 * NT], pl[2 * NT];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const float p0 = ex2f(x[2 * i] + off), p1 = ex2f(x[2 * i + 1] + off);
+    for (int n = 0; n < 2 * NT; ++n) {
+        const float p0 = ex2f(x[n][0] + off), p1 = ex2f(x[n][1] + off);
         st.l += p0 + p1;
         const __half2 h = __floats2half2_rn(p0, p1);
         const __half2 l = __floats2half2_rn(p0 - __low2float(h), p1 - __high2float(h));
-        ph[i] = *reinterpret_cast<const uint32_t*>(&h);
-        pl[i] = *reinterpret_cast<const uint32_t*>(&l);
+        ph[n] = *reinterpret_cast<const uint32_t*>(&h);
+        pl[n] = *reinterpret_cast<const uint32_t*>(&l);
     }
-    // ---- O^T += V^T P^T
-    const uint32_t vb = *reinterpret_cast<const uint32_t*>(tile + OFF_VS + lane * 4);
-    const Scale16 sa = scale16(scale_pair(__byte_perm(vb, 0u, 0x4140)));
-    const Scale16 sb = scale16(scale_pair(__byte_perm(vb, 0u, 0x4342)));
+    // ---- O^T += V^T P^T.  The matrix instruction adds to its f32 accumulator with truncation
+    // (n additions leave it about n 2^-24 short: 5e-6 over 148 tiles when O was the
+    // accumulator), so the tiles' product starts from 0 and is added to O rounded to nearest.
+    Scale16 sa[NT], sb[NT];
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+        const uint32_t vb = *reinterpret_cast<const uint32_t*>(tiles + k * Q4_TILE_BYTES + OFF_VS + lane * 4);
+        sa[k] = scale16(scale_pair(__byte_perm(vb, 0u, 0x4140)));
+        sb[k] = scale16(scale_pair(__byte_perm(vb, 0u, 0x4342)));
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint4 w4 = *reinterpret_cast<const uint4*>(tile + OFF_V + i * 512 + lane * 16);
-        const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w};
+        float d[4][4];
+#pragma unroll
+        for (int k = 0; k < NT; ++k) {
+            const uint4 w4 = *reinterpret_cast<const uint4*>(tiles + k * Q4_TILE_BYTES + OFF_V + i * 512 + lane * 16);
+            const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const uint32_t w = ws[u], w8 = w >> 8;
+                const uint32_t a0 = unpack_lo(w, sa[k]), a2 = unpack_hi(w, sb[k]);
+                const uint32_t a1 = unpack_lo(w8, sa[k]), a3 = unpack_hi(w8, sb[k]);
+                if (k == 0) mma0(d[u], a0, a1, a2, a3, ph[0], ph[1]);
+                else mma(d[u], a0, a1, a2, a3, ph[2 * k], ph[2 * k + 1]);
+                mma(d[u], a0, a1, a2, a3, pl[2 * k], pl[2 * k + 1]);
+            }
+        }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const uint32_t w = ws[u], w8 = w >> 8;
-            const uint32_t a0 = unpack_lo(w, sa), a2 = unpack_hi(w, sb);
-            const uint32_t a1 = unpack_lo(w8, sa), a3 = unpack_hi(w8, sb);
-            mma(st.o[4 * i + u], a0, a1, a2, a3, ph[0], ph[1]);
-            mma(st.o[4 * i + u], a0, a1, a2, a3, pl[0], pl[1]);
+            add2(st.o[4 * i + u][0], d[u][0], d[u][1]);
+            add2(st.o[4 * i + u][1], d[u][2], d[u][3]);
         }
     }
 }
@@ -298,7 +346,6 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
     const int64_t W = d.tiles(), run0 = run_start(W, run, R), run1 = run_start(W, run + 1, R);
     if (lane == 0) {
         for (int s = 0; s < STAGES; ++s) mbar_init(&ring.full[s], 1);
-        mbar_init(&ring.q_full, 1);
         fence_mbar_init();
     }
     __syncwarp();
@@ -321,38 +368,37 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
             p_end += ps.t1 - ps.t0;
             p_t = ps.t0;
         }
-        if (p_t == d.row_tiles(ps.b) - 1) wait_prep();
+        const int nt = min(2, ps.t1 - p_t);
+        if (p_t + nt == d.row_tiles(ps.b)) wait_prep();
         if (lane == 0) {
-            mbar_arrive_expect_tx(&ring.full[stage], Q4_TILE_BYTES);
-            bulk_g2s(ring.tile[stage], ps.base + (size_t)p_t * Q4_TILE_BYTES, Q4_TILE_BYTES, &ring.full[stage]);
+            mbar_arrive_expect_tx(&ring.full[stage], nt * Q4_TILE_BYTES);
+            bulk_g2s(ring.pair[stage], ps.base + (size_t)p_t * Q4_TILE_BYTES, nt * Q4_TILE_BYTES, &ring.full[stage]);
         }
-        ++p_t;
+        p_t += nt;
     };
     for (int s = 0; s < STAGES; ++s) produce(s);
     wait_prep();                                 // q_frag
 
     int stage = 0;
-    uint32_t phase = 0, q_phase = 0;
-    for (int64_t at = run0; at < run1; q_phase ^= 1u) {
+    uint32_t phase = 0;
+    for (int64_t at = run0; at < run1;) {
         const Segment sg = segment_at(d, slots, at, run1);
-        if (lane == 0) {
-            mbar_arrive_expect_tx(&ring.q_full, FRAG_WORDS * 4);
-            bulk_g2s(ring.q, q_frag + (size_t)sg.row * FRAG_WORDS, FRAG_WORDS * 4, &ring.q_full);
-        }
-        if (!mbar_wait(&ring.q_full, q_phase, err)) return;
-        const float qs = __uint_as_float(ring.q[FRAG_SCALES + r]);
+        const uint32_t* frag = q_frag + (size_t)sg.row * FRAG_WORDS;
+        uint4 q[16];
+#pragma unroll
+        for (int s = 0; s < 16; ++s) q[s] = reinterpret_cast<const uint4*>(frag)[s * 32 + lane];
+        const float qs = __uint_as_float(frag[FRAG_SCALES + r]);
         const int n = d.len[sg.b] + 1;
         State st;
 #pragma unroll
-        for (int m = 0; m < 16; ++m)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) st.o[m][e] = 0.0f;
+        for (int m = 0; m < 16; ++m) st.o[m][0] = st.o[m][1] = 0ull;
         st.m = -INFINITY;
         st.l = 0.0f;
-        for (int t = sg.t0; t < sg.t1; ++t, ++at) {
+        for (int t = sg.t0; t < sg.t1; t += 2) {
             if (!mbar_wait(&ring.full[stage], phase, err)) return;
-            attend_tile<TRACK>(st, ring.tile[stage], ring.q, qs, n - t * Q4_TILE,
-                               TRACK ? scores + (size_t)at * (GRP * Q4_TILE) : nullptr, lane);
+            float* sc = TRACK ? scores + (size_t)(at + (t - sg.t0)) * (GRP * Q4_TILE) : nullptr;
+            if (t + 1 < sg.t1) attend<2, TRACK>(st, ring.pair[stage], q, qs, n - t * Q4_TILE, sc, lane);
+            else attend<1, TRACK>(st, ring.pair[stage], q, qs, n - t * Q4_TILE, sc, lane);
             __syncwarp();
             produce(stage);
             if (++stage == STAGES) {
@@ -360,6 +406,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
                 phase ^= 1u;
             }
         }
+        at += sg.t1 - sg.t0;
         // ---- the segment's partial: thread (r, c) holds dims 32 r .. + 31 of heads 2c, 2c + 1
         st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
         st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
@@ -368,10 +415,11 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
             float* po = part_o + (part * GRP + 2 * c) * HD + 32 * r;
 #pragma unroll
             for (int m = 0; m < 16; m += 2) {    // V came as V / 16
-                *reinterpret_cast<float4*>(po + 2 * m) =
-                    make_float4(16.0f * st.o[m][0], 16.0f * st.o[m][2], 16.0f * st.o[m + 1][0], 16.0f * st.o[m + 1][2]);
+                const float2 a0 = halves(st.o[m][0]), b0 = halves(st.o[m][1]);
+                const float2 a1 = halves(st.o[m + 1][0]), b1 = halves(st.o[m + 1][1]);
+                *reinterpret_cast<float4*>(po + 2 * m) = make_float4(16.0f * a0.x, 16.0f * b0.x, 16.0f * a1.x, 16.0f * b1.x);
                 *reinterpret_cast<float4*>(po + HD + 2 * m) =
-                    make_float4(16.0f * st.o[m][1], 16.0f * st.o[m][3], 16.0f * st.o[m + 1][1], 16.0f * st.o[m + 1][3]);
+                    make_float4(16.0f * a0.y, 16.0f * b0.y, 16.0f * a1.y, 16.0f * b1.y);
             }
         }
         if (c == 0 && r < GRP)

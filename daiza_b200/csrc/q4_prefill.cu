@@ -6,15 +6,14 @@
 // 0 .. base + t as the cache holds them (4 bits), its own row included: the same as one
 // decode call per token.
 //
-// Kernels (stream-ordered):
-//   1. q4_pf_angles : (cos, sin) of every token's 32 pairs, f64.
-//   2. q4_pf_query  : Q normed, rotated, scaled, as f16 [head][token][256].
-//   3. q4_pf_append : K (normed, rotated, f64) and V quantised into the sequences' tiles.
-//   4. q4_pf_values : every held row as f16 [kv head][key][256] -- exact -- each sequence
-//                     padded with zeros to whole blocks of 128 keys, so that a block never
-//                     meets another sequence's values.
-//   5. pf_attn      : (pf_attn.cuh) tcgen05 attention, f16 operands: K and V are exact, Q and
-//                     P are rounded to 11 bits (bf16's 8 would cost the output's last bits).
+// Two kernels:
+//   1. q4_pf_prep : Q normed, rotated, scaled, as f16 [head][token][256]; K (normed, rotated,
+//                   f64) and V quantised into the sequences' tiles; and every held row, old
+//                   and new, as f16 [kv head][key][256] -- exact -- each sequence padded with
+//                   zeros to whole blocks of 128 keys, so that a block never meets another
+//                   sequence's values.  Blocks of three kinds, all independent.
+//   2. pf_attn    : (pf_attn.cuh) tcgen05 attention, f16 operands: K and V are exact, Q and P
+//                   are rounded to 11 bits (bf16's 8 would cost the output's last bits).
 #include "pf_attn.cuh"
 #include "q4.cuh"
 
@@ -28,7 +27,11 @@ struct Prompt {
     int32_t sid[MAXB], base[MAXB];
     int32_t row0[MAXB + 1], key0[MAXB + 1];      // key0: multiples of 128
     int32_t at0[MAXB + 1];                       // tiles that the new tokens touch
+    int32_t old0[MAXB + 1];                      // tiles with cached rows or padding
     __host__ __device__ int T(int i) const { return row0[i + 1] - row0[i]; }
+    // tiles of cached rows come first, then those of the padding
+    __host__ __device__ int cached_tiles(int i) const { return (base[i] + Q4_TILE - 1) / Q4_TILE; }
+    __host__ __device__ int first_pad_tile(int i) const { return (base[i] + T(i)) / Q4_TILE; }
 };
 __device__ __forceinline__ int last_at_or_before(const int32_t* start, int n, int at) {   // last i with start[i] <= at
     int lo = 0, hi = n - 1;
@@ -39,118 +42,123 @@ __device__ __forceinline__ int last_at_or_before(const int32_t* start, int n, in
     return lo;
 }
 
-__global__ void __launch_bounds__(256) q4_pf_angles_kernel(const __grid_constant__ Prompt d, RopeAxes axes,
-                                                           const int32_t* __restrict__ pos, double2* __restrict__ cs) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int t = (int)(i / (ROPE / 2)), pair = (int)(i % (ROPE / 2));
-    if (t >= d.row0[d.n]) return;
-    if (pos) {
-        cs[i] = rope_cs(axes, pair, pos[3 * (int64_t)t], pos[3 * (int64_t)t + 1], pos[3 * (int64_t)t + 2]);
-    } else {
-        const int s = last_at_or_before(d.row0, d.n, t), p = d.base[s] + (t - d.row0[s]);
-        cs[i] = rope_cs(axes, pair, p, p, p);
-    }
-}
-
-__device__ __forceinline__ void load_row(const float* p, float (&x)[8]) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+template <typename T>
+__device__ __forceinline__ void load_row(const T* p, double (&x)[8]) {
+    const float4 a = as_f32(load4(p)), b = as_f32(load4(p + 4));
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
     x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
 }
-__device__ __forceinline__ void load_row(const __nv_bfloat16* p, float (&x)[8]) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// codes + 8 and the group's scale byte -> 8 held values
+__device__ __forceinline__ uint4 held(const uint32_t (&code)[8], uint32_t sb) {
+    const uint32_t s = scale_pair(sb | sb << 16), c = hmul2_u(s, NEG72);
+    uint32_t h[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[2 * i] = tc::bf16_lo_f(w[i]);
-        x[2 * i + 1] = tc::bf16_hi_f(w[i]);
-    }
+    for (int i = 0; i < 4; ++i) h[i] = unpack(code[2 * i] << 4 | code[2 * i + 1] << 20, s, c);
+    return make_uint4(h[0], h[1], h[2], h[3]);
 }
 
-// one warp per (token, q head)
+constexpr int PREP_WARPS = 16, PREP_HEADS = 6;   // heads of a token that a warp takes
+
+// Blocks [0, at0 kvc): a tile of new rows and a kv head, a warp per position.
+// Then (old0 kvc) blocks: a tile of cached rows or padding, a warp per position.
+// Then: a warp per (token, PREP_HEADS heads).
 template <typename T>
-__global__ void __launch_bounds__(256) q4_pf_query_kernel(int n_tokens, int nq, const double2* __restrict__ cs,
-                                                          const float* __restrict__ q_norm, const T* __restrict__ q_gate,
-                                                          __half* __restrict__ q, float eps) {
-    const int t = blockIdx.x, head = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (head >= nq) return;
-    float x[8];
-    load_row(q_gate + ((size_t)t * nq + head) * QG_ROW + 8 * lane, x);
-    norm_rotate(x, q_norm, cs + (size_t)t * (ROPE / 2), eps, lane);
-    constexpr float QS = 0.0625f * LOG2E;        // scores in log2 units
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = pf::pack2<__half>(x[2 * i] * QS, x[2 * i + 1] * QS);
-    *reinterpret_cast<uint4*>(q + ((size_t)head * n_tokens + t) * HD + 8 * lane) = make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// one warp per (tile that a new token lies in, kv head); the tile's other positions stay
-template <typename T>
-__global__ void __launch_bounds__(256) q4_pf_append_kernel(const __grid_constant__ Prompt d, int kvc,
-                                                           const Q4Slot* __restrict__ slots,
-                                                           const double2* __restrict__ cs,
-                                                           const float* __restrict__ k_norm, const T* __restrict__ k,
-                                                           const T* __restrict__ v, bool track, float eps) {
-    const int64_t task = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (task >= (int64_t)d.at0[d.n] * kvc) return;
-    const int at = (int)(task / kvc), kvh = (int)(task - (int64_t)at * kvc);
-    const int s = last_at_or_before(d.at0, d.n, at);
-    const int base = d.base[s], end = base + d.T(s);
-    const int t16 = (base >> 4) + (at - d.at0[s]);
-    const Q4Slot slot = slots[d.sid[s]];
-    uint8_t* tile = slot.tile(kvh, t16);
-    uint4 w[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) w[c] = *v_words(tile, lane, c);
-#pragma unroll
-    for (int p = 0; p < Q4_TILE; ++p) {
-        const int at_pos = t16 * Q4_TILE + p;
-        if (at_pos < base || at_pos >= end) continue;
-        const int64_t row = d.row0[s] + (at_pos - base);
-        float f[8];
-        load_row(k + (row * kvc + kvh) * HD + 8 * lane, f);
-        double x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = f[e];
-        norm_rotate(x, k_norm, cs + row * (ROPE / 2), eps, lane);
-        uint32_t code[8];
-        uint32_t sb = quantise(x, code);
-        put_k(tile, p, lane, code, sb);
-        load_row(v + (row * kvc + kvh) * HD + 8 * lane, f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = f[e];
-        sb = quantise(x, code);
-        merge_v(w[(p & 7) >> 1], p, code);
-        put_v_scale(tile, p, lane, sb);
-        if (track && lane == 0) slot.wts[(size_t)kvh * slot.cap + at_pos] = 0.0f;
-    }
-#pragma unroll
-    for (int c = 0; c < 4; ++c) *v_words(tile, lane, c) = w[c];
-}
-
-// one warp per (16 key rows, kv head)
-__global__ void __launch_bounds__(256) q4_pf_values_kernel(const __grid_constant__ Prompt d, int kvc,
-                                                           const Q4Slot* __restrict__ slots, __half* __restrict__ kf,
-                                                           __half* __restrict__ vf) {
-    const int64_t keys = d.key0[d.n];
-    const int64_t task = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (task >= keys / Q4_TILE * kvc) return;
-    const int kvh = (int)(task % kvc), row = (int)(task / kvc) * Q4_TILE;
-    const int s = last_at_or_before(d.key0, d.n, row);
-    const int pos = row - d.key0[s], len = d.base[s] + d.T(s);
-    const uint8_t* tile = slots[d.sid[s]].tile(kvh, pos >> 4);
-    uint4* ko = reinterpret_cast<uint4*>(kf + ((size_t)kvh * keys + row) * HD) + lane;
-    uint4* vo = reinterpret_cast<uint4*>(vf + ((size_t)kvh * keys + row) * HD) + lane;
-    for (int p = 0; p < Q4_TILE; ++p, ko += HD / 8, vo += HD / 8) {
-        uint32_t a[4] = {}, b[4] = {};
-        if (pos + p < len) {
-            get_k(tile, p, lane, a);
-            get_v(tile, p, lane, b);
+__global__ void __launch_bounds__(32 * PREP_WARPS)
+    q4_pf_prep_kernel(const __grid_constant__ Prompt d, const __grid_constant__ RopeAxes axes, int kvc,
+                      const Q4Slot* __restrict__ slots, const int32_t* __restrict__ pos, const float* __restrict__ q_norm,
+                      const float* __restrict__ k_norm, const T* __restrict__ q_gate, const T* __restrict__ k,
+                      const T* __restrict__ v, __half* __restrict__ qf, __half* __restrict__ kf, __half* __restrict__ vf,
+                      bool track, float eps) {
+    __shared__ TileMerge merge;
+    __shared__ double2 cs[PREP_WARPS][ROPE / 2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nq = GRP * kvc;
+    const int64_t keys = d.key0[d.n], tokens = d.row0[d.n];
+    int64_t block = blockIdx.x;
+    auto angles_at = [&](int s, int64_t row, int (&p)[3]) {
+        if (pos) {
+            for (int i = 0; i < 3; ++i) p[i] = pos[3 * row + i];
+        } else {
+            p[0] = p[1] = p[2] = d.base[s] + (int)(row - d.row0[s]);
         }
-        *ko = make_uint4(a[0], a[1], a[2], a[3]);
-        *vo = make_uint4(b[0], b[1], b[2], b[3]);
+    };
+    if (block < (int64_t)d.at0[d.n] * kvc) {
+        const int at = (int)(block / kvc), kvh = (int)(block - (int64_t)at * kvc);
+        const int s = last_at_or_before(d.at0, d.n, at);
+        const int base = d.base[s], t16 = (base >> 4) + (at - d.at0[s]), slot_pos = t16 * Q4_TILE + warp;
+        const Q4Slot slot = slots[d.sid[s]];
+        uint8_t* tile = slot.tile(kvh, t16);
+        merge.begin();
+        if (slot_pos >= base && slot_pos < base + d.T(s)) {
+            const int64_t row = d.row0[s] + (slot_pos - base);
+            int p[3];
+            angles_at(s, row, p);
+            cs[warp][lane] = rope_cs(axes, lane, p[0], p[1], p[2]);
+            __syncwarp();
+            const size_t out = ((size_t)kvh * keys + d.key0[s] + slot_pos) * HD + 8 * lane;
+            double x[8];
+            load_row(k + (row * kvc + kvh) * HD + 8 * lane, x);
+            norm_rotate(x, k_norm, cs[warp], eps, lane);
+            uint32_t code[8];
+            uint32_t sb = quantise(x, code);
+            put_k(tile, warp, lane, code, sb);
+            *reinterpret_cast<uint4*>(kf + out) = held(code, sb);
+            load_row(v + (row * kvc + kvh) * HD + 8 * lane, x);
+            sb = quantise(x, code);
+            merge.add(warp, lane, code);
+            put_v_scale(tile, warp, lane, sb);
+            *reinterpret_cast<uint4*>(vf + out) = held(code, sb);
+            if (track && lane == 0) slot.wts[(size_t)kvh * slot.cap + slot_pos] = 0.0f;
+        }
+        merge.end(tile);
+        return;
+    }
+    block -= (int64_t)d.at0[d.n] * kvc;
+    if (block < (int64_t)d.old0[d.n] * kvc) {
+        const int ot = (int)(block / kvc), kvh = (int)(block - (int64_t)ot * kvc);
+        const int s = last_at_or_before(d.old0, d.n, ot);
+        const int i = ot - d.old0[s], cached = d.cached_tiles(s);
+        const int t16 = i < cached ? i : d.first_pad_tile(s) + (i - cached), at = t16 * Q4_TILE + warp;
+        const bool old = i < cached;
+        if (old ? at >= d.base[s] : at < d.base[s] + d.T(s)) return;   // a new row
+        uint32_t a[4] = {}, b[4] = {};
+        if (old) {
+            const uint8_t* tile = slots[d.sid[s]].tile(kvh, t16);
+            get_k(tile, warp, lane, a);
+            get_v(tile, warp, lane, b);
+        }
+        const size_t out = ((size_t)kvh * keys + d.key0[s] + at) * HD + 8 * lane;
+        *reinterpret_cast<uint4*>(kf + out) = make_uint4(a[0], a[1], a[2], a[3]);
+        *reinterpret_cast<uint4*>(vf + out) = make_uint4(b[0], b[1], b[2], b[3]);
+        return;
+    }
+    block -= (int64_t)d.old0[d.n] * kvc;
+    const int parts = (nq + PREP_HEADS - 1) / PREP_HEADS;
+    const int64_t task = block * PREP_WARPS + warp, row = task / parts;
+    if (row >= tokens) return;
+    const int h0 = (int)(task - row * parts) * PREP_HEADS, h1 = min(nq, h0 + PREP_HEADS);
+    int p[3];
+    angles_at(pos ? 0 : last_at_or_before(d.row0, d.n, (int)row), row, p);
+    float2 c4[4];
+    spread_pairs(rope_cs_f32(axes, lane, p[0], p[1], p[2]), c4, lane);
+    float w[8];
+    load_split(q_norm, lane, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] *= 0.0625f * LOG2E;   // scores in log2 units
+    SplitRow<T> in[PREP_HEADS];
+#pragma unroll
+    for (int i = 0; i < PREP_HEADS; ++i)
+        if (h0 + i < h1) in[i].load(q_gate + (row * nq + h0 + i) * QG_ROW, lane);
+#pragma unroll
+    for (int i = 0; i < PREP_HEADS; ++i) {
+        if (h0 + i >= h1) break;
+        float x[8];
+        in[i].values(x);
+        norm_rotate_split(x, w, c4, eps, lane);
+        __half* out = qf + ((size_t)(h0 + i) * tokens + row) * HD;
+        *reinterpret_cast<uint2*>(out + split_dim(lane, 0)) =
+            make_uint2(pf::pack2<__half>(x[0], x[1]), pf::pack2<__half>(x[2], x[3]));
+        *reinterpret_cast<uint2*>(out + split_dim(lane, 1)) =
+            make_uint2(pf::pack2<__half>(x[4], x[5]), pf::pack2<__half>(x[6], x[7]));
     }
 }
 
@@ -183,10 +191,9 @@ static cudaError_t launch_group(dz_ctx* ctx, int layer, const q4::Prompt& d, con
     const int kvc = ctx->cfg.kv_head_count, nq = GRP * kvc;
     const int64_t tokens = d.row0[d.n], keys = d.key0[d.n];
     const size_t qn = (size_t)nq * tokens * HD, kn = (size_t)kvc * keys * HD;
-    cudaError_t e = ensure_q4_scratch(ctx, (qn + 2 * kn) * sizeof(__half) + (size_t)tokens * (ROPE / 2) * sizeof(double2));
+    cudaError_t e = ensure_q4_scratch(ctx, (qn + 2 * kn) * sizeof(__half));
     if (e != cudaSuccess) return e;
-    double2* cs = static_cast<double2*>(ctx->q4_scratch);
-    __half* qf = reinterpret_cast<__half*>(cs + (size_t)tokens * (ROPE / 2));
+    __half* qf = static_cast<__half*>(ctx->q4_scratch);
     __half *kf = qf + qn, *vf = kf + kn;
     CUtensorMap mq, mk, mv;
     if (!pf::make_map<__half>(&mq, qf, tokens, nq, pf::BM) || !pf::make_map<__half>(&mk, kf, keys, kvc, pf::BN) ||
@@ -211,13 +218,11 @@ static cudaError_t launch_group(dz_ctx* ctx, int layer, const q4::Prompt& d, con
         map.key[i] = d.key0[s];
         map.first[i + 1] = map.first[i] + pf::Packed::own_tiles(d.T(s), map.split_idx, map.split_cnt);
     }
-    q4::q4_pf_angles_kernel<<<(unsigned)((tokens * (ROPE / 2) + 255) / 256), 256, 0, st>>>(d, ctx->axes, pos, cs);
-    q4::q4_pf_query_kernel<T><<<dim3((unsigned)tokens, (nq + 7) / 8), 256, 0, st>>>((int)tokens, nq, cs, L.q_norm, q_gate,
-                                                                                 qf, ctx->cfg.rms_eps);
-    q4::q4_pf_append_kernel<T><<<(unsigned)(((int64_t)d.at0[d.n] * kvc + 7) / 8), 256, 0, st>>>(
-        d, kvc, L.d_q4, cs, L.k_norm, k, v, ctx->q4_track, ctx->cfg.rms_eps);
-    q4::q4_pf_values_kernel<<<(unsigned)((keys / Q4_TILE * kvc + 7) / 8), 256, 0, st>>>(d, kvc, L.d_q4, kf, vf);
-    *n_launch += 4;
+    const int64_t q_tasks = tokens * ((nq + q4::PREP_HEADS - 1) / q4::PREP_HEADS);
+    const int64_t blocks = (int64_t)(d.at0[d.n] + d.old0[d.n]) * kvc + (q_tasks + q4::PREP_WARPS - 1) / q4::PREP_WARPS;
+    q4::q4_pf_prep_kernel<T><<<(unsigned)blocks, 32 * q4::PREP_WARPS, 0, st>>>(
+        d, ctx->axes, kvc, L.d_q4, pos, L.q_norm, L.k_norm, q_gate, k, v, qf, kf, vf, ctx->q4_track, ctx->cfg.rms_eps);
+    *n_launch += 1;
     if (map.first[d.n] > 0) {
         const size_t smem = sizeof(pf::Smem) + 1024;
         auto kernel = pf_attn_kernel<T, T, __half, pf::Packed>;
@@ -242,12 +247,12 @@ static cudaError_t launch_prompts(dz_ctx* ctx, int layer, int n, const int32_t* 
     for (int i = 0; i < n;) {
         q4::Prompt d;
         d.n = 0;
-        d.row0[0] = d.key0[0] = d.at0[0] = 0;
+        d.row0[0] = d.key0[0] = d.at0[0] = d.old0[0] = 0;
         int64_t bytes = 0;
         for (; i < n && d.n < MAXB; ++i) {
             const int64_t base = L.len[seq_ids[i]], T_i = lens[i];
             const int64_t keys = (base + T_i + pf::BN - 1) / pf::BN * pf::BN;
-            const int64_t more = T_i * (nq * HD * 2 + ROPE / 2 * 16) + keys * kvc * HD * 4;
+            const int64_t more = T_i * nq * HD * 2 + keys * kvc * HD * 4;
             if (T_i == 0) continue;
             if (d.n > 0 && bytes + more > GROUP_BYTES) break;
             bytes += more;
@@ -257,6 +262,7 @@ static cudaError_t launch_prompts(dz_ctx* ctx, int layer, int n, const int32_t* 
             d.row0[d.n] = d.row0[s] + (int32_t)T_i;
             d.key0[d.n] = d.key0[s] + (int32_t)keys;
             d.at0[d.n] = d.at0[s] + (int32_t)((base + T_i - 1) / Q4_TILE - base / Q4_TILE + 1);
+            d.old0[d.n] = d.old0[s] + d.cached_tiles(s) + (int32_t)(keys / Q4_TILE - d.first_pad_tile(s));
         }
         if (d.n == 0) break;
         const cudaError_t e = launch_group<T>(ctx, layer, d, pos, q_gate, k, v, out, st, n_launch);

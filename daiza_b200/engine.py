@@ -45,22 +45,34 @@ def _stream(stream):
 
 
 def _tensor(name, t, dtype, numel):
-    """Pointer of a contiguous CUDA tensor that a 4-bit cache call reads or writes; DZ_EINVAL otherwise."""
+    """Address of a contiguous CUDA tensor that a 4-bit cache call reads or writes; DZ_EINVAL otherwise."""
     if not (t.is_cuda and t.dtype == dtype and t.is_contiguous() and t.numel() == numel):
         raise _ffi.DzError(_ffi.DZ_EINVAL, f"{name} must be a contiguous CUDA {dtype} tensor of {numel} values, got "
                                            f"{tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
-    return _ptr(t)
+    return t.data_ptr()
+
+
+def _ints(name, values, ctype, count=None):
+    """ctypes array of whole numbers (a number, list or array); DZ_EINVAL if they do not fit or are not `count`.
+    A list goes straight into the array: the numpy route costs as much as a small launch."""
+    v = values if type(values) in (list, tuple) else np.atleast_1d(values).tolist()
+    bits = 8 * C.sizeof(ctype) - 1
+    try:
+        if count is not None and len(v) != count:
+            raise ValueError(f"{count} numbers wanted, {len(v)} given")
+        if v and not (-(1 << bits) <= min(v) and max(v) < 1 << bits):
+            raise ValueError("out of range")
+        return (ctype * len(v))(*v)
+    except (TypeError, ValueError) as e:
+        raise _ffi.DzError(_ffi.DZ_EINVAL, f"{name}: {e}") from None
 
 
 def _ids(seq_ids):
-    return np.ascontiguousarray(np.atleast_1d(seq_ids), np.int32)
+    return _ints("seq_ids", seq_ids, C.c_int32)
 
 
 def _per_seq(name, values, ids):
-    a = np.ascontiguousarray(np.atleast_1d(values), np.int64)
-    if a.shape != ids.shape:
-        raise _ffi.DzError(_ffi.DZ_EINVAL, f"{name} needs one number per sequence ({len(ids)}), got {a.shape}")
-    return a
+    return _ints(name, values, C.c_int64, len(ids))
 
 
 def default_config(n_layers=64, full_attention_interval=4, kv_heads=None, v_heads=None, qtile_split=None):
@@ -287,10 +299,13 @@ class Context:
 
     def set_rope_axes(self, sections=(11, 11, 10), interleaved=False):
         """Which of a token's (time, height, width) positions turns each of the 32 rotary pairs."""
-        s = np.ascontiguousarray(sections, np.int32)
-        if s.shape != (3,):
-            raise _ffi.DzError(_ffi.DZ_EINVAL, f"sections has three numbers, got {s.shape}")
-        self._chk(self.lib.dz_set_rope_axes(self.h, _np_ptr(s), int(bool(interleaved))))
+        s = _ints("sections", sections, C.c_int32, 3)
+        self._chk(self.lib.dz_set_rope_axes(self.h, s, int(bool(interleaved))))
+
+    def _on(self, stream):
+        """Handle of `stream`, or of the context's device's current one."""
+        import torch
+        return (torch.cuda.current_stream(self.device) if stream is None else stream).cuda_stream
 
     def qk_mrope(self, layer, pos, q_gate, k, q_out, k_out, stream=None):
         """QK-RMSNorm, rotation by pos [T][3] (int32) and q's 1/16; q_gate [T][6*kvc][512] and k [T][kvc][256] f32 or
@@ -302,7 +317,7 @@ class Context:
         self._chk(fn(self.h, layer, T, _tensor("pos", pos, torch.int32, 3 * T),
                      _tensor("q_gate", q_gate, dt, T * self.nq * QG_ROW), _tensor("k", k, dt, T * self.kvc * HD),
                      _tensor("q_out", q_out, dt, T * self.nq * HD), _tensor("k_out", k_out, dt, T * self.kvc * HD),
-                     _stream(stream)))
+                     self._on(stream)))
 
     def gqa_decode_q4(self, layer, seq_ids, q_gate, k, v, out, stream=None, pos=None):
         """gqa_decode on 4-bit caches; pos: [B][3] rotary positions (host), default the cache lengths."""
@@ -310,13 +325,11 @@ class Context:
         ids, f = _ids(seq_ids), torch.float32
         B, p3 = len(ids), None
         if pos is not None:
-            p3 = np.ascontiguousarray(pos, np.int32)
-            if p3.shape != (B, 3):
-                raise _ffi.DzError(_ffi.DZ_EINVAL, f"pos is [{B}][3], got {p3.shape}")
+            p3 = _ints("pos", [p for row in pos for p in row], C.c_int32, 3 * B)
         self._chk(self.lib.dz_gqa_decode_q4(
-            self.h, layer, B, _np_ptr(ids), None if p3 is None else _np_ptr(p3),
+            self.h, layer, B, ids, p3,
             _tensor("q_gate", q_gate, f, B * self.nq * QG_ROW), _tensor("k", k, f, B * self.kvc * HD),
-            _tensor("v", v, f, B * self.kvc * HD), _tensor("out", out, f, B * self.nq * HD), _stream(stream)))
+            _tensor("v", v, f, B * self.kvc * HD), _tensor("out", out, f, B * self.nq * HD), self._on(stream)))
 
     def gqa_prefill_q4(self, layer, seq_ids, lens, q_gate, k, v, out, stream=None, pos=None):
         """lens[i] new tokens of each sequence, packed: q_gate [sum][6*kvc][512], k and v [sum][kvc][256], out
@@ -324,42 +337,42 @@ class Context:
         import torch
         ids = _ids(seq_ids)
         n = _per_seq("lens", lens, ids)
-        T = int(np.maximum(n, 0).sum())
+        T = sum(c for c in n if c > 0)
         dt = torch.bfloat16 if k.dtype == torch.bfloat16 else torch.float32
         fn = self.lib.dz_gqa_prefill_q4_bf16 if dt == torch.bfloat16 else self.lib.dz_gqa_prefill_q4
-        self._chk(fn(self.h, layer, len(ids), _np_ptr(ids), _np_ptr(n),
+        self._chk(fn(self.h, layer, len(ids), ids, n,
                      None if pos is None else _tensor("pos", pos, torch.int32, 3 * T),
                      _tensor("q_gate", q_gate, dt, T * self.nq * QG_ROW), _tensor("k", k, dt, T * self.kvc * HD),
                      _tensor("v", v, dt, T * self.kvc * HD), _tensor("out", out, dt, T * self.nq * HD),
-                     _stream(stream)))
+                     self._on(stream)))
 
     def kv_rows_q4(self, layer, seq_ids, first, count, k, v, stream=None):
         """Held rows [first, first + count) of each sequence as f32 [sum count][kvc][256]."""
         import torch
         ids = _ids(seq_ids)
         a, n = _per_seq("first", first, ids), _per_seq("count", count, ids)
-        total = int(np.maximum(n, 0).sum()) * self.kvc * HD
-        self._chk(self.lib.dz_kv_rows_q4(self.h, layer, len(ids), _np_ptr(ids), _np_ptr(a), _np_ptr(n),
+        total = sum(c for c in n if c > 0) * self.kvc * HD
+        self._chk(self.lib.dz_kv_rows_q4(self.h, layer, len(ids), ids, a, n,
                                          _tensor("k", k, torch.float32, total), _tensor("v", v, torch.float32, total),
-                                         _stream(stream)))
+                                         self._on(stream)))
 
     def _weights_numel(self, layer, ids):
-        return self.kvc * sum(self.kv_len(layer, int(s)) for s in ids)
+        return self.kvc * sum(self.kv_len(layer, s) for s in ids)
 
     def kv_weights_q4(self, layer, seq_ids, out, stream=None):
         """Accumulated attention weights, sequence by sequence [kvc][length]."""
         import torch
         ids = _ids(seq_ids)
         self._chk(self.lib.dz_kv_weights_q4(
-            self.h, layer, len(ids), _np_ptr(ids),
-            _tensor("out", out, torch.float32, self._weights_numel(layer, ids)), _stream(stream)))
+            self.h, layer, len(ids), ids,
+            _tensor("out", out, torch.float32, self._weights_numel(layer, ids)), self._on(stream)))
 
     def kv_set_weights_q4(self, layer, seq_ids, weights, stream=None):
         import torch
         ids = _ids(seq_ids)
         self._chk(self.lib.dz_kv_set_weights_q4(
-            self.h, layer, len(ids), _np_ptr(ids),
-            _tensor("weights", weights, torch.float32, self._weights_numel(layer, ids)), _stream(stream)))
+            self.h, layer, len(ids), ids,
+            _tensor("weights", weights, torch.float32, self._weights_numel(layer, ids)), self._on(stream)))
 
     def kv_evict_q4(self, layer, seq_ids, keep, recent, kept=None, into=None, stream=None):
         """Keeps the last recent[b] and the heaviest other entries, keep[b] in all, per kv head; in place, or into the
@@ -367,15 +380,13 @@ class Context:
         import torch
         ids = _ids(seq_ids)
         k, r = _per_seq("keep", keep, ids), _per_seq("recent", recent, ids)
-        to = None if into is None else _ids(into)
-        if to is not None and to.shape != ids.shape:
-            raise _ffi.DzError(_ffi.DZ_EINVAL, f"into needs one sequence per source ({len(ids)}), got {to.shape}")
+        to = None if into is None else _ints("into", into, C.c_int32, len(ids))
         out = None
         if kept is not None:
-            n = sum(max(0, min(int(a), self.kv_len(layer, int(s)))) for a, s in zip(k, ids))
+            n = sum(max(0, min(a, self.kv_len(layer, s))) for a, s in zip(k, ids))
             out = _tensor("kept", kept, torch.int32, n * self.kvc)
-        self._chk(self.lib.dz_kv_evict_q4(self.h, layer, len(ids), _np_ptr(ids), None if to is None else _np_ptr(to),
-                                          _np_ptr(k), _np_ptr(r), out, _stream(stream)))
+        self._chk(self.lib.dz_kv_evict_q4(self.h, layer, len(ids), ids, to,
+                                          k, r, out, self._on(stream)))
 
     def gdn_decode(self, layer, seq_ids, qkv, alpha, beta, z, y, stream=None):
         ids = np.ascontiguousarray(np.atleast_1d(seq_ids), np.int32)

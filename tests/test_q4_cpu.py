@@ -97,5 +97,11 @@ def test_host_tensors_wrong_types_and_sizes_are_refused():
         with pytest.raises(DzError) as e:
             engine._tensor("x", bad, torch.float32, 4)
         assert e.value.status == DZ_EINVAL
+    for name, bad in (("too many", [1, 2]), ("not whole", [1.5]), ("too large", [1 << 63]), ("no number", ["a"])):
+        with pytest.raises(DzError) as e:
+            engine._per_seq(name, bad, engine._ids([0]))
+        assert e.value.status == DZ_EINVAL
     with pytest.raises(DzError):
-        engine._per_seq("count", [1, 2], engine._ids([0]))
+        engine._ids([1 << 31])
+    assert list(engine._ids(np.array([3, 1]))) == [3, 1] and list(engine._ids(2)) == [2]
+    assert list(engine._per_seq("count", (4, 5), engine._ids([0, 1]))) == [4, 5]
