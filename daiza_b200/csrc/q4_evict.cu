@@ -5,8 +5,9 @@
 //
 // One kernel, a cluster of CTAs per (sequence, kv head):
 //   1. the weight of the last entry that stays: radix selection over the weights as ordered
-//      32-bit keys, 11 + 11 + 10 bits, histograms per CTA, summed over the cluster through
-//      distributed shared memory;
+//      32-bit keys, 11 + 11 + 10 bits, a histogram per CTA, which every CTA reads from all
+//      (distributed shared memory, 16 bytes at a time; adding them up by remote atomics
+//      took 45 ns an instruction);
 //   2. the indices that stay: each CTA counts its stretch of entries, prefix sums over the
 //      cluster, then writes its part of the list in order;
 //   3. the rows move, 16 positions a warp at a time: a round of destination tiles is built
@@ -23,8 +24,8 @@ namespace dz {
 namespace q4 {
 
 constexpr int EV_CTAS = 8, EV_THREADS = 512, EV_WARPS = EV_THREADS / 32;
-constexpr int EV_TILES = 2;                      // tiles that a warp builds in a round
-constexpr int EV_PER = 4;                        // consecutive entries of a thread in step 2
+constexpr int EV_PER = 8;                        // consecutive entries of a thread
+constexpr int EV_BATCH = EV_PER * EV_THREADS;    // entries that a CTA looks at at a time
 
 struct Evict {
     int B, kvc;
@@ -33,13 +34,19 @@ struct Evict {
     int64_t out[MAXB];                           // first index of the sequence in the list
 };
 
-struct EvictSmem {
-    uint8_t tile[EV_WARPS * EV_TILES][Q4_TILE_BYTES];
-    float wts[EV_WARPS * EV_TILES][Q4_TILE];
-    uint32_t hist[3][2048];
+struct alignas(16) EvictSmem {
+    union {
+        struct {                                 // step 3: one tile per warp
+            uint8_t tile[EV_WARPS][Q4_TILE_BYTES];
+            float wts[EV_WARPS][Q4_TILE];
+        };
+        struct {                                 // step 1
+            uint32_t hist[3][2048];
+        };
+    };
     uint32_t scan[EV_WARPS], scan2[EV_WARPS];
     uint32_t found[2];                           // bin, entries above it
-    uint32_t count[2];                           // this CTA's entries above the threshold, and at it
+    alignas(8) uint32_t count[2];                // this CTA's entries above the threshold, and at it
 };
 
 // Weights in order as unsigned keys; NaN lowest, -0 as 0.
@@ -52,11 +59,20 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// a word of the same shared-memory place in CTA `rank` of the cluster
-__device__ __forceinline__ uint32_t peer_word(const uint32_t* p, uint32_t rank) {
-    uint32_t a, v;
+// 16 or 8 bytes of the same shared-memory place in CTA `rank` of the cluster
+__device__ __forceinline__ uint4 peer_16(const uint32_t* p, uint32_t rank) {
+    uint32_t a;
+    uint4 v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 peer_8(const uint32_t* p, uint32_t rank) {
+    uint32_t a;
+    uint2 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
     return v;
 }
 
@@ -134,7 +150,7 @@ __device__ __forceinline__ void build_tile(uint8_t* out, float* wts_out, const Q
     *reinterpret_cast<uint32_t*>(out + OFF_VS + lane * 4) = scales;
 }
 
-__global__ void __cluster_dims__(EV_CTAS, 1, 1) __launch_bounds__(EV_THREADS, 1)
+__global__ void __cluster_dims__(EV_CTAS, 1, 1) __launch_bounds__(EV_THREADS, 2)
     q4_evict_kernel(const __grid_constant__ Evict d, const Q4Slot* __restrict__ slots, int32_t* list,
                     int32_t* __restrict__ kept) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -147,45 +163,63 @@ __global__ void __cluster_dims__(EV_CTAS, 1, 1) __launch_bounds__(EV_THREADS, 1)
     const float* wts = src.wts + (size_t)kvh * src.cap;
     list += d.out[b] * d.kvc + (int64_t)kvh * keep;
     if (kept) kept += d.out[b] * d.kvc + (int64_t)kvh * keep;
-    const int per = ((old + EV_CTAS - 1) / EV_CTAS + EV_PER - 1) / EV_PER * EV_PER;
-    const int lo = min(old, rank * per), hi = min(old, lo + per);
+    // this CTA's stretch, in batches of EV_BATCH; a stretch of one batch stays in registers
+    const int per = (int)(((int64_t)old + EV_CTAS - 1) / EV_CTAS);
+    const int lo = (int)min((int64_t)old, (int64_t)rank * per), hi = (int)min((int64_t)old, (int64_t)lo + per);
+    const bool select = need > 0 && need < old;                // the same for the whole cluster
+    uint32_t key[EV_PER];
+    auto load = [&](int at) {
+#pragma unroll
+        for (int i = 0; i < EV_PER; ++i) {
+            const int j = at + EV_PER * tid + i;
+            key[i] = j < hi ? weight_key(wts[j]) : 0u;
+        }
+    };
+    const bool one = hi - lo <= EV_BATCH;
+    if (select && one) load(lo);
 
     // ---- 1. threshold: entries with a larger key stay, and the first `ties` with this key
     uint32_t threshold = 0, ties = 0;
-    const bool select = need > 0 && need < old;                // the same for the whole cluster
     if (select) {
         for (int i = tid; i < 3 * 2048; i += EV_THREADS) (&sm.hist[0][0])[i] = 0;
         __syncthreads();
         uint32_t prefix = 0, left = (uint32_t)need;            // key bits found so far; entries still to find below them
-#pragma unroll
+#pragma unroll 1
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048;
-            for (int j = lo + tid; j < hi; j += EV_THREADS) {
-                const uint32_t k = weight_key(wts[j]);
-                const bool in = pass == 0 || (k >> (pass == 1 ? 21 : 10)) == prefix;
-                if (in) atomicAdd(&sm.hist[pass][(k >> shift) & (bins - 1)], 1u);
+            for (int at = lo; at < hi; at += EV_BATCH) {
+                if (!one) load(at);
+#pragma unroll
+                for (int i = 0; i < EV_PER; ++i) {
+                    const bool in = at + EV_PER * tid + i < hi &&
+                                    (pass == 0 || (key[i] >> (pass == 1 ? 21 : 10)) == prefix);
+                    if (in) atomicAdd(&sm.hist[pass][(key[i] >> shift) & (bins - 1)], 1u);
+                }
             }
             cluster_sync();
             // this thread's 4 bins, from the highest bin down, over the cluster
-            uint32_t c[4] = {}, sum = 0;
+            uint32_t c[4] = {};
             const int top = bins - 1 - 4 * tid;
             if (top >= 0) {
+                uint4 v[EV_CTAS];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    for (int q = 0; q < EV_CTAS; ++q) c[i] += peer_word(&sm.hist[pass][top - i], q);
-                    sum += c[i];
+                for (int q = 0; q < EV_CTAS; ++q) v[q] = peer_16(&sm.hist[pass][top - 3], q);
+#pragma unroll
+                for (int q = 0; q < EV_CTAS; ++q) {
+                    c[0] += v[q].w;
+                    c[1] += v[q].z;
+                    c[2] += v[q].y;
+                    c[3] += v[q].x;
                 }
             }
-            uint32_t total, above = block_scan(sum, sm.scan, total);
-            if (top >= 0) {
+            uint32_t total, above = block_scan(c[0] + c[1] + c[2] + c[3], sm.scan, total);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (above < left && left <= above + c[i]) {
-                        sm.found[0] = (uint32_t)(top - i);
-                        sm.found[1] = above;
-                    }
-                    above += c[i];
+            for (int i = 0; i < 4; ++i) {
+                if (above < left && left <= above + c[i]) {
+                    sm.found[0] = (uint32_t)(top - i);
+                    sm.found[1] = above;
                 }
+                above += c[i];
             }
             __syncthreads();
             prefix = prefix << (pass == 2 ? 10 : 11) | sm.found[0];
@@ -199,10 +233,14 @@ __global__ void __cluster_dims__(EV_CTAS, 1, 1) __launch_bounds__(EV_THREADS, 1)
     // ---- 2. the list of entries that stay
     if (select) {
         uint32_t gt = 0, eq = 0;
-        for (int j = lo + tid; j < hi; j += EV_THREADS) {
-            const uint32_t k = weight_key(wts[j]);
-            gt += k > threshold;
-            eq += k == threshold;
+        for (int at = lo; at < hi; at += EV_BATCH) {
+            if (!one) load(at);
+#pragma unroll
+            for (int i = 0; i < EV_PER; ++i)
+                if (at + EV_PER * tid + i < hi) {
+                    gt += key[i] > threshold;
+                    eq += key[i] == threshold;
+                }
         }
         uint32_t all_gt, all_eq;
         block_scan(gt, sm.scan, all_gt);
@@ -212,39 +250,36 @@ __global__ void __cluster_dims__(EV_CTAS, 1, 1) __launch_bounds__(EV_THREADS, 1)
             sm.count[1] = all_eq;
         }
         cluster_sync();
-        uint32_t gt_before = 0, eq_before = 0;
-        for (int q = 0; q < rank; ++q) {
-            gt_before += peer_word(&sm.count[0], q);
-            eq_before += peer_word(&sm.count[1], q);
-        }
-        uint32_t at = gt_before + min(eq_before, ties);
-        for (int j0 = lo; j0 < hi; j0 += EV_PER * EV_THREADS) {
-            uint32_t g = 0, e = 0;
-            uint32_t is[EV_PER];
-            const int first = j0 + EV_PER * tid;
-#pragma unroll
-            for (int i = 0; i < EV_PER; ++i) {
-                const int j = first + i;
-                const uint32_t k = j < hi ? weight_key(wts[j]) : 0u;
-                is[i] = j >= hi ? 0u : (k > threshold ? 1u : (k == threshold ? 2u : 0u));
-                e += is[i] == 2u;
-            }
-            uint32_t chunk_eq, eq_at = block_scan(e, sm.scan, chunk_eq) + eq_before;
-#pragma unroll
-            for (int i = 0; i < EV_PER; ++i) {
-                if (is[i] == 2u && eq_at++ >= ties) is[i] = 0u;
-                g += is[i] != 0u;
-            }
-            uint32_t chunk, to = block_scan(g, sm.scan2, chunk) + at;
+        // the CTAs before this one: lane q reads CTA q's counts
+        const uint2 theirs = lane < EV_CTAS ? peer_8(sm.count, lane) : make_uint2(0u, 0u);
+        const uint32_t gt_before = __reduce_add_sync(0xffffffffu, lane < rank ? theirs.x : 0u);
+        uint32_t eq_before = __reduce_add_sync(0xffffffffu, lane < rank ? theirs.y : 0u);
+        uint32_t to0 = gt_before + min(eq_before, ties);
+        for (int at = lo; at < hi; at += EV_BATCH) {
+            if (!one) load(at);
+            uint32_t e = 0, stays = 0, at_threshold = 0;       // bit i: entry i
 #pragma unroll
             for (int i = 0; i < EV_PER; ++i)
-                if (is[i]) {
-                    list[to] = first + i;
-                    if (kept) kept[to] = first + i;
+                if (at + EV_PER * tid + i < hi) {
+                    stays |= (uint32_t)(key[i] > threshold) << i;
+                    at_threshold |= (uint32_t)(key[i] == threshold) << i;
+                }
+            e = __popc(at_threshold);
+            uint32_t batch_eq, eq_at = block_scan(e, sm.scan, batch_eq) + eq_before;
+#pragma unroll
+            for (int i = 0; i < EV_PER; ++i)
+                if (at_threshold >> i & 1u) stays |= (uint32_t)(eq_at++ < ties) << i;
+            uint32_t batch, to = block_scan(__popc(stays), sm.scan2, batch) + to0;
+#pragma unroll
+            for (int i = 0; i < EV_PER; ++i)
+                if (stays >> i & 1u) {
+                    const int j = at + EV_PER * tid + i;
+                    list[to] = j;
+                    if (kept) kept[to] = j;
                     ++to;
                 }
-            eq_before += chunk_eq;
-            at += chunk;
+            eq_before += batch_eq;
+            to0 += batch;
         }
     } else if (need > 0) {                                     // nothing leaves
         for (int j = lo + tid; j < hi; j += EV_THREADS) {
@@ -261,29 +296,20 @@ __global__ void __cluster_dims__(EV_CTAS, 1, 1) __launch_bounds__(EV_THREADS, 1)
     // ---- 3. the rows move
     if (d.src[b] == d.dst[b] && keep == n) return;             // nothing leaves: already in place (the whole cluster)
     const int tiles = (keep + Q4_TILE - 1) / Q4_TILE;
-    constexpr int ROUND = EV_CTAS * EV_WARPS * EV_TILES;
-    for (int t0 = 0; t0 < tiles; t0 += ROUND) {
-        const int w0 = (warp * EV_CTAS + rank) * EV_TILES;     // few tiles: spread over the CTAs first
-#pragma unroll 1
-        for (int k = 0; k < EV_TILES; ++k) {
-            const int t = t0 + w0 + k;
-            if (t < tiles)
-                build_tile(sm.tile[warp * EV_TILES + k], sm.wts[warp * EV_TILES + k], src, kvh, list + (int64_t)t * Q4_TILE,
-                           min(Q4_TILE, keep - t * Q4_TILE), lane);
-        }
+    for (int t0 = 0; t0 < tiles; t0 += EV_CTAS * EV_WARPS) {
+        const int t = t0 + warp * EV_CTAS + rank;              // few tiles: spread over the CTAs first
+        if (t < tiles)
+            build_tile(sm.tile[warp], sm.wts[warp], src, kvh, list + (int64_t)t * Q4_TILE,
+                       min(Q4_TILE, keep - t * Q4_TILE), lane);
         cluster_sync();                                        // every source of this round has been read
-#pragma unroll 1
-        for (int k = 0; k < EV_TILES; ++k) {
-            const int t = t0 + w0 + k;
-            if (t < tiles) {
-                const uint4* from = reinterpret_cast<const uint4*>(sm.tile[warp * EV_TILES + k]);
-                uint4* to = reinterpret_cast<uint4*>(dst.tile(kvh, t));
-                for (int i = lane; i < Q4_TILE_BYTES / 16; i += 32) to[i] = from[i];
-                const int j = t * Q4_TILE + lane;
-                if (lane < Q4_TILE && j < keep) dst.wts[(size_t)kvh * dst.cap + j] = sm.wts[warp * EV_TILES + k][lane];
-            }
+        if (t < tiles) {
+            const uint4* from = reinterpret_cast<const uint4*>(sm.tile[warp]);
+            uint4* to = reinterpret_cast<uint4*>(dst.tile(kvh, t));
+            for (int i = lane; i < Q4_TILE_BYTES / 16; i += 32) to[i] = from[i];
+            const int j = t * Q4_TILE + lane;
+            if (lane < Q4_TILE && j < keep) dst.wts[(size_t)kvh * dst.cap + j] = sm.wts[warp][lane];
         }
-        __syncwarp();                                          // the warp's staging tiles are free again
+        __syncwarp();                                          // the warp's staging tile is free again
     }
 }
 
