@@ -23,9 +23,11 @@
 // reads a tile with 16-byte loads and no shuffles.  With r = lane / 4, c = lane % 4:
 //   K codes  [pos / 8][i 0..1][lane (r = pos % 8)][4 words]: word w = 4 i + j holds
 //            dims 64 c + 8 w .. + 7 of that position, dim e at bit (e & 1) * 16 + (e >> 1) * 4
-//   V codes  [i 0..3][lane][4 words]: word m = 4 i + j holds dims 32 r + 2 m (A) and
+//   V codes  [i 0..3][c][(r + 2 c) % 8][4 words]: word m = 4 i + j holds dims 32 r + 2 m (A) and
 //            32 r + 2 m + 1 (B) at positions 2c, 2c+1, 2c+8, 2c+9: position 2c + u + 8 w
-//            at bit u * 16 + w * 4, dim B 8 bits above dim A
+//            at bit u * 16 + w * 4, dim B 8 bits above dim A.  A position lies in four
+//            lines of 128 bytes (its c); the rotation by 2 c keeps a warp's 16-byte loads
+//            free of bank conflicts.
 //   K scales [lane][4]: (pos r, group 2c), (r, 2c+1), (r + 8, 2c), (r + 8, 2c+1)
 //   V scales [lane][4]: group r at positions 2c, 2c+1, 2c+8, 2c+9
 // Codes are stored as code + 8.  Unwritten positions hold finite scales always
@@ -257,9 +259,11 @@ __device__ __forceinline__ void put_k(uint8_t* tile, int p, int lane, const uint
     const int g = lane >> 2;
     if ((lane & 3) == 0) tile[OFF_KS + (n * 4 + (g >> 1)) * 4 + (p >> 3) * 2 + (g & 1)] = (uint8_t)sb;
 }
+// Byte offset of V's words 4 i .. 4 i + 3 of (r, c).
+__device__ __forceinline__ int v_at(int i, int r, int c) { return OFF_V + i * 512 + c * 128 + ((r + 2 * c) & 7) * 16; }
 // The four V words of lane l's dims at column c: group r = l / 4, words 4 (l % 4) .. + 3.
 __device__ __forceinline__ uint4* v_words(uint8_t* tile, int lane, int c) {
-    return reinterpret_cast<uint4*>(tile + OFF_V + (lane & 3) * 512 + ((lane >> 2) * 4 + c) * 16);
+    return reinterpret_cast<uint4*>(tile + v_at(lane & 3, lane >> 2, c));
 }
 // The same words with position p's nibbles replaced by the codes.
 __device__ __forceinline__ void merge_v(uint4& w, int p, const uint32_t (&code)[8]) {
@@ -285,7 +289,7 @@ struct TileMerge {
     }
     // position p's codes, by one warp
     __device__ __forceinline__ void add(int p, int lane, const uint32_t (&c)[8]) {
-        const int at = (lane & 3) * 128 + ((lane >> 2) * 4 + ((p & 7) >> 1)) * 4, sh = (p & 1) * 16 + (p >> 3) * 4;
+        const int at = (v_at(lane & 3, lane >> 2, (p & 7) >> 1) - OFF_V) / 4, sh = (p & 1) * 16 + (p >> 3) * 4;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             atomicOr(&code[at + i], (c[2 * i] | c[2 * i + 1] << 8) << sh);
@@ -315,7 +319,7 @@ __device__ __forceinline__ void get_k(const uint8_t* tile, int p, int lane, uint
 }
 __device__ __forceinline__ void get_v(const uint8_t* tile, int p, int lane, uint32_t (&h)[4]) {
     const int c = (p & 7) >> 1;
-    const uint4 w = *reinterpret_cast<const uint4*>(tile + OFF_V + (lane & 3) * 512 + ((lane >> 2) * 4 + c) * 16);
+    const uint4 w = *reinterpret_cast<const uint4*>(tile + v_at(lane & 3, lane >> 2, c));
     const uint32_t b = tile[OFF_VS + ((lane >> 2) * 4 + c) * 4 + (p & 1) + (p >> 3) * 2];
     const uint32_t s = scale_pair(b | b << 16), k = hmul2_u(s, NEG72);
     const int sh = (p & 1) * 16 + (p >> 3) * 4;

@@ -312,7 +312,7 @@ __device__ __forceinline__ void attend(State& st, const uint8_t* tiles, const ui
         float d[4][4];
 #pragma unroll
         for (int k = 0; k < NT; ++k) {
-            const uint4 w4 = *reinterpret_cast<const uint4*>(tiles + k * Q4_TILE_BYTES + OFF_V + i * 512 + lane * 16);
+            const uint4 w4 = *reinterpret_cast<const uint4*>(tiles + k * Q4_TILE_BYTES + v_at(i, r, c));
             const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
             for (int u = 0; u < 4; ++u) {

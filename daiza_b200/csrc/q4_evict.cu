@@ -23,7 +23,7 @@
 namespace dz {
 namespace q4 {
 
-constexpr int EV_CTAS = 8, EV_THREADS = 512, EV_WARPS = EV_THREADS / 32;
+constexpr int EV_THREADS = 512, EV_WARPS = EV_THREADS / 32;
 constexpr int EV_PER = 8;                        // consecutive entries of a thread
 constexpr int EV_BATCH = EV_PER * EV_THREADS;    // entries that a CTA looks at at a time
 
@@ -134,11 +134,11 @@ __device__ __forceinline__ void build_tile(uint8_t* out, float* wts_out, const Q
         const int32_t s = __shfl_sync(0xffffffffu, mine, 2 * c + u + 8 * hi);
         if (s < 0) continue;
         const uint8_t* tile = slot.tile(kvh, s >> 4);
-        const int from = r * 4 + ((s & 7) >> 1), sh = (s & 1) * 16 + ((s >> 3) & 1) * 4, to = u * 16 + hi * 4;
-        scales |= (uint32_t)tile[OFF_VS + from * 4 + (s & 1) + ((s >> 3) & 1) * 2] << (8 * q);
+        const int c_from = (s & 7) >> 1, sh = (s & 1) * 16 + ((s >> 3) & 1) * 4, to = u * 16 + hi * 4;
+        scales |= (uint32_t)tile[OFF_VS + (r * 4 + c_from) * 4 + (s & 1) + ((s >> 3) & 1) * 2] << (8 * q);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint4 x = *reinterpret_cast<const uint4*>(tile + OFF_V + i * 512 + from * 16);
+            const uint4 x = *reinterpret_cast<const uint4*>(tile + v_at(i, r, c_from));
             w[i].x |= ((x.x >> sh) & 0x0F0Fu) << to;
             w[i].y |= ((x.y >> sh) & 0x0F0Fu) << to;
             w[i].z |= ((x.z >> sh) & 0x0F0Fu) << to;
@@ -146,11 +146,13 @@ __device__ __forceinline__ void build_tile(uint8_t* out, float* wts_out, const Q
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(out + OFF_V + i * 512 + lane * 16) = w[i];
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(out + v_at(i, r, c)) = w[i];
     *reinterpret_cast<uint32_t*>(out + OFF_VS + lane * 4) = scales;
 }
 
-__global__ void __cluster_dims__(EV_CTAS, 1, 1) __launch_bounds__(EV_THREADS, 2)
+// EV_CTAS: CTAs of a cluster
+template <int EV_CTAS>
+__global__ void __launch_bounds__(EV_THREADS, 2)
     q4_evict_kernel(const __grid_constant__ Evict d, const Q4Slot* __restrict__ slots, int32_t* list,
                     int32_t* __restrict__ kept) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -315,13 +317,30 @@ __global__ void __cluster_dims__(EV_CTAS, 1, 1) __launch_bounds__(EV_THREADS, 2)
 
 }  // namespace q4
 
+template <int CTAS>
+static cudaError_t launch_evict(const q4::Evict& d, const Q4Slot* slots, int32_t* list, int32_t* kept, cudaStream_t st) {
+    cudaError_t e = cudaFuncSetAttribute(q4::q4_evict_kernel<CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)sizeof(q4::EvictSmem));
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = CTAS;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t lc{};
+    lc.gridDim = dim3(d.B * d.kvc * CTAS);
+    lc.blockDim = dim3(q4::EV_THREADS);
+    lc.dynamicSmemBytes = sizeof(q4::EvictSmem);
+    lc.stream = st;
+    lc.attrs = at;
+    lc.numAttrs = 1;
+    return cudaLaunchKernelEx(&lc, q4::q4_evict_kernel<CTAS>, d, slots, list, kept);
+}
+
 cudaError_t launch_q4_evict(dz_ctx* ctx, int layer, int B, const int32_t* src, const int32_t* dst, const int64_t* keep,
                             const int64_t* recent, int32_t* kept, cudaStream_t st, int* n_launch) {
     const LayerState& L = ctx->layers[layer];
     const int kvc = ctx->cfg.kv_head_count;
-    cudaError_t e = cudaFuncSetAttribute(q4::q4_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)sizeof(q4::EvictSmem));
-    if (e != cudaSuccess) return e;
+    cudaError_t e;
     int64_t rows = 0;
     for (int b = 0; b < B; ++b) rows += std::min<int64_t>(keep[b], L.len[src[b]]);
     if ((e = ensure_q4_scratch(ctx, std::max<int64_t>(rows, 1) * kvc * sizeof(int32_t))) != cudaSuccess) return e;
@@ -340,9 +359,13 @@ cudaError_t launch_q4_evict(dz_ctx* ctx, int layer, int B, const int32_t* src, c
             d.out[b] = at;
             at += k;
         }
-        q4::q4_evict_kernel<<<d.B * kvc * q4::EV_CTAS, q4::EV_THREADS, sizeof(q4::EvictSmem), st>>>(
-            d, L.d_q4, static_cast<int32_t*>(ctx->q4_scratch), kept);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        // as many CTAs per (sequence, kv head) as fit the GPU at once, two per SM
+        const int pairs = d.B * kvc;
+        int32_t* list = static_cast<int32_t*>(ctx->q4_scratch);
+        e = pairs * 8 <= 2 * ctx->n_sm   ? launch_evict<8>(d, L.d_q4, list, kept, st)
+            : pairs * 4 <= 2 * ctx->n_sm ? launch_evict<4>(d, L.d_q4, list, kept, st)
+                                         : launch_evict<2>(d, L.d_q4, list, kept, st);
+        if (e != cudaSuccess) return e;
         *n_launch += 1;
     }
     return cudaSuccess;
