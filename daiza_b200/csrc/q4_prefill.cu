@@ -12,10 +12,15 @@
 //                   and new, as f16 [kv head][key][256] -- exact -- each sequence padded with
 //                   zeros to whole blocks of 128 keys, so that a block never meets another
 //                   sequence's values.  Blocks of three kinds, all independent.
-//   2. pf_attn    : (pf_attn.cuh) tcgen05 attention, f16 operands: K and V are exact, Q and P
-//                   are rounded to 11 bits (bf16's 8 would cost the output's last bits).
-#include "pf_attn.cuh"
+//   2. q4_pf_attn : causal flash attention on tcgen05, f16 operands (K and V are exact, Q and P
+//                   rounded to 11 bits; bf16's 8 would cost the output's last bits), two
+//                   heads of a group to a CTA pair.
+#include <cuda.h>
+#include <algorithm>
+#include <cstddef>
+
 #include "q4.cuh"
+#include "tc_common.cuh"
 
 namespace dz {
 namespace q4 {
@@ -42,6 +47,10 @@ __device__ __forceinline__ int last_at_or_before(const int32_t* start, int n, in
     return lo;
 }
 
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);   // a in the low half
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
 template <typename T>
 __device__ __forceinline__ void load_row(const T* p, double (&x)[8]) {
     const float4 a = as_f32(load4(p)), b = as_f32(load4(p + 4));
@@ -156,33 +165,437 @@ __global__ void __launch_bounds__(32 * PREP_WARPS)
         norm_rotate_split(x, w, c4, eps, lane);
         __half* out = qf + ((size_t)(h0 + i) * tokens + row) * HD;
         *reinterpret_cast<uint2*>(out + split_dim(lane, 0)) =
-            make_uint2(pf::pack2<__half>(x[0], x[1]), pf::pack2<__half>(x[2], x[3]));
+            make_uint2(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]));
         *reinterpret_cast<uint2*>(out + split_dim(lane, 1)) =
-            make_uint2(pf::pack2<__half>(x[4], x[5]), pf::pack2<__half>(x[6], x[7]));
+            make_uint2(pack_f16(x[4], x[5]), pack_f16(x[6], x[7]));
     }
 }
 
-}  // namespace q4
+// ---------------------------------------------------------------------------
+// Attention.  A cluster of two CTAs takes a query tile of 128 tokens of two q heads of one
+// group, a head each, with tcgen05.mma.cta_group::2: M = 256 rows, each CTA's 128 in its own
+// TMEM, and every K and V block fetched once for both, half by each CTA.  (One CTA per
+// tile had to take in 128 KB per block of 128 keys, about 2000 cycles at an SM's 64
+// bytes a cycle, beside 2100 cycles of products: 3300 cycles a block.)
+//   warps 0-7  softmax: thread = (query row, half of a block's 128 keys); scores in log2
+//              units, running max rescaled lazily (only when it grows by more than 2^8), P
+//              as f16 over its S columns, finally O / l * sigmoid(gate)
+//   warp 8     TMA of Q and of this CTA's 64 keys of each K block (slots of 64 dims)
+//   warp 9     (first CTA) issues S = Q K^T (N = 128, K = 256) into one of two TMEM buffers
+//              and O += P V (N = 256, K = 128, P from TMEM)
+//   warp 10    TMA of this CTA's 128 dims of each V block (slots of 32 keys)
+// The first CTA's barriers count both CTAs' bytes and arrivals; the products' completion
+// goes to both.  Every wait is bounded; a CTA that gave one up still meets its barriers.
+// ---------------------------------------------------------------------------
+namespace attn {
+using namespace tc;
 
-namespace pf {
+constexpr int BM = 128, BN = 128;                // query rows of a CTA, keys of a block
+constexpr int NK = 10, NV = 9;                   // ring slots of 8 KB (a block is 4 of each)
+constexpr int NTHREADS = 352;
+__host__ __device__ constexpr uint32_t S_COL(int st) { return 128u * (uint32_t)st; }
+constexpr uint32_t O_COL = 256;
+constexpr float RESCALE_THRESHOLD = 8.0f;        // log2 units: P stays below 2^8, far inside f16
+
+struct alignas(1024) Smem {
+    uint16_t q[4][BM][64];                       // 4 boxes of 64 dims, 16 KB each
+    uint16_t k[NK][BN / 2][64];
+    uint16_t v[NV][2][32][64];
+    uint64_t q_full;
+    uint64_t k_full[NK], k_empty[NK], v_full[NV], v_empty[NV];
+    uint64_t s_full[2], p_full[2], pv_done[2];
+    float red_max[2][2][BM];                     // [block parity][key half][row] partial row maxima
+    float red_l[2][BM];                          // [key half][row] partial row sums
+    uint32_t tmem_base;
+};
+static_assert(offsetof(Smem, k) % 1024 == 0 && offsetof(Smem, v) % 1024 == 0, "swizzle atoms need 1 KB alignment");
+
+// ---- the pair's forms of the PTX wrappers ------------------------------------------
+__device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+// a load into this CTA, counted on a barrier of the pair (a shared::cluster address)
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+        "[%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+__device__ __forceinline__ void alloc(uint32_t* dst, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void dealloc(uint32_t taddr, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+// Issued by the one lane whose `go` is set, in code that its whole warp runs: the operands
+// then stay in uniform registers (issued under `if (lane == 0)` an instruction took about
+// 100 cycles, more than the product itself).
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t go;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(go));
+    return go;
+}
+// the issued products' completion, to this barrier of both CTAs
+__device__ __forceinline__ void commit(uint32_t go, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t.reg .b16 m;\n\tsetp.ne.b32 q, %1, 0;\n\tmov.b16 m, 3;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}"
+        ::"r"(bar), "r"(go) : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t go, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(go) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t go, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(go) : "memory");
+}
+// f16 A and B, f32 accumulator; B optionally MN-major
+constexpr uint32_t idesc(int M, int N, bool b_mn_major) {
+    return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+// What crosses CTAs under these barriers is TMEM and TMA data, ordered by tcgen05 fences and
+// by the copies' own completion: a release or acquire at cluster scope would only add
+// memory barriers (they cost a tenth of the kernel).
+__device__ __forceinline__ void arrive_at(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* err, bool& ok) {
+    return wait_or_flag(bar, parity, err, ok);
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void f2_split(uint64_t r, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t sub_f2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ void store4(float* p, float4 x) { *reinterpret_cast<float4*>(p) = x; }
+__device__ __forceinline__ void store4(__nv_bfloat16* p, float4 x) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
+    *reinterpret_cast<uint2*>(p) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+// One query tile: rows [q0, q0 + 128) of a sequence of T new tokens behind `base` keys.  row:
+// the tile's first row in the Q map, q_gate and out; key: the sequence's first row in K and V.
+struct Tile { int64_t q0, T, base, row, key; };
 // Packed sequences, those with the most keys first and their latest query tiles first: the
-// heaviest tiles start first.
+// heaviest tiles start first.  A context owns the tiles t % split_cnt == split_idx.
 struct Packed {
     int n, split_idx, split_cnt;
     int32_t first[MAXB + 1];                     // query tiles before the i-th sequence of this order
     int32_t T[MAXB], base[MAXB], row[MAXB], key[MAXB];
-    __host__ __device__ static int own_tiles(int64_t T, int idx, int cnt) {
+    static int own_tiles(int64_t T, int idx, int cnt) {
         const int n_qt = (int)((T + BM - 1) / BM);
         return n_qt > idx ? (n_qt - 1 - idx) / cnt + 1 : 0;
     }
     __device__ __forceinline__ Tile tile(int i) const {
-        const int s = q4::last_at_or_before(first, n, i);
+        const int s = last_at_or_before(first, n, i);
         const int own = first[s + 1] - first[s];
         const int64_t q0 = (int64_t)(split_idx + split_cnt * (own - 1 - (i - first[s]))) * BM;
         return {q0, T[s], base[s], row[s] + q0, key[s]};
     }
 };
-}  // namespace pf
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
+    q4_pf_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Packed map, int kvc,
+                      const T* __restrict__ q_gate, T* __restrict__ out, int* err) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    // dynamic shared memory is only 16-byte aligned: round up to 1 KB (the same place in both CTAs)
+    Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int nq = GRP * kvc, pairs = nq / 2, rank = blockIdx.x & 1;
+    const Tile tl = map.tile((int)(blockIdx.x / 2 / pairs));
+    const int qh = 2 * (int)(blockIdx.x / 2 % pairs) + rank, kvh = qh / GRP;
+    const int64_t q_last = min(tl.q0 + BM, tl.T) - 1;                  // last valid query row of the sequence
+    const int nblk = (int)((tl.base + q_last) / BN) + 1;               // key blocks that touch the causal range
+
+    if (tid == 0) {
+        mbar_init(&sm.q_full, 1);
+        for (int i = 0; i < NK; ++i) {
+            mbar_init(&sm.k_full[i], 1);
+            mbar_init(&sm.k_empty[i], 1);
+        }
+        for (int i = 0; i < NV; ++i) {
+            mbar_init(&sm.v_full[i], 1);
+            mbar_init(&sm.v_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sm.s_full[i], 1);
+            mbar_init(&sm.p_full[i], 16);                              // the softmax warps of both CTAs
+            mbar_init(&sm.pv_done[i], 1);
+        }
+        fence_mbar_init();
+    }
+    if (warp == 0) alloc(&sm.tmem_base, 512);
+    fence_before_sync();
+    __syncthreads();
+    cluster_sync();
+    fence_after_sync();
+    const uint32_t tmem = sm.tmem_base;
+    bool ok = true;
+
+    if (warp == 8) {
+        // ---------------- TMA of Q and K ----------------
+        if (lane == 0) {
+            if (rank == 0) mbar_arrive_expect_tx(&sm.q_full, 2 * BM * HD * 2);
+            const uint32_t qb = peer_addr(&sm.q_full, 0);
+            for (int b = 0; b < 4; ++b) tma_load(&sm.q[b][0][0], &tm_q, 64 * b, (int)tl.row, qh, qb);
+            for (int idx = 0; idx < 4 * nblk && ok; ++idx) {
+                const int slot = idx % NK, j = idx >> 2, b = idx & 3;
+                if (idx >= NK && !wait(&sm.k_empty[slot], ((idx / NK) - 1) & 1, err, ok)) break;
+                if (rank == 0) mbar_arrive_expect_tx(&sm.k_full[slot], BN * 64 * 2);
+                tma_load(&sm.k[slot][0][0], &tm_k, 64 * b, (int)tl.key + j * BN + rank * (BN / 2), kvh,
+                         peer_addr(&sm.k_full[slot], 0));
+            }
+        }
+    } else if (warp == 10) {
+        // ---------------- TMA of V ----------------
+        if (lane == 0) {
+            for (int idx = 0; idx < 4 * nblk && ok; ++idx) {
+                const int slot = idx % NV, j = idx >> 2, kg = idx & 3;
+                if (idx >= NV && !wait(&sm.v_empty[slot], ((idx / NV) - 1) & 1, err, ok)) break;
+                if (rank == 0) mbar_arrive_expect_tx(&sm.v_full[slot], 32 * HD * 2);
+                for (int d = 0; d < 2; ++d)
+                    tma_load(&sm.v[slot][d][0][0], &tm_v, 128 * rank + 64 * d, (int)tl.key + j * BN + 32 * kg, kvh,
+                             peer_addr(&sm.v_full[slot], 0));
+            }
+        }
+    } else if (warp == 9) {
+        // ---------------- products (first CTA; the whole warp, one lane issues) ----------------
+        if (rank == 0) {
+            constexpr uint32_t ID_QK = idesc(2 * BM, BN, false), ID_PV = idesc(2 * BM, HD, true);
+            // matrix descriptors count 16 bytes in their low bits: offsets are added
+            const uint64_t q_d = sw128_desc(smem_u32(&sm.q[0][0][0]), 16, 1024);
+            const uint64_t k_d = sw128_desc(smem_u32(&sm.k[0][0][0]), 16, 1024);
+            // V: [16 keys][dims], MN-major: 64-dim boxes 4 KB apart (LBO), 8-key swizzle atoms 1 KB apart (SBO)
+            const uint64_t v_d = sw128_desc(smem_u32(&sm.v[0][0][0][0]), 32 * 128, 1024);
+            const uint32_t k_empty = smem_u32(&sm.k_empty[0]), v_empty = smem_u32(&sm.v_empty[0]);
+            const uint32_t go = elect_one();
+            int k_slot = 0, v_slot = 0;
+            uint32_t k_phase = 0, v_phase = 0;
+            auto issue_s = [&](int st) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    if (!wait(&sm.k_full[k_slot], k_phase, err, ok)) return;
+                    fence_after_sync();
+                    const uint64_t kd = k_d + (uint64_t)(uint32_t)(k_slot * (BN / 2 * 128 / 16));
+#pragma unroll
+                    for (int s4 = 0; s4 < 4; ++s4)
+                        mma_ss(go, tmem + S_COL(st), q_d + (uint32_t)(b * (BM * 128 / 16) + s4 * 2), kd + (uint32_t)(s4 * 2),
+                               ID_QK, (b > 0 || s4 > 0) ? 1u : 0u);
+                    commit(go, k_empty + 8 * k_slot);
+                    if (++k_slot == NK) {
+                        k_slot = 0;
+                        k_phase ^= 1u;
+                    }
+                }
+                commit(go, smem_u32(&sm.s_full[st]));
+            };
+            if (wait(&sm.q_full, 0, err, ok)) {
+                issue_s(0);
+                if (nblk > 1) issue_s(1);
+                for (int j = 0; j < nblk && ok; ++j) {
+                    const int st = j & 1;
+                    if (!wait(&sm.p_full[st], (j >> 1) & 1, err, ok)) break;
+#pragma unroll
+                    for (int kg = 0; kg < 4; ++kg) {
+                        if (!wait(&sm.v_full[v_slot], v_phase, err, ok)) break;
+                        fence_after_sync();
+                        const uint64_t vd = v_d + (uint64_t)(uint32_t)(v_slot * (32 * 128 * 2 / 16));
+#pragma unroll
+                        for (int s2 = 0; s2 < 2; ++s2)         // A = P columns of 16 keys
+                            mma_ts(go, tmem + O_COL, tmem + S_COL(st) + 8 * (2 * kg + s2), vd + (uint32_t)(s2 * 16 * 128 / 16),
+                                   ID_PV, (j > 0 || kg > 0 || s2 > 0) ? 1u : 0u);
+                        commit(go, v_empty + 8 * v_slot);
+                        if (++v_slot == NV) {
+                            v_slot = 0;
+                            v_phase ^= 1u;
+                        }
+                    }
+                    commit(go, smem_u32(&sm.pv_done[st]));
+                    if (j + 2 < nblk) issue_s(st);
+                }
+            }
+        }
+    } else {
+        // ---------------- softmax: 8 warps, thread = (query row, key half) ----------------
+        const int r = 32 * (warp & 3) + lane;                          // TMEM lane = query row
+        const int hf = warp >> 2;                                      // keys [64 hf, 64 hf + 64) of a block
+        const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
+        const int64_t qpos = tl.base + tl.q0 + r;                      // absolute position of this query row
+        const uint32_t p_bar[2] = {peer_addr(&sm.p_full[0], 0), peer_addr(&sm.p_full[1], 0)};
+        float m_run = -INFINITY, l_run = 0.0f;                         // m identical in both halves; l partial per half
+        for (int j = 0; j < nblk; ++j) {
+            const int st = j & 1;
+            if (!wait(&sm.s_full[st], (j >> 1) & 1, err, ok)) break;
+            fence_after_sync();
+            float s[64];
+            {
+                uint32_t raw[64];
+                tmem_ld32_async(tmem + lane_off + S_COL(st) + 64 * hf, raw);
+                tmem_ld32_async(tmem + lane_off + S_COL(st) + 64 * hf + 32, raw + 32);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 64; ++c) s[c] = __uint_as_float(raw[c]);
+            }
+            // causal mask: keys k0 + c with c > lim are in the future (only blocks on the diagonal)
+            const int64_t lim64 = qpos - ((int64_t)j * BN + 64 * hf);
+            if (lim64 < 63) {
+                const int lim = lim64 < -1 ? -1 : (int)lim64;
+#pragma unroll
+                for (int c = 0; c < 64; ++c) s[c] = c > lim ? -INFINITY : s[c];
+            }
+            float mx;
+            {
+                float a0 = s[0], a1 = s[1], a2 = s[2], a3 = s[3];
+#pragma unroll
+                for (int c = 4; c < 60; c += 8) {
+                    a0 = max3f(a0, s[c], s[c + 1]);
+                    a1 = max3f(a1, s[c + 2], s[c + 3]);
+                    a2 = max3f(a2, s[c + 4], s[c + 5]);
+                    a3 = max3f(a3, s[c + 6], s[c + 7]);
+                }
+                a0 = max3f(a0, s[60], s[61]);
+                a1 = max3f(a1, s[62], s[63]);
+                mx = fmaxf(max3f(a0, a1, a2), a3);
+            }
+            sm.red_max[st][hf][r] = mx;
+            named_bar_sync(1, 256);                                    // also: every S read of this block is done
+            mx = fmaxf(mx, sm.red_max[st][hf ^ 1][r]);
+            const float m_new = fmaxf(m_run, mx);
+            if (m_new > m_run + RESCALE_THRESHOLD) {
+                // the running max moved a lot: scale l and this half-row of O
+                const float f = ex2(m_run - m_new);
+                l_run *= f;
+                if (j > 0) {
+                    const int pj = (j - 1) & 1;
+                    if (!wait(&sm.pv_done[pj], ((j - 1) >> 1) & 1, err, ok)) break;
+                    fence_after_sync();
+#pragma unroll 1
+                    for (int c = 128 * hf; c < 128 * hf + 128; c += 32) {
+                        float o[32];
+                        uint32_t ob[32];
+                        tmem_ld32(tmem + lane_off + O_COL + c, o);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) ob[i] = __float_as_uint(o[i] * f);
+                        tmem_st32(tmem + lane_off + O_COL + c, ob);
+                    }
+                }
+                m_run = m_new;
+            }
+            uint32_t pk[32];
+            {
+                const uint64_t mm = f2(m_run, m_run);
+                uint64_t acc0 = f2(0.0f, 0.0f), acc1 = acc0;
+#pragma unroll
+                for (int c = 0; c < 64; c += 4) {
+                    float x0, x1, x2, x3;
+                    f2_split(sub_f2(f2(s[c], s[c + 1]), mm), x0, x1);
+                    f2_split(sub_f2(f2(s[c + 2], s[c + 3]), mm), x2, x3);
+                    const float p0 = ex2(x0), p1 = ex2(x1), p2 = ex2(x2), p3 = ex2(x3);
+                    acc0 = add_f2(acc0, f2(p0, p1));
+                    acc1 = add_f2(acc1, f2(p2, p3));
+                    pk[c / 2] = pack_f16(p0, p1);
+                    pk[c / 2 + 1] = pack_f16(p2, p3);
+                }
+                float u0, u1;
+                f2_split(add_f2(acc0, acc1), u0, u1);
+                l_run += u0 + u1;
+            }
+            // P goes over the first 64 columns of its own S buffer (the previous reader of these
+            // columns, PV(j-2), completed before S(j) did)
+            tmem_st32(tmem + lane_off + S_COL(st) + 32 * hf, pk);
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) arrive_at(p_bar[st]);
+        }
+        // epilogue: O / l * sigmoid(gate); this thread covers dims [128 hf, 128 hf + 128)
+        sm.red_l[hf][r] = l_run;
+        named_bar_sync(1, 256);
+        const float l_tot = l_run + sm.red_l[hf ^ 1][r];
+        if (ok) {
+            const int jl = nblk - 1;
+            if (wait(&sm.pv_done[jl & 1], (jl >> 1) & 1, err, ok)) {
+                fence_after_sync();
+                const int64_t t = tl.row + r;
+                const float inv_l = 1.0f / l_tot;
+#pragma unroll 1
+                for (int c = 128 * hf; c < 128 * hf + 128; c += 32) {
+                    float o[32];
+                    tmem_ld32(tmem + lane_off + O_COL + c, o);
+                    if (tl.q0 + r < tl.T) {
+                        const T* g = q_gate + (t * nq + qh) * QG_ROW + HD + c;
+                        T* dst = out + (t * nq + qh) * HD + c;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 gv = as_f32(load4(g + i));
+                            store4(dst + i, make_float4(o[i + 0] * inv_l * sigmoidf_acc(gv.x),
+                                                        o[i + 1] * inv_l * sigmoidf_acc(gv.y),
+                                                        o[i + 2] * inv_l * sigmoidf_acc(gv.z),
+                                                        o[i + 3] * inv_l * sigmoidf_acc(gv.w)));
+                        }
+                    }
+                }
+            }
+        }
+    }
+    // neither CTA leaves, or frees TMEM, while the other's products or arrivals may touch it
+    fence_before_sync();
+    __syncthreads();
+    cluster_sync();
+    if (warp == 0) dealloc(tmem, 512);
+}
+
+// f16 tensor [d2][d1][256] with a (64 x rows x 1) box, 128-byte swizzle
+static bool make_map(CUtensorMap* m, const void* base, int64_t d1, int64_t d2, int box_rows) {
+    const EncodeTiledFn fn = tensor_map_encoder();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)HD, (cuuint64_t)d1, (cuuint64_t)d2};
+    const cuuint64_t strides[2] = {(cuuint64_t)HD * 2, (cuuint64_t)d1 * HD * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, estr[3] = {1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace attn
+}  // namespace q4
 
 template <typename T>
 static cudaError_t launch_group(dz_ctx* ctx, int layer, const q4::Prompt& d, const int32_t* pos, const T* q_gate,
@@ -196,10 +609,11 @@ static cudaError_t launch_group(dz_ctx* ctx, int layer, const q4::Prompt& d, con
     __half* qf = static_cast<__half*>(ctx->q4_scratch);
     __half *kf = qf + qn, *vf = kf + kn;
     CUtensorMap mq, mk, mv;
-    if (!pf::make_map<__half>(&mq, qf, tokens, nq, pf::BM) || !pf::make_map<__half>(&mk, kf, keys, kvc, pf::BN) ||
-        !pf::make_map<__half>(&mv, vf, keys, kvc, 32))
+    using namespace q4;
+    if (!attn::make_map(&mq, qf, tokens, nq, attn::BM) || !attn::make_map(&mk, kf, keys, kvc, attn::BN / 2) ||
+        !attn::make_map(&mv, vf, keys, kvc, 32))
         return cudaErrorInvalidValue;
-    pf::Packed map;
+    attn::Packed map;
     map.n = d.n;
     map.split_idx = ctx->cfg.qtile_split_index;
     map.split_cnt = ctx->cfg.qtile_split_count;
@@ -216,7 +630,7 @@ static cudaError_t launch_group(dz_ctx* ctx, int layer, const q4::Prompt& d, con
         map.base[i] = d.base[s];
         map.row[i] = d.row0[s];
         map.key[i] = d.key0[s];
-        map.first[i + 1] = map.first[i] + pf::Packed::own_tiles(d.T(s), map.split_idx, map.split_cnt);
+        map.first[i + 1] = map.first[i] + attn::Packed::own_tiles(d.T(s), map.split_idx, map.split_cnt);
     }
     const int64_t q_tasks = tokens * ((nq + q4::PREP_HEADS - 1) / q4::PREP_HEADS);
     const int64_t blocks = (int64_t)(d.at0[d.n] + d.old0[d.n]) * kvc + (q_tasks + q4::PREP_WARPS - 1) / q4::PREP_WARPS;
@@ -224,11 +638,11 @@ static cudaError_t launch_group(dz_ctx* ctx, int layer, const q4::Prompt& d, con
         d, ctx->axes, kvc, L.d_q4, pos, L.q_norm, L.k_norm, q_gate, k, v, qf, kf, vf, ctx->q4_track, ctx->cfg.rms_eps);
     *n_launch += 1;
     if (map.first[d.n] > 0) {
-        const size_t smem = sizeof(pf::Smem) + 1024;
-        auto kernel = pf_attn_kernel<T, T, __half, pf::Packed>;
+        const size_t smem = sizeof(attn::Smem) + 1024;
+        auto kernel = attn::q4_pf_attn_kernel<T>;
         if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess)
             return e;
-        kernel<<<(unsigned)(map.first[d.n] * nq), pf::NTHREADS, smem, st>>>(mq, mk, mv, map, kvc, q_gate, out, ctx->d_err);
+        kernel<<<(unsigned)(map.first[d.n] * nq), attn::NTHREADS, smem, st>>>(mq, mk, mv, map, kvc, q_gate, out, ctx->d_err);
         *n_launch += 1;
     }
     return cudaGetLastError();
@@ -251,7 +665,7 @@ static cudaError_t launch_prompts(dz_ctx* ctx, int layer, int n, const int32_t* 
         int64_t bytes = 0;
         for (; i < n && d.n < MAXB; ++i) {
             const int64_t base = L.len[seq_ids[i]], T_i = lens[i];
-            const int64_t keys = (base + T_i + pf::BN - 1) / pf::BN * pf::BN;
+            const int64_t keys = (base + T_i + q4::attn::BN - 1) / q4::attn::BN * q4::attn::BN;
             const int64_t more = T_i * nq * HD * 2 + keys * kvc * HD * 4;
             if (T_i == 0) continue;
             if (d.n > 0 && bytes + more > GROUP_BYTES) break;
