@@ -208,6 +208,8 @@ struct alignas(1024) Smem {
     float red_l[2][BM];                          // [key half][row] partial row sums
     uint32_t tmem_base;
 };
+constexpr int OUT_PITCH = 68;                    // floats a staged output row (16-byte aligned, no bank conflicts)
+static_assert(8 * 32 * OUT_PITCH * 4 <= offsetof(Smem, q_full), "the staged output fits below the barriers");
 static_assert(offsetof(Smem, k) % 1024 == 0 && offsetof(Smem, v) % 1024 == 0, "swizzle atoms need 1 KB alignment");
 
 // ---- the pair's forms of the PTX wrappers ------------------------------------------
@@ -279,6 +281,8 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// to 2^-21 or so, below the products' f16 rounding
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + ex2(-LOG2E * x)); }
 __device__ __forceinline__ float max3f(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -545,32 +549,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
             __syncwarp();
             if (lane == 0) arrive_at(p_bar[st]);
         }
-        // epilogue: O / l * sigmoid(gate); this thread covers dims [128 hf, 128 hf + 128)
+        // epilogue: O / l * sigmoid(gate), the warp's 32 rows x 128 dims [128 hf, 128 hf + 128) in four
+        // parts of 16 rows x 64 dims, through shared memory (every product is done by then: Q's and the
+        // rings' place is free), so that gates are read and outputs written in whole lines.  The gates
+        // of a part are requested before the part ahead of it is worked on.
+        const int64_t row0 = tl.row + 32 * (warp & 3);
+        const int rows = (int)max((int64_t)0, min((int64_t)32, tl.T - tl.q0 - 32 * (warp & 3)));   // that exist
+        const int c = 4 * (lane & 15), half = lane >> 4;
+        decltype(load4(q_gate)) gate[8];
+        auto load_gates = [&](int part) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int row = min(16 * (part & 1) + 2 * i + half, rows - 1);
+                gate[i] = load4(q_gate + ((row0 + row) * nq + qh) * QG_ROW + HD + 128 * hf + 64 * (part >> 1) + c);
+            }
+        };
+        if (rows > 0) load_gates(0);
         sm.red_l[hf][r] = l_run;
         named_bar_sync(1, 256);
-        const float l_tot = l_run + sm.red_l[hf ^ 1][r];
-        if (ok) {
-            const int jl = nblk - 1;
-            if (wait(&sm.pv_done[jl & 1], (jl >> 1) & 1, err, ok)) {
-                fence_after_sync();
-                const int64_t t = tl.row + r;
-                const float inv_l = 1.0f / l_tot;
-#pragma unroll 1
-                for (int c = 128 * hf; c < 128 * hf + 128; c += 32) {
-                    float o[32];
-                    tmem_ld32(tmem + lane_off + O_COL + c, o);
-                    if (tl.q0 + r < tl.T) {
-                        const T* g = q_gate + (t * nq + qh) * QG_ROW + HD + c;
-                        T* dst = out + (t * nq + qh) * HD + c;
+        const float inv_l = 1.0f / (l_run + sm.red_l[hf ^ 1][r]);
+        const int jl = nblk - 1;
+        if (ok && wait(&sm.pv_done[jl & 1], (jl >> 1) & 1, err, ok) && rows > 0) {
+            fence_after_sync();
+            float* stage = reinterpret_cast<float*>(&sm) + (size_t)warp * 32 * OUT_PITCH;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            const float4 gv = as_f32(load4(g + i));
-                            store4(dst + i, make_float4(o[i + 0] * inv_l * sigmoidf_acc(gv.x),
-                                                        o[i + 1] * inv_l * sigmoidf_acc(gv.y),
-                                                        o[i + 2] * inv_l * sigmoidf_acc(gv.z),
-                                                        o[i + 3] * inv_l * sigmoidf_acc(gv.w)));
-                        }
+            for (int part = 0; part < 4; ++part) {
+                const int c0 = 128 * hf + 64 * (part >> 1);
+                if ((part & 1) == 0) {
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 64; k += 32) {
+                        float o[32];
+                        tmem_ld32(tmem + lane_off + O_COL + c0 + k, o);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<float4*>(stage + lane * OUT_PITCH + k + i) =
+                                make_float4(o[i] * inv_l, o[i + 1] * inv_l, o[i + 2] * inv_l, o[i + 3] * inv_l);
                     }
+                    __syncwarp();
+                }
+                float4 g[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) g[i] = as_f32(gate[i]);
+                if (part < 3) load_gates(part + 1);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int row = 16 * (part & 1) + 2 * i + half;
+                    const float4 o = *reinterpret_cast<const float4*>(stage + row * OUT_PITCH + c);
+                    if (row < rows)
+                        store4(out + ((row0 + row) * nq + qh) * HD + c0 + c,
+                               make_float4(o.x * sigmoid(g[i].x), o.y * sigmoid(g[i].y), o.z * sigmoid(g[i].z),
+                                           o.w * sigmoid(g[i].w)));
                 }
             }
         }
