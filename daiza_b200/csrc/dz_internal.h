@@ -51,11 +51,13 @@ struct Q4Rows {
     int B, kvc;
     int32_t sid[MAXB], len[MAXB];                // slot of sequence b, its length before this token
     int32_t cum[MAXB + 1];
-    __host__ __device__ int64_t tiles() const { return (int64_t)cum[B] * kvc; }
+    int runs, run_base, run_rem;                 // the tiles are cut into `runs`, run_rem of them one longer
+    // (32 bits: a GPU's memory holds some 40 million tiles)
+    __host__ __device__ int tiles() const { return cum[B] * kvc; }
     __host__ __device__ int row_tiles(int b) const { return cum[b + 1] - cum[b]; }
-    __host__ __device__ int64_t row_start(int row) const {
+    __host__ __device__ int row_start(int row) const {
         const int b = row / kvc;
-        return (int64_t)cum[b] * kvc + (int64_t)(row - b * kvc) * row_tiles(b);
+        return cum[b] * kvc + (row - b * kvc) * row_tiles(b);
     }
 };
 constexpr int Q4_FRAG_WORDS = 16 * 32 * 4 + 16;   // q as matrix operand, one row (q4_decode.cu)
@@ -302,7 +304,7 @@ cudaError_t launch_q1_gemv(dz_ctx* ctx, int n_mats, const uint8_t* const* w, con
 cudaError_t launch_rmsnorm_rows(const float* x, const float* w, float eps, int T, int n, float* out, cudaStream_t st);
 cudaError_t launch_swiglu(float* gate, const float* up, int64_t n, cudaStream_t st);
 // 4-bit KV caches (q4_*.cu)
-cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, const Q4Rows& d, const Q4Pos& pos, const float* q_gate,
+cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, Q4Rows& d, const Q4Pos& pos, const float* q_gate,
                              const float* k, const float* v, float* out, cudaStream_t st, int* n_launch);
 // prompts: lens[i] new tokens of each sequence, packed; f32 or bf16 (uint16_t) tensors
 cudaError_t launch_q4_prefill(dz_ctx* ctx, int layer, int n, const int32_t* seq_ids, const int64_t* lens,

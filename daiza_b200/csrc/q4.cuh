@@ -42,21 +42,38 @@ namespace dz {
 namespace q4 {
 
 constexpr float SCALE_MAX = 896.0f;
+constexpr uint32_t SCALE_MAX_BYTE = 24u << 3 | 6u;            // 896 = 1.75 * 2^9
 constexpr int OFF_V = 2048, OFF_KS = 4096, OFF_VS = 4224;
 static_assert(OFF_VS + 128 == Q4_TILE_BYTES, "tile layout");
 static_assert(Q4_TILE_BYTES % 16 == 0, "tiles move by bulk copies");
 
+// About a millisecond, for what is in flight after a wait that ran into its limit.
+__device__ __forceinline__ void settle() {
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+}
+
 // ---- scales ------------------------------------------------------------------------
-// s (as stored byte) from the group's largest magnitude.  t's significand is cut to 4
-// bits in integer arithmetic; below 2^-14 the grid is 2^-17.
+// s (as stored byte) from the group's largest magnitude: 4 significant bits of amax / 7 by
+// f32, then decided exactly.  A border lies half a step from s, at 7 s +- 3.5 steps of
+// amax, and amax - 7 s is exact there; so no division, and K's f64 and V's f32 values
+// are treated alike.
 __device__ __forceinline__ uint32_t scale_byte(double amax) {
-    const double t = fmin(amax / 7.0, (double)SCALE_MAX);
-    if (t < 6.103515625e-05)                                   // 2^-14: f16 subnormals
-        return (uint32_t)__double2int_rn(t * 131072.0);        // 0..8 (8 = the smallest normal)
-    const long long b = __double_as_longlong(t);
-    const long long odd = (b >> 49) & 1;                       // keep 3 fraction bits of 52, nearest even
-    const long long r = (b + ((1ll << 48) - 1) + odd) >> 49;   // exponent and 3 fraction bits
-    return (uint32_t)(r - ((1023 - 15) << 3));                 // rebias to f16: exponent << 3 | fraction
+    const float t = fminf((float)amax * (1.0f / 7.0f), SCALE_MAX);
+    uint32_t byte;                                             // exponent << 3 | 3 fraction bits, of f16
+    if (t < 6.103515625e-05f) {                                // 2^-14: the grid is 2^-17, f16's subnormals
+        byte = (uint32_t)__float2int_rn(t * 131072.0f);        // 0..8 (8 = the smallest normal)
+    } else {
+        const uint32_t b = __float_as_uint(t);
+        byte = ((b + 0x7FFFFu + ((b >> 20) & 1u)) >> 20) - ((127 - 15) << 3);
+    }
+    const float s = __half2float(__ushort_as_half((unsigned short)(byte << 7)));
+    const float step = __half2float(__ushort_as_half((unsigned short)((byte + 1) << 7))) - s;
+    const bool binade = (byte & 7u) == 0u && byte > 8u;        // the step below is half as long
+    const double d = fma(-7.0, (double)s, amax), up = 3.5 * (double)step, down = binade ? 0.5 * up : up;
+    const bool odd = byte & 1u;
+    if (d > up || (d == up && odd)) byte += 1;
+    else if (d < -down || (d == -down && odd)) byte -= 1;
+    return min(byte, SCALE_MAX_BYTE);
 }
 __device__ __forceinline__ float scale_value(uint32_t byte) {
     return __half2float(__ushort_as_half((unsigned short)(byte << 7)));
@@ -139,7 +156,13 @@ __device__ __forceinline__ double2 rope_cs(const RopeAxes& a, int i, int t, int 
 // both halves, math/rope.rs:205-210), in f64 for rows that are quantised and in f32 for
 // the others.  cs: (cos, sin) of the 32 pairs.  The partner of dim i < 32 is i + 32:
 // lane ^ 4.
-__device__ __forceinline__ double inv_sqrt(double x) { return 1.0 / sqrt(x); }
+__device__ __forceinline__ double inv_sqrt(double x) {         // Newton's iteration from f32's: 2^-23, 2^-45, 2^-53
+    if (!(x > 1e-30 && x < 1e30)) return 1.0 / sqrt(x);        // where f32's would lose bits or overflow
+    double g = (double)rsqrtf((float)x);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) g = fma(fma(-x * g, g, 1.0), 0.5 * g, g);
+    return g;
+}
 __device__ __forceinline__ float inv_sqrt(float x) { return 1.0f / sqrtf(x); }
 template <typename F, typename C>
 __device__ __forceinline__ void norm_rotate(F (&x)[8], const float* __restrict__ w, const C* cs, float eps, int lane) {

@@ -37,22 +37,25 @@ __global__ void __launch_bounds__(256) q4_prep_kernel(const __grid_constant__ Ro
                                                       const float* __restrict__ q_gate, const float* __restrict__ k_in,
                                                       const float* __restrict__ v_in, uint32_t* __restrict__ q_frag,
                                                       float eps) {
-    __shared__ double2 cs[ROPE / 2];
+    __shared__ double2 cs[8][ROPE / 2];
     const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == 0) cs[lane] = rope_cs(axes, lane, pos.p[b][0], pos.p[b][1], pos.p[b][2]);
-    __syncthreads();
+    const int kvc = d.kvc, nq = GRP * kvc;
+    const int task = blockIdx.y * 8 + warp;
+    // before the wait: the angles (f32 for q, f64 for K)
+    float2* csf = reinterpret_cast<float2*>(cs[warp]);
+    if (task < nq) csf[lane] = rope_cs_f32(axes, lane, pos.p[b][0], pos.p[b][1], pos.p[b][2]);
+    else cs[warp][lane] = rope_cs(axes, lane, pos.p[b][0], pos.p[b][1], pos.p[b][2]);
+    __syncwarp();
     // As in gqa_prep: everything before this grid is complete (inputs, caches, q_frag)
     // before the split grid may start streaming old tiles.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-    const int kvc = d.kvc, nq = GRP * kvc;
-    const int task = blockIdx.y * 8 + warp;
     if (task >= nq + kvc) return;
     if (task < nq) {
         const float4* src = reinterpret_cast<const float4*>(q_gate + ((size_t)b * nq + task) * QG_ROW);
         const float4 a0 = src[2 * lane], a1 = src[2 * lane + 1];
         float x[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
-        norm_rotate(x, q_norm, cs, eps, lane);
+        norm_rotate(x, q_norm, csf, eps, lane);
         float amax = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -91,7 +94,7 @@ __global__ void __launch_bounds__(256) q4_prep_kernel(const __grid_constant__ Ro
         const float4 k0 = *reinterpret_cast<const float4*>(k_in + at), k1 = *reinterpret_cast<const float4*>(k_in + at + 4);
         const float4 v0 = *reinterpret_cast<const float4*>(v_in + at), v1 = *reinterpret_cast<const float4*>(v_in + at + 4);
         double x[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
-        norm_rotate(x, k_norm, cs, eps, lane);
+        norm_rotate(x, k_norm, cs[warp], eps, lane);
         uint32_t code[8];
         uint32_t sb = quantise(x, code);
         put_k(tile, p, lane, code, sb);
@@ -131,37 +134,35 @@ struct alignas(128) Ring {
 };
 static_assert(Q4_TILE_BYTES % 128 == 0 && sizeof(Ring) % 128 == 0, "bulk copies need 16-byte alignment");
 
-// W c overflows nothing: W is below 2^36 tiles, c below 2^12 runs
-__host__ __device__ inline int64_t run_start(int64_t W, int c, int R) { return W * c / R; }
+// Run c starts at tile c * run_base + min(c, run_rem) (tiles = runs * run_base + run_rem).
+__host__ __device__ inline int run_start(const Rows& d, int c) { return c * d.run_base + min(c, d.run_rem); }
 // the run that holds a tile
-__device__ __forceinline__ int run_of(int64_t tile, int64_t W, int R) {
-    int c = (int)(tile * R / W);
-    while (run_start(W, c + 1, R) <= tile) ++c;
-    while (run_start(W, c, R) > tile) --c;
-    return c;
+__device__ __forceinline__ int run_of(const Rows& d, int tile) {
+    const int longer = d.run_rem * (d.run_base + 1);           // tiles of the runs that have one more
+    return tile < longer ? (int)((uint32_t)tile / (uint32_t)(d.run_base + 1))
+                         : d.run_rem + (int)((uint32_t)(tile - longer) / (uint32_t)d.run_base);
 }
 
 // The part of a row that a run covers: tiles [t0, t1) of the row.
 struct Segment { int b, row, t0, t1; const uint8_t* base; };
 
-__device__ __forceinline__ Segment segment_at(const Rows& d, const Q4Slot* __restrict__ slots, int64_t tile, int64_t end) {
+__device__ __forceinline__ Segment segment_at(const Rows& d, const Q4Slot* __restrict__ slots, int tile, int end) {
     Segment s;
     int lo = 0, hi = d.B - 1;                    // last b whose rows start at or before the tile
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if ((int64_t)d.cum[mid] * d.kvc <= tile) lo = mid; else hi = mid - 1;
+        if (d.cum[mid] * d.kvc <= tile) lo = mid; else hi = mid - 1;
     }
     s.b = lo;
     const int n = d.row_tiles(lo);
-    int64_t in = tile - (int64_t)d.cum[lo] * d.kvc;
-    int kvh = 0;
+    int in = tile - d.cum[lo] * d.kvc, kvh = 0;
     while (in >= n) {
         in -= n;
         ++kvh;
     }
     s.row = lo * d.kvc + kvh;
-    s.t0 = (int)in;
-    s.t1 = (int)min((int64_t)n, s.t0 + (end - tile));
+    s.t0 = in;
+    s.t1 = min(n, in + (end - tile));
     s.base = slots[d.sid[lo]].tile(kvh, 0);
     return s;
 }
@@ -334,7 +335,7 @@ __device__ __forceinline__ void attend(State& st, const uint8_t* tiles, const ui
 
 template <bool TRACK>
 __global__ void __launch_bounds__(32 * WARPS, 1)
-    q4_split_kernel(const __grid_constant__ Rows d, int R, const Q4Slot* __restrict__ slots,
+    q4_split_kernel(const __grid_constant__ Rows d, const Q4Slot* __restrict__ slots,
                     const uint32_t* __restrict__ q_frag, float* __restrict__ part_o, float* __restrict__ part_ml,
                     float* __restrict__ scores, int* err) {
     extern __shared__ __align__(128) unsigned char smem_raw[];
@@ -342,15 +343,15 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
     Ring& ring = reinterpret_cast<Ring*>(smem_raw)[warp];
     asm volatile("griddepcontrol.launch_dependents;");
     const int run = warp * gridDim.x + blockIdx.x;   // few runs: spread over the SMs first
-    if (run >= R) return;
-    const int64_t W = d.tiles(), run0 = run_start(W, run, R), run1 = run_start(W, run + 1, R);
+    if (run >= d.runs) return;
+    const int run0 = run_start(d, run), run1 = run_start(d, run + 1);
     if (lane == 0) {
         for (int s = 0; s < STAGES; ++s) mbar_init(&ring.full[s], 1);
         fence_mbar_init();
     }
     __syncwarp();
     // producer: the next tile to request
-    int64_t p_end = run0;                        // end of the producer's segment
+    int p_end = run0;                        // end of the producer's segment
     Segment ps{};
     int p_t = 0;
     // the tile that holds slot len is written by q4_prep: requested after the grid-dependency wait
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
 
     int stage = 0;
     uint32_t phase = 0;
-    for (int64_t at = run0; at < run1;) {
+    for (int at = run0; at < run1;) {
         const Segment sg = segment_at(d, slots, at, run1);
         const uint32_t* frag = q_frag + (size_t)sg.row * FRAG_WORDS;
         uint4 q[16];
@@ -395,7 +396,10 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
         st.m = -INFINITY;
         st.l = 0.0f;
         for (int t = sg.t0; t < sg.t1; t += 2) {
-            if (!mbar_wait(&ring.full[stage], phase, err)) return;
+            if (!mbar_wait(&ring.full[stage], phase, err)) {   // given up: copies already issued get time to end
+                settle();
+                return;
+            }
             float* sc = TRACK ? scores + (size_t)(at + (t - sg.t0)) * (GRP * Q4_TILE) : nullptr;
             if (t + 1 < sg.t1) attend<2, TRACK>(st, ring.pair[stage], q, qs, n - t * Q4_TILE, sc, lane);
             else attend<1, TRACK>(st, ring.pair[stage], q, qs, n - t * Q4_TILE, sc, lane);
@@ -431,10 +435,10 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
 // 3. combine: merge a row's partials, divide, gate.  Grid (6 kvc, B, 4 quarters of the
 //    dims), 16 groups of 16 threads that take partials in turn, 4 dims a thread.
 // ---------------------------------------------------------------------------
-constexpr int MAX_RUNS = 2048;                   // warps of the split grid (148 SMs: 1776)
+constexpr int MAX_RUNS = 2048;                   // warps of the split grid (148 SMs: 1184)
 constexpr int CMB_DIMS = 64;
 
-__global__ void __launch_bounds__(256) q4_combine_kernel(const __grid_constant__ Rows d, int R,
+__global__ void __launch_bounds__(256) q4_combine_kernel(const __grid_constant__ Rows d,
                                                          const float* __restrict__ part_o,
                                                          const float* __restrict__ part_ml,
                                                          const float* __restrict__ q_gate, float* __restrict__ out) {
@@ -446,8 +450,7 @@ __global__ void __launch_bounds__(256) q4_combine_kernel(const __grid_constant__
     const int kvh = qh / GRP, h = qh - kvh * GRP, row = b * d.kvc + kvh;
     const int warp = tid >> 5, lane = tid & 31;
     const float gate = tid < CMB_DIMS ? q_gate[((size_t)b * nq + qh) * QG_ROW + HD + d0 + tid] : 0.0f;
-    const int64_t W = d.tiles(), start = d.row_start(row);
-    const int c0 = run_of(start, W, R), nc = run_of(start + d.row_tiles(b) - 1, W, R) - c0 + 1;
+    const int start = d.row_start(row), c0 = run_of(d, start), nc = run_of(d, start + d.row_tiles(b) - 1) - c0 + 1;
     const size_t part0 = (size_t)c0 + row;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const float2* ml = reinterpret_cast<const float2*>(part_ml) + part0 * GRP + h;
@@ -499,7 +502,7 @@ __global__ void __launch_bounds__(256) q4_combine_kernel(const __grid_constant__
 // ---------------------------------------------------------------------------
 constexpr int WT_SPAN = 1024;
 
-__global__ void __launch_bounds__(256) q4_weights_kernel(const __grid_constant__ Rows d, int R,
+__global__ void __launch_bounds__(256) q4_weights_kernel(const __grid_constant__ Rows d,
                                                          const Q4Slot* __restrict__ slots,
                                                          const float* __restrict__ part_ml,
                                                          const float* __restrict__ scores) {
@@ -507,9 +510,9 @@ __global__ void __launch_bounds__(256) q4_weights_kernel(const __grid_constant__
     const int b = blockIdx.z, kvh = blockIdx.y, n = d.len[b] + 1, j0 = blockIdx.x * WT_SPAN;
     if (j0 >= n) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = b * d.kvc + kvh;
-    const int64_t W = d.tiles(), start = d.row_start(row);
+    const int start = d.row_start(row);
     if (warp < GRP) {
-        const int c0 = run_of(start, W, R), nc = run_of(start + d.row_tiles(b) - 1, W, R) - c0 + 1;
+        const int c0 = run_of(d, start), nc = run_of(d, start + d.row_tiles(b) - 1) - c0 + 1;
         const float2* ml = reinterpret_cast<const float2*>(part_ml) + ((size_t)c0 + row) * GRP + warp;
         float m = -INFINITY;
         for (int i = lane; i < nc; i += 32) m = fmaxf(m, ml[(size_t)i * GRP].x);
@@ -541,12 +544,14 @@ __global__ void __launch_bounds__(256) q4_weights_kernel(const __grid_constant__
 
 int q4_decode_runs(int n_sm) { return std::min(q4::WARPS * n_sm, q4::MAX_RUNS); }
 
-cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, const Q4Rows& d, const Q4Pos& pos, const float* q_gate,
+cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, Q4Rows& d, const Q4Pos& pos, const float* q_gate,
                              const float* k, const float* v, float* out, cudaStream_t st, int* n_launch) {
     using namespace q4;
     const LayerState& L = ctx->layers[layer];
     const int kvc = d.kvc;
-    const int R = (int)std::min<int64_t>(d.tiles(), q4_decode_runs(ctx->n_sm));
+    d.runs = std::min(d.tiles(), q4_decode_runs(ctx->n_sm));
+    d.run_base = d.tiles() / d.runs;
+    d.run_rem = d.tiles() % d.runs;
     const int smem = WARPS * (int)sizeof(Ring);
     auto split = ctx->q4_track ? q4_split_kernel<true> : q4_split_kernel<false>;
     cudaError_t e = cudaFuncSetAttribute(split, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -563,16 +568,16 @@ cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, const Q4Rows& d, const Q4Po
     e = cudaLaunchKernelEx(&lc, q4_prep_kernel, d, pos, ctx->axes, (const Q4Slot*)L.d_q4, (const float*)L.q_norm,
                            (const float*)L.k_norm, q_gate, k, v, ctx->q4_frag, ctx->cfg.rms_eps);
     if (e != cudaSuccess) return e;
-    lc.gridDim = dim3(std::min(R, ctx->n_sm));
+    lc.gridDim = dim3(std::min(d.runs, ctx->n_sm));
     lc.blockDim = dim3(32 * WARPS);
     lc.dynamicSmemBytes = smem;
-    e = cudaLaunchKernelEx(&lc, split, d, R, (const Q4Slot*)L.d_q4, (const uint32_t*)ctx->q4_frag, ctx->part_o,
+    e = cudaLaunchKernelEx(&lc, split, d, (const Q4Slot*)L.d_q4, (const uint32_t*)ctx->q4_frag, ctx->part_o,
                            ctx->part_ml, ctx->q4_sc, ctx->d_err);
     if (e != cudaSuccess) return e;
     lc.gridDim = dim3(GRP * kvc, d.B, HD / CMB_DIMS);
     lc.blockDim = dim3(256);
     lc.dynamicSmemBytes = 0;
-    e = cudaLaunchKernelEx(&lc, q4_combine_kernel, d, R, (const float*)ctx->part_o, (const float*)ctx->part_ml, q_gate,
+    e = cudaLaunchKernelEx(&lc, q4_combine_kernel, d, (const float*)ctx->part_o, (const float*)ctx->part_ml, q_gate,
                            out);
     if (e != cudaSuccess) return e;
     *n_launch += 3;
@@ -580,7 +585,7 @@ cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, const Q4Rows& d, const Q4Po
         int longest = 0;
         for (int b = 0; b < d.B; ++b) longest = std::max(longest, d.len[b] + 1);
         q4_weights_kernel<<<dim3((longest + WT_SPAN - 1) / WT_SPAN, kvc, d.B), 256, 0, st>>>(
-            d, R, (const Q4Slot*)L.d_q4, ctx->part_ml, ctx->q4_sc);
+            d, (const Q4Slot*)L.d_q4, (const float*)ctx->part_ml, (const float*)ctx->q4_sc);
         *n_launch += 1;
     }
     return cudaGetLastError();

@@ -222,6 +222,20 @@ def test_decode_extreme_inputs():
     m.done()
 
 
+@pytest.mark.parametrize("size", [1e-30, 1e-20, 1e12, 1e19, 1e30, 3e38])
+def test_decode_keys_of_any_size(size):
+    """K is normalised in f64: squares below and above f32's range count as they are."""
+    m = Model([40], seed=31)
+    m.fill(0, 19)
+    qg, k, v = m.inputs(1)
+    k = np.clip(k, -1, 1) * np.float32(size)
+    k[0, 1, 100:] = 0.0
+    got, want = m.decode([0], inputs=(qg, k, v))
+    assert np.abs(got - want).max() <= OUT_TOL * np.abs(m.refs[0].v).max()
+    m.check_held(0)
+    m.done()
+
+
 def test_decode_zero_query_and_equal_keys():
     m = Model([20], seed=26, track=True)
     k = np.repeat(m.normal(1, 4, 256), 17, 0)
