@@ -1,10 +1,11 @@
 // q4_cache.cu -- entry points of the 4-bit KV cache (format: q4.cuh) and its small
 // kernels: import and export of rows, accumulated weights, and the rotary positions
 // of three axes as a pass of their own.
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
-#include <new>
+#include <exception>
 
 #include "q4.cuh"
 
@@ -25,12 +26,18 @@ void rope_axes_set(RopeAxes& a, const int32_t sections[3], bool interleaved, dou
 cudaError_t ensure_q4_scratch(dz_ctx* ctx, size_t bytes) {
     if (ctx->q4_scratch_bytes >= bytes) return cudaSuccess;
     ctx->q4_retired.reserve(ctx->q4_retired.size() + 1);
+    // at least twice the size before, so that all the old ones together are smaller than the new one
+    size_t size = std::max(bytes, 2 * ctx->q4_scratch_bytes);
     void* p = nullptr;
-    const cudaError_t e = cudaMalloc(&p, bytes);
+    cudaError_t e = cudaMalloc(&p, size);
+    if (e == cudaErrorMemoryAllocation && size > bytes) {
+        cudaGetLastError();
+        e = cudaMalloc(&p, size = bytes);
+    }
     if (e != cudaSuccess) return e;
     if (ctx->q4_scratch) ctx->q4_retired.push_back(ctx->q4_scratch);
     ctx->q4_scratch = p;
-    ctx->q4_scratch_bytes = bytes;
+    ctx->q4_scratch_bytes = size;
     return cudaSuccess;
 }
 
@@ -222,13 +229,14 @@ dz_status cuda_fail(dz_ctx* ctx, cudaError_t e, const char* what) {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// no C++ exception leaves a C entry point
+// no C++ exception leaves a C entry point: what can be thrown here is a failed or too large
+// allocation of a host vector
 template <typename F>
 dz_status guarded(dz_ctx* ctx, F&& body) {
     if (!ctx) return DZ_EINVAL;
     try {
         return body();
-    } catch (const std::bad_alloc&) {
+    } catch (const std::exception&) {
         return DZ_ENOMEM;
     }
 }

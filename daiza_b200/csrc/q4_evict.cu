@@ -101,7 +101,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* warp_sums, 
 // A warp builds the tile of 16 entries whose sources are src[0 .. n) (n <= 16; the rest
 // becomes zeros) in shared memory, codes, scales and weights.
 __device__ __forceinline__ void build_tile(uint8_t* out, float* wts_out, const Q4Slot& slot, int kvh,
-                                           const int32_t* __restrict__ src, int n, int lane) {
+                                           const int32_t* src, int n, int lane) {   // src: written by this kernel
     const int32_t mine = lane < n ? src[lane] : -1;            // source of destination position `lane`
     if (lane < Q4_TILE) wts_out[lane] = mine >= 0 ? slot.wts[(size_t)kvh * slot.cap + mine] : 0.0f;
 #pragma unroll

@@ -129,6 +129,8 @@ __global__ void __launch_bounds__(32 * PREP_WARPS)
         const int t16 = i < cached ? i : d.first_pad_tile(s) + (i - cached), at = t16 * Q4_TILE + warp;
         const bool old = i < cached;
         if (old ? at >= d.base[s] : at < d.base[s] + d.T(s)) return;   // a new row
+        // (in the last cached tile, words that hold old and new rows may be written meanwhile by
+        // the block that appends: the old rows' bits stay the same)
         uint32_t a[4] = {}, b[4] = {};
         if (old) {
             const uint8_t* tile = slots[d.sid[s]].tile(kvh, t16);
@@ -467,7 +469,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
         float m_run = -INFINITY, l_run = 0.0f;                         // m identical in both halves; l partial per half
         for (int j = 0; j < nblk; ++j) {
             const int st = j & 1;
-            if (!wait(&sm.s_full[st], (j >> 1) & 1, err, ok)) break;
+            // a wait given up (the rest is skipped then, and nothing is stored) leaves no named barrier out
+            wait(&sm.s_full[st], (j >> 1) & 1, err, ok);
             fence_after_sync();
             float s[64];
             {
@@ -509,7 +512,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
                 l_run *= f;
                 if (j > 0) {
                     const int pj = (j - 1) & 1;
-                    if (!wait(&sm.pv_done[pj], ((j - 1) >> 1) & 1, err, ok)) break;
+                    wait(&sm.pv_done[pj], ((j - 1) >> 1) & 1, err, ok);
                     fence_after_sync();
 #pragma unroll 1
                     for (int c = 128 * hf; c < 128 * hf + 128; c += 32) {
@@ -604,7 +607,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
             }
         }
     }
-    // neither CTA leaves, or frees TMEM, while the other's products or arrivals may touch it
+    // neither CTA leaves, or frees TMEM, while the other's products or arrivals may touch it; after
+    // a wait that was given up, copies and products already issued get time to end
+    if (!ok) settle();
     fence_before_sync();
     __syncthreads();
     cluster_sync();

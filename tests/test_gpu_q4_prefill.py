@@ -206,6 +206,45 @@ def test_prompt_on_another_stream_and_in_graphs():
     m.done()
 
 
+def test_scratch_of_growing_prompts_stays_bounded():
+    """Scratch that was outgrown stays (captured graphs may hold it): all of it together below the last one's size."""
+    m = Model([1300], kvc=4, seed=119)
+    tensors = [dev(x) for x in m.inputs(1300)]
+    out = torch.empty(1300, 24 * 256, device="cuda")
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    for T in range(20, 1301, 16):
+        m.ctx.kv_truncate(0, 0, 0)
+        m.ctx.gqa_prefill_q4(0, [0], [T], *(x[:T] for x in tensors), out[:T])
+    torch.cuda.synchronize()
+    need = 1300 * 24 * 512 + 1408 * 4 * 1024
+    assert free - torch.cuda.mem_get_info()[0] <= 4 * need + (64 << 20)
+    m.done()
+
+
+def test_two_contexts_at_once():
+    """Contexts share nothing: calls of two of them overlap on two streams."""
+    ms = [Model([700], kvc=1, seed=120 + i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in ms]
+    work = []
+    for m in ms:
+        t, u = m.inputs(600), m.inputs(1)
+        work.append((t, [dev(x) for x in t], u, [dev(x) for x in u], torch.empty(600, 1536, device="cuda"),
+                     torch.empty(1, 1536, device="cuda")))
+    torch.cuda.synchronize()
+    for m, st, (_, t, _, u, o, o1) in zip(ms, streams, work):
+        m.ctx.gqa_prefill_q4(0, [0], [600], *t, o, stream=st)
+        m.ctx.gqa_decode_q4(0, [0], *u, o1, stream=st)
+    torch.cuda.synchronize()
+    for m, (t, _, u, _, o, o1) in zip(ms, work):
+        for x, got, tol in ((t, o, MAX_TOL), (u, o1, OUT_TOL)):
+            want = m.refs[0].extend(*x, m.qn, m.kn)
+            got = got.cpu().numpy().reshape(want.shape)
+            assert np.abs(got - want).max() <= tol * np.abs(m.refs[0].v).max()
+        m.check_held(0)
+        m.done()
+
+
 def test_refusals():
     m = Model([20, 20], kvc=1, seed=118)
     m.fill(0, 15)
