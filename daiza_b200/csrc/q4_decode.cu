@@ -396,10 +396,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
         st.m = -INFINITY;
         st.l = 0.0f;
         for (int t = sg.t0; t < sg.t1; t += 2) {
-            if (!mbar_wait(&ring.full[stage], phase, err)) {   // given up: copies already issued get time to end
-                settle();
-                return;
-            }
+            // given up: the warp's other copies, all issued before, have had the whole limit to end
+            if (!mbar_wait(&ring.full[stage], phase, err)) return;
             float* sc = TRACK ? scores + (size_t)(at + (t - sg.t0)) * (GRP * Q4_TILE) : nullptr;
             if (t + 1 < sg.t1) attend<2, TRACK>(st, ring.pair[stage], q, qs, n - t * Q4_TILE, sc, lane);
             else attend<1, TRACK>(st, ring.pair[stage], q, qs, n - t * Q4_TILE, sc, lane);
