@@ -193,7 +193,7 @@ namespace attn {
 using namespace tc;
 
 constexpr int BM = 128, BN = 128;                // query rows of a CTA, keys of a block
-constexpr int NK = 10, NV = 9;                   // ring slots of 8 KB (a block is 4 of each)
+constexpr int NK = 8, NV = 7;                    // ring slots of 8 KB (a block is 4 of each)
 constexpr int NTHREADS = 352;
 __host__ __device__ constexpr uint32_t S_COL(int st) { return 128u * (uint32_t)st; }
 constexpr uint32_t O_COL = 256;
@@ -203,15 +203,14 @@ struct alignas(1024) Smem {
     uint16_t q[4][BM][64];                       // 4 boxes of 64 dims, 16 KB each
     uint16_t k[NK][BN / 2][64];
     uint16_t v[NV][2][32][64];
-    uint64_t q_full;
+    float out[8][32][32];                        // the softmax warps' outputs on their way out
+    uint64_t q_full, q_empty;
     uint64_t k_full[NK], k_empty[NK], v_full[NV], v_empty[NV];
     uint64_t s_full[2], p_full[2], pv_done[2];
     float red_max[2][2][BM];                     // [block parity][key half][row] partial row maxima
     float red_l[2][BM];                          // [key half][row] partial row sums
     uint32_t tmem_base;
 };
-constexpr int OUT_PITCH = 68;                    // floats a staged output row (16-byte aligned, no bank conflicts)
-static_assert(8 * 32 * OUT_PITCH * 4 <= offsetof(Smem, q_full), "the staged output fits below the barriers");
 static_assert(offsetof(Smem, k) % 1024 == 0 && offsetof(Smem, v) % 1024 == 0, "swizzle atoms need 1 KB alignment");
 
 // ---- the pair's forms of the PTX wrappers ------------------------------------------
@@ -346,13 +345,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int nq = GRP * kvc, pairs = nq / 2, rank = blockIdx.x & 1;
-    const Tile tl = map.tile((int)(blockIdx.x / 2 / pairs));
-    const int qh = 2 * (int)(blockIdx.x / 2 % pairs) + rank, kvh = qh / GRP;
-    const int64_t q_last = min(tl.q0 + BM, tl.T) - 1;                  // last valid query row of the sequence
-    const int nblk = (int)((tl.base + q_last) / BN) + 1;               // key blocks that touch the causal range
+    // the cluster's tiles, heaviest first: in rounds over all clusters, there and back
+    const int clusters = gridDim.x / 2, cluster = blockIdx.x / 2, total = map.first[map.n] * pairs;
+    int round = 0, qh, kvh, nblk;                                      // nblk: key blocks that touch the causal range
+    Tile tl;
+    auto next_tile = [&]() -> bool {
+        const int at = round * clusters + (round & 1 ? clusters - 1 - cluster : cluster);
+        if (at >= total) return false;
+        tl = map.tile(at / pairs);
+        qh = 2 * (at % pairs) + rank;
+        kvh = qh / GRP;
+        nblk = (int)((tl.base + min(tl.q0 + BM, tl.T) - 1) / BN) + 1;
+        ++round;
+        return true;
+    };
 
     if (tid == 0) {
         mbar_init(&sm.q_full, 1);
+        mbar_init(&sm.q_empty, 1);
         for (int i = 0; i < NK; ++i) {
             mbar_init(&sm.k_full[i], 1);
             mbar_init(&sm.k_empty[i], 1);
@@ -379,27 +389,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
     if (warp == 8) {
         // ---------------- TMA of Q and K ----------------
         if (lane == 0) {
-            if (rank == 0) mbar_arrive_expect_tx(&sm.q_full, 2 * BM * HD * 2);
             const uint32_t qb = peer_addr(&sm.q_full, 0);
-            for (int b = 0; b < 4; ++b) tma_load(&sm.q[b][0][0], &tm_q, 64 * b, (int)tl.row, qh, qb);
-            for (int idx = 0; idx < 4 * nblk && ok; ++idx) {
-                const int slot = idx % NK, j = idx >> 2, b = idx & 3;
-                if (idx >= NK && !wait(&sm.k_empty[slot], ((idx / NK) - 1) & 1, err, ok)) break;
-                if (rank == 0) mbar_arrive_expect_tx(&sm.k_full[slot], BN * 64 * 2);
-                tma_load(&sm.k[slot][0][0], &tm_k, 64 * b, (int)tl.key + j * BN + rank * (BN / 2), kvh,
-                         peer_addr(&sm.k_full[slot], 0));
+            int slot = 0;
+            uint32_t phase = 1;                                        // of the slot before: passes on a fresh ring
+            while (ok && next_tile()) {
+                if (round > 1 && !wait(&sm.q_empty, round & 1, err, ok)) break;
+                if (rank == 0) mbar_arrive_expect_tx(&sm.q_full, 2 * BM * HD * 2);
+                for (int b = 0; b < 4; ++b) tma_load(&sm.q[b][0][0], &tm_q, 64 * b, (int)tl.row, qh, qb);
+                for (int idx = 0; idx < 4 * nblk; ++idx) {
+                    const int j = idx >> 2, b = idx & 3;
+                    if (!wait(&sm.k_empty[slot], phase, err, ok)) break;
+                    if (rank == 0) mbar_arrive_expect_tx(&sm.k_full[slot], BN * 64 * 2);
+                    tma_load(&sm.k[slot][0][0], &tm_k, 64 * b, (int)tl.key + j * BN + rank * (BN / 2), kvh,
+                             peer_addr(&sm.k_full[slot], 0));
+                    if (++slot == NK) {
+                        slot = 0;
+                        phase ^= 1u;
+                    }
+                }
             }
         }
     } else if (warp == 10) {
         // ---------------- TMA of V ----------------
         if (lane == 0) {
-            for (int idx = 0; idx < 4 * nblk && ok; ++idx) {
-                const int slot = idx % NV, j = idx >> 2, kg = idx & 3;
-                if (idx >= NV && !wait(&sm.v_empty[slot], ((idx / NV) - 1) & 1, err, ok)) break;
-                if (rank == 0) mbar_arrive_expect_tx(&sm.v_full[slot], 32 * HD * 2);
-                for (int d = 0; d < 2; ++d)
-                    tma_load(&sm.v[slot][d][0][0], &tm_v, 128 * rank + 64 * d, (int)tl.key + j * BN + 32 * kg, kvh,
-                             peer_addr(&sm.v_full[slot], 0));
+            int slot = 0;
+            uint32_t phase = 1;
+            while (ok && next_tile()) {
+                for (int idx = 0; idx < 4 * nblk; ++idx) {
+                    const int j = idx >> 2, kg = idx & 3;
+                    if (!wait(&sm.v_empty[slot], phase, err, ok)) break;
+                    if (rank == 0) mbar_arrive_expect_tx(&sm.v_full[slot], 32 * HD * 2);
+                    for (int d = 0; d < 2; ++d)
+                        tma_load(&sm.v[slot][d][0][0], &tm_v, 128 * rank + 64 * d, (int)tl.key + j * BN + 32 * kg, kvh,
+                                 peer_addr(&sm.v_full[slot], 0));
+                    if (++slot == NV) {
+                        slot = 0;
+                        phase ^= 1u;
+                    }
+                }
             }
         }
     } else if (warp == 9) {
@@ -414,8 +441,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
             const uint32_t k_empty = smem_u32(&sm.k_empty[0]), v_empty = smem_u32(&sm.v_empty[0]);
             const uint32_t go = elect_one();
             int k_slot = 0, v_slot = 0;
-            uint32_t k_phase = 0, v_phase = 0;
-            auto issue_s = [&](int st) {
+            uint32_t k_phase = 0, v_phase = 0, g = 0;                  // g: blocks of the cluster's earlier tiles
+            auto issue_s = [&](int j) {
+                const int st = (g + j) & 1;
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     if (!wait(&sm.k_full[k_slot], k_phase, err, ok)) return;
@@ -432,13 +460,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
                     }
                 }
                 commit(go, smem_u32(&sm.s_full[st]));
+                if (j == nblk - 1) commit(go, smem_u32(&sm.q_empty));
             };
-            if (wait(&sm.q_full, 0, err, ok)) {
+            while (ok && next_tile()) {
+                if (!wait(&sm.q_full, (round - 1) & 1, err, ok)) break;
                 issue_s(0);
                 if (nblk > 1) issue_s(1);
                 for (int j = 0; j < nblk && ok; ++j) {
-                    const int st = j & 1;
-                    if (!wait(&sm.p_full[st], (j >> 1) & 1, err, ok)) break;
+                    const int st = (g + j) & 1;
+                    // the first block's P also says that the last tile's O has been read
+                    if (!wait(&sm.p_full[st], ((g + j) >> 1) & 1, err, ok)) break;
 #pragma unroll
                     for (int kg = 0; kg < 4; ++kg) {
                         if (!wait(&sm.v_full[v_slot], v_phase, err, ok)) break;
@@ -455,8 +486,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
                         }
                     }
                     commit(go, smem_u32(&sm.pv_done[st]));
-                    if (j + 2 < nblk) issue_s(st);
+                    if (j + 2 < nblk) issue_s(j + 2);
                 }
+                g += nblk;
             }
         }
     } else {
@@ -464,145 +496,144 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
         const int r = 32 * (warp & 3) + lane;                          // TMEM lane = query row
         const int hf = warp >> 2;                                      // keys [64 hf, 64 hf + 64) of a block
         const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
-        const int64_t qpos = tl.base + tl.q0 + r;                      // absolute position of this query row
         const uint32_t p_bar[2] = {peer_addr(&sm.p_full[0], 0), peer_addr(&sm.p_full[1], 0)};
-        float m_run = -INFINITY, l_run = 0.0f;                         // m identical in both halves; l partial per half
-        for (int j = 0; j < nblk; ++j) {
-            const int st = j & 1;
-            // a wait given up (the rest is skipped then, and nothing is stored) leaves no named barrier out
-            wait(&sm.s_full[st], (j >> 1) & 1, err, ok);
-            fence_after_sync();
-            float s[64];
-            {
-                uint32_t raw[64];
-                tmem_ld32_async(tmem + lane_off + S_COL(st) + 64 * hf, raw);
-                tmem_ld32_async(tmem + lane_off + S_COL(st) + 64 * hf + 32, raw + 32);
-                tmem_wait_ld();
+        float (*stage)[32] = sm.out[warp];
+        uint32_t g = 0;                                                // blocks so far
+        while (next_tile()) {
+            const int64_t qpos = tl.base + tl.q0 + r;                      // absolute position of this query row
+            float m_run = -INFINITY, l_run = 0.0f;                         // m identical in both halves; l partial per half
+            for (int j = 0; j < nblk; ++j, ++g) {
+                const int st = g & 1;
+                // a wait given up (the rest is skipped then, and nothing is stored) leaves no named barrier out
+                wait(&sm.s_full[st], (g >> 1) & 1, err, ok);
+                fence_after_sync();
+                float s[64];
+                {
+                    uint32_t raw[64];
+                    tmem_ld32_async(tmem + lane_off + S_COL(st) + 64 * hf, raw);
+                    tmem_ld32_async(tmem + lane_off + S_COL(st) + 64 * hf + 32, raw + 32);
+                    tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < 64; ++c) s[c] = __uint_as_float(raw[c]);
-            }
-            // causal mask: keys k0 + c with c > lim are in the future (only blocks on the diagonal)
-            const int64_t lim64 = qpos - ((int64_t)j * BN + 64 * hf);
-            if (lim64 < 63) {
-                const int lim = lim64 < -1 ? -1 : (int)lim64;
-#pragma unroll
-                for (int c = 0; c < 64; ++c) s[c] = c > lim ? -INFINITY : s[c];
-            }
-            float mx;
-            {
-                float a0 = s[0], a1 = s[1], a2 = s[2], a3 = s[3];
-#pragma unroll
-                for (int c = 4; c < 60; c += 8) {
-                    a0 = max3f(a0, s[c], s[c + 1]);
-                    a1 = max3f(a1, s[c + 2], s[c + 3]);
-                    a2 = max3f(a2, s[c + 4], s[c + 5]);
-                    a3 = max3f(a3, s[c + 6], s[c + 7]);
+                    for (int c = 0; c < 64; ++c) s[c] = __uint_as_float(raw[c]);
                 }
-                a0 = max3f(a0, s[60], s[61]);
-                a1 = max3f(a1, s[62], s[63]);
-                mx = fmaxf(max3f(a0, a1, a2), a3);
-            }
-            sm.red_max[st][hf][r] = mx;
-            named_bar_sync(1, 256);                                    // also: every S read of this block is done
-            mx = fmaxf(mx, sm.red_max[st][hf ^ 1][r]);
-            const float m_new = fmaxf(m_run, mx);
-            if (m_new > m_run + RESCALE_THRESHOLD) {
-                // the running max moved a lot: scale l and this half-row of O
-                const float f = ex2(m_run - m_new);
-                l_run *= f;
-                if (j > 0) {
-                    const int pj = (j - 1) & 1;
-                    wait(&sm.pv_done[pj], ((j - 1) >> 1) & 1, err, ok);
-                    fence_after_sync();
+                // causal mask: keys k0 + c with c > lim are in the future (only blocks on the diagonal)
+                const int64_t lim64 = qpos - ((int64_t)j * BN + 64 * hf);
+                if (lim64 < 63) {
+                    const int lim = lim64 < -1 ? -1 : (int)lim64;
+#pragma unroll
+                    for (int c = 0; c < 64; ++c) s[c] = c > lim ? -INFINITY : s[c];
+                }
+                float mx;
+                {
+                    float a0 = s[0], a1 = s[1], a2 = s[2], a3 = s[3];
+#pragma unroll
+                    for (int c = 4; c < 60; c += 8) {
+                        a0 = max3f(a0, s[c], s[c + 1]);
+                        a1 = max3f(a1, s[c + 2], s[c + 3]);
+                        a2 = max3f(a2, s[c + 4], s[c + 5]);
+                        a3 = max3f(a3, s[c + 6], s[c + 7]);
+                    }
+                    a0 = max3f(a0, s[60], s[61]);
+                    a1 = max3f(a1, s[62], s[63]);
+                    mx = fmaxf(max3f(a0, a1, a2), a3);
+                }
+                sm.red_max[st][hf][r] = mx;
+                named_bar_sync(1, 256);                                    // also: every S read of this block is done
+                mx = fmaxf(mx, sm.red_max[st][hf ^ 1][r]);
+                const float m_new = fmaxf(m_run, mx);
+                const bool grown = m_new > m_run + RESCALE_THRESHOLD;
+                if (__any_sync(0xffffffffu, grown)) {
+                    // a running max of the warp moved a lot: scale l and this half of the rows of O (by 1
+                    // where it did not: TMEM is read and written by whole warps)
+                    const float f = grown ? ex2(m_run - m_new) : 1.0f;
+                    l_run *= f;
+                    if (j > 0) {
+                        wait(&sm.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, err, ok);
+                        __syncwarp();
+                        fence_after_sync();
 #pragma unroll 1
-                    for (int c = 128 * hf; c < 128 * hf + 128; c += 32) {
-                        float o[32];
-                        uint32_t ob[32];
-                        tmem_ld32(tmem + lane_off + O_COL + c, o);
+                        for (int c = 128 * hf; c < 128 * hf + 128; c += 32) {
+                            float o[32];
+                            uint32_t ob[32];
+                            tmem_ld32(tmem + lane_off + O_COL + c, o);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) ob[i] = __float_as_uint(o[i] * f);
-                        tmem_st32(tmem + lane_off + O_COL + c, ob);
+                            for (int i = 0; i < 32; ++i) ob[i] = __float_as_uint(o[i] * f);
+                            tmem_st32(tmem + lane_off + O_COL + c, ob);
+                        }
                     }
+                    if (grown) m_run = m_new;
                 }
-                m_run = m_new;
-            }
-            uint32_t pk[32];
-            {
-                const uint64_t mm = f2(m_run, m_run);
-                uint64_t acc0 = f2(0.0f, 0.0f), acc1 = acc0;
+                uint32_t pk[32];
+                {
+                    const uint64_t mm = f2(m_run, m_run);
+                    uint64_t acc0 = f2(0.0f, 0.0f), acc1 = acc0;
 #pragma unroll
-                for (int c = 0; c < 64; c += 4) {
-                    float x0, x1, x2, x3;
-                    f2_split(sub_f2(f2(s[c], s[c + 1]), mm), x0, x1);
-                    f2_split(sub_f2(f2(s[c + 2], s[c + 3]), mm), x2, x3);
-                    const float p0 = ex2(x0), p1 = ex2(x1), p2 = ex2(x2), p3 = ex2(x3);
-                    acc0 = add_f2(acc0, f2(p0, p1));
-                    acc1 = add_f2(acc1, f2(p2, p3));
-                    pk[c / 2] = pack_f16(p0, p1);
-                    pk[c / 2 + 1] = pack_f16(p2, p3);
-                }
-                float u0, u1;
-                f2_split(add_f2(acc0, acc1), u0, u1);
-                l_run += u0 + u1;
-            }
-            // P goes over the first 64 columns of its own S buffer (the previous reader of these
-            // columns, PV(j-2), completed before S(j) did)
-            tmem_st32(tmem + lane_off + S_COL(st) + 32 * hf, pk);
-            fence_before_sync();
-            __syncwarp();
-            if (lane == 0) arrive_at(p_bar[st]);
-        }
-        // epilogue: O / l * sigmoid(gate), the warp's 32 rows x 128 dims [128 hf, 128 hf + 128) in four
-        // parts of 16 rows x 64 dims, through shared memory (every product is done by then: Q's and the
-        // rings' place is free), so that gates are read and outputs written in whole lines.  The gates
-        // of a part are requested before the part ahead of it is worked on.
-        const int64_t row0 = tl.row + 32 * (warp & 3);
-        const int rows = (int)max((int64_t)0, min((int64_t)32, tl.T - tl.q0 - 32 * (warp & 3)));   // that exist
-        const int c = 4 * (lane & 15), half = lane >> 4;
-        decltype(load4(q_gate)) gate[8];
-        auto load_gates = [&](int part) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int row = min(16 * (part & 1) + 2 * i + half, rows - 1);
-                gate[i] = load4(q_gate + ((row0 + row) * nq + qh) * QG_ROW + HD + 128 * hf + 64 * (part >> 1) + c);
-            }
-        };
-        if (rows > 0) load_gates(0);
-        sm.red_l[hf][r] = l_run;
-        named_bar_sync(1, 256);
-        const float inv_l = 1.0f / (l_run + sm.red_l[hf ^ 1][r]);
-        const int jl = nblk - 1;
-        if (ok && wait(&sm.pv_done[jl & 1], (jl >> 1) & 1, err, ok) && rows > 0) {
-            fence_after_sync();
-            float* stage = reinterpret_cast<float*>(&sm) + (size_t)warp * 32 * OUT_PITCH;
-#pragma unroll
-            for (int part = 0; part < 4; ++part) {
-                const int c0 = 128 * hf + 64 * (part >> 1);
-                if ((part & 1) == 0) {
-                    __syncwarp();
-#pragma unroll
-                    for (int k = 0; k < 64; k += 32) {
-                        float o[32];
-                        tmem_ld32(tmem + lane_off + O_COL + c0 + k, o);
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<float4*>(stage + lane * OUT_PITCH + k + i) =
-                                make_float4(o[i] * inv_l, o[i + 1] * inv_l, o[i + 2] * inv_l, o[i + 3] * inv_l);
+                    for (int c = 0; c < 64; c += 4) {
+                        float x0, x1, x2, x3;
+                        f2_split(sub_f2(f2(s[c], s[c + 1]), mm), x0, x1);
+                        f2_split(sub_f2(f2(s[c + 2], s[c + 3]), mm), x2, x3);
+                        const float p0 = ex2(x0), p1 = ex2(x1), p2 = ex2(x2), p3 = ex2(x3);
+                        acc0 = add_f2(acc0, f2(p0, p1));
+                        acc1 = add_f2(acc1, f2(p2, p3));
+                        pk[c / 2] = pack_f16(p0, p1);
+                        pk[c / 2 + 1] = pack_f16(p2, p3);
                     }
-                    __syncwarp();
+                    float u0, u1;
+                    f2_split(add_f2(acc0, acc1), u0, u1);
+                    l_run += u0 + u1;
                 }
-                float4 g[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) g[i] = as_f32(gate[i]);
-                if (part < 3) load_gates(part + 1);
+                // P goes over the first 64 columns of its own S buffer (the previous reader of these
+                // columns, PV(j-2), completed before S(j) did)
+                tmem_st32(tmem + lane_off + S_COL(st) + 32 * hf, pk);
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) arrive_at(p_bar[st]);
+            }
+            // epilogue: O / l * sigmoid(gate), the warp's 32 rows x 128 dims [128 hf, 128 hf + 128) in four
+            // parts of 32 dims, through shared memory, so that gates are read and outputs written 8 lanes a
+            // row.  The gates of a part are requested before the part ahead of it is worked on.
+            const int64_t row0 = tl.row + 32 * (warp & 3);
+            const int rows = (int)max((int64_t)0, min((int64_t)32, tl.T - tl.q0 - 32 * (warp & 3)));   // that exist
+            const int c = lane & 7, quarter = lane >> 3;                   // 4 dims of every fourth row
+            decltype(load4(q_gate)) gate[8];
+            auto load_gates = [&](int part) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const int row = 16 * (part & 1) + 2 * i + half;
-                    const float4 o = *reinterpret_cast<const float4*>(stage + row * OUT_PITCH + c);
-                    if (row < rows)
-                        store4(out + ((row0 + row) * nq + qh) * HD + c0 + c,
-                               make_float4(o.x * sigmoid(g[i].x), o.y * sigmoid(g[i].y), o.z * sigmoid(g[i].z),
-                                           o.w * sigmoid(g[i].w)));
+                    const int row = min(4 * i + quarter, rows - 1);
+                    gate[i] = load4(q_gate + ((row0 + row) * nq + qh) * QG_ROW + HD + 128 * hf + 32 * part + 4 * c);
+                }
+            };
+            if (rows > 0) load_gates(0);
+            sm.red_l[hf][r] = l_run;
+            named_bar_sync(1, 256);
+            const float inv_l = 1.0f / (l_run + sm.red_l[hf ^ 1][r]);
+            wait(&sm.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, err, ok);
+            if (__all_sync(0xffffffffu, ok) && rows > 0) {
+                fence_after_sync();
+#pragma unroll
+                for (int part = 0; part < 4; ++part) {
+                    const int c0 = 128 * hf + 32 * part;
+                    float o[32];
+                    tmem_ld32(tmem + lane_off + O_COL + c0, o);
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)                            // 16-byte words in swizzled order
+                        *reinterpret_cast<float4*>(&stage[lane][4 * (i ^ (lane & 7))]) =
+                            make_float4(o[4 * i] * inv_l, o[4 * i + 1] * inv_l, o[4 * i + 2] * inv_l, o[4 * i + 3] * inv_l);
+                    __syncwarp();
+                    float4 w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) w[i] = as_f32(gate[i]);
+                    if (part < 3) load_gates(part + 1);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int row = 4 * i + quarter;
+                        const float4 x = *reinterpret_cast<const float4*>(&stage[row][4 * (c ^ (row & 7))]);
+                        if (row < rows)
+                            store4(out + ((row0 + row) * nq + qh) * HD + c0 + 4 * c,
+                                   make_float4(x.x * sigmoid(w[i].x), x.y * sigmoid(w[i].y), x.z * sigmoid(w[i].z),
+                                               x.w * sigmoid(w[i].w)));
+                    }
                 }
             }
         }
@@ -676,7 +707,8 @@ static cudaError_t launch_group(dz_ctx* ctx, int layer, const q4::Prompt& d, con
         auto kernel = attn::q4_pf_attn_kernel<T>;
         if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess)
             return e;
-        kernel<<<(unsigned)(map.first[d.n] * nq), attn::NTHREADS, smem, st>>>(mq, mk, mv, map, kvc, q_gate, out, ctx->d_err);
+        const unsigned clusters = (unsigned)std::min((int64_t)map.first[d.n] * nq / 2, (int64_t)ctx->n_sm / 2);
+        kernel<<<2 * clusters, attn::NTHREADS, smem, st>>>(mq, mk, mv, map, kvc, q_gate, out, ctx->d_err);
         *n_launch += 1;
     }
     return cudaGetLastError();

@@ -87,6 +87,20 @@ def test_many_short_prompts():
     m.done()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_more_query_tiles_than_fit_the_gpu_at_once(dtype):
+    """Several tiles per cluster, of one and of many key blocks."""
+    rng = np.random.default_rng(121)
+    lens = [int(n) for n in rng.integers(1, 300, 40)]
+    bases = [int(n) for n in rng.integers(0, 2, 40) * rng.integers(1, 500, 40)]
+    m = Model([a + b for a, b in zip(lens, bases)], seed=121)
+    for s, b in enumerate(bases):
+        if b:
+            m.fill(s, b)
+    check(m, list(range(40)), lens, dtype)
+    m.done()
+
+
 def test_prompt_then_decode_then_prompt():
     m = Model([400, 200], seed=112, track=True)
     check(m, [0, 1], [150, 37])
