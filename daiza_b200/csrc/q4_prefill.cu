@@ -193,8 +193,8 @@ namespace attn {
 using namespace tc;
 
 constexpr int BM = 128, BN = 128;                // query rows of a CTA, keys of a block
-constexpr int NK = 8, NV = 7;                    // ring slots of 8 KB (a block is 4 of each)
-constexpr int NTHREADS = 352;
+constexpr int NK = 6, NV = 5;                    // ring slots of 8 KB (a block is 4 of each)
+constexpr int NTHREADS = 512;
 __host__ __device__ constexpr uint32_t S_COL(int st) { return 128u * (uint32_t)st; }
 constexpr uint32_t O_COL = 256;
 constexpr float RESCALE_THRESHOLD = 8.0f;        // log2 units: P stays below 2^8, far inside f16
@@ -203,8 +203,8 @@ struct alignas(1024) Smem {
     uint16_t q[4][BM][64];                       // 4 boxes of 64 dims, 16 KB each
     uint16_t k[NK][BN / 2][64];
     uint16_t v[NV][2][32][64];
-    float out[8][32][32];                        // the softmax warps' outputs on their way out
-    uint64_t q_full, q_empty;
+    uint4 out[BM][HD / 8];                       // O / l as f16, 16-byte words of a row in swizzled order
+    uint64_t q_full, q_empty, out_full, out_empty;
     uint64_t k_full[NK], k_empty[NK], v_full[NV], v_empty[NV];
     uint64_t s_full[2], p_full[2], pv_done[2];
     float red_max[2][2][BM];                     // [block parity][key half][row] partial row maxima
@@ -282,8 +282,6 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// to 2^-21 or so, below the products' f16 rounding
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + ex2(-LOG2E * x)); }
 __device__ __forceinline__ float max3f(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -307,11 +305,59 @@ __device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-__device__ __forceinline__ void store4(float* p, float4 x) { *reinterpret_cast<float4*>(p) = x; }
-__device__ __forceinline__ void store4(__nv_bfloat16* p, float4 x) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
-    *reinterpret_cast<uint2*>(p) =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+// 2^x without the special-function unit, x at most 2^7: x = n + f with n nearest, a polynomial of
+// degree 4 for 2^f (least squares weighted towards the smallest largest error: 2.6e-6, far below P's
+// f16 rounding), n added to its exponent.  Below -126: 2^-126.
+__device__ __forceinline__ void ex2_poly(uint64_t x, float& p0, float& p1) {
+    float a, b;
+    f2_split(x, a, b);
+    x = f2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+    const uint64_t big = f2(12582912.0f, 12582912.0f);                 // 1.5 * 2^23: sums are rounded to integers
+    const uint64_t t = add_f2(x, big), f = sub_f2(x, sub_f2(t, big));
+    uint64_t y = fma_f2(f2(0.0095701f, 0.0095701f), f, f2(0.05591786f, 0.05591786f));
+    y = fma_f2(y, f, f2(0.24024745f, 0.24024745f));
+    y = fma_f2(y, f, f2(0.69312181f, 0.69312181f));
+    y = fma_f2(y, f, f2(0.99999926f, 0.99999926f));
+    float t0, t1;
+    f2_split(t, t0, t1);
+    f2_split(y, a, b);
+    p0 = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
+    p1 = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
+}
+__device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// (a sigmoid(x), b sigmoid(y)) of f16 a and b, to 2^-20 or so, below the products' f16 rounding; one
+// reciprocal for both.  Below 2^-60 a sigmoid counts as 2^-60: the denominators' product is finite.
+__device__ __forceinline__ float2 gate2(uint32_t ab, float x, float y) {
+    float s, t, u, w, r;
+    f2_split(mul_f2(f2(x, y), f2(-LOG2E, -LOG2E)), s, t);
+    const uint64_t uw = add_f2(f2(ex2(fminf(s, 60.0f)), ex2(fminf(t, 60.0f))), f2(1.0f, 1.0f));
+    f2_split(uw, u, w);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(u * w));
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&ab));
+    float2 out;
+    f2_split(mul_f2(f2(h.x, h.y), mul_f2(f2(w, u), f2(r, r))), out.x, out.y);
+    return out;
+}
+__device__ __forceinline__ void store8(float* p, float4 a, float4 b) {
+    reinterpret_cast<float4*>(p)[0] = a;
+    reinterpret_cast<float4*>(p)[1] = b;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, float4 a, float4 b) {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w), pack_bf16(b.x, b.y), pack_bf16(b.z, b.w));
 }
 
 // One query tile: rows [q0, q0 + 128) of a sequence of T new tokens behind `base` keys.  row:
@@ -363,6 +409,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
     if (tid == 0) {
         mbar_init(&sm.q_full, 1);
         mbar_init(&sm.q_empty, 1);
+        mbar_init(&sm.out_full, 8);                                    // the softmax warps of this CTA
+        mbar_init(&sm.out_empty, 4);                                   // the output warps
         for (int i = 0; i < NK; ++i) {
             mbar_init(&sm.k_full[i], 1);
             mbar_init(&sm.k_empty[i], 1);
@@ -386,6 +434,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
     const uint32_t tmem = sm.tmem_base;
     bool ok = true;
 
+    if (warp >= 8 && warp < 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 8) {
         // ---------------- TMA of Q and K ----------------
         if (lane == 0) {
@@ -491,13 +541,59 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
                 g += nblk;
             }
         }
+    }
+    } else if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        // ---------------- output: O / l * sigmoid(gate), 32 rows a warp ----------------
+        // a lane has 8 dims of a row; gates are fetched to L2 at the tile's start, to registers
+        // AHEAD rows ahead
+        constexpr int AHEAD = 8;
+        const int r0 = 32 * (warp - 12);
+        while (next_tile()) {
+            const int rows = (int)max((int64_t)0, min((int64_t)32, tl.T - tl.q0 - r0));   // that exist
+            const int64_t first = (tl.row + r0) * nq + qh;             // (row, head) of the first
+            const T* gates = q_gate + first * QG_ROW + HD + 8 * lane;
+            T* to = out + first * HD + 8 * lane;
+            for (int i = lane; i < rows * (HD * (int)sizeof(T) / 128); i += 32) {
+                constexpr int LINES = HD * (int)sizeof(T) / 128;       // 128-byte lines of a row's gates
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(
+                    q_gate + (first + (int64_t)(i / LINES) * nq) * QG_ROW + HD + (i % LINES) * (128 / (int)sizeof(T))));
+            }
+            decltype(load4(q_gate)) g0[AHEAD], g1[AHEAD];
+            auto load_gates = [&](int i) {
+                const T* p = gates + min(i, rows - 1) * (nq * QG_ROW);
+                g0[i % AHEAD] = load4(p);
+                g1[i % AHEAD] = load4(p + 4);
+            };
+            if (rows > 0) {
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) load_gates(i);
+            }
+            wait(&sm.out_full, (round - 1) & 1, err, ok);
+#pragma unroll 1
+            for (int i0 = 0; ok && i0 < rows; i0 += AHEAD) {
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    const int i = i0 + k;
+                    const uint4 h = sm.out[r0 + i][lane ^ (i & 7)];
+                    const float4 w0 = as_f32(g0[k]), w1 = as_f32(g1[k]);
+                    load_gates(i + AHEAD);
+                    const float2 a = gate2(h.x, w0.x, w0.y), b = gate2(h.y, w0.z, w0.w);
+                    const float2 c = gate2(h.z, w1.x, w1.y), e = gate2(h.w, w1.z, w1.w);
+                    if (i < rows)
+                        store8(to + i * (nq * HD), make_float4(a.x, a.y, b.x, b.y), make_float4(c.x, c.y, e.x, e.y));
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.out_empty);
+        }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
         // ---------------- softmax: 8 warps, thread = (query row, key half) ----------------
         const int r = 32 * (warp & 3) + lane;                          // TMEM lane = query row
         const int hf = warp >> 2;                                      // keys [64 hf, 64 hf + 64) of a block
         const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t p_bar[2] = {peer_addr(&sm.p_full[0], 0), peer_addr(&sm.p_full[1], 0)};
-        float (*stage)[32] = sm.out[warp];
         uint32_t g = 0;                                                // blocks so far
         while (next_tile()) {
             const int64_t qpos = tl.base + tl.q0 + r;                      // absolute position of this query row
@@ -569,10 +665,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
                     uint64_t acc0 = f2(0.0f, 0.0f), acc1 = acc0;
 #pragma unroll
                     for (int c = 0; c < 64; c += 4) {
-                        float x0, x1, x2, x3;
+                        float x0, x1, p2, p3;
                         f2_split(sub_f2(f2(s[c], s[c + 1]), mm), x0, x1);
-                        f2_split(sub_f2(f2(s[c + 2], s[c + 3]), mm), x2, x3);
-                        const float p0 = ex2(x0), p1 = ex2(x1), p2 = ex2(x2), p3 = ex2(x3);
+                        const float p0 = ex2(x0), p1 = ex2(x1);
+                        const uint64_t x23 = sub_f2(f2(s[c + 2], s[c + 3]), mm);
+                        if (c % 8 == 0) {                                  // a quarter of them off the special-function unit
+                            ex2_poly(x23, p2, p3);
+                        } else {
+                            float x2, x3;
+                            f2_split(x23, x2, x3);
+                            p2 = ex2(x2);
+                            p3 = ex2(x3);
+                        }
                         acc0 = add_f2(acc0, f2(p0, p1));
                         acc1 = add_f2(acc1, f2(p2, p3));
                         pk[c / 2] = pack_f16(p0, p1);
@@ -589,53 +693,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
                 __syncwarp();
                 if (lane == 0) arrive_at(p_bar[st]);
             }
-            // epilogue: O / l * sigmoid(gate), the warp's 32 rows x 128 dims [128 hf, 128 hf + 128) in four
-            // parts of 32 dims, through shared memory, so that gates are read and outputs written 8 lanes a
-            // row.  The gates of a part are requested before the part ahead of it is worked on.
-            const int64_t row0 = tl.row + 32 * (warp & 3);
-            const int rows = (int)max((int64_t)0, min((int64_t)32, tl.T - tl.q0 - 32 * (warp & 3)));   // that exist
-            const int c = lane & 7, quarter = lane >> 3;                   // 4 dims of every fourth row
-            decltype(load4(q_gate)) gate[8];
-            auto load_gates = [&](int part) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int row = min(4 * i + quarter, rows - 1);
-                    gate[i] = load4(q_gate + ((row0 + row) * nq + qh) * QG_ROW + HD + 128 * hf + 32 * part + 4 * c);
-                }
-            };
-            if (rows > 0) load_gates(0);
+            // O / l of this thread's row, dims [128 hf, 128 hf + 128), to the output warps
             sm.red_l[hf][r] = l_run;
             named_bar_sync(1, 256);
             const float inv_l = 1.0f / (l_run + sm.red_l[hf ^ 1][r]);
+            if (round > 1) wait(&sm.out_empty, round & 1, err, ok);
             wait(&sm.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, err, ok);
-            if (__all_sync(0xffffffffu, ok) && rows > 0) {
-                fence_after_sync();
+            __syncwarp();
+            fence_after_sync();
 #pragma unroll
-                for (int part = 0; part < 4; ++part) {
-                    const int c0 = 128 * hf + 32 * part;
-                    float o[32];
-                    tmem_ld32(tmem + lane_off + O_COL + c0, o);
-                    __syncwarp();
+            for (int c0 = 0; c0 < 128; c0 += 32) {
+                float o[32];
+                tmem_ld32(tmem + lane_off + O_COL + 128 * hf + c0, o);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)                            // 16-byte words in swizzled order
-                        *reinterpret_cast<float4*>(&stage[lane][4 * (i ^ (lane & 7))]) =
-                            make_float4(o[4 * i] * inv_l, o[4 * i + 1] * inv_l, o[4 * i + 2] * inv_l, o[4 * i + 3] * inv_l);
-                    __syncwarp();
-                    float4 w[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) w[i] = as_f32(gate[i]);
-                    if (part < 3) load_gates(part + 1);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int row = 4 * i + quarter;
-                        const float4 x = *reinterpret_cast<const float4*>(&stage[row][4 * (c ^ (row & 7))]);
-                        if (row < rows)
-                            store4(out + ((row0 + row) * nq + qh) * HD + c0 + 4 * c,
-                                   make_float4(x.x * sigmoid(w[i].x), x.y * sigmoid(w[i].y), x.z * sigmoid(w[i].z),
-                                               x.w * sigmoid(w[i].w)));
-                    }
-                }
+                for (int i = 0; i < 32; i += 8)
+                    sm.out[r][((128 * hf + c0 + i) / 8) ^ (r & 7)] =
+                        make_uint4(pack_f16(o[i] * inv_l, o[i + 1] * inv_l), pack_f16(o[i + 2] * inv_l, o[i + 3] * inv_l),
+                                   pack_f16(o[i + 4] * inv_l, o[i + 5] * inv_l), pack_f16(o[i + 6] * inv_l, o[i + 7] * inv_l));
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.out_full);
         }
     }
     // neither CTA leaves, or frees TMEM, while the other's products or arrivals may touch it; after
