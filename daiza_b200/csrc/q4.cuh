@@ -52,12 +52,33 @@ __device__ __forceinline__ void settle() {
     for (int i = 0; i < 1000; ++i) __nanosleep(1000);
 }
 
+// ---- f32 pairs in one operation --------------------------------------------------------
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+    return d;
+}
+__device__ __forceinline__ void unpack2(uint64_t a, float& x, float& y) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
 // ---- scales ------------------------------------------------------------------------
 // s (as stored byte) from the group's largest magnitude: 4 significant bits of amax / 7 by
 // f32, then decided exactly.  A border lies half a step from s, at 7 s +- 3.5 steps of
-// amax, and amax - 7 s is exact there; so no division, and K's f64 and V's f32 values
-// are treated alike.
-__device__ __forceinline__ uint32_t scale_byte(double amax) {
+// amax, and amax - 7 s is exact there (the two are within a factor of 2), in F's precision:
+// no division, and f64 for f64 values alone.
+template <typename F>
+__device__ __forceinline__ uint32_t scale_byte(F amax) {
     const float t = fminf((float)amax * (1.0f / 7.0f), SCALE_MAX);
     uint32_t byte;                                             // exponent << 3 | 3 fraction bits, of f16
     if (t < 6.103515625e-05f) {                                // 2^-14: the grid is 2^-17, f16's subnormals
@@ -69,7 +90,7 @@ __device__ __forceinline__ uint32_t scale_byte(double amax) {
     const float s = __half2float(__ushort_as_half((unsigned short)(byte << 7)));
     const float step = __half2float(__ushort_as_half((unsigned short)((byte + 1) << 7))) - s;
     const bool binade = (byte & 7u) == 0u && byte > 8u;        // the step below is half as long
-    const double d = fma(-7.0, (double)s, amax), up = 3.5 * (double)step, down = binade ? 0.5 * up : up;
+    const F d = fma((F)-7, (F)s, amax), up = (F)3.5 * (F)step, down = binade ? (F)0.5 * up : up;
     const bool odd = byte & 1u;
     if (d > up || (d == up && odd)) byte += 1;
     else if (d < -down || (d == -down && odd)) byte -= 1;
@@ -78,18 +99,21 @@ __device__ __forceinline__ uint32_t scale_byte(double amax) {
 __device__ __forceinline__ float scale_value(uint32_t byte) {
     return __half2float(__ushort_as_half((unsigned short)(byte << 7)));
 }
-// code + 8 of x: the nearest whole multiple of s (ties to even), decided exactly.
-// inv = 1 / s (0 if s is 0), an approximation that the remainder corrects.
-__device__ __forceinline__ uint32_t code8(double x, double s, float inv) {
-    float kf = rintf(fminf(fmaxf((float)x * inv, -7.0f), 7.0f));
-    const double d = fma((double)-kf, s, x), h = 0.5 * s;      // exact where it is near a border
-    const bool odd = ((int)kf) & 1;
-    if (d > h || (d == h && odd)) kf += 1.0f;
-    else if (d < -h || (d == -h && odd)) kf -= 1.0f;
-    kf = fminf(fmaxf(kf, -7.0f), 7.0f);
-    return s > 0.0 ? (uint32_t)((int)kf + 8) : 8u;
+// code + 8 of x: the nearest whole multiple k s (ties to even) within 7 s, decided exactly.
+// inv = 1 / s (0 if s is 0), an approximation that the remainder corrects.  The remainder is
+// exact in F where k s and x are within a factor of 2, and for k = 0; that leaves |k| = 1 with
+// |x| just below s / 2, where it may be rounded to s / 2: the tie goes to 0, as x does.
+// half, below: s / 2 and the next smaller F.
+template <typename F>
+__device__ __forceinline__ uint32_t code8(F x, F s, float inv, F half, F below) {
+    x = fmin(fmax(x, (F)-7 * s), (F)7 * s);
+    float t = fmaf((float)x, inv, 12582920.0f);                // 1.5 * 2^23 + 8: rounds to an integer, k + 8 its low bits
+    const F d = fma((F)(12582920.0f - t), s, x);
+    if (fabs(d) > ((__float_as_uint(t) & 1u) ? below : half)) t += d > (F)0 ? 1.0f : -1.0f;
+    return __float_as_uint(t) & 15u;
 }
-__device__ __forceinline__ double not_nan(double x) { return x == x ? x : 0.0; }
+__device__ __forceinline__ float next_below(float x) { return __uint_as_float(__float_as_uint(x) - 1u); }   // x > 0
+__device__ __forceinline__ double next_below(double x) { return __longlong_as_double(__double_as_longlong(x) - 1); }
 
 // two scale bytes (bits 0..7 and 16..23) -> an f16 pair
 __device__ __forceinline__ uint32_t scale_pair(uint32_t bytes) { return bytes << 7; }
@@ -195,21 +219,29 @@ __device__ __forceinline__ int split_dim(int lane, int run) {
 // 4 l .. 4 l + 3 in lanes 0..7.
 __device__ __forceinline__ void norm_rotate_split(float (&x)[8], const float (&w)[8], const float2 (&cs)[4], float eps,
                                                   int lane) {
-    float ss = 0.0f;
+    uint64_t y[4], ss = 0ull;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-    const float v = fmaf(warp_sum(ss), 1.0f / (float)HD, eps), g = rsqrtf(v);
+    for (int i = 0; i < 4; ++i) {
+        y[i] = pack2(x[2 * i], x[2 * i + 1]);
+        ss = fma2(y[i], y[i], ss);
+    }
+    float s0, s1;
+    unpack2(ss, s0, s1);
+    const float v = fmaf(warp_sum(s0 + s1), 1.0f / (float)HD, eps), g = rsqrtf(v);
     const float inv = fmaf(fmaf(-v * g, g, 1.0f), 0.5f * g, g);   // one Newton step: to the last bit or so
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = (x[e] * inv) * w[e];
+    for (int i = 0; i < 4; ++i) y[i] = mul2(mul2(y[i], pack2(inv, inv)), pack2(w[2 * i], w[2 * i + 1]));
     if (lane < 8) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float a = x[e], b = x[e + 4];
-            x[e] = fmaf(a, cs[e].x, b * cs[e].y);
-            x[e + 4] = fmaf(b, cs[e].x, a * cs[e].y);
+        for (int i = 0; i < 2; ++i) {
+            const uint64_t c = pack2(cs[2 * i].x, cs[2 * i + 1].x), s = pack2(cs[2 * i].y, cs[2 * i + 1].y);
+            const uint64_t a = y[i], b = y[i + 2];
+            y[i] = fma2(a, c, mul2(b, s));
+            y[i + 2] = fma2(b, c, mul2(a, s));
         }
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpack2(y[i], x[2 * i], x[2 * i + 1]);
 }
 // The (cos, sin) that norm_rotate_split wants, from a lane's own pair (lane = pair).
 __device__ __forceinline__ void spread_pairs(float2 own, float2 (&cs)[4], int lane) {
@@ -254,20 +286,103 @@ __device__ __forceinline__ void load_split(const T* row, int lane, float (&x)[8]
     r.values(x);
 }
 
-// Quantise the row: the stored scale byte of this lane's group and the 8 codes + 8.
-__device__ __forceinline__ uint32_t quantise(double (&x)[8], uint32_t (&code)[8]) {
-    double a = 0.0;
+// Quantise the row, exactly: the stored scale byte of this lane's group and the 8 codes + 8.
+template <typename F>
+__device__ __forceinline__ uint32_t quantise(F (&x)[8], uint32_t (&code)[8]) {
+    F a = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        x[e] = not_nan(x[e]);
+        x[e] = x[e] == x[e] ? x[e] : (F)0;
         a = fmax(a, fabs(x[e]));
     }
     a = fmax(a, __shfl_xor_sync(0xffffffffu, a, 1));
     a = fmax(a, __shfl_xor_sync(0xffffffffu, a, 2));
     const uint32_t sb = scale_byte(a);
-    const float s = scale_value(sb), inv = s > 0.0f ? 1.0f / s : 0.0f;
+    const float s = scale_value(sb);
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    inv = s > 0.0f ? inv : 0.0f;
+    const F half = (F)0.5 * (F)s, below = s > 0.0f ? next_below(half) : half;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) code[e] = code8(x[e], (double)s, inv);
+    for (int e = 0; e < 8; ++e) code[e] = code8(x[e], (F)s, inv, half, below);
+    return sb;
+}
+
+// The same from f32 values that are off by at most 7e-7 of their own magnitude and of `from`
+// (0, or what they were computed from): false where that could change a code or a scale, that
+// is where one lies within about 1e-5 of a border, and for NaN.  A row is undecided about once
+// in 50 times; f64 for every row took three times as many instructions.
+__device__ __forceinline__ bool quantise_f32(const float (&x)[8], float from, uint32_t (&code)[8], uint32_t& sb) {
+    float a = 0.0f, sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        a = fmaxf(a, fabsf(x[e]));
+        sum += x[e];
+    }
+    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
+    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+    // |error of a value| <= 7e-7 (a + from) <= 3.5e-6 a = 2.5e-5 s where `from` is at most 4 a
+    bool ok = sum == sum && from <= 4.0f * a;
+    const float t = fminf(a * (1.0f / 7.0f), SCALE_MAX);
+    if (t < 6.103515625e-05f) {                                // as in scale_byte
+        const float u = t * 131072.0f, r = rintf(u);
+        sb = (uint32_t)(int)r;
+        ok = ok && fabsf(u - r) < 0.4999f;
+    } else {
+        const uint32_t b = __float_as_uint(t);
+        sb = ((b + 0x7FFFFu + ((b >> 20) & 1u)) >> 20) - ((127 - 15) << 3);
+        ok = ok && (b & 0xFFFFFu) - (0x80000u - 128u) > 256u;  // 128 steps of 2^-24..2^-23 from a border
+    }
+    const float s = scale_value(sb);
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    inv = s > 0.0f ? inv : 0.0f;
+    float off = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float u = fminf(fmaxf(x[e] * inv, -7.0f), 7.0f), r = u + 12582920.0f;   // 1.5 * 2^23 + 8: rounds to integers
+        code[e] = __float_as_uint(r) & 15u;
+        off = fmaxf(off, fabsf(u - (r - 12582920.0f)));
+    }
+    return ok && off < 0.5f - 4e-5f;
+}
+// A row of K: normalised, rotated, quantised as in f64.  cs: the warp's place for 32 angles, in
+// which float2 (rope_cs_f32) are ready; t, h, w: the positions they are of.
+__device__ __forceinline__ uint32_t quantise_key(const float (&x)[8], const float* __restrict__ weight, double2* cs,
+                                                 const RopeAxes& axes, int t, int h, int w, float eps, int lane,
+                                                 uint32_t (&code)[8]) {
+    uint32_t sb;
+    // f32: the norm is off by at most 5e-7 (13 roundings of its sum, halved, and its root), a value by two
+    // roundings more, sine and cosine by 3.1e-7 (1.9e-7 of them the angle's rounding)
+    float y[8], ss = 0.0f, from = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+    const float v = fmaf(warp_sum(ss), 1.0f / (float)HD, eps), inv = 1.0f / sqrtf(v);
+    const float4* wp = reinterpret_cast<const float4*>(weight) + 2 * lane;
+    const float4 w0 = wp[0], w1 = wp[1];
+    const float wv[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (x[e] * inv) * wv[e];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float p = __shfl_xor_sync(0xffffffffu, y[e], 4);
+        if (lane < 8) {
+            const float2 c = reinterpret_cast<const float2*>(cs)[8 * (lane & 3) + e];
+            from = fmaxf(from, fmaxf(fabsf(y[e]), fabsf(p)));
+            y[e] = fmaf(y[e], c.x, p * c.y);
+        }
+    }
+    bool ok = quantise_f32(y, from, code, sb);
+    ok = ok && v > 1e-30f && v < 1e30f;                        // no overflow or lost bits on the way
+    if (__any_sync(0xffffffffu, !ok)) {
+        cs[lane] = rope_cs(axes, lane, t, h, w);
+        __syncwarp();
+        double z[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] = x[e];
+        norm_rotate(z, weight, cs, eps, lane);
+        sb = quantise(z, code);
+    }
     return sb;
 }
 
@@ -302,27 +417,29 @@ __device__ __forceinline__ void put_v_scale(uint8_t* tile, int p, int lane, uint
         tile[OFF_VS + ((lane >> 2) * 4 + ((p & 7) >> 1)) * 4 + (p & 1) + (p >> 3) * 2] = (uint8_t)sb;
 }
 
-// V codes of several positions of one tile, from the warps of a block of 512 threads (a
-// word holds four positions): gathered in shared memory, then merged into the tile.
+// V codes of positions [p0, p1) of one tile, from the warps of a block of 512 threads (a word
+// holds four positions): gathered in shared memory, then merged into the tile.
 struct TileMerge {
-    uint32_t code[512], mask[512];
+    uint32_t code[512];
     __device__ __forceinline__ void begin() {
-        code[threadIdx.x] = mask[threadIdx.x] = 0u;
+        code[threadIdx.x] = 0u;
         __syncthreads();
     }
     // position p's codes, by one warp
     __device__ __forceinline__ void add(int p, int lane, const uint32_t (&c)[8]) {
         const int at = (v_at(lane & 3, lane >> 2, (p & 7) >> 1) - OFF_V) / 4, sh = (p & 1) * 16 + (p >> 3) * 4;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            atomicOr(&code[at + i], (c[2 * i] | c[2 * i + 1] << 8) << sh);
-            atomicOr(&mask[at + i], 0x0F0Fu << sh);
-        }
+        for (int i = 0; i < 4; ++i) atomicOr(&code[at + i], (c[2 * i] | c[2 * i + 1] << 8) << sh);
     }
-    __device__ __forceinline__ void end(uint8_t* tile) {
+    __device__ __forceinline__ void end(uint8_t* tile, int p0, int p1) {
         __syncthreads();
         uint32_t* w = reinterpret_cast<uint32_t*>(tile + OFF_V) + threadIdx.x;
-        const uint32_t m = mask[threadIdx.x];
+        uint32_t m = 0;                                        // the nibbles of column c's positions 2c, 2c + 1, 2c + 8, 2c + 9
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int p = 2 * ((threadIdx.x >> 5) & 3) + (k & 1) + 8 * (k >> 1);
+            if (p >= p0 && p < p1) m |= 0x0F0Fu << ((p & 1) * 16 + (p >> 3) * 4);
+        }
         if (m == 0xFFFFFFFFu) *w = code[threadIdx.x];
         else if (m) *w = (*w & ~m) | code[threadIdx.x];
     }

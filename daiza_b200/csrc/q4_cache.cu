@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(512) q4_import_kernel(Q4Slot slot, int kvc, in
     const int64_t row = t * Q4_TILE + p;
     if (row0 + row < len) {
         const size_t at = ((size_t)row * kvc + kvh) * HD + 8 * lane;
-        double x[8], y[8];
+        float x[8], y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             x[e] = k[at + e];
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(512) q4_import_kernel(Q4Slot slot, int kvc, in
         merge.add(p, lane, code);
         put_v_scale(tile, p, lane, sb);
     }
-    merge.end(tile);
+    merge.end(tile, 0, (int)min((int64_t)Q4_TILE, len - row0 - t * Q4_TILE));
 }
 
 // ---- accumulated weights ---------------------------------------------------------------

@@ -41,10 +41,9 @@ __global__ void __launch_bounds__(256) q4_prep_kernel(const __grid_constant__ Ro
     const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int kvc = d.kvc, nq = GRP * kvc;
     const int task = blockIdx.y * 8 + warp;
-    // before the wait: the angles (f32 for q, f64 for K)
+    // before the wait: the angles
     float2* csf = reinterpret_cast<float2*>(cs[warp]);
-    if (task < nq) csf[lane] = rope_cs_f32(axes, lane, pos.p[b][0], pos.p[b][1], pos.p[b][2]);
-    else cs[warp][lane] = rope_cs(axes, lane, pos.p[b][0], pos.p[b][1], pos.p[b][2]);
+    csf[lane] = rope_cs_f32(axes, lane, pos.p[b][0], pos.p[b][1], pos.p[b][2]);
     __syncwarp();
     // As in gqa_prep: everything before this grid is complete (inputs, caches, q_frag)
     // before the split grid may start streaming old tiles.
@@ -93,12 +92,11 @@ __global__ void __launch_bounds__(256) q4_prep_kernel(const __grid_constant__ Ro
         const size_t at = ((size_t)b * kvc + kvh) * HD + 8 * lane;
         const float4 k0 = *reinterpret_cast<const float4*>(k_in + at), k1 = *reinterpret_cast<const float4*>(k_in + at + 4);
         const float4 v0 = *reinterpret_cast<const float4*>(v_in + at), v1 = *reinterpret_cast<const float4*>(v_in + at + 4);
-        double x[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
-        norm_rotate(x, k_norm, cs[warp], eps, lane);
+        const float x[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
+        float y[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
         uint32_t code[8];
-        uint32_t sb = quantise(x, code);
+        uint32_t sb = quantise_key(x, k_norm, cs[warp], axes, pos.p[b][0], pos.p[b][1], pos.p[b][2], eps, lane, code);
         put_k(tile, p, lane, code, sb);
-        double y[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
         sb = quantise(y, code);
         uint4* vw = v_words(tile, lane, (p & 7) >> 1);
         uint4 w = *vw;
@@ -180,21 +178,13 @@ __device__ __forceinline__ void mma0(float (&c)[4], uint32_t a0, uint32_t a1, ui
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
-// f32 pairs: a += (x, y), a *= s
+// f32 pairs: a += (x, y)
 __device__ __forceinline__ void add2(uint64_t& a, float x, float y) {
     asm("{.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tadd.rn.f32x2 %0, %0, t;}" : "+l"(a) : "f"(x), "f"(y));
 }
-__device__ __forceinline__ void mul2(uint64_t& a, uint64_t s) {
-    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a) : "l"(s));
-}
-__device__ __forceinline__ uint64_t pair_of(float x, float y) {
-    uint64_t d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
-    return d;
-}
 __device__ __forceinline__ float2 halves(uint64_t a) {
     float2 d;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(a));
+    unpack2(a, d.x, d.y);
     return d;
 }
 __device__ __forceinline__ float ex2f(float x) {
@@ -280,11 +270,11 @@ __device__ __forceinline__ void attend(State& st, const uint8_t* tiles, const ui
         st.l *= a;
         st.m = m_new;
         const float a0 = __shfl_sync(0xffffffffu, a, 8 * c), a1 = __shfl_sync(0xffffffffu, a, 8 * c + 4);
-        const uint64_t aa = pair_of(a0, a1);
+        const uint64_t aa = pack2(a0, a1);
 #pragma unroll
         for (int m = 0; m < 16; ++m) {
-            mul2(st.o[m][0], aa);
-            mul2(st.o[m][1], aa);
+            st.o[m][0] = mul2(st.o[m][0], aa);
+            st.o[m][1] = mul2(st.o[m][1], aa);
         }
     }
     const float off = P_LOG2 - st.m;

@@ -52,7 +52,7 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 template <typename T>
-__device__ __forceinline__ void load_row(const T* p, double (&x)[8]) {
+__device__ __forceinline__ void load_row(const T* p, float (&x)[8]) {
     const float4 a = as_f32(load4(p)), b = as_f32(load4(p + 4));
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
     x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
@@ -101,24 +101,23 @@ __global__ void __launch_bounds__(32 * PREP_WARPS)
             const int64_t row = d.row0[s] + (slot_pos - base);
             int p[3];
             angles_at(s, row, p);
-            cs[warp][lane] = rope_cs(axes, lane, p[0], p[1], p[2]);
+            reinterpret_cast<float2*>(cs[warp])[lane] = rope_cs_f32(axes, lane, p[0], p[1], p[2]);
             __syncwarp();
             const size_t out = ((size_t)kvh * keys + d.key0[s] + slot_pos) * HD + 8 * lane;
-            double x[8];
+            float x[8], y[8];
             load_row(k + (row * kvc + kvh) * HD + 8 * lane, x);
-            norm_rotate(x, k_norm, cs[warp], eps, lane);
+            load_row(v + (row * kvc + kvh) * HD + 8 * lane, y);
             uint32_t code[8];
-            uint32_t sb = quantise(x, code);
+            uint32_t sb = quantise_key(x, k_norm, cs[warp], axes, p[0], p[1], p[2], eps, lane, code);
             put_k(tile, warp, lane, code, sb);
             *reinterpret_cast<uint4*>(kf + out) = held(code, sb);
-            load_row(v + (row * kvc + kvh) * HD + 8 * lane, x);
-            sb = quantise(x, code);
+            sb = quantise(y, code);
             merge.add(warp, lane, code);
             put_v_scale(tile, warp, lane, sb);
             *reinterpret_cast<uint4*>(vf + out) = held(code, sb);
             if (track && lane == 0) slot.wts[(size_t)kvh * slot.cap + slot_pos] = 0.0f;
         }
-        merge.end(tile);
+        merge.end(tile, base - t16 * Q4_TILE, base + d.T(s) - t16 * Q4_TILE);
         return;
     }
     block -= (int64_t)d.at0[d.n] * kvc;
@@ -287,27 +286,14 @@ __device__ __forceinline__ float max3f(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-__device__ __forceinline__ uint64_t f2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void f2_split(uint64_t r, float& a, float& b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
-}
-__device__ __forceinline__ uint64_t sub_f2(uint64_t a, uint64_t b) {
+__device__ __forceinline__ uint64_t sub2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
 // 2^x without the special-function unit, x at most 2^7: x = n + f with n nearest, a polynomial of
@@ -315,36 +301,31 @@ __device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
 // f16 rounding), n added to its exponent.  Below -126: 2^-126.
 __device__ __forceinline__ void ex2_poly(uint64_t x, float& p0, float& p1) {
     float a, b;
-    f2_split(x, a, b);
-    x = f2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
-    const uint64_t big = f2(12582912.0f, 12582912.0f);                 // 1.5 * 2^23: sums are rounded to integers
-    const uint64_t t = add_f2(x, big), f = sub_f2(x, sub_f2(t, big));
-    uint64_t y = fma_f2(f2(0.0095701f, 0.0095701f), f, f2(0.05591786f, 0.05591786f));
-    y = fma_f2(y, f, f2(0.24024745f, 0.24024745f));
-    y = fma_f2(y, f, f2(0.69312181f, 0.69312181f));
-    y = fma_f2(y, f, f2(0.99999926f, 0.99999926f));
+    unpack2(x, a, b);
+    x = pack2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+    const uint64_t big = pack2(12582912.0f, 12582912.0f);                 // 1.5 * 2^23: sums are rounded to integers
+    const uint64_t t = add2(x, big), f = sub2(x, sub2(t, big));
+    uint64_t y = fma2(pack2(0.0095701f, 0.0095701f), f, pack2(0.05591786f, 0.05591786f));
+    y = fma2(y, f, pack2(0.24024745f, 0.24024745f));
+    y = fma2(y, f, pack2(0.69312181f, 0.69312181f));
+    y = fma2(y, f, pack2(0.99999926f, 0.99999926f));
     float t0, t1;
-    f2_split(t, t0, t1);
-    f2_split(y, a, b);
+    unpack2(t, t0, t1);
+    unpack2(y, a, b);
     p0 = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
     p1 = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
-}
-__device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
 }
 // (a sigmoid(x), b sigmoid(y)) of f16 a and b, to 2^-20 or so, below the products' f16 rounding; one
 // reciprocal for both.  Below 2^-60 a sigmoid counts as 2^-60: the denominators' product is finite.
 __device__ __forceinline__ float2 gate2(uint32_t ab, float x, float y) {
     float s, t, u, w, r;
-    f2_split(mul_f2(f2(x, y), f2(-LOG2E, -LOG2E)), s, t);
-    const uint64_t uw = add_f2(f2(ex2(fminf(s, 60.0f)), ex2(fminf(t, 60.0f))), f2(1.0f, 1.0f));
-    f2_split(uw, u, w);
+    unpack2(mul2(pack2(x, y), pack2(-LOG2E, -LOG2E)), s, t);
+    const uint64_t uw = add2(pack2(ex2(fminf(s, 60.0f)), ex2(fminf(t, 60.0f))), pack2(1.0f, 1.0f));
+    unpack2(uw, u, w);
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(u * w));
     const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&ab));
     float2 out;
-    f2_split(mul_f2(f2(h.x, h.y), mul_f2(f2(w, u), f2(r, r))), out.x, out.y);
+    unpack2(mul2(pack2(h.x, h.y), mul2(pack2(w, u), pack2(r, r))), out.x, out.y);
     return out;
 }
 __device__ __forceinline__ void store8(float* p, float4 a, float4 b) {
@@ -661,29 +642,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
                 }
                 uint32_t pk[32];
                 {
-                    const uint64_t mm = f2(m_run, m_run);
-                    uint64_t acc0 = f2(0.0f, 0.0f), acc1 = acc0;
+                    const uint64_t mm = pack2(m_run, m_run);
+                    uint64_t acc0 = pack2(0.0f, 0.0f), acc1 = acc0;
 #pragma unroll
                     for (int c = 0; c < 64; c += 4) {
                         float x0, x1, p2, p3;
-                        f2_split(sub_f2(f2(s[c], s[c + 1]), mm), x0, x1);
+                        unpack2(sub2(pack2(s[c], s[c + 1]), mm), x0, x1);
                         const float p0 = ex2(x0), p1 = ex2(x1);
-                        const uint64_t x23 = sub_f2(f2(s[c + 2], s[c + 3]), mm);
+                        const uint64_t x23 = sub2(pack2(s[c + 2], s[c + 3]), mm);
                         if (c % 8 == 0) {                                  // a quarter of them off the special-function unit
                             ex2_poly(x23, p2, p3);
                         } else {
                             float x2, x3;
-                            f2_split(x23, x2, x3);
+                            unpack2(x23, x2, x3);
                             p2 = ex2(x2);
                             p3 = ex2(x3);
                         }
-                        acc0 = add_f2(acc0, f2(p0, p1));
-                        acc1 = add_f2(acc1, f2(p2, p3));
+                        acc0 = add2(acc0, pack2(p0, p1));
+                        acc1 = add2(acc1, pack2(p2, p3));
                         pk[c / 2] = pack_f16(p0, p1);
                         pk[c / 2 + 1] = pack_f16(p2, p3);
                     }
                     float u0, u1;
-                    f2_split(add_f2(acc0, acc1), u0, u1);
+                    unpack2(add2(acc0, acc1), u0, u1);
                     l_run += u0 + u1;
                 }
                 // P goes over the first 64 columns of its own S buffer (the previous reader of these
