@@ -219,29 +219,21 @@ __device__ __forceinline__ int split_dim(int lane, int run) {
 // 4 l .. 4 l + 3 in lanes 0..7.
 __device__ __forceinline__ void norm_rotate_split(float (&x)[8], const float (&w)[8], const float2 (&cs)[4], float eps,
                                                   int lane) {
-    uint64_t y[4], ss = 0ull;
+    float ss = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        y[i] = pack2(x[2 * i], x[2 * i + 1]);
-        ss = fma2(y[i], y[i], ss);
-    }
-    float s0, s1;
-    unpack2(ss, s0, s1);
-    const float v = fmaf(warp_sum(s0 + s1), 1.0f / (float)HD, eps), g = rsqrtf(v);
+    for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+    const float v = fmaf(warp_sum(ss), 1.0f / (float)HD, eps), g = rsqrtf(v);
     const float inv = fmaf(fmaf(-v * g, g, 1.0f), 0.5f * g, g);   // one Newton step: to the last bit or so
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = mul2(mul2(y[i], pack2(inv, inv)), pack2(w[2 * i], w[2 * i + 1]));
+    for (int e = 0; e < 8; ++e) x[e] = (x[e] * inv) * w[e];
     if (lane < 8) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint64_t c = pack2(cs[2 * i].x, cs[2 * i + 1].x), s = pack2(cs[2 * i].y, cs[2 * i + 1].y);
-            const uint64_t a = y[i], b = y[i + 2];
-            y[i] = fma2(a, c, mul2(b, s));
-            y[i + 2] = fma2(b, c, mul2(a, s));
+        for (int e = 0; e < 4; ++e) {
+            const float a = x[e], b = x[e + 4];
+            x[e] = fmaf(a, cs[e].x, b * cs[e].y);
+            x[e + 4] = fmaf(b, cs[e].x, a * cs[e].y);
         }
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) unpack2(y[i], x[2 * i], x[2 * i + 1]);
 }
 // The (cos, sin) that norm_rotate_split wants, from a lane's own pair (lane = pair).
 __device__ __forceinline__ void spread_pairs(float2 own, float2 (&cs)[4], int lane) {
@@ -357,7 +349,8 @@ __device__ __forceinline__ uint32_t quantise_key(const float (&x)[8], const floa
     float y[8], ss = 0.0f, from = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-    const float v = fmaf(warp_sum(ss), 1.0f / (float)HD, eps), inv = 1.0f / sqrtf(v);
+    const float v = fmaf(warp_sum(ss), 1.0f / (float)HD, eps), g = rsqrtf(v);
+    const float inv = fmaf(fmaf(-v * g, g, 1.0f), 0.5f * g, g);
     const float4* wp = reinterpret_cast<const float4*>(weight) + 2 * lane;
     const float4 w0 = wp[0], w1 = wp[1];
     const float wv[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
@@ -421,11 +414,9 @@ __device__ __forceinline__ void put_v_scale(uint8_t* tile, int p, int lane, uint
 // holds four positions): gathered in shared memory, then merged into the tile.
 struct TileMerge {
     uint32_t code[512];
-    __device__ __forceinline__ void begin() {
-        code[threadIdx.x] = 0u;
-        __syncthreads();
-    }
-    // position p's codes, by one warp
+    // by every thread before the first tile (end() leaves it ready for the next)
+    __device__ __forceinline__ void begin() { code[threadIdx.x] = 0u; }
+    // position p's codes, by one warp, after a barrier behind begin() or the last end()
     __device__ __forceinline__ void add(int p, int lane, const uint32_t (&c)[8]) {
         const int at = (v_at(lane & 3, lane >> 2, (p & 7) >> 1) - OFF_V) / 4, sh = (p & 1) * 16 + (p >> 3) * 4;
 #pragma unroll
@@ -440,8 +431,10 @@ struct TileMerge {
             const int p = 2 * ((threadIdx.x >> 5) & 3) + (k & 1) + 8 * (k >> 1);
             if (p >= p0 && p < p1) m |= 0x0F0Fu << ((p & 1) * 16 + (p >> 3) * 4);
         }
-        if (m == 0xFFFFFFFFu) *w = code[threadIdx.x];
-        else if (m) *w = (*w & ~m) | code[threadIdx.x];
+        const uint32_t c = code[threadIdx.x];
+        if (m == 0xFFFFFFFFu) *w = c;
+        else if (m) *w = (*w & ~m) | c;
+        code[threadIdx.x] = 0u;
     }
 };
 

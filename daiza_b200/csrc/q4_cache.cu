@@ -99,6 +99,7 @@ __global__ void __launch_bounds__(512) q4_import_kernel(Q4Slot slot, int kvc, in
     const int kvh = (int)(blockIdx.x - t * kvc), p = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint8_t* tile = slot.tile(kvh, (row0 >> 4) + t);
     merge.begin();
+    __syncthreads();
     const int64_t row = t * Q4_TILE + p;
     if (row0 + row < len) {
         const size_t at = ((size_t)row * kvc + kvh) * HD + 8 * lane;
@@ -161,7 +162,7 @@ __device__ __forceinline__ void store_split(__nv_bfloat16* row, int lane, const 
 
 // A warp per token and share of its heads: grid (ceil(T / 8), shares).  Several rows are
 // in flight per warp: reading one at a time held the pass at 4.3 TB/s.
-constexpr int MROPE_ROWS = 7;
+constexpr int MROPE_ROWS = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) qk_mrope_kernel(const __grid_constant__ RopeAxes axes, int kvc, int64_t n_tokens,
                                                        const int32_t* __restrict__ pos, const T* __restrict__ q_gate,

@@ -66,18 +66,18 @@ __device__ __forceinline__ uint4 held(const uint32_t (&code)[8], uint32_t sb) {
     return make_uint4(h[0], h[1], h[2], h[3]);
 }
 
-constexpr int PREP_WARPS = 16, PREP_HEADS = 6;   // heads of a token that a warp takes
+constexpr int PREP_WARPS = 16, PREP_ROWS = 4;    // query rows that a warp has in flight
 
-// Blocks [0, at0 kvc): a tile of new rows and a kv head, a warp per position.
+// Blocks [0, at0 kvc / key_heads): a tile of new rows and key_heads kv heads, a warp per position.
 // Then (old0 kvc) blocks: a tile of cached rows or padding, a warp per position.
-// Then: a warp per (token, PREP_HEADS heads).
+// Then: a warp per token and q_heads of its heads.
 template <typename T>
-__global__ void __launch_bounds__(32 * PREP_WARPS)
+__global__ void __launch_bounds__(32 * PREP_WARPS, 2)
     q4_pf_prep_kernel(const __grid_constant__ Prompt d, const __grid_constant__ RopeAxes axes, int kvc,
                       const Q4Slot* __restrict__ slots, const int32_t* __restrict__ pos, const float* __restrict__ q_norm,
                       const float* __restrict__ k_norm, const T* __restrict__ q_gate, const T* __restrict__ k,
                       const T* __restrict__ v, __half* __restrict__ qf, __half* __restrict__ kf, __half* __restrict__ vf,
-                      bool track, float eps) {
+                      int key_heads, int q_heads, bool track, float eps) {
     __shared__ TileMerge merge;
     __shared__ double2 cs[PREP_WARPS][ROPE / 2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nq = GRP * kvc;
@@ -90,37 +90,43 @@ __global__ void __launch_bounds__(32 * PREP_WARPS)
             p[0] = p[1] = p[2] = d.base[s] + (int)(row - d.row0[s]);
         }
     };
-    if (block < (int64_t)d.at0[d.n] * kvc) {
-        const int at = (int)(block / kvc), kvh = (int)(block - (int64_t)at * kvc);
+    const int shares = kvc / key_heads;
+    if (block < (int64_t)d.at0[d.n] * shares) {
+        const int at = (int)(block / shares), kvh0 = (int)(block - (int64_t)at * shares) * key_heads;
         const int s = last_at_or_before(d.at0, d.n, at);
         const int base = d.base[s], t16 = (base >> 4) + (at - d.at0[s]), slot_pos = t16 * Q4_TILE + warp;
         const Q4Slot slot = slots[d.sid[s]];
-        uint8_t* tile = slot.tile(kvh, t16);
+        const bool mine = slot_pos >= base && slot_pos < base + d.T(s);
+        const int64_t row = d.row0[s] + (slot_pos - base);
+        int p[3];
         merge.begin();
-        if (slot_pos >= base && slot_pos < base + d.T(s)) {
-            const int64_t row = d.row0[s] + (slot_pos - base);
-            int p[3];
-            angles_at(s, row, p);
-            reinterpret_cast<float2*>(cs[warp])[lane] = rope_cs_f32(axes, lane, p[0], p[1], p[2]);
-            __syncwarp();
-            const size_t out = ((size_t)kvh * keys + d.key0[s] + slot_pos) * HD + 8 * lane;
-            float x[8], y[8];
-            load_row(k + (row * kvc + kvh) * HD + 8 * lane, x);
-            load_row(v + (row * kvc + kvh) * HD + 8 * lane, y);
-            uint32_t code[8];
-            uint32_t sb = quantise_key(x, k_norm, cs[warp], axes, p[0], p[1], p[2], eps, lane, code);
-            put_k(tile, warp, lane, code, sb);
-            *reinterpret_cast<uint4*>(kf + out) = held(code, sb);
-            sb = quantise(y, code);
-            merge.add(warp, lane, code);
-            put_v_scale(tile, warp, lane, sb);
-            *reinterpret_cast<uint4*>(vf + out) = held(code, sb);
-            if (track && lane == 0) slot.wts[(size_t)kvh * slot.cap + slot_pos] = 0.0f;
+        if (mine) angles_at(s, row, p);
+#pragma unroll 1
+        for (int kvh = kvh0; kvh < kvh0 + key_heads; ++kvh) {
+            uint8_t* tile = slot.tile(kvh, t16);
+            __syncthreads();
+            if (mine) {
+                float x[8], y[8];
+                load_row(k + (row * kvc + kvh) * HD + 8 * lane, x);
+                load_row(v + (row * kvc + kvh) * HD + 8 * lane, y);
+                reinterpret_cast<float2*>(cs[warp])[lane] = rope_cs_f32(axes, lane, p[0], p[1], p[2]);
+                __syncwarp();
+                const size_t out = ((size_t)kvh * keys + d.key0[s] + slot_pos) * HD + 8 * lane;
+                uint32_t code[8];
+                uint32_t sb = quantise_key(x, k_norm, cs[warp], axes, p[0], p[1], p[2], eps, lane, code);
+                put_k(tile, warp, lane, code, sb);
+                *reinterpret_cast<uint4*>(kf + out) = held(code, sb);
+                sb = quantise(y, code);
+                merge.add(warp, lane, code);
+                put_v_scale(tile, warp, lane, sb);
+                *reinterpret_cast<uint4*>(vf + out) = held(code, sb);
+                if (track && lane == 0) slot.wts[(size_t)kvh * slot.cap + slot_pos] = 0.0f;
+            }
+            merge.end(tile, base - t16 * Q4_TILE, base + d.T(s) - t16 * Q4_TILE);
         }
-        merge.end(tile, base - t16 * Q4_TILE, base + d.T(s) - t16 * Q4_TILE);
         return;
     }
-    block -= (int64_t)d.at0[d.n] * kvc;
+    block -= (int64_t)d.at0[d.n] * shares;
     if (block < (int64_t)d.old0[d.n] * kvc) {
         const int ot = (int)(block / kvc), kvh = (int)(block - (int64_t)ot * kvc);
         const int s = last_at_or_before(d.old0, d.n, ot);
@@ -142,10 +148,10 @@ __global__ void __launch_bounds__(32 * PREP_WARPS)
         return;
     }
     block -= (int64_t)d.old0[d.n] * kvc;
-    const int parts = (nq + PREP_HEADS - 1) / PREP_HEADS;
+    const int parts = (nq + q_heads - 1) / q_heads;
     const int64_t task = block * PREP_WARPS + warp, row = task / parts;
     if (row >= tokens) return;
-    const int h0 = (int)(task - row * parts) * PREP_HEADS, h1 = min(nq, h0 + PREP_HEADS);
+    const int h_first = (int)(task - row * parts) * q_heads, h1 = min(nq, h_first + q_heads);
     int p[3];
     angles_at(pos ? 0 : last_at_or_before(d.row0, d.n, (int)row), row, p);
     float2 c4[4];
@@ -154,21 +160,22 @@ __global__ void __launch_bounds__(32 * PREP_WARPS)
     load_split(q_norm, lane, w);
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] *= 0.0625f * LOG2E;   // scores in log2 units
-    SplitRow<T> in[PREP_HEADS];
+#pragma unroll 1
+    for (int h0 = h_first; h0 < h1; h0 += PREP_ROWS) {
+        SplitRow<T> in[PREP_ROWS];
 #pragma unroll
-    for (int i = 0; i < PREP_HEADS; ++i)
-        if (h0 + i < h1) in[i].load(q_gate + (row * nq + h0 + i) * QG_ROW, lane);
+        for (int i = 0; i < PREP_ROWS; ++i)
+            if (h0 + i < h1) in[i].load(q_gate + (row * nq + h0 + i) * QG_ROW, lane);
 #pragma unroll
-    for (int i = 0; i < PREP_HEADS; ++i) {
-        if (h0 + i >= h1) break;
-        float x[8];
-        in[i].values(x);
-        norm_rotate_split(x, w, c4, eps, lane);
-        __half* out = qf + ((size_t)(h0 + i) * tokens + row) * HD;
-        *reinterpret_cast<uint2*>(out + split_dim(lane, 0)) =
-            make_uint2(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]));
-        *reinterpret_cast<uint2*>(out + split_dim(lane, 1)) =
-            make_uint2(pack_f16(x[4], x[5]), pack_f16(x[6], x[7]));
+        for (int i = 0; i < PREP_ROWS; ++i) {
+            if (h0 + i >= h1) break;
+            float x[8];
+            in[i].values(x);
+            norm_rotate_split(x, w, c4, eps, lane);
+            __half* out = qf + ((size_t)(h0 + i) * tokens + row) * HD;
+            *reinterpret_cast<uint2*>(out + split_dim(lane, 0)) = make_uint2(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]));
+            *reinterpret_cast<uint2*>(out + split_dim(lane, 1)) = make_uint2(pack_f16(x[4], x[5]), pack_f16(x[6], x[7]));
+        }
     }
 }
 
@@ -755,10 +762,17 @@ static cudaError_t launch_group(dz_ctx* ctx, int layer, const q4::Prompt& d, con
         map.key[i] = d.key0[s];
         map.first[i + 1] = map.first[i] + attn::Packed::own_tiles(d.T(s), map.split_idx, map.split_cnt);
     }
-    const int64_t q_tasks = tokens * ((nq + q4::PREP_HEADS - 1) / q4::PREP_HEADS);
-    const int64_t blocks = (int64_t)(d.at0[d.n] + d.old0[d.n]) * kvc + (q_tasks + q4::PREP_WARPS - 1) / q4::PREP_WARPS;
-    q4::q4_pf_prep_kernel<T><<<(unsigned)blocks, 32 * q4::PREP_WARPS, 0, st>>>(
-        d, ctx->axes, kvc, L.d_q4, pos, L.q_norm, L.k_norm, q_gate, k, v, qf, kf, vf, ctx->q4_track, ctx->cfg.rms_eps);
+    // Heads that share a warp's set-up (positions, angles, weights): half of them, and a tile's kv heads,
+    // where that leaves 20 warps per SM, else 4 and one (the call with 1000 tokens: 37 us, 42 with half
+    // and all; with 1500: 56 and 55; with 2000 after 5555: 246 and 240).
+    const bool many = tokens >= 10 * (int64_t)ctx->n_sm;
+    const int q_heads = many ? nq / 2 : PREP_ROWS, key_heads = many ? kvc : 1;
+    const int64_t q_tasks = tokens * ((nq + q_heads - 1) / q_heads);
+    const int64_t blocks = (int64_t)d.at0[d.n] * (kvc / key_heads) + (int64_t)d.old0[d.n] * kvc +
+                           (q_tasks + PREP_WARPS - 1) / PREP_WARPS;
+    q4_pf_prep_kernel<T><<<(unsigned)blocks, 32 * PREP_WARPS, 0, st>>>(
+        d, ctx->axes, kvc, L.d_q4, pos, L.q_norm, L.k_norm, q_gate, k, v, qf, kf, vf, key_heads, q_heads, ctx->q4_track,
+        ctx->cfg.rms_eps);
     *n_launch += 1;
     if (map.first[d.n] > 0) {
         const size_t smem = sizeof(attn::Smem) + 1024;
