@@ -100,20 +100,26 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
     return __half2float(__ushort_as_half((unsigned short)(byte << 7)));
 }
 // code + 8 of x: the nearest whole multiple k s (ties to even) within 7 s, decided exactly.
-// inv = 1 / s (0 if s is 0), an approximation that the remainder corrects.  The remainder is
-// exact in F where k s and x are within a factor of 2, and for k = 0; that leaves |k| = 1 with
-// |x| just below s / 2, where it may be rounded to s / 2: the tie goes to 0, as x does.
-// half, below: s / 2 and the next smaller F.
-template <typename F>
-__device__ __forceinline__ uint32_t code8(F x, F s, float inv, F half, F below) {
-    x = fmin(fmax(x, (F)-7 * s), (F)7 * s);
-    float t = fmaf((float)x, inv, 12582920.0f);                // 1.5 * 2^23 + 8: rounds to an integer, k + 8 its low bits
-    const F d = fma((F)(12582920.0f - t), s, x);
-    if (fabs(d) > ((__float_as_uint(t) & 1u) ? below : half)) t += d > (F)0 ? 1.0f : -1.0f;
-    return __float_as_uint(t) & 15u;
+// inv = 1 / s (0 if s is 0), an approximation.
+constexpr float ROUND8 = 12582920.0f;                          // 1.5 * 2^23 + 8: x + this is an integer, x + 8 its low bits
+// f64: an approximate k, corrected by the remainder, which is exact where k s and x are within
+// a factor of 2, and for k = 0; that leaves |k| = 1 with |x| just below s / 2, where it may be
+// rounded to s / 2: the tie goes to 0, as x does.
+__device__ __forceinline__ uint32_t code8(double x, float s, float inv) {
+    x = fmin(fmax(x, -7.0 * s), 7.0 * s);
+    const float t = fmaf((float)x, inv, ROUND8);
+    const double d = fma((double)(ROUND8 - t), (double)s, x), h = 0.5 * s;
+    const bool odd = __float_as_uint(t) & 1u;
+    const float up = d > 0.0 ? 1.0f : -1.0f;
+    return __float_as_uint(fabs(d) > h || (odd && fabs(d) == h && s > 0.0f) ? t + up : t) & 15u;
 }
-__device__ __forceinline__ float next_below(float x) { return __uint_as_float(__float_as_uint(x) - 1u); }   // x > 0
-__device__ __forceinline__ double next_below(double x) { return __longlong_as_double(__double_as_longlong(x) - 1); }
+// f32: the quotient, corrected to the nearest f32.  x has 24 bits and s 4, so a quotient that is
+// no tie lies at least 0.53 units in the last place from one (1 / 1.875), and a tie is an f32.
+__device__ __forceinline__ uint32_t code8(float x, float s, float inv) {
+    x = fminf(fmaxf(x, -7.0f * s), 7.0f * s);
+    const float u = x * inv;
+    return __float_as_uint(fmaf(fmaf(-u, s, x), inv, u) + ROUND8) & 15u;
+}
 
 // two scale bytes (bits 0..7 and 16..23) -> an f16 pair
 __device__ __forceinline__ uint32_t scale_pair(uint32_t bytes) { return bytes << 7; }
@@ -294,9 +300,8 @@ __device__ __forceinline__ uint32_t quantise(F (&x)[8], uint32_t (&code)[8]) {
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
     inv = s > 0.0f ? inv : 0.0f;
-    const F half = (F)0.5 * (F)s, below = s > 0.0f ? next_below(half) : half;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) code[e] = code8(x[e], (F)s, inv, half, below);
+    for (int e = 0; e < 8; ++e) code[e] = code8(x[e], s, inv);
     return sb;
 }
 
@@ -332,17 +337,17 @@ __device__ __forceinline__ bool quantise_f32(const float (&x)[8], float from, ui
     float off = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const float u = fminf(fmaxf(x[e] * inv, -7.0f), 7.0f), r = u + 12582920.0f;   // 1.5 * 2^23 + 8: rounds to integers
+        const float u = fminf(fmaxf(x[e] * inv, -7.0f), 7.0f), r = u + ROUND8;
         code[e] = __float_as_uint(r) & 15u;
-        off = fmaxf(off, fabsf(u - (r - 12582920.0f)));
+        off = fmaxf(off, fabsf(u - (r - ROUND8)));
     }
     return ok && off < 0.5f - 4e-5f;
 }
-// A row of K: normalised, rotated, quantised as in f64.  cs: the warp's place for 32 angles, in
-// which float2 (rope_cs_f32) are ready; t, h, w: the positions they are of.
-__device__ __forceinline__ uint32_t quantise_key(const float (&x)[8], const float* __restrict__ weight, double2* cs,
-                                                 const RopeAxes& axes, int t, int h, int w, float eps, int lane,
-                                                 uint32_t (&code)[8]) {
+// A row of K: normalised, rotated, quantised as in f64.  csf: its 32 angles (rope_cs_f32), t, h, w:
+// the positions they are of; cs: the warp's place for them in f64.
+__device__ __forceinline__ uint32_t quantise_key(const float (&x)[8], const float* __restrict__ weight,
+                                                 const float2* csf, double2* cs, const RopeAxes& axes, int t, int h, int w,
+                                                 float eps, int lane, uint32_t (&code)[8]) {
     uint32_t sb;
     // f32: the norm is off by at most 5e-7 (13 roundings of its sum, halved, and its root), a value by two
     // roundings more, sine and cosine by 3.1e-7 (1.9e-7 of them the angle's rounding)
@@ -355,13 +360,16 @@ __device__ __forceinline__ uint32_t quantise_key(const float (&x)[8], const floa
     const float4 w0 = wp[0], w1 = wp[1];
     const float wv[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = (x[e] * inv) * wv[e];
+    for (int e = 0; e < 8; ++e) {
+        y[e] = (x[e] * inv) * wv[e];
+        from = fmaxf(from, fabsf(y[e]));
+    }
+    from = lane < 8 ? fmaxf(from, __shfl_xor_sync(0xffu, from, 4)) : 0.0f;   // the rotated dims and their partners
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const float p = __shfl_xor_sync(0xffffffffu, y[e], 4);
         if (lane < 8) {
-            const float2 c = reinterpret_cast<const float2*>(cs)[8 * (lane & 3) + e];
-            from = fmaxf(from, fmaxf(fabsf(y[e]), fabsf(p)));
+            const float2 c = csf[8 * (lane & 3) + e];
             y[e] = fmaf(y[e], c.x, p * c.y);
         }
     }

@@ -8,6 +8,9 @@
 //                    over the SMs; unnormalised partials out.
 //   3. q4_combine  : per (sequence, q head) -- merge, normalise, gate.
 //   4. q4_weights  : tracked caches -- the new attention weights are added.
+// One call, 24 q heads on 4 kv heads: one sequence of 2048, 10.5 us (three dependent grids:
+// latency); 64 of 512-32768 (1.17 GB), 296 us, 3.95 TB/s; 8 of 131072 (1.14 GB), 276 us,
+// 4.1 TB/s, 0.63 of a plain copy's rate.
 #include <algorithm>
 #include <cstddef>
 
@@ -27,6 +30,9 @@ namespace q4 {
 //      q_frag [b][kvh][step 16][lane][hi 0,1 | lo 0,1 | hi 2,3 | lo 2,3]
 //    where step s, lane (r, c) covers dims 64 c + 4 s .. + 3 of head r.
 //    and behind the 16 steps the heads' factors back (f32 [8], 0 for the empty heads).
+//    K goes through f32 first (quantise_key): with f64 throughout, the call for one
+//    sequence took 13.0 us.  Running this inside the split grid (each CTA its own rows)
+//    was slower: 64 CTAs of few sequences wait for it as for a grid.
 // ---------------------------------------------------------------------------
 using Rows = Q4Rows;
 constexpr int FRAG_WORDS = Q4_FRAG_WORDS, FRAG_SCALES = 16 * 32 * 4;
@@ -38,12 +44,12 @@ __global__ void __launch_bounds__(256) q4_prep_kernel(const __grid_constant__ Ro
                                                       const float* __restrict__ v_in, uint32_t* __restrict__ q_frag,
                                                       float eps) {
     __shared__ double2 cs[8][ROPE / 2];
+    __shared__ float2 csf[8][ROPE / 2];
     const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int kvc = d.kvc, nq = GRP * kvc;
     const int task = blockIdx.y * 8 + warp;
     // before the wait: the angles
-    float2* csf = reinterpret_cast<float2*>(cs[warp]);
-    csf[lane] = rope_cs_f32(axes, lane, pos.p[b][0], pos.p[b][1], pos.p[b][2]);
+    csf[warp][lane] = rope_cs_f32(axes, lane, pos.p[b][0], pos.p[b][1], pos.p[b][2]);
     __syncwarp();
     // As in gqa_prep: everything before this grid is complete (inputs, caches, q_frag)
     // before the split grid may start streaming old tiles.
@@ -54,7 +60,7 @@ __global__ void __launch_bounds__(256) q4_prep_kernel(const __grid_constant__ Ro
         const float4* src = reinterpret_cast<const float4*>(q_gate + ((size_t)b * nq + task) * QG_ROW);
         const float4 a0 = src[2 * lane], a1 = src[2 * lane + 1];
         float x[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
-        norm_rotate(x, q_norm, csf, eps, lane);
+        norm_rotate(x, q_norm, csf[warp], eps, lane);
         float amax = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -95,7 +101,8 @@ __global__ void __launch_bounds__(256) q4_prep_kernel(const __grid_constant__ Ro
         const float x[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
         float y[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
         uint32_t code[8];
-        uint32_t sb = quantise_key(x, k_norm, cs[warp], axes, pos.p[b][0], pos.p[b][1], pos.p[b][2], eps, lane, code);
+        uint32_t sb = quantise_key(x, k_norm, csf[warp], cs[warp], axes, pos.p[b][0], pos.p[b][1], pos.p[b][2], eps,
+                                   lane, code);
         put_k(tile, p, lane, code, sb);
         sb = quantise(y, code);
         uint4* vw = v_words(tile, lane, (p & 7) >> 1);
@@ -120,6 +127,14 @@ __global__ void __launch_bounds__(256) q4_prep_kernel(const __grid_constant__ Ro
 //    added).  That is the B operand's own layout, so P needs no shuffle: O^T += V^T P^T,
 //    A = V's dims x 16 positions, B = P (hi, then lo), 16 tiles of 16 dims accumulated in
 //    64 registers.
+//    Bound by issue: the 64 matrix instructions of a tile take 131 cycles of an SM (a
+//    sub-core is held 8 cycles by each), unpacking, softmax and sums bring it to 235; the
+//    tile's bytes take 189 at the copy rate.  tcgen05 would want the codes unpacked into
+//    shared memory for 6 of 128 rows.  8 warps with 255 registers: 12 with 168 kept q in
+//    shared memory, and 64 sequences took 342 us; e4m3 products (a conversion and two f16
+//    products on this GPU) were slower still; adding partial sums of single tiles instead of
+//    pairs: 315 us.  Equal runs of tiles per warp against per CTA: 285 and 303 us with the
+//    12 warps.
 // ---------------------------------------------------------------------------
 constexpr int STAGES = 3, WARPS = 8;
 // p is taken against a maximum that may be stale by P_SLACK and is scaled by 2^P_LOG2: at
@@ -421,7 +436,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
 
 // ---------------------------------------------------------------------------
 // 3. combine: merge a row's partials, divide, gate.  Grid (6 kvc, B, 4 quarters of the
-//    dims), 16 groups of 16 threads that take partials in turn, 4 dims a thread.
+//    dims), 16 groups of 16 threads that take partials in turn, 4 dims a thread.  Latency:
+//    about 3 us of a call.
 // ---------------------------------------------------------------------------
 constexpr int MAX_RUNS = 2048;                   // warps of the split grid (148 SMs: 1184)
 constexpr int CMB_DIMS = 64;
@@ -486,7 +502,9 @@ __global__ void __launch_bounds__(256) q4_combine_kernel(const __grid_constant__
 // ---------------------------------------------------------------------------
 // 4. tracked caches: weight of position j of a kv head += sum over its 6 q heads of
 //    exp2(score - M) / L, with M and L merged from the partials' (m, l).  The new
-//    position's weight starts here.  Grid (ceil(longest / 1024), kvc, B).
+//    position's weight starts here.  Grid (ceil(longest / 1024), kvc, B).  12 sequences of
+//    1137-7414: 39 us the call, 30 without weights; as a programmatic dependent it took the
+//    same time.
 // ---------------------------------------------------------------------------
 constexpr int WT_SPAN = 1024;
 

@@ -66,6 +66,8 @@ __device__ __forceinline__ uint4 held(const uint32_t (&code)[8], uint32_t sb) {
     return make_uint4(h[0], h[1], h[2], h[3]);
 }
 
+// 8192 bf16 tokens: 84 us for 0.28 GB (3.3 TB/s).  Bound by issue (57 % of the slots, at two
+// blocks per SM; more blocks spill): norms, rotation, the codes and their f16 values.
 constexpr int PREP_WARPS = 16, PREP_ROWS = 4;    // query rows that a warp has in flight
 
 // Blocks [0, at0 kvc / key_heads): a tile of new rows and key_heads kv heads, a warp per position.
@@ -80,6 +82,7 @@ __global__ void __launch_bounds__(32 * PREP_WARPS, 2)
                       int key_heads, int q_heads, bool track, float eps) {
     __shared__ TileMerge merge;
     __shared__ double2 cs[PREP_WARPS][ROPE / 2];
+    __shared__ float2 csf[PREP_WARPS][ROPE / 2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nq = GRP * kvc;
     const int64_t keys = d.key0[d.n], tokens = d.row0[d.n];
     int64_t block = blockIdx.x;
@@ -100,7 +103,10 @@ __global__ void __launch_bounds__(32 * PREP_WARPS, 2)
         const int64_t row = d.row0[s] + (slot_pos - base);
         int p[3];
         merge.begin();
-        if (mine) angles_at(s, row, p);
+        if (mine) {
+            angles_at(s, row, p);
+            csf[warp][lane] = rope_cs_f32(axes, lane, p[0], p[1], p[2]);
+        }
 #pragma unroll 1
         for (int kvh = kvh0; kvh < kvh0 + key_heads; ++kvh) {
             uint8_t* tile = slot.tile(kvh, t16);
@@ -109,11 +115,9 @@ __global__ void __launch_bounds__(32 * PREP_WARPS, 2)
                 float x[8], y[8];
                 load_row(k + (row * kvc + kvh) * HD + 8 * lane, x);
                 load_row(v + (row * kvc + kvh) * HD + 8 * lane, y);
-                reinterpret_cast<float2*>(cs[warp])[lane] = rope_cs_f32(axes, lane, p[0], p[1], p[2]);
-                __syncwarp();
                 const size_t out = ((size_t)kvh * keys + d.key0[s] + slot_pos) * HD + 8 * lane;
                 uint32_t code[8];
-                uint32_t sb = quantise_key(x, k_norm, cs[warp], axes, p[0], p[1], p[2], eps, lane, code);
+                uint32_t sb = quantise_key(x, k_norm, csf[warp], cs[warp], axes, p[0], p[1], p[2], eps, lane, code);
                 put_k(tile, warp, lane, code, sb);
                 *reinterpret_cast<uint4*>(kf + out) = held(code, sb);
                 sb = quantise(y, code);
@@ -192,6 +196,16 @@ __global__ void __launch_bounds__(32 * PREP_WARPS, 2)
 //   warp 9     (first CTA) issues S = Q K^T (N = 128, K = 256) into one of two TMEM buffers
 //              and O += P V (N = 256, K = 128, P from TMEM)
 //   warp 10    TMA of this CTA's 128 dims of each V block (slots of 32 keys)
+//   warps 12-15  outputs: O / l from shared memory (f16: P was rounded to f16 already, and the
+//              sum over many keys is off by more), times the gate's sigmoid, in whole rows
+// A cluster takes several query tiles in turn; while the outputs of one leave, the next one's
+// queries are fetched and its first blocks worked on.  (A cluster per tile, the softmax warps
+// writing the outputs: packed prompts of 1-1500 took 378 us, all of the call, instead of 247:
+// set-up and outputs were 15 us of each tile's time, next to 1.3 us per block of keys.)
+// Bound by the products and the softmax together: a block of 128 keys takes 2270 cycles, of
+// which the products 2048; the softmax of one block (1950 cycles, 1100 of them exponentials)
+// runs beside the products of another.  8192 tokens: 825 GFLOP, 1.35-1.5 PFLOP/s with the SM
+// clock at 1.6-1.8 GHz.
 // The first CTA's barriers count both CTAs' bytes and arrivals; the products' completion
 // goes to both.  Every wait is bounded; a CTA that gave one up still meets its barriers.
 // ---------------------------------------------------------------------------
