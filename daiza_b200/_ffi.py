@@ -44,6 +44,7 @@ SIGNATURES = {
     "dz_layer_set_ssm_params": [_P, _I, _P, _P, _P, _P],
     "dz_cache_create": [_P, _I, _P],
     "dz_kv_len": [_P, _I, _I, C.POINTER(_I64)],
+    "dz_kv_lens": [_P, _I, _I, _P, _P],
     "dz_kv_truncate": [_P, _I, _I, _I64],
     "dz_cache_reset": [_P, _I],
     "dz_kv_export": [_P, _I, _I, _P, _P],

@@ -466,6 +466,9 @@ static dz_status cache_create(dz_ctx* ctx, int n_seqs, const int64_t* max_len, b
                 return st;
             }
             ctx->q4_frag = static_cast<uint32_t*>(d);
+            DZ_CUDA(q4_decode_setup());
+            DZ_CUDA(q4_prefill_setup());
+            DZ_CUDA(q4_evict_setup());
             if (track) {
                 const size_t tiles = (size_t)(sum_n / Q4_TILE) + nb;
                 if ((st = dev_alloc(ctx, &d, tiles * kvc * GRP * Q4_TILE * sizeof(float), false)) != DZ_OK) {
@@ -500,6 +503,14 @@ dz_status dz_kv_len(const dz_ctx* ctx, int layer, int seq, int64_t* out_len) {
     if (!layer_ok(ctx, layer) || !out_len || !ctx->layers[layer].is_attn || seq < 0 || seq >= ctx->n_seqs)
         return DZ_EINVAL;
     *out_len = ctx->layers[layer].len[seq];
+    return DZ_OK;
+}
+
+dz_status dz_kv_lens(const dz_ctx* ctx, int layer, int B, const int32_t* seq_ids, int64_t* out_lens) {
+    if (!layer_ok(ctx, layer) || !ctx->layers[layer].is_attn || B <= 0 || !seq_ids || !out_lens) return DZ_EINVAL;
+    for (int b = 0; b < B; ++b)
+        if (seq_ids[b] < 0 || seq_ids[b] >= ctx->n_seqs) return DZ_EINVAL;
+    for (int b = 0; b < B; ++b) out_lens[b] = ctx->layers[layer].len[seq_ids[b]];
     return DZ_OK;
 }
 

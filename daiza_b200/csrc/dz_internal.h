@@ -155,8 +155,9 @@ struct dz_ctx {
         cudaEvent_t landed = nullptr, done = nullptr;
     } hs[2];                     // 0: gated GQA, 1: Gated DeltaNet
     cudaEvent_t pf_ev[dz::PF_MAX_SEGMENTS + 1] = {};
-    // 4-bit KV caches (dz_cache_create_q4): the decode kernels' q operand, the scores of tracked caches, and scratch of prompts and evictions.  A buffer that is
-    // outgrown stays allocated until the context goes: a captured graph may hold it.
+    // 4-bit KV caches (dz_cache_create_q4): the decode kernels' q operand, the scores of tracked
+    // caches, and scratch of prompts and evictions.  A buffer that is outgrown stays allocated
+    // until the context goes: a captured graph may hold it.
     bool q4 = false, q4_track = false;
     dz::RopeAxes axes{};
     uint32_t* q4_frag = nullptr;  // [min(n_seqs, MAXB)][kvc][Q4_FRAG_WORDS]
@@ -304,6 +305,10 @@ cudaError_t launch_q1_gemv(dz_ctx* ctx, int n_mats, const uint8_t* const* w, con
 cudaError_t launch_rmsnorm_rows(const float* x, const float* w, float eps, int T, int n, float* out, cudaStream_t st);
 cudaError_t launch_swiglu(float* gate, const float* up, int64_t n, cudaStream_t st);
 // 4-bit KV caches (q4_*.cu)
+// shared memory of the kernels that take more than 48 KB, set once (a call of 1 us each)
+cudaError_t q4_decode_setup();
+cudaError_t q4_prefill_setup();
+cudaError_t q4_evict_setup();
 cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, Q4Rows& d, const Q4Pos& pos, const float* q_gate,
                              const float* k, const float* v, float* out, cudaStream_t st, int* n_launch);
 // prompts: lens[i] new tokens of each sequence, packed; f32 or bf16 (uint16_t) tensors

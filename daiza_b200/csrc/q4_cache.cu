@@ -364,9 +364,11 @@ static dz_status qk_mrope(dz_ctx* ctx, int layer, int64_t n, const int32_t* pos,
         if (!g.ok) return fail(ctx, DZ_ECUDA, "cudaSetDevice(%d) failed", ctx->device);
         const LayerState& L = ctx->layers[layer];
         const int kvc = ctx->cfg.kv_head_count;
-        // few tokens: a warp per head, so that their latencies overlap; then 4 shares, then one
+        // Few tokens: a warp per head, so that their latencies overlap, while that leaves at most 20
+        // warps per SM (f32, 64 tokens: 3.5 us, 4.8 with 4 shares; 200: 7.6 and 5.0); then 4 shares, up
+        // to 40 (1200: 14.5 us, 16.5 with one; 2368: 29.6 and 24.8); then one share.
         const int heads = GRP * kvc + kvc;
-        const int shares = n * 4 <= 64 * ctx->n_sm ? (n * heads <= 64 * ctx->n_sm ? heads : 4) : 1;
+        const int shares = n * heads <= 20 * ctx->n_sm ? heads : (n * 4 <= 40 * ctx->n_sm ? 4 : 1);
         q4::qk_mrope_kernel<T><<<dim3((unsigned)((n + 7) / 8), shares), 256, 0, static_cast<cudaStream_t>(stream)>>>(
             ctx->axes, kvc, n, pos, q_gate, k, L.q_norm, L.k_norm, q_out, k_out, ctx->cfg.rms_eps);
         Q4_CUDA(cudaGetLastError());

@@ -145,6 +145,7 @@ struct alignas(128) Ring {
     uint8_t pair[STAGES][2 * Q4_TILE_BYTES];
     uint64_t full[STAGES];
 };
+constexpr int SPLIT_SMEM = WARPS * (int)sizeof(Ring);
 static_assert(Q4_TILE_BYTES % 128 == 0 && sizeof(Ring) % 128 == 0, "bulk copies need 16-byte alignment");
 
 // Run c starts at tile c * run_base + min(c, run_rem) (tiles = runs * run_base + run_rem).
@@ -548,6 +549,14 @@ __global__ void __launch_bounds__(256) q4_weights_kernel(const __grid_constant__
 
 }  // namespace q4
 
+cudaError_t q4_decode_setup() {
+    const cudaError_t e = cudaFuncSetAttribute(q4::q4_split_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               q4::SPLIT_SMEM);
+    return e != cudaSuccess ? e
+                            : cudaFuncSetAttribute(q4::q4_split_kernel<true>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, q4::SPLIT_SMEM);
+}
+
 int q4_decode_runs(int n_sm) { return std::min(q4::WARPS * n_sm, q4::MAX_RUNS); }
 
 cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, Q4Rows& d, const Q4Pos& pos, const float* q_gate,
@@ -558,10 +567,7 @@ cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, Q4Rows& d, const Q4Pos& pos
     d.runs = std::min(d.tiles(), q4_decode_runs(ctx->n_sm));
     d.run_base = d.tiles() / d.runs;
     d.run_rem = d.tiles() % d.runs;
-    const int smem = WARPS * (int)sizeof(Ring);
     auto split = ctx->q4_track ? q4_split_kernel<true> : q4_split_kernel<false>;
-    cudaError_t e = cudaFuncSetAttribute(split, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -571,12 +577,12 @@ cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, Q4Rows& d, const Q4Pos& pos
     lc.stream = st;
     lc.attrs = at;
     lc.numAttrs = 1;
-    e = cudaLaunchKernelEx(&lc, q4_prep_kernel, d, pos, ctx->axes, (const Q4Slot*)L.d_q4, (const float*)L.q_norm,
+    cudaError_t e = cudaLaunchKernelEx(&lc, q4_prep_kernel, d, pos, ctx->axes, (const Q4Slot*)L.d_q4, (const float*)L.q_norm,
                            (const float*)L.k_norm, q_gate, k, v, ctx->q4_frag, ctx->cfg.rms_eps);
     if (e != cudaSuccess) return e;
     lc.gridDim = dim3(std::min(d.runs, ctx->n_sm));
     lc.blockDim = dim3(32 * WARPS);
-    lc.dynamicSmemBytes = smem;
+    lc.dynamicSmemBytes = SPLIT_SMEM;
     e = cudaLaunchKernelEx(&lc, split, d, (const Q4Slot*)L.d_q4, (const uint32_t*)ctx->q4_frag, ctx->part_o,
                            ctx->part_ml, ctx->q4_sc, ctx->d_err);
     if (e != cudaSuccess) return e;

@@ -319,11 +319,16 @@ __global__ void __launch_bounds__(EV_THREADS, 2)
 
 }  // namespace q4
 
+cudaError_t q4_evict_setup() {
+    cudaError_t e = cudaSuccess;
+    for (auto kernel : {q4::q4_evict_kernel<8>, q4::q4_evict_kernel<4>, q4::q4_evict_kernel<2>})
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(q4::EvictSmem));
+    return e;
+}
+
 template <int CTAS>
 static cudaError_t launch_evict(const q4::Evict& d, const Q4Slot* slots, int32_t* list, int32_t* kept, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(q4::q4_evict_kernel<CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)sizeof(q4::EvictSmem));
-    if (e != cudaSuccess) return e;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = CTAS;
@@ -362,7 +367,7 @@ cudaError_t launch_q4_evict(dz_ctx* ctx, int layer, int B, const int32_t* src, c
             at += k;
         }
         // as many CTAs per (sequence, kv head) as fit the GPU at once, two per SM (52 pairs of 20000
-        // entries: 64 us with 4, 76 with 8)
+        // entries: 64 us with 4, 79 with 8, 96 with 2; 4 pairs: 27 us with 8, 37 and 60 with 4 and 2)
         const int pairs = d.B * kvc;
         int32_t* list = static_cast<int32_t*>(ctx->q4_scratch);
         e = pairs * 8 <= 2 * ctx->n_sm   ? launch_evict<8>(d, L.d_q4, list, kept, st)

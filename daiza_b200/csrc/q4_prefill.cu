@@ -231,6 +231,7 @@ struct alignas(1024) Smem {
     float red_l[2][BM];                          // [key half][row] partial row sums
     uint32_t tmem_base;
 };
+constexpr int SMEM_BYTES = (int)sizeof(Smem) + 1024;           // the kernel rounds its address up to 1 KB
 static_assert(offsetof(Smem, k) % 1024 == 0 && offsetof(Smem, v) % 1024 == 0, "swizzle atoms need 1 KB alignment");
 
 // ---- the pair's forms of the PTX wrappers ------------------------------------------
@@ -741,6 +742,14 @@ static bool make_map(CUtensorMap* m, const void* base, int64_t d1, int64_t d2, i
 }  // namespace attn
 }  // namespace q4
 
+cudaError_t q4_prefill_setup() {
+    const cudaError_t e = cudaFuncSetAttribute(q4::attn::q4_pf_attn_kernel<float>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, q4::attn::SMEM_BYTES);
+    return e != cudaSuccess ? e
+                            : cudaFuncSetAttribute(q4::attn::q4_pf_attn_kernel<__nv_bfloat16>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, q4::attn::SMEM_BYTES);
+}
+
 template <typename T>
 static cudaError_t launch_group(dz_ctx* ctx, int layer, const q4::Prompt& d, const int32_t* pos, const T* q_gate,
                                 const T* k, const T* v, T* out, cudaStream_t st, int* n_launch) {
@@ -789,12 +798,9 @@ static cudaError_t launch_group(dz_ctx* ctx, int layer, const q4::Prompt& d, con
         ctx->cfg.rms_eps);
     *n_launch += 1;
     if (map.first[d.n] > 0) {
-        const size_t smem = sizeof(attn::Smem) + 1024;
-        auto kernel = attn::q4_pf_attn_kernel<T>;
-        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess)
-            return e;
         const unsigned clusters = (unsigned)std::min((int64_t)map.first[d.n] * nq / 2, (int64_t)ctx->n_sm / 2);
-        kernel<<<2 * clusters, attn::NTHREADS, smem, st>>>(mq, mk, mv, map, kvc, q_gate, out, ctx->d_err);
+        attn::q4_pf_attn_kernel<T><<<2 * clusters, attn::NTHREADS, attn::SMEM_BYTES, st>>>(mq, mk, mv, map, kvc, q_gate,
+                                                                                          out, ctx->d_err);
         *n_launch += 1;
     }
     return cudaGetLastError();

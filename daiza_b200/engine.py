@@ -52,17 +52,24 @@ def _tensor(name, t, dtype, numel):
     return t.data_ptr()
 
 
+_arrays = {}                                     # ctypes array types by (type, length)
+
+
 def _ints(name, values, ctype, count=None):
     """ctypes array of whole numbers (a number, list or array); DZ_EINVAL if they do not fit or are not `count`.
     A list goes straight into the array: the numpy route costs as much as a small launch."""
-    v = values if type(values) in (list, tuple) else np.atleast_1d(values).tolist()
-    bits = 8 * C.sizeof(ctype) - 1
+    v = values if type(values) is list or type(values) is tuple else np.atleast_1d(values).tolist()
+    n = len(v)
     try:
-        if count is not None and len(v) != count:
-            raise ValueError(f"{count} numbers wanted, {len(v)} given")
-        if v and not (-(1 << bits) <= min(v) and max(v) < 1 << bits):
+        if count is not None and n != count:
+            raise ValueError(f"{count} numbers wanted, {n} given")
+        top = 1 << 31 if ctype is C.c_int32 else 1 << 63
+        if n and not (-top <= min(v) and max(v) < top):
             raise ValueError("out of range")
-        return (ctype * len(v))(*v)
+        array = _arrays.get((ctype, n))
+        if array is None:
+            array = _arrays[ctype, n] = ctype * n
+        return array(*v)
     except (TypeError, ValueError) as e:
         raise _ffi.DzError(_ffi.DZ_EINVAL, f"{name}: {e}") from None
 
@@ -73,6 +80,12 @@ def _ids(seq_ids):
 
 def _per_seq(name, values, ids):
     return _ints(name, values, C.c_int64, len(ids))
+
+
+def _total(counts):
+    """Sum of those of a ctypes array that are not negative (the call refuses the others)."""
+    n = list(counts)
+    return sum(n) if min(n, default=0) >= 0 else sum(c for c in n if c > 0)
 
 
 def default_config(n_layers=64, full_attention_interval=4, kv_heads=None, v_heads=None, qtile_split=None):
@@ -153,6 +166,16 @@ class Context:
         n = C.c_int64()
         self._chk(self.lib.dz_kv_len(self.h, layer, seq, C.byref(n)))
         return n.value
+
+    def kv_lens(self, layer, seq_ids):
+        """kv_len of several sequences, as a list."""
+        ids = _ids(seq_ids)
+        return list(self._lens(layer, ids))
+
+    def _lens(self, layer, ids):
+        out = _ints("lens", [0] * len(ids), C.c_int64)
+        self._chk(self.lib.dz_kv_lens(self.h, layer, len(ids), ids, out))
+        return out
 
     def kv_truncate(self, layer, seq, new_len):
         self._chk(self.lib.dz_kv_truncate(self.h, layer, seq, int(new_len)))
@@ -303,9 +326,12 @@ class Context:
         self._chk(self.lib.dz_set_rope_axes(self.h, s, int(bool(interleaved))))
 
     def _on(self, stream):
-        """Handle of `stream`, or of the context's device's current one."""
+        """Handle of `stream`, or of the context's device's current one (the raw handle: making a Stream object of it
+        takes 1.3 us)."""
+        if stream is not None:
+            return stream.cuda_stream
         import torch
-        return (torch.cuda.current_stream(self.device) if stream is None else stream).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.device)
 
     def qk_mrope(self, layer, pos, q_gate, k, q_out, k_out, stream=None):
         """QK-RMSNorm, rotation by pos [T][3] (int32) and q's 1/16; q_gate [T][6*kvc][512] and k [T][kvc][256] f32 or
@@ -337,7 +363,7 @@ class Context:
         import torch
         ids = _ids(seq_ids)
         n = _per_seq("lens", lens, ids)
-        T = sum(c for c in n if c > 0)
+        T = _total(n)
         dt = torch.bfloat16 if k.dtype == torch.bfloat16 else torch.float32
         fn = self.lib.dz_gqa_prefill_q4_bf16 if dt == torch.bfloat16 else self.lib.dz_gqa_prefill_q4
         self._chk(fn(self.h, layer, len(ids), ids, n,
@@ -351,13 +377,13 @@ class Context:
         import torch
         ids = _ids(seq_ids)
         a, n = _per_seq("first", first, ids), _per_seq("count", count, ids)
-        total = sum(c for c in n if c > 0) * self.kvc * HD
+        total = _total(n) * self.kvc * HD
         self._chk(self.lib.dz_kv_rows_q4(self.h, layer, len(ids), ids, a, n,
                                          _tensor("k", k, torch.float32, total), _tensor("v", v, torch.float32, total),
                                          self._on(stream)))
 
     def _weights_numel(self, layer, ids):
-        return self.kvc * sum(self.kv_len(layer, s) for s in ids)
+        return self.kvc * sum(self._lens(layer, ids))
 
     def kv_weights_q4(self, layer, seq_ids, out, stream=None):
         """Accumulated attention weights, sequence by sequence [kvc][length]."""
@@ -383,7 +409,7 @@ class Context:
         to = None if into is None else _ints("into", into, C.c_int32, len(ids))
         out = None
         if kept is not None:
-            n = sum(max(0, min(a, self.kv_len(layer, s))) for a, s in zip(k, ids))
+            n = sum(max(0, min(a, b)) for a, b in zip(k, self._lens(layer, ids)))
             out = _tensor("kept", kept, torch.int32, n * self.kvc)
         self._chk(self.lib.dz_kv_evict_q4(self.h, layer, len(ids), ids, to,
                                           k, r, out, self._on(stream)))

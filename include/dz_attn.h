@@ -98,6 +98,8 @@ dz_status dz_layer_set_ssm_params(dz_ctx* ctx, int layer, const float* conv1d_t,
 dz_status dz_cache_create(dz_ctx* ctx, int n_seqs, const int64_t* max_len);
 /* KvCache::len (kv_cache.rs:23) */
 dz_status dz_kv_len(const dz_ctx* ctx, int layer, int seq, int64_t* out_len);
+/* The same of B sequences (host arrays; an id may come twice). */
+dz_status dz_kv_lens(const dz_ctx* ctx, int layer, int B, const int32_t* seq_ids, int64_t* out_lens);
 /* KvCache::truncate (kv_cache.rs:119-129): no-op if new_len >= len. */
 dz_status dz_kv_truncate(dz_ctx* ctx, int layer, int seq, int64_t new_len);
 /* KvCache::reset + SsmState::reset for every layer of one sequence
@@ -301,8 +303,8 @@ dz_status dz_gqa_decode_q4(dz_ctx* ctx, int layer, int B, const int32_t* seq_ids
  * All tensors 16-byte aligned.  Tracked caches: new rows start with weight 0; prompts
  * add no weights.  Scratch grows with the largest prompt (12 KB per new token and 4 KB
  * per key with 4 kv heads; beyond 2 GB a call takes its sequences in groups); make one
- * such call before capturing a graph: old scratch stays for captured graphs until the
- * caches are created anew. */
+ * such call before capturing a graph: outgrown scratch stays for captured graphs until
+ * the context is destroyed. */
 dz_status dz_gqa_prefill_q4(dz_ctx* ctx, int layer, int n_seqs, const int32_t* seq_ids, const int64_t* T,
                             const int32_t* pos, const float* q_gate, const float* k, const float* v, float* out,
                             void* stream);

@@ -116,6 +116,18 @@ def test_import_of_extremes():
     m.done()
 
 
+def test_lengths_of_several_sequences():
+    m = Model([50, 33, 20], seed=41)
+    for s, n in enumerate((50, 0, 20)):
+        if n:
+            m.fill(s, n)
+    assert m.ctx.kv_lens(0, [2, 0, 1, 2]) == [20, 50, 0, 20]
+    for bad in ([3], [-1], []):
+        refused(DZ_EINVAL, m.ctx.kv_lens, 0, bad)
+    refused(DZ_EINVAL, m.ctx.kv_lens, 1, [0])
+    m.done()
+
+
 def test_rows_of_several_sequences():
     m = Model([50, 33, 20], seed=4)
     for s, n in enumerate((50, 33, 20)):

@@ -83,6 +83,7 @@ def test_null_contexts_are_refused():
     assert lib.dz_gqa_decode_q4(none, 0, 1, ids, none, none, none, none, none, none) == _ffi.DZ_EINVAL
     assert lib.dz_gqa_prefill_q4(none, 0, 1, ids, one, none, none, none, none, none, none) == _ffi.DZ_EINVAL
     assert lib.dz_gqa_prefill_q4_bf16(none, 0, 1, ids, one, none, none, none, none, none, none) == _ffi.DZ_EINVAL
+    assert lib.dz_kv_lens(none, 0, 1, ids, one) == _ffi.DZ_EINVAL
     assert lib.dz_kv_rows_q4(none, 0, 1, ids, one, one, none, none, none) == _ffi.DZ_EINVAL
     assert lib.dz_kv_evict_q4(none, 0, 1, ids, none, one, one, none, none) == _ffi.DZ_EINVAL
     assert lib.dz_kv_weights_q4(none, 0, 1, ids, none, none) == _ffi.DZ_EINVAL
