@@ -217,9 +217,10 @@ __device__ __forceinline__ void norm_rotate(F (&x)[8], const float* __restrict__
 }
 
 // Rows that are not quantised: lane l holds two runs of 4 dims, at split_dim(l, 0) and
-// split_dim(l, 1), such that a rotary pair (i, i + 32) lies in one lane (lanes 0..7).
+// split_dim(l, 1), such that a rotary pair (i, i + 32) lies in one lane (lanes 0..7), and
+// neighbouring lanes' runs are neighbours: a store fills whole sectors.
 __device__ __forceinline__ int split_dim(int lane, int run) {
-    return lane < 8 ? 4 * lane + 32 * run : 8 * lane + 4 * run;
+    return lane < 8 ? 4 * lane + 32 * run : 32 + 4 * lane + 96 * run;
 }
 // RMS norm, weight (w: this lane's 8) and rotation in f32; cs: (cos, sin) of pairs
 // 4 l .. 4 l + 3 in lanes 0..7.
@@ -467,6 +468,27 @@ __device__ __forceinline__ void get_v(const uint8_t* tile, int p, int lane, uint
     const uint32_t x[4] = {w.x >> sh, w.y >> sh, w.z >> sh, w.w >> sh};
 #pragma unroll
     for (int i = 0; i < 4; ++i) h[i] = unpack((x[i] & 0xFu) << 4 | (x[i] & 0xF00u) << 12, s, k);
+}
+
+// The same for 4 dims, 4 l + 128 half.
+__device__ __forceinline__ void get_k4(const uint8_t* tile, int p, int lane, int half, uint32_t (&h)[2]) {
+    const int w8 = (lane >> 1) + 16 * half, c = w8 >> 3, ws = w8 & 7, n = p & 7, g = w8 >> 2;
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + ((p >> 3) * 2 + (ws >> 2)) * 512 + (n * 4 + c) * 16 +
+                                                          (ws & 3) * 4) >> (8 * (lane & 1));
+    const uint32_t b = tile[OFF_KS + (n * 4 + (g >> 1)) * 4 + (p >> 3) * 2 + (g & 1)];
+    const uint32_t s = scale_pair(b | b << 16), k = hmul2_u(s, NEG72);
+    h[0] = unpack(w << 4, s, k);
+    h[1] = unpack(w, s, k);
+}
+__device__ __forceinline__ void get_v4(const uint8_t* tile, int p, int lane, int half, uint32_t (&h)[2]) {
+    const int w8 = (lane >> 1) + 16 * half, c = (p & 7) >> 1;
+    const uint2 w = *reinterpret_cast<const uint2*>(tile + v_at(w8 & 3, w8 >> 2, c) + 8 * (lane & 1));
+    const uint32_t b = tile[OFF_VS + ((w8 >> 2) * 4 + c) * 4 + (p & 1) + (p >> 3) * 2];
+    const uint32_t s = scale_pair(b | b << 16), k = hmul2_u(s, NEG72);
+    const int sh = (p & 1) * 16 + (p >> 3) * 4;
+    const uint32_t x[2] = {w.x >> sh, w.y >> sh};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) h[i] = unpack((x[i] & 0xFu) << 4 | (x[i] & 0xF00u) << 12, s, k);
 }
 
 }  // namespace q4

@@ -60,8 +60,9 @@ __device__ __forceinline__ int range_of(const int32_t* start, int B, int at) {  
     return lo;
 }
 
-// One warp per (row, kv head), 8 dims per lane.  HBM bound for many rows: 8192 in 20.5 us
-// (76 MB, 3.7 TB/s); 4 rows per warp took 23.6 us, and 5.2 for 142 rows instead of 2.8.
+// One warp per (row, kv head); a lane writes 4 dims of either half of K and V, whole lines a warp.
+// 8192 rows (76 MB): 12.5 us, 6.1 TB/s.  With 8 dims a lane a store fills half sectors: 19 us;
+// several heads to a warp, their loads ahead: 26 to 33 us.
 __global__ void __launch_bounds__(256) q4_rows_kernel(Ranges d, int kvc, const Q4Slot* __restrict__ slots,
                                                       float* __restrict__ k, float* __restrict__ v) {
     const int64_t task = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -71,23 +72,19 @@ __global__ void __launch_bounds__(256) q4_rows_kernel(Ranges d, int kvc, const Q
     const int b = range_of(d.row0, d.B, row);
     const int pos = d.first[b] + (row - d.row0[b]);
     const uint8_t* tile = slots[d.sid[b]].tile(kvh, pos >> 4);
-    const size_t at = (size_t)task * HD + 8 * lane;
-    uint32_t h[4];
-    auto put = [&](float* dst) {
-        float f[8];
+    const size_t at = (size_t)task * HD + 4 * lane;
+    uint32_t h[4][2];                            // K's halves, V's halves
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-            f[2 * i] = t.x;
-            f[2 * i + 1] = t.y;
-        }
-        reinterpret_cast<float4*>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
-        reinterpret_cast<float4*>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
-    };
-    get_k(tile, pos & 15, lane, h);
-    put(k + at);
-    get_v(tile, pos & 15, lane, h);
-    put(v + at);
+    for (int half = 0; half < 2; ++half) {
+        get_k4(tile, pos & 15, lane, half, h[half]);
+        get_v4(tile, pos & 15, lane, half, h[2 + half]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h[i][0]));
+        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&h[i][1]));
+        *reinterpret_cast<float4*>((i < 2 ? k : v) + at + 128 * (i & 1)) = make_float4(x.x, x.y, y.x, y.y);
+    }
 }
 
 // One block per (tile, kv head), a warp per position: rows [row0, len) from f32
