@@ -197,7 +197,8 @@ __global__ void __launch_bounds__(32 * PREP_WARPS, 2)
 //              and O += P V (N = 256, K = 128, P from TMEM)
 //   warp 10    TMA of this CTA's 128 dims of each V block (slots of 32 keys)
 //   warps 12-15  outputs: O / l from shared memory (f16: P was rounded to f16 already, and the
-//              sum over many keys is off by more), times the gate's sigmoid, in whole rows
+//              sum over many keys is off by more; times 8, which keeps |V| <= 7 * 896 in range
+//              and small values' bits), times the gate's sigmoid, in whole rows
 // A cluster takes several query tiles in turn; while the outputs of one leave, the next one's
 // queries are fetched and its first blocks worked on.  (A cluster per tile, the softmax warps
 // writing the outputs: packed prompts of 1-1500 took 378 us, all of the call, instead of 247:
@@ -217,6 +218,7 @@ constexpr int NK = 6, NV = 5;                    // ring slots of 8 KB (a block 
 constexpr int NTHREADS = 512;
 __host__ __device__ constexpr uint32_t S_COL(int st) { return 128u * (uint32_t)st; }
 constexpr uint32_t O_COL = 256;
+constexpr float OUT_SCALE = 8.0f;
 constexpr float RESCALE_THRESHOLD = 8.0f;        // log2 units: P stays below 2^8, far inside f16
 
 struct alignas(1024) Smem {
@@ -337,7 +339,7 @@ __device__ __forceinline__ void ex2_poly(uint64_t x, float& p0, float& p1) {
     p0 = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
     p1 = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
 }
-// (a sigmoid(x), b sigmoid(y)) of f16 a and b, to 2^-20 or so, below the products' f16 rounding; one
+// (a sigmoid(x), b sigmoid(y)) / OUT_SCALE of f16 a and b, to 2^-20 or so, below the products' f16 rounding; one
 // reciprocal for both.  Below 2^-60 a sigmoid counts as 2^-60: the denominators' product is finite.
 __device__ __forceinline__ float2 gate2(uint32_t ab, float x, float y) {
     float s, t, u, w, r;
@@ -345,6 +347,7 @@ __device__ __forceinline__ float2 gate2(uint32_t ab, float x, float y) {
     const uint64_t uw = add2(pack2(ex2(fminf(s, 60.0f)), ex2(fminf(t, 60.0f))), pack2(1.0f, 1.0f));
     unpack2(uw, u, w);
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(u * w));
+    r *= 1.0f / OUT_SCALE;
     const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&ab));
     float2 out;
     unpack2(mul2(pack2(h.x, h.y), mul2(pack2(w, u), pack2(r, r))), out.x, out.y);
@@ -699,7 +702,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
             // O / l of this thread's row, dims [128 hf, 128 hf + 128), to the output warps
             sm.red_l[hf][r] = l_run;
             named_bar_sync(1, 256);
-            const float inv_l = 1.0f / (l_run + sm.red_l[hf ^ 1][r]);
+            const float inv_l = OUT_SCALE / (l_run + sm.red_l[hf ^ 1][r]);
             if (round > 1) wait(&sm.out_empty, round & 1, err, ok);
             wait(&sm.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, err, ok);
             __syncwarp();

@@ -168,6 +168,16 @@ def test_prompt_extremes_stay_in_their_rows():
     m.done()
 
 
+@pytest.mark.parametrize("loud", [1e-4, 2000.0])
+def test_prompt_values_near_the_ends_of_the_scales(loud):
+    """Values on the smallest scales' grid, and held near 7 * 896: the outputs keep their bits on the way out."""
+    m = Model([500], kvc=1, seed=122)
+    m.fill(0, 200, loud=loud)
+    q, k, v = m.inputs(300)
+    check(m, [0], [300], inputs=(q, k, np.float32(loud) * v))
+    m.done()
+
+
 def test_prompt_query_tile_split():
     """Two contexts that share a kv head's query tiles (qtile_split): together they give the whole, each holds all
     rows; the other's output rows are left as they were."""
