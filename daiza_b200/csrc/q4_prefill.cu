@@ -83,6 +83,8 @@ __global__ void __launch_bounds__(32 * PREP_WARPS, 2)
     __shared__ TileMerge merge;
     __shared__ double2 cs[PREP_WARPS][ROPE / 2];
     __shared__ float2 csf[PREP_WARPS][ROPE / 2];
+    // the attention grid's CTAs may take their places as these blocks leave
+    asm volatile("griddepcontrol.launch_dependents;");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nq = GRP * kvc;
     const int64_t keys = d.key0[d.n], tokens = d.row0[d.n];
     int64_t block = blockIdx.x;
@@ -445,6 +447,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
     if (warp == 8) {
         // ---------------- TMA of Q and K ----------------
         if (lane == 0) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");         // for q4_pf_prep
             const uint32_t qb = peer_addr(&sm.q_full, 0);
             int slot = 0;
             uint32_t phase = 1;                                        // of the slot before: passes on a fresh ring
@@ -468,6 +471,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
     } else if (warp == 10) {
         // ---------------- TMA of V ----------------
         if (lane == 0) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
             int slot = 0;
             uint32_t phase = 1;
             while (ok && next_tile()) {
@@ -802,8 +806,18 @@ static cudaError_t launch_group(dz_ctx* ctx, int layer, const q4::Prompt& d, con
     *n_launch += 1;
     if (map.first[d.n] > 0) {
         const unsigned clusters = (unsigned)std::min((int64_t)map.first[d.n] * nq / 2, (int64_t)ctx->n_sm / 2);
-        attn::q4_pf_attn_kernel<T><<<2 * clusters, attn::NTHREADS, attn::SMEM_BYTES, st>>>(mq, mk, mv, map, kvc, q_gate,
-                                                                                          out, ctx->d_err);
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t lc{};
+        lc.gridDim = dim3(2 * clusters);
+        lc.blockDim = dim3(attn::NTHREADS);
+        lc.dynamicSmemBytes = attn::SMEM_BYTES;
+        lc.stream = st;
+        lc.attrs = at;
+        lc.numAttrs = 1;
+        e = cudaLaunchKernelEx(&lc, attn::q4_pf_attn_kernel<T>, mq, mk, mv, map, kvc, q_gate, out, ctx->d_err);
+        if (e != cudaSuccess) return e;
         *n_launch += 1;
     }
     return cudaGetLastError();
