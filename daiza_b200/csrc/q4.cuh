@@ -6,17 +6,18 @@
 //   even, grid 2^-17 below 2^-14), at most 896; code = clamp(rint(x / s), -7, 7);
 //   the held value is code * s.  NaN is held as 0, infinities saturate, a group
 //   whose s rounds to 0 is held as 0.
-// Rounding the scale to the nearest (not up) loses nothing: t / s <= 17/16, so the
-// largest |x| / s is 7.44 and still lands within half a step of code 7.
+// Rounding the scale to the nearest (not up) loses nothing from 2^-14 on: t / s <= 17/16,
+// so the largest |x| / s is 7.44 and still lands within half a step of code 7.
 // s is a positive f16 whose low 7 bits are zero, so 8 bits of it are stored
 // (f16 bits >> 7).  code * s has at most 3 + 4 significant bits: exact in f16, so
 // the matrix instructions multiply the held values themselves, with no second
 // rounding and no scale in an epilogue.  896 is the largest s for which 72 * s,
 // the constant of the unpacking below, is still an f16.
 //
-// Where a value next to a border falls must not depend on rounding in the
-// arithmetic before it: K's norm and rotation run in f64 on the way here, and the
-// code is decided from the exact remainder x - code * s.
+// Where a value next to a border falls must not depend on rounding in the arithmetic
+// before it, so K's codes are those of a norm and rotation in f64: f32 with a bound on
+// its error decides nearly every row, f64 the others.  Given values (V, imported rows)
+// are decided exactly in f32.
 //
 // Tile: 16 positions of one kv head, 4352 bytes (K codes 2048, V codes 2048, K
 // scales 128, V scales 128), in the register order of mma.m16n8k16, so that a warp

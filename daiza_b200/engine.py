@@ -331,7 +331,7 @@ class Context:
         if stream is not None:
             return stream.cuda_stream
         import torch
-        return torch._C._cuda_getCurrentRawStream(self.device)
+        return torch._C._cuda_getCurrentRawStream(int(self.device))
 
     def qk_mrope(self, layer, pos, q_gate, k, q_out, k_out, stream=None):
         """QK-RMSNorm, rotation by pos [T][3] (int32) and q's 1/16; q_gate [T][6*kvc][512] and k [T][kvc][256] f32 or
