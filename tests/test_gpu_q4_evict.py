@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 from daiza_b200._ffi import DZ_EINVAL, DZ_ESTATE
+from oracle import q4_ref as R
 from tests.test_gpu_q4 import Model, dev, refused
 
 pytestmark = pytest.mark.gpu
@@ -124,6 +125,50 @@ def test_serving_on_a_budget():
                 m.refs[s].w = got[s].astype(np.float64)
             evict(m, full, [64] * len(full), [16] * len(full))
     assert m.ctx.kv_len(0, 0) < 96 and at == [120, 90]
+    m.done()
+
+
+def test_offsets_beyond_32_bits():
+    """The last kv head of a sequence of 6 million slots lies 4.9 GB behind the first: prompt, decode, rows, weights
+    and eviction there, and in the sequence behind it."""
+    m = Model([6_000_000, 200], kvc=4, seed=218, track=True)
+    qg, k, v = m.inputs(130)
+    out = torch.empty(130, m.nq * 256, device="cuda")
+    m.ctx.gqa_prefill_q4(0, [1, 0], [50, 80], dev(qg), dev(k), dev(v), out)
+    for s, a, n in ((1, 0, 50), (0, 50, 80)):
+        want = m.refs[s].extend(qg[a:a + n], k[a:a + n], v[a:a + n], m.qn, m.kn)
+        got = out[a:a + n].cpu().numpy().reshape(want.shape)
+        assert np.abs(got - want).max() <= 2.2e-3 * np.abs(m.refs[s].v).max()
+        m.refs[s].w[:] = 0
+        m.check_held(s)
+    m.check_decode([0, 1])
+    m.check_weights([0, 1])
+    for s in (0, 1):
+        weigh(m, s, heavy_tailed(m, m.ctx.kv_len(0, s)))
+    evict(m, [0, 1], [33, 20], [5, 0])
+    m.done()
+
+
+def test_many_long_sequences_at_once():
+    """More pairs than clusters of four CTAs fit the GPU, each with more entries than a CTA keeps in registers."""
+    n = 9000
+    m = Model([n] * 80, kvc=1, seed=219, track=True)
+    k, v = m.normal(n, 1, 256), m.normal(n, 1, 256)
+    w = heavy_tailed(m, n)
+    for s in range(80):
+        m.ctx.kv_import(0, s, dev(k), dev(v))
+    m.ctx.kv_set_weights_q4(0, list(range(80)), dev(np.concatenate([np.roll(w.ravel(), s) for s in range(80)])))
+    keep, recent = 1500, 100
+    kept = torch.empty(80 * keep, dtype=torch.int32, device="cuda")
+    m.ctx.kv_evict_q4(0, list(range(80)), [keep] * 80, [recent] * 80, kept=kept)
+    for s in range(80):
+        m.refs[0] = R.Cache(1, k, v)
+        m.refs[0].w = np.roll(w.ravel(), s)[None].astype(np.float64)
+        idx = m.refs[0].evict(keep, recent)
+        assert np.array_equal(kept[s * keep:(s + 1) * keep].cpu().numpy(), idx[0]), f"seq {s}"
+        if s % 27 == 0:
+            got = m.ctx.kv_export(0, s)
+            assert np.array_equal(got[0], m.refs[0].k) and np.array_equal(got[1], m.refs[0].v)
     m.done()
 
 
