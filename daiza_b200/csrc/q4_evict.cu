@@ -47,7 +47,7 @@ struct alignas(16) EvictSmem {
         };
     };
     uint32_t scan[EV_WARPS], scan2[EV_WARPS];
-    uint32_t found[2];                           // bin, entries above it
+    uint32_t found[3];                           // bin, entries above it, entries in it
     alignas(8) uint32_t count[2];                // this CTA's entries above the threshold, and at it
 };
 
@@ -222,15 +222,23 @@ __global__ void __launch_bounds__(EV_THREADS, 2)
                 if (above < left && left <= above + c[i]) {
                     sm.found[0] = (uint32_t)(top - i);
                     sm.found[1] = above;
+                    sm.found[2] = c[i];
                 }
                 above += c[i];
             }
             __syncthreads();
             prefix = prefix << (pass == 2 ? 10 : 11) | sm.found[0];
             left -= sm.found[1];
+            const uint32_t in_bin = sm.found[2];
             __syncthreads();
+            // every entry of the bin stays (it often has just one): the key below it is a threshold
+            if (pass < 2 && left == in_bin && prefix > 0u) {
+                threshold = (prefix << shift) - 1u;
+                left = 0;
+                break;
+            }
+            threshold = prefix;
         }
-        threshold = prefix;
         ties = left;
     }
 
