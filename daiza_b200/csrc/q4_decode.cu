@@ -8,9 +8,9 @@
 //                    over the SMs; unnormalised partials out.
 //   3. q4_combine  : per (sequence, q head) -- merge, normalise, gate.
 //   4. q4_weights  : tracked caches -- the new attention weights are added.
-// One call, 24 q heads on 4 kv heads: one sequence of 2048, 10.5 us (three dependent grids:
-// latency); 64 of 512-32768 (1.17 GB), 296 us, 3.95 TB/s; 8 of 131072 (1.14 GB), 276 us,
-// 4.1 TB/s, 0.63 of a plain copy's rate.
+// One call, 24 q heads on 4 kv heads: one sequence of 2048, 10.4 us (three dependent grids:
+// latency); 64 of 512-32768 (1.17 GB), 295 us, 3.96 TB/s; 8 of 131072 (1.14 GB), 275 us,
+// 4.15 TB/s, 0.63 of a plain copy's rate.
 #include <algorithm>
 #include <cstddef>
 
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(256) q4_combine_kernel(const __grid_constant__
 // 4. tracked caches: weight of position j of a kv head += sum over its 6 q heads of
 //    exp2(score - M) / L, with M and L merged from the partials' (m, l).  The new
 //    position's weight starts here.  Grid (ceil(longest / 1024), kvc, B).  12 sequences of
-//    1137-7414: 39 us the call, 30 without weights; as a programmatic dependent it took the
+//    1137-7414: 38 us the call, 30 without weights; as a programmatic dependent it took the
 //    same time.
 // ---------------------------------------------------------------------------
 constexpr int WT_SPAN = 1024;

@@ -16,8 +16,8 @@
 //      round lie behind everything that an earlier one writes: source and destination may
 //      be the same sequence.
 // Bound by latency (cluster barriers and block scans of the selection, then two dependent
-// reads per moved row): one sequence of 4352 to 4096, 27 us; 13 of 9000-32768 to 2048 (63 MB),
-// 64 us.
+// reads per moved row): one sequence of 4352 to 4096, 25 us; 13 of 9000-32768 to 2048 (63 MB),
+// 60 us, half of it the scattered reads (about 900 bytes in pieces of 32 to 128 per kept row).
 #include <algorithm>
 
 #include "q4.cuh"
@@ -375,7 +375,7 @@ cudaError_t launch_q4_evict(dz_ctx* ctx, int layer, int B, const int32_t* src, c
             at += k;
         }
         // as many CTAs per (sequence, kv head) as fit the GPU at once, two per SM (52 pairs of 20000
-        // entries: 64 us with 4, 79 with 8, 96 with 2; 4 pairs: 27 us with 8, 37 and 60 with 4 and 2)
+        // entries: 60 us with 4, 73 with 8, 91 with 2; 4 pairs: 25 us with 8, 35 and 60 with 4 and 2)
         const int pairs = d.B * kvc;
         int32_t* list = static_cast<int32_t*>(ctx->q4_scratch);
         e = pairs * 8 <= 2 * ctx->n_sm   ? launch_evict<8>(d, L.d_q4, list, kept, st)

@@ -66,7 +66,7 @@ __device__ __forceinline__ uint4 held(const uint32_t (&code)[8], uint32_t sb) {
     return make_uint4(h[0], h[1], h[2], h[3]);
 }
 
-// 8192 bf16 tokens: 84 us for 0.28 GB (3.3 TB/s).  Bound by issue (57 % of the slots, at two
+// 8192 bf16 tokens: 77 us for 0.28 GB (3.6 TB/s).  Bound by issue (59 % of the slots, at two
 // blocks per SM; more blocks spill): norms, rotation, the codes and their f16 values.
 constexpr int PREP_WARPS = 16, PREP_ROWS = 4;    // query rows that a warp has in flight
 
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(32 * PREP_WARPS, 2)
 //              and small values' bits), times the gate's sigmoid, in whole rows
 // A cluster takes several query tiles in turn; while the outputs of one leave, the next one's
 // queries are fetched and its first blocks worked on.  (A cluster per tile, the softmax warps
-// writing the outputs: packed prompts of 1-1500 took 378 us, all of the call, instead of 247:
+// writing the outputs: packed prompts of 1-1500 took 378 us, all of the call, instead of 240:
 // set-up and outputs were 15 us of each tile's time, next to 1.3 us per block of keys.)
 // Bound by the products and the softmax together: a block of 128 keys takes 2270 cycles, of
 // which the products 2048; the softmax of one block (1950 cycles, 1100 of them exponentials)
