@@ -6,10 +6,10 @@
 //                    rotation; q as matrix operand, K and V quantised into slot len.
 //   2. q4_split    : scores, online softmax and P V over the cached tiles, cut evenly
 //                    over the SMs; unnormalised partials out.
-//   3. q4_combine  : per (sequence, q head) -- merge, normalise, gate.
-//   4. q4_weights  : tracked caches -- the new attention weights are added.
+//   3. q4_combine  : per (sequence, q head) -- merge, normalise, gate; tracked caches: further
+//                    blocks add the new attention weights.
 // One call, 24 q heads on 4 kv heads: one sequence of 2048, 10.4 us (three dependent grids:
-// latency); 64 of 512-32768 (1.17 GB), 295 us, 3.96 TB/s; 8 of 131072 (1.14 GB), 275 us,
+// latency); 64 of 512-32768 (1.17 GB), 294 us, 3.98 TB/s; 8 of 131072 (1.14 GB), 275 us,
 // 4.15 TB/s, 0.63 of a plain copy's rate.
 #include <algorithm>
 #include <cstddef>
@@ -436,22 +436,76 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
 }
 
 // ---------------------------------------------------------------------------
-// 3. combine: merge a row's partials, divide, gate.  Grid (6 kvc, B, 4 quarters of the
-//    dims), 16 groups of 16 threads that take partials in turn, 4 dims a thread.  Latency:
+// 3. tracked caches: weight of position j of a kv head += sum over its 6 q heads of
+//    exp2(score - M) / L, with M and L merged from the partials' (m, l).  The new
+//    position's weight starts here.  A block takes WT_SPAN positions of a (sequence, kv head).
+//    In the combine grid, beside its blocks: 12 sequences of 1137-7414 take 34.5 us (30 without
+//    weights; 38 as a kernel of its own behind it; 35.0 and 34.7 with spans of 1024 and 256).
+// ---------------------------------------------------------------------------
+constexpr int WT_SPAN = 512;
+
+__device__ __forceinline__ void add_weights(const Rows& d, int b, int kvh, int span, const Q4Slot* __restrict__ slots,
+                                            const float* __restrict__ part_ml, const float* __restrict__ scores) {
+    __shared__ float M[GRP], L[GRP];
+    const int n = d.len[b] + 1, j0 = span * WT_SPAN;
+    if (j0 >= n) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = b * d.kvc + kvh;
+    const int start = d.row_start(row), c0 = run_of(d, start), nc = run_of(d, start + d.row_tiles(b) - 1) - c0 + 1;
+    const Q4Slot slot = slots[d.sid[b]];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (warp < GRP) {
+        const float2* ml = reinterpret_cast<const float2*>(part_ml) + ((size_t)c0 + row) * GRP + warp;
+        float m = -INFINITY;
+        for (int i = lane; i < nc; i += 32) m = fmaxf(m, ml[(size_t)i * GRP].x);
+        m = warp_max(m);
+        float l = 0.0f;
+        for (int i = lane; i < nc; i += 32) {
+            const float2 v = ml[(size_t)i * GRP];
+            l += v.y * exp2f(v.x - m);
+        }
+        l = warp_sum(l);
+        if (lane == 0) {
+            M[warp] = m;
+            L[warp] = 1.0f / l;
+        }
+    }
+    __syncthreads();
+    float* wts = slot.wts + (size_t)kvh * slot.cap;
+    for (int j = j0 + threadIdx.x; j < min(n, j0 + WT_SPAN); j += 256) {
+        const float* sc = scores + (size_t)(start + (j >> 4)) * (GRP * Q4_TILE) + (j & 15);
+        float w = 0.0f;
+#pragma unroll
+        for (int h = 0; h < GRP; ++h) w += ex2f(sc[h * Q4_TILE] - M[h]) * L[h];
+        wts[j] = w + (j < n - 1 ? wts[j] : 0.0f);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// 4. combine: merge a row's partials, divide, gate.  Grid (6 kvc x 4 quarters of the
+//    dims, then the blocks of the weights; B), 16 groups of 16 threads that take partials in turn, 4 dims a thread.  Latency:
 //    about 3 us of a call.
 // ---------------------------------------------------------------------------
 constexpr int MAX_RUNS = 2048;                   // warps of the split grid (148 SMs: 1184)
 constexpr int CMB_DIMS = 64;
 
+template <bool TRACK>
 __global__ void __launch_bounds__(256) q4_combine_kernel(const __grid_constant__ Rows d,
                                                          const float* __restrict__ part_o,
                                                          const float* __restrict__ part_ml,
-                                                         const float* __restrict__ q_gate, float* __restrict__ out) {
+                                                         const float* __restrict__ q_gate, float* __restrict__ out,
+                                                         const Q4Slot* __restrict__ slots,
+                                                         const float* __restrict__ scores) {
     __shared__ float wgt[MAX_RUNS];
     __shared__ float red[2][8];
     __shared__ float4 acc[16][CMB_DIMS / 4];
     asm volatile("griddepcontrol.launch_dependents;");
-    const int nq = GRP * d.kvc, qh = blockIdx.x, b = blockIdx.y, d0 = blockIdx.z * CMB_DIMS, tid = threadIdx.x;
+    const int nq = GRP * d.kvc, b = blockIdx.y, quarter = blockIdx.x / nq, tid = threadIdx.x;
+    const int qh = blockIdx.x - quarter * nq, d0 = quarter * CMB_DIMS;
+    if (TRACK && quarter >= HD / CMB_DIMS) {
+        const int at = blockIdx.x - HD / CMB_DIMS * nq;
+        add_weights(d, b, at % d.kvc, at / d.kvc, slots, part_ml, scores);
+        return;
+    }
     const int kvh = qh / GRP, h = qh - kvh * GRP, row = b * d.kvc + kvh;
     const int warp = tid >> 5, lane = tid & 31;
     const float gate = tid < CMB_DIMS ? q_gate[((size_t)b * nq + qh) * QG_ROW + HD + d0 + tid] : 0.0f;
@@ -500,53 +554,6 @@ __global__ void __launch_bounds__(256) q4_combine_kernel(const __grid_constant__
     }
 }
 
-// ---------------------------------------------------------------------------
-// 4. tracked caches: weight of position j of a kv head += sum over its 6 q heads of
-//    exp2(score - M) / L, with M and L merged from the partials' (m, l).  The new
-//    position's weight starts here.  Grid (ceil(longest / 1024), kvc, B).  12 sequences of
-//    1137-7414: 38 us the call, 30 without weights; as a programmatic dependent it took the
-//    same time.
-// ---------------------------------------------------------------------------
-constexpr int WT_SPAN = 1024;
-
-__global__ void __launch_bounds__(256) q4_weights_kernel(const __grid_constant__ Rows d,
-                                                         const Q4Slot* __restrict__ slots,
-                                                         const float* __restrict__ part_ml,
-                                                         const float* __restrict__ scores) {
-    __shared__ float M[GRP], L[GRP];
-    const int b = blockIdx.z, kvh = blockIdx.y, n = d.len[b] + 1, j0 = blockIdx.x * WT_SPAN;
-    if (j0 >= n) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = b * d.kvc + kvh;
-    const int start = d.row_start(row);
-    if (warp < GRP) {
-        const int c0 = run_of(d, start), nc = run_of(d, start + d.row_tiles(b) - 1) - c0 + 1;
-        const float2* ml = reinterpret_cast<const float2*>(part_ml) + ((size_t)c0 + row) * GRP + warp;
-        float m = -INFINITY;
-        for (int i = lane; i < nc; i += 32) m = fmaxf(m, ml[(size_t)i * GRP].x);
-        m = warp_max(m);
-        float l = 0.0f;
-        for (int i = lane; i < nc; i += 32) {
-            const float2 v = ml[(size_t)i * GRP];
-            l += v.y * exp2f(v.x - m);
-        }
-        l = warp_sum(l);
-        if (lane == 0) {
-            M[warp] = m;
-            L[warp] = 1.0f / l;
-        }
-    }
-    __syncthreads();
-    const Q4Slot slot = slots[d.sid[b]];
-    float* wts = slot.wts + (size_t)kvh * slot.cap;
-    for (int j = j0 + threadIdx.x; j < min(n, j0 + WT_SPAN); j += 256) {
-        const float* sc = scores + (size_t)(start + (j >> 4)) * (GRP * Q4_TILE) + (j & 15);
-        float w = 0.0f;
-#pragma unroll
-        for (int h = 0; h < GRP; ++h) w += ex2f(sc[h * Q4_TILE] - M[h]) * L[h];
-        wts[j] = w + (j < n - 1 ? wts[j] : 0.0f);
-    }
-}
-
 }  // namespace q4
 
 cudaError_t q4_decode_setup() {
@@ -586,20 +593,19 @@ cudaError_t launch_q4_decode(dz_ctx* ctx, int layer, Q4Rows& d, const Q4Pos& pos
     e = cudaLaunchKernelEx(&lc, split, d, (const Q4Slot*)L.d_q4, (const uint32_t*)ctx->q4_frag, ctx->part_o,
                            ctx->part_ml, ctx->q4_sc, ctx->d_err);
     if (e != cudaSuccess) return e;
-    lc.gridDim = dim3(GRP * kvc, d.B, HD / CMB_DIMS);
+    int blocks = GRP * kvc * (HD / CMB_DIMS);
+    if (ctx->q4_track) {
+        const int longest = *std::max_element(d.len, d.len + d.B) + 1;
+        blocks += kvc * ((longest + WT_SPAN - 1) / WT_SPAN);
+    }
+    auto combine = ctx->q4_track ? q4_combine_kernel<true> : q4_combine_kernel<false>;
+    lc.gridDim = dim3(blocks, d.B);
     lc.blockDim = dim3(256);
     lc.dynamicSmemBytes = 0;
-    e = cudaLaunchKernelEx(&lc, q4_combine_kernel, d, (const float*)ctx->part_o, (const float*)ctx->part_ml, q_gate,
-                           out);
+    e = cudaLaunchKernelEx(&lc, combine, d, (const float*)ctx->part_o, (const float*)ctx->part_ml, q_gate, out,
+                           (const Q4Slot*)L.d_q4, (const float*)ctx->q4_sc);
     if (e != cudaSuccess) return e;
     *n_launch += 3;
-    if (ctx->q4_track) {
-        int longest = 0;
-        for (int b = 0; b < d.B; ++b) longest = std::max(longest, d.len[b] + 1);
-        q4_weights_kernel<<<dim3((longest + WT_SPAN - 1) / WT_SPAN, kvc, d.B), 256, 0, st>>>(
-            d, (const Q4Slot*)L.d_q4, (const float*)ctx->part_ml, (const float*)ctx->q4_sc);
-        *n_launch += 1;
-    }
     return cudaGetLastError();
 }
 
