@@ -324,7 +324,8 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 }
 // 2^x without the special-function unit, x at most 2^7: x = n + f with n nearest, a polynomial of
 // degree 4 for 2^f (least squares weighted towards the smallest largest error: 2.6e-6, far below P's
-// f16 rounding), n added to its exponent.  Below -126: 2^-126.
+// f16 rounding), n added to its exponent.  Below -126: 2^-126.  A quarter of the exponentials
+// this way: 2000 tokens after 5555 took 252 us instead of 253.5.
 __device__ __forceinline__ void ex2_poly(uint64_t x, float& p0, float& p1) {
     float a, b;
     unpack2(x, a, b);
