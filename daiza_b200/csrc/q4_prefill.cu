@@ -342,18 +342,18 @@ __device__ __forceinline__ void ex2_poly(uint64_t x, float& p0, float& p1) {
     p0 = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
     p1 = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
 }
-// (a sigmoid(x), b sigmoid(y)) / OUT_SCALE of f16 a and b, to 2^-20 or so, below the products' f16 rounding; one
-// reciprocal for both.  Below 2^-60 a sigmoid counts as 2^-60: the denominators' product is finite.
+// (a sigmoid(x), b sigmoid(y)) / OUT_SCALE of f16 a and b, to 2^-20 or so, below the products' f16 rounding: 1 / (8 + 2^(3 - x
+// log2 e)).  (One reciprocal of both denominators' product has to be kept from overflowing: it took as long.)
 __device__ __forceinline__ float2 gate2(uint32_t ab, float x, float y) {
-    float s, t, u, w, r;
-    unpack2(mul2(pack2(x, y), pack2(-LOG2E, -LOG2E)), s, t);
-    const uint64_t uw = add2(pack2(ex2(fminf(s, 60.0f)), ex2(fminf(t, 60.0f))), pack2(1.0f, 1.0f));
-    unpack2(uw, u, w);
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(u * w));
-    r *= 1.0f / OUT_SCALE;
-    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&ab));
+    static_assert(OUT_SCALE == 8.0f, "the exponent's 3");
+    float s, t, u, w, g, h;
+    unpack2(fma2(pack2(x, y), pack2(-LOG2E, -LOG2E), pack2(3.0f, 3.0f)), s, t);
+    unpack2(add2(pack2(ex2(s), ex2(t)), pack2(OUT_SCALE, OUT_SCALE)), u, w);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(g) : "f"(u));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(h) : "f"(w));
+    const float2 o = __half22float2(*reinterpret_cast<const __half2*>(&ab));
     float2 out;
-    unpack2(mul2(pack2(h.x, h.y), mul2(pack2(w, u), pack2(r, r))), out.x, out.y);
+    unpack2(mul2(pack2(o.x, o.y), pack2(g, h)), out.x, out.y);
     return out;
 }
 __device__ __forceinline__ void store8(float* p, float4 a, float4 b) {

@@ -1,12 +1,36 @@
 """What the calls on 4-bit caches take at their limits: values, weights and gates of any size, more prompts than one
 group of scratch holds, and scratch that grows."""
+import numpy as np
 import pytest
 
 from tests.test_gpu_q4 import Model, dev
+from tests.test_gpu_q4_prefill import MAX_TOL, prompt
 
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_prompt_gates_of_any_size(dtype):
+    """A NaN gate gives NaN, -inf 0, and a nearly closed one sigmoid's own small value.  An eighth of it is a reciprocal
+    whose results below 2^-126 are flushed to 0: sigmoids below 2^-123 count as 0."""
+    m = Model([40], kvc=1, seed=310)
+    q, k, v = m.inputs(30)
+    gates = np.array([np.nan, np.inf, -np.inf, 200, -200, -30, -45, -60, -80, 60, 0, -87], np.float32)
+    q[:, :, 256:256 + 12], q[:, :, 300:312], q[:, :, 399:411] = gates, gates[::-1], gates
+    with np.errstate(over="ignore"):
+        (got, want), = prompt(m, [0], [30], dtype, inputs=(q, k, v))
+    top = np.abs(m.refs[0].v).max()
+    nan = np.isnan(want)
+    assert nan.any() and np.array_equal(np.isnan(got), nan)
+    g = dev(q, getattr(torch, dtype)).double().cpu().numpy()[..., 256:]
+    with np.errstate(over="ignore"):
+        open_ = 1 / (1 + np.exp(-g))
+    step = 2.0 ** -8 if dtype == "bfloat16" else 0.0
+    bound = MAX_TOL * top * open_ + step * np.abs(want) + 2.0 ** -123 * top
+    assert np.all((np.abs(got - want) <= bound)[~nan])
+    m.done()
 
 
 def test_prompt_groups_of_sequences():
