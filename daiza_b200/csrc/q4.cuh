@@ -195,6 +195,16 @@ __device__ __forceinline__ double inv_sqrt(double x) {         // Newton's itera
     return g;
 }
 __device__ __forceinline__ float inv_sqrt(float x) { return 1.0f / sqrtf(x); }
+// 1 / rms of a row whose mean square v = sum / 256 + eps left f32, or the range where it keeps its bits: taken of the row
+// times a power of two.  (An infinity in the row: 0, as 1 / sqrt has it.)
+__device__ __forceinline__ bool out_of_range(float v) { return !(v > 1e-30f && v < 1e38f); }   // the same for the whole warp
+__device__ __forceinline__ float scaled_inv_rms(const float (&x)[8], float v, float eps) {
+    const float up = v < 1.0f ? 0x1p80f : 0x1p-80f;
+    float ss = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(x[e] * up, x[e] * up, ss);
+    return up * inv_sqrt(fmaf(warp_sum(ss), 1.0f / (float)HD, eps * up * up));
+}
 template <typename F, typename C>
 __device__ __forceinline__ void norm_rotate(F (&x)[8], const float* __restrict__ w, const C* cs, float eps, int lane) {
     F ss = 0;
@@ -202,7 +212,11 @@ __device__ __forceinline__ void norm_rotate(F (&x)[8], const float* __restrict__
     for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const F inv = inv_sqrt(ss / (F)HD + (F)eps);
+    const F v = ss / (F)HD + (F)eps;
+    F inv = inv_sqrt(v);
+    if constexpr (sizeof(F) == sizeof(float)) {
+        if (out_of_range(v)) inv = scaled_inv_rms(x, v, eps);
+    }
     const float4 w0 = reinterpret_cast<const float4*>(w)[2 * lane], w1 = reinterpret_cast<const float4*>(w)[2 * lane + 1];
     const float wv[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
@@ -223,15 +237,9 @@ __device__ __forceinline__ void norm_rotate(F (&x)[8], const float* __restrict__
 __device__ __forceinline__ int split_dim(int lane, int run) {
     return lane < 8 ? 4 * lane + 32 * run : 32 + 4 * lane + 96 * run;
 }
-// RMS norm, weight (w: this lane's 8) and rotation in f32; cs: (cos, sin) of pairs
-// 4 l .. 4 l + 3 in lanes 0..7.
-__device__ __forceinline__ void norm_rotate_split(float (&x)[8], const float (&w)[8], const float2 (&cs)[4], float eps,
-                                                  int lane) {
-    float ss = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-    const float v = fmaf(warp_sum(ss), 1.0f / (float)HD, eps), g = rsqrtf(v);
-    const float inv = fmaf(fmaf(-v * g, g, 1.0f), 0.5f * g, g);   // one Newton step: to the last bit or so
+// Weight (w: this lane's 8) and rotation of a row times inv, in f32; cs: (cos, sin) of pairs 4 l .. 4 l + 3 in lanes 0..7.
+__device__ __forceinline__ void scale_rotate_split(float (&x)[8], float inv, const float (&w)[8], const float2 (&cs)[4],
+                                                   int lane) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = (x[e] * inv) * w[e];
     if (lane < 8) {
@@ -242,6 +250,24 @@ __device__ __forceinline__ void norm_rotate_split(float (&x)[8], const float (&w
             x[e + 4] = fmaf(b, cs[e].x, a * cs[e].y);
         }
     }
+}
+// RMS norm, weight and rotation.  False, the same for the whole warp, where the row's mean square is out of range: the
+// caller takes such rows again behind its loop (norm_rotate_far).  A branch to that in here costs registers and keeps
+// rows in flight from overlapping: the rotary pass of 32768 bf16 tokens took 193 us instead of 166.
+__device__ __forceinline__ bool norm_rotate_split(float (&x)[8], const float (&w)[8], const float2 (&cs)[4], float eps,
+                                                  int lane) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+    const float v = fmaf(warp_sum(ss), 1.0f / (float)HD, eps), g = rsqrtf(v);
+    scale_rotate_split(x, fmaf(fmaf(-v * g, g, 1.0f), 0.5f * g, g), w, cs, lane);   // one Newton step: to the last bit or so
+    return !out_of_range(v);
+}
+__device__ __forceinline__ void norm_rotate_far(float (&x)[8], const float (&w)[8], const float2 (&cs)[4], float eps, int lane) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+    scale_rotate_split(x, scaled_inv_rms(x, fmaf(warp_sum(ss), 1.0f / (float)HD, eps), eps), w, cs, lane);
 }
 // The (cos, sin) that norm_rotate_split wants, from a lane's own pair (lane = pair).
 __device__ __forceinline__ void spread_pairs(float2 own, float2 (&cs)[4], int lane) {

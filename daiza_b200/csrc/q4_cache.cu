@@ -178,8 +178,10 @@ __global__ void __launch_bounds__(256) qk_mrope_kernel(const __grid_constant__ R
     load_split(k_norm, lane, wk);
 #pragma unroll
     for (int e = 0; e < 8; ++e) wq[e] *= 0.0625f;
+    static_assert(HQ + HKV <= 32, "a bit per head");
     const int heads = nq + kvc, share = (heads + gridDim.y - 1) / gridDim.y;
     const int h1 = min(heads, ((int)blockIdx.y + 1) * share);
+    uint32_t far = 0;                            // heads whose row is out of range
     for (int h0 = blockIdx.y * share; h0 < h1; h0 += MROPE_ROWS) {
         SplitRow<T> in[MROPE_ROWS];
 #pragma unroll
@@ -193,10 +195,18 @@ __global__ void __launch_bounds__(256) qk_mrope_kernel(const __grid_constant__ R
             if (h >= h1) break;
             float x[8];
             in[i].values(x);
-            if (h < nq) norm_rotate_split(x, wq, cs, eps, lane);
-            else norm_rotate_split(x, wk, cs, eps, lane);
-            store_split(h < nq ? q_out + (t * nq + h) * HD : k_out + (t * kvc + (h - nq)) * HD, lane, x);
+            const bool near = h < nq ? norm_rotate_split(x, wq, cs, eps, lane) : norm_rotate_split(x, wk, cs, eps, lane);
+            if (near) store_split(h < nq ? q_out + (t * nq + h) * HD : k_out + (t * kvc + (h - nq)) * HD, lane, x);
+            else far |= 1u << h;
         }
+    }
+    for (; far; far &= far - 1) {
+        const int h = __ffs(far) - 1;
+        float x[8];
+        load_split(h < nq ? q_gate + (t * nq + h) * QG_ROW : k + (t * kvc + (h - nq)) * HD, lane, x);
+        if (h < nq) norm_rotate_far(x, wq, cs, eps, lane);
+        else norm_rotate_far(x, wk, cs, eps, lane);
+        store_split(h < nq ? q_out + (t * nq + h) * HD : k_out + (t * kvc + (h - nq)) * HD, lane, x);
     }
 }
 

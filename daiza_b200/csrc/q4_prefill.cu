@@ -166,6 +166,12 @@ __global__ void __launch_bounds__(32 * PREP_WARPS, 2)
     load_split(q_norm, lane, w);
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] *= 0.0625f * LOG2E;   // scores in log2 units
+    auto store_q = [&](int h, const float (&x)[8]) {
+        __half* out = qf + ((size_t)h * tokens + row) * HD;
+        *reinterpret_cast<uint2*>(out + split_dim(lane, 0)) = make_uint2(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]));
+        *reinterpret_cast<uint2*>(out + split_dim(lane, 1)) = make_uint2(pack_f16(x[4], x[5]), pack_f16(x[6], x[7]));
+    };
+    uint32_t far = 0;                            // heads whose row is out of range
 #pragma unroll 1
     for (int h0 = h_first; h0 < h1; h0 += PREP_ROWS) {
         SplitRow<T> in[PREP_ROWS];
@@ -177,11 +183,16 @@ __global__ void __launch_bounds__(32 * PREP_WARPS, 2)
             if (h0 + i >= h1) break;
             float x[8];
             in[i].values(x);
-            norm_rotate_split(x, w, c4, eps, lane);
-            __half* out = qf + ((size_t)(h0 + i) * tokens + row) * HD;
-            *reinterpret_cast<uint2*>(out + split_dim(lane, 0)) = make_uint2(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]));
-            *reinterpret_cast<uint2*>(out + split_dim(lane, 1)) = make_uint2(pack_f16(x[4], x[5]), pack_f16(x[6], x[7]));
+            if (!norm_rotate_split(x, w, c4, eps, lane)) far |= 1u << (h0 + i);
+            store_q(h0 + i, x);
         }
+    }
+    for (; far; far &= far - 1) {
+        const int h = __ffs(far) - 1;
+        float x[8];
+        load_split(q_gate + (row * nq + h) * QG_ROW, lane, x);
+        norm_rotate_far(x, w, c4, eps, lane);
+        store_q(h, x);
     }
 }
 

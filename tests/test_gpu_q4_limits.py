@@ -3,8 +3,9 @@ group of scratch holds, and scratch that grows."""
 import numpy as np
 import pytest
 
-from tests.test_gpu_q4 import Model, dev
-from tests.test_gpu_q4_prefill import MAX_TOL, prompt
+from oracle import q4_ref as R
+from tests.test_gpu_q4 import OUT_TOL, Model, dev
+from tests.test_gpu_q4_prefill import MAX_TOL, check, prompt
 
 pytestmark = pytest.mark.gpu
 
@@ -30,6 +31,36 @@ def test_prompt_gates_of_any_size(dtype):
     step = 2.0 ** -8 if dtype == "bfloat16" else 0.0
     bound = MAX_TOL * top * open_ + step * np.abs(want) + 2.0 ** -123 * top
     assert np.all((np.abs(got - want) <= bound)[~nan])
+    m.done()
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e12, 1e19, 1e30, 3e38])
+def test_queries_of_any_size(size):
+    """Rows are normalised whatever their size: squares beyond f32's range count as they are, in decode, prompts and the
+    rotary pass."""
+    m = Model([60, 60], kvc=2, seed=311)
+    m.fill(0, 19)
+    qg, k, v = m.inputs(40)
+    qg[..., :256] = np.clip(qg[..., :256], -1, 1) * np.float32(size)
+    k = np.clip(k, -1, 1) * np.float32(size)
+    got, want = m.decode([0], inputs=(qg[:1], k[:1], v[:1]))
+    assert np.abs(got - want).max() <= OUT_TOL * np.abs(m.refs[0].v).max()
+    for dtype in ("float32", "bfloat16"):
+        m.ctx.kv_truncate(0, 1, 0)
+        m.refs[1] = R.Cache(2)
+        check(m, [1], [40], dtype, inputs=(qg, k, v))
+        dt = getattr(torch, dtype)
+        tq, tk = dev(qg, dt), dev(k, dt)
+        pos = m.rng.integers(0, 1 << 20, (40, 3))
+        q_out, k_out = torch.empty(40, m.nq, 256, dtype=dt, device="cuda"), torch.empty_like(tk)
+        m.ctx.qk_mrope(0, dev(pos, torch.int32), tq, tk, q_out, k_out)
+        for out, x, norm, c in ((q_out, tq[..., :256], m.qn, 1 / 16), (k_out, tk, m.kn, 1.0)):
+            want = c * R.turn(x.double().cpu().numpy(), norm, pos, m.axis)
+            rounding = 2.0 ** -8 * np.abs(want) if dtype == "bfloat16" else 0.0
+            err = np.abs(out.double().cpu().numpy() - want)
+            assert np.all(err <= 2e-6 * np.abs(want).max(-1, keepdims=True) + rounding + 1e-30), err.max()
+        m.ctx.qk_mrope(0, dev(pos, torch.int32), tq, tk, q_out, tk)    # k in place
+        assert torch.equal(tk, k_out)
     m.done()
 
 
