@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(256) q4_weights_clear_kernel(Q4Slot slot, int 
 // ---- rotary positions of three axes ------------------------------------------------------
 // QK-RMSNorm, rotation and q's 1/16 for T tokens.  HBM bound: q's halves of q_gate and k
 // read once, q and k written once.  The angle is reduced in f64, sine and cosine taken
-// in f32.
+// in f32.  k_out may be k: a row is loaded whole by the warp that writes it.
 __device__ __forceinline__ void store_split(float* row, int lane, const float (&x)[8]) {
     *reinterpret_cast<float4*>(row + split_dim(lane, 0)) = make_float4(x[0], x[1], x[2], x[3]);
     *reinterpret_cast<float4*>(row + split_dim(lane, 1)) = make_float4(x[4], x[5], x[6], x[7]);
@@ -165,9 +165,9 @@ constexpr int MROPE_ROWS = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) qk_mrope_kernel(const __grid_constant__ RopeAxes axes, int kvc, int64_t n_tokens,
                                                        const int32_t* __restrict__ pos, const T* __restrict__ q_gate,
-                                                       const T* __restrict__ k, const float* __restrict__ q_norm,
-                                                       const float* __restrict__ k_norm, T* __restrict__ q_out,
-                                                       T* __restrict__ k_out, float eps) {
+                                                       const T* k, const float* __restrict__ q_norm,
+                                                       const float* __restrict__ k_norm, T* __restrict__ q_out, T* k_out,
+                                                       float eps) {
     const int lane = threadIdx.x & 31, nq = GRP * kvc;
     const int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (t >= n_tokens) return;
