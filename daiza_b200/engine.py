@@ -44,10 +44,12 @@ def _stream(stream):
     return C.c_void_p(s.cuda_stream)
 
 
-def _tensor(name, t, dtype, numel):
-    """Address of a contiguous CUDA tensor that a 4-bit cache call reads or writes; DZ_EINVAL otherwise."""
-    if not (t.is_cuda and t.dtype == dtype and t.is_contiguous() and t.numel() == numel):
-        raise _ffi.DzError(_ffi.DZ_EINVAL, f"{name} must be a contiguous CUDA {dtype} tensor of {numel} values, got "
+def _tensor(name, t, dtype, numel, device=None):
+    """Address of a contiguous CUDA tensor (on that device) that a 4-bit cache call takes; DZ_EINVAL otherwise."""
+    if not (t.is_cuda and t.dtype == dtype and t.is_contiguous() and t.numel() == numel and
+            (device is None or t.get_device() == device)):
+        where = "CUDA" if device is None else f"cuda:{device}"
+        raise _ffi.DzError(_ffi.DZ_EINVAL, f"{name} must be a contiguous {where} {dtype} tensor of {numel} values, got "
                                            f"{tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
     return t.data_ptr()
 
@@ -325,6 +327,9 @@ class Context:
         s = _ints("sections", sections, C.c_int32, 3)
         self._chk(self.lib.dz_set_rope_axes(self.h, s, int(bool(interleaved))))
 
+    def _tensor(self, name, t, dtype, numel):
+        return _tensor(name, t, dtype, numel, int(self.device))
+
     def _on(self, stream):
         """Handle of `stream`, or of the context's device's current one (the raw handle: making a Stream object of it
         takes 1.3 us)."""
@@ -340,10 +345,11 @@ class Context:
         T = k.numel() // (self.kvc * HD)
         dt = torch.bfloat16 if k.dtype == torch.bfloat16 else torch.float32
         fn = self.lib.dz_qk_mrope_bf16 if dt == torch.bfloat16 else self.lib.dz_qk_mrope
-        self._chk(fn(self.h, layer, T, _tensor("pos", pos, torch.int32, 3 * T),
-                     _tensor("q_gate", q_gate, dt, T * self.nq * QG_ROW), _tensor("k", k, dt, T * self.kvc * HD),
-                     _tensor("q_out", q_out, dt, T * self.nq * HD), _tensor("k_out", k_out, dt, T * self.kvc * HD),
-                     self._on(stream)))
+        self._chk(fn(self.h, layer, T, self._tensor("pos", pos, torch.int32, 3 * T),
+                     self._tensor("q_gate", q_gate, dt, T * self.nq * QG_ROW),
+                     self._tensor("k", k, dt, T * self.kvc * HD),
+                     self._tensor("q_out", q_out, dt, T * self.nq * HD),
+                     self._tensor("k_out", k_out, dt, T * self.kvc * HD), self._on(stream)))
 
     def gqa_decode_q4(self, layer, seq_ids, q_gate, k, v, out, stream=None, pos=None):
         """gqa_decode on 4-bit caches; pos: [B][3] rotary positions (host), default the cache lengths."""
@@ -354,8 +360,9 @@ class Context:
             p3 = _ints("pos", [p for row in pos for p in row], C.c_int32, 3 * B)
         self._chk(self.lib.dz_gqa_decode_q4(
             self.h, layer, B, ids, p3,
-            _tensor("q_gate", q_gate, f, B * self.nq * QG_ROW), _tensor("k", k, f, B * self.kvc * HD),
-            _tensor("v", v, f, B * self.kvc * HD), _tensor("out", out, f, B * self.nq * HD), self._on(stream)))
+            self._tensor("q_gate", q_gate, f, B * self.nq * QG_ROW), self._tensor("k", k, f, B * self.kvc * HD),
+            self._tensor("v", v, f, B * self.kvc * HD), self._tensor("out", out, f, B * self.nq * HD),
+            self._on(stream)))
 
     def gqa_prefill_q4(self, layer, seq_ids, lens, q_gate, k, v, out, stream=None, pos=None):
         """lens[i] new tokens of each sequence, packed: q_gate [sum][6*kvc][512], k and v [sum][kvc][256], out
@@ -367,9 +374,10 @@ class Context:
         dt = torch.bfloat16 if k.dtype == torch.bfloat16 else torch.float32
         fn = self.lib.dz_gqa_prefill_q4_bf16 if dt == torch.bfloat16 else self.lib.dz_gqa_prefill_q4
         self._chk(fn(self.h, layer, len(ids), ids, n,
-                     None if pos is None else _tensor("pos", pos, torch.int32, 3 * T),
-                     _tensor("q_gate", q_gate, dt, T * self.nq * QG_ROW), _tensor("k", k, dt, T * self.kvc * HD),
-                     _tensor("v", v, dt, T * self.kvc * HD), _tensor("out", out, dt, T * self.nq * HD),
+                     None if pos is None else self._tensor("pos", pos, torch.int32, 3 * T),
+                     self._tensor("q_gate", q_gate, dt, T * self.nq * QG_ROW),
+                     self._tensor("k", k, dt, T * self.kvc * HD),
+                     self._tensor("v", v, dt, T * self.kvc * HD), self._tensor("out", out, dt, T * self.nq * HD),
                      self._on(stream)))
 
     def kv_rows_q4(self, layer, seq_ids, first, count, k, v, stream=None):
@@ -379,8 +387,8 @@ class Context:
         a, n = _per_seq("first", first, ids), _per_seq("count", count, ids)
         total = _total(n) * self.kvc * HD
         self._chk(self.lib.dz_kv_rows_q4(self.h, layer, len(ids), ids, a, n,
-                                         _tensor("k", k, torch.float32, total), _tensor("v", v, torch.float32, total),
-                                         self._on(stream)))
+                                         self._tensor("k", k, torch.float32, total),
+                                         self._tensor("v", v, torch.float32, total), self._on(stream)))
 
     def _weights_numel(self, layer, ids):
         return self.kvc * sum(self._lens(layer, ids))
@@ -391,14 +399,14 @@ class Context:
         ids = _ids(seq_ids)
         self._chk(self.lib.dz_kv_weights_q4(
             self.h, layer, len(ids), ids,
-            _tensor("out", out, torch.float32, self._weights_numel(layer, ids)), self._on(stream)))
+            self._tensor("out", out, torch.float32, self._weights_numel(layer, ids)), self._on(stream)))
 
     def kv_set_weights_q4(self, layer, seq_ids, weights, stream=None):
         import torch
         ids = _ids(seq_ids)
         self._chk(self.lib.dz_kv_set_weights_q4(
             self.h, layer, len(ids), ids,
-            _tensor("weights", weights, torch.float32, self._weights_numel(layer, ids)), self._on(stream)))
+            self._tensor("weights", weights, torch.float32, self._weights_numel(layer, ids)), self._on(stream)))
 
     def kv_evict_q4(self, layer, seq_ids, keep, recent, kept=None, into=None, stream=None):
         """Keeps the last recent[b] and the heaviest other entries, keep[b] in all, per kv head; in place, or into the
@@ -410,7 +418,7 @@ class Context:
         out = None
         if kept is not None:
             n = sum(max(0, min(a, b)) for a, b in zip(k, self._lens(layer, ids)))
-            out = _tensor("kept", kept, torch.int32, n * self.kvc)
+            out = self._tensor("kept", kept, torch.int32, n * self.kvc)
         self._chk(self.lib.dz_kv_evict_q4(self.h, layer, len(ids), ids, to,
                                           k, r, out, self._on(stream)))
 

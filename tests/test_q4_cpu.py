@@ -106,3 +106,39 @@ def test_host_tensors_wrong_types_and_sizes_are_refused():
         engine._ids([1 << 31])
     assert list(engine._ids(np.array([3, 1]))) == [3, 1] and list(engine._ids(2)) == [2]
     assert list(engine._per_seq("count", (4, 5), engine._ids([0, 1]))) == [4, 5]
+
+
+class OfAnotherGpu:
+    """What the checks ask of a tensor, for one that lies on cuda:1."""
+    is_cuda, shape, device = True, (4,), "cuda:1"
+
+    def __init__(self, torch):
+        self.dtype = torch.float32
+
+    def get_device(self):
+        return 1
+
+    def is_contiguous(self):
+        return True
+
+    def numel(self):
+        return 4
+
+    def stride(self):
+        return (1,)
+
+    def data_ptr(self):
+        return 4096
+
+
+def test_tensors_of_another_gpu_are_refused():
+    torch = pytest.importorskip("torch")
+    from daiza_b200 import engine
+    from daiza_b200._ffi import DZ_EINVAL, DzError
+    there = OfAnotherGpu(torch)
+    assert engine._tensor("x", there, torch.float32, 4, 1) == 4096
+    ctx = engine.Context.__new__(engine.Context)     # a context of cuda:0, as far as its checks go
+    ctx.device, ctx.h = 0, None
+    with pytest.raises(DzError) as e:
+        ctx._tensor("x", there, torch.float32, 4)
+    assert e.value.status == DZ_EINVAL and "cuda:0" in str(e.value)
