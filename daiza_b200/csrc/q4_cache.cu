@@ -435,8 +435,8 @@ dz_status dz_gqa_decode_q4(dz_ctx* ctx, int layer, int B, const int32_t* seq_ids
             Q4_CUDA(launch_q4_decode(ctx, layer, d, p3, q_gate + (size_t)b0 * nq * QG_ROW, k + (size_t)b0 * kvc * HD,
                                      v + (size_t)b0 * kvc * HD, out + (size_t)b0 * nq * HD,
                                      static_cast<cudaStream_t>(stream), &launches));
-            for (int b = 0; b < d.B; ++b) L.len[d.sid[b]] += 1;
         }
+        for (int b = 0; b < B; ++b) L.len[seq_ids[b]] += 1;
         ctx->last_launches = launches;
         return DZ_OK;
     });

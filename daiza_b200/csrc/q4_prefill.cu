@@ -776,8 +776,7 @@ static cudaError_t launch_group(dz_ctx* ctx, int layer, const q4::Prompt& d, con
     const int kvc = ctx->cfg.kv_head_count, nq = GRP * kvc;
     const int64_t tokens = d.row0[d.n], keys = d.key0[d.n];
     const size_t qn = (size_t)nq * tokens * HD, kn = (size_t)kvc * keys * HD;
-    cudaError_t e = ensure_q4_scratch(ctx, (qn + 2 * kn) * sizeof(__half));
-    if (e != cudaSuccess) return e;
+    cudaError_t e;
     __half* qf = static_cast<__half*>(ctx->q4_scratch);
     __half *kf = qf + qn, *vf = kf + kn;
     CUtensorMap mq, mk, mv;
@@ -839,43 +838,53 @@ static cudaError_t launch_group(dz_ctx* ctx, int layer, const q4::Prompt& d, con
 // this, unless one alone is larger.
 static constexpr int64_t GROUP_BYTES = (int64_t)2 << 30;
 
+// The group that begins at sequence i (i moves behind it); its scratch in bytes, 0 if no tokens are left.
+static int64_t next_group(const LayerState& L, int kvc, int& i, int n, const int32_t* seq_ids, const int64_t* lens,
+                          q4::Prompt& d) {
+    d.n = 0;
+    d.row0[0] = d.key0[0] = d.at0[0] = d.old0[0] = 0;
+    int64_t bytes = 0;
+    for (; i < n && d.n < MAXB; ++i) {
+        const int64_t base = L.len[seq_ids[i]], T_i = lens[i];
+        const int64_t keys = (base + T_i + q4::attn::BN - 1) / q4::attn::BN * q4::attn::BN;
+        const int64_t more = (T_i * GRP + 2 * keys) * kvc * HD * (int64_t)sizeof(__half);
+        if (T_i == 0) continue;
+        if (d.n > 0 && bytes + more > GROUP_BYTES) break;
+        bytes += more;
+        const int s = d.n++;
+        d.sid[s] = seq_ids[i];
+        d.base[s] = (int32_t)base;
+        d.row0[d.n] = d.row0[s] + (int32_t)T_i;
+        d.key0[d.n] = d.key0[s] + (int32_t)keys;
+        d.at0[d.n] = d.at0[s] + (int32_t)((base + T_i - 1) / Q4_TILE - base / Q4_TILE + 1);
+        d.old0[d.n] = d.old0[s] + d.cached_tiles(s) + (int32_t)(keys / Q4_TILE - d.first_pad_tile(s));
+    }
+    return bytes;
+}
+
+// All or nothing: scratch for the largest group before the first launch, lengths after the last.
 template <typename T>
 static cudaError_t launch_prompts(dz_ctx* ctx, int layer, int n, const int32_t* seq_ids, const int64_t* lens,
                                   const int32_t* pos, const T* q_gate, const T* k, const T* v, T* out, cudaStream_t st,
                                   int* n_launch) {
     LayerState& L = ctx->layers[layer];
     const int kvc = ctx->cfg.kv_head_count, nq = GRP * kvc;
+    q4::Prompt d;
+    int64_t most = 0;
+    for (int i = 0; i < n;) most = std::max(most, next_group(L, kvc, i, n, seq_ids, lens, d));
+    cudaError_t e = ensure_q4_scratch(ctx, most);
+    if (e != cudaSuccess) return e;
     for (int i = 0; i < n;) {
-        q4::Prompt d;
-        d.n = 0;
-        d.row0[0] = d.key0[0] = d.at0[0] = d.old0[0] = 0;
-        int64_t bytes = 0;
-        for (; i < n && d.n < MAXB; ++i) {
-            const int64_t base = L.len[seq_ids[i]], T_i = lens[i];
-            const int64_t keys = (base + T_i + q4::attn::BN - 1) / q4::attn::BN * q4::attn::BN;
-            const int64_t more = T_i * nq * HD * 2 + keys * kvc * HD * 4;
-            if (T_i == 0) continue;
-            if (d.n > 0 && bytes + more > GROUP_BYTES) break;
-            bytes += more;
-            const int s = d.n++;
-            d.sid[s] = seq_ids[i];
-            d.base[s] = (int32_t)base;
-            d.row0[d.n] = d.row0[s] + (int32_t)T_i;
-            d.key0[d.n] = d.key0[s] + (int32_t)keys;
-            d.at0[d.n] = d.at0[s] + (int32_t)((base + T_i - 1) / Q4_TILE - base / Q4_TILE + 1);
-            d.old0[d.n] = d.old0[s] + d.cached_tiles(s) + (int32_t)(keys / Q4_TILE - d.first_pad_tile(s));
-        }
-        if (d.n == 0) break;
-        const cudaError_t e = launch_group<T>(ctx, layer, d, pos, q_gate, k, v, out, st, n_launch);
-        if (e != cudaSuccess) return e;
+        if (next_group(L, kvc, i, n, seq_ids, lens, d) == 0) break;
+        if ((e = launch_group<T>(ctx, layer, d, pos, q_gate, k, v, out, st, n_launch)) != cudaSuccess) return e;
         const size_t rows = d.row0[d.n];
-        for (int s = 0; s < d.n; ++s) L.len[d.sid[s]] += d.T(s);
         if (pos) pos += 3 * rows;
         q_gate += rows * nq * QG_ROW;
         k += rows * kvc * HD;
         v += rows * kvc * HD;
         out += rows * nq * HD;
     }
+    for (int i = 0; i < n; ++i) L.len[seq_ids[i]] += lens[i];
     return cudaSuccess;
 }
 

@@ -3,6 +3,7 @@ group of scratch holds, and scratch that grows."""
 import numpy as np
 import pytest
 
+from daiza_b200._ffi import DZ_ENOMEM, DzError
 from oracle import q4_ref as R
 from tests.test_gpu_q4 import OUT_TOL, Model, dev
 from tests.test_gpu_q4_prefill import MAX_TOL, check, prompt
@@ -83,4 +84,28 @@ def test_prompt_groups_of_sequences():
         m.ctx.gqa_prefill_q4(0, [s], [t], qg[b], k[b], v[b], one, pos=pos[b])
         assert torch.equal(one, out[b]), s
         a += t
+    m.done()
+
+
+def test_prompt_that_finds_no_memory_leaves_every_length():
+    """The second sequence's scratch (2.6 GB) is more than what is left: none of the prompts is appended."""
+    n = 640000
+    m = Model([100, n + 8], kvc=4, seed=315)
+    zeros = torch.zeros(n, 4, 256, device="cuda")
+    m.ctx.kv_import(0, 1, zeros, zeros)
+    del zeros
+    torch.cuda.empty_cache()
+    qg, k, v = (dev(x) for x in m.inputs(24))
+    out = torch.empty(24, m.nq * 256, device="cuda")
+    torch.cuda.synchronize()
+    rest = torch.empty(torch.cuda.mem_get_info()[0] - (1 << 30), dtype=torch.uint8, device="cuda")
+    with pytest.raises(DzError) as e:
+        m.ctx.gqa_prefill_q4(0, [0, 1], [16, 8], qg, k, v, out)
+    assert e.value.status == DZ_ENOMEM
+    lens = m.ctx.kv_lens(0, [0, 1])
+    del rest
+    torch.cuda.empty_cache()
+    assert lens == [0, n]
+    m.ctx.gqa_prefill_q4(0, [0, 1], [16, 8], qg, k, v, out)
+    assert m.ctx.kv_lens(0, [0, 1]) == [16, n + 8]
     m.done()
