@@ -23,17 +23,30 @@ void rope_axes_set(RopeAxes& a, const int32_t sections[3], bool interleaved, dou
     }
 }
 
+// An allocation is no work of the stream: it may be made while a graph is captured, on this thread or another
+// (the buffer stays until the context goes, so the graph may hold it).
+static cudaError_t alloc_uncaptured(void** p, size_t bytes) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return e;
+    e = cudaMalloc(p, bytes);
+    const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e == cudaErrorMemoryAllocation) cudaGetLastError();
+    return e != cudaSuccess ? e : back;
+}
+
 cudaError_t ensure_q4_scratch(dz_ctx* ctx, size_t bytes) {
     if (ctx->q4_scratch_bytes >= bytes) return cudaSuccess;
-    ctx->q4_retired.reserve(ctx->q4_retired.size() + 1);
+    try {
+        ctx->q4_retired.reserve(ctx->q4_retired.size() + 1);
+    } catch (const std::exception&) {
+        return cudaErrorMemoryAllocation;
+    }
     // at least twice the size before, so that all the old ones together are smaller than the new one
     size_t size = std::max(bytes, 2 * ctx->q4_scratch_bytes);
     void* p = nullptr;
-    cudaError_t e = cudaMalloc(&p, size);
-    if (e == cudaErrorMemoryAllocation && size > bytes) {
-        cudaGetLastError();
-        e = cudaMalloc(&p, size = bytes);
-    }
+    cudaError_t e = alloc_uncaptured(&p, size);
+    if (e == cudaErrorMemoryAllocation && size > bytes) e = alloc_uncaptured(&p, size = bytes);
     if (e != cudaSuccess) return e;
     if (ctx->q4_scratch) ctx->q4_retired.push_back(ctx->q4_scratch);
     ctx->q4_scratch = p;
@@ -225,11 +238,8 @@ dz_status fail(dz_ctx* ctx, dz_status st, const char* fmt, ...) {
     return st;
 }
 dz_status cuda_fail(dz_ctx* ctx, cudaError_t e, const char* what) {
-    if (e == cudaErrorMemoryAllocation) {
-        cudaGetLastError();
-        return fail(ctx, DZ_ENOMEM, "%s: %s", what, cudaGetErrorString(e));
-    }
-    return fail(ctx, DZ_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+    cudaGetLastError();   // reported here: the next call's launch check must not find it again
+    return fail(ctx, e == cudaErrorMemoryAllocation ? DZ_ENOMEM : DZ_ECUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 #define Q4_CUDA(call)                                            \
     do {                                                         \

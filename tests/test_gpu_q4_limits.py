@@ -109,3 +109,51 @@ def test_prompt_that_finds_no_memory_leaves_every_length():
     m.ctx.gqa_prefill_q4(0, [0, 1], [16, 8], qg, k, v, out)
     assert m.ctx.kv_lens(0, [0, 1]) == [16, n + 8]
     m.done()
+
+
+def test_scratch_grows_within_a_capture():
+    """The first prompts and evictions of a context may be captured ones: replays give what the plain calls give."""
+    m = Model([600] * 4, kvc=1, seed=316, track=True)
+    tensors = [dev(x) for x in m.inputs(500)]
+    outs = torch.zeros(2, 500, m.nq * 256, device="cuda")
+    weights = torch.rand(500, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    kept = torch.zeros(2, 400, dtype=torch.int32, device="cuda")
+    prompt_graph, evict_graph = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(prompt_graph):
+        m.ctx.gqa_prefill_q4(0, [0], [500], *tensors, outs[0])
+    with torch.cuda.graph(evict_graph):
+        m.ctx.kv_evict_q4(0, [0], [400], [30], kept=kept[0], into=[2])
+    prompt_graph.replay()
+    m.ctx.kv_set_weights_q4(0, [0], weights)
+    evict_graph.replay()
+    m.ctx.gqa_prefill_q4(0, [1], [500], *tensors, outs[1])
+    m.ctx.kv_set_weights_q4(0, [1], weights)
+    m.ctx.kv_evict_q4(0, [1], [400], [30], kept=kept[1], into=[3])
+    torch.cuda.synchronize()
+    assert torch.equal(*outs) and torch.equal(*kept)
+    for a, b in ((0, 1), (2, 3)):
+        assert all(np.array_equal(x, y) for x, y in zip(m.ctx.kv_export(0, a), m.ctx.kv_export(0, b)))
+    m.done()
+
+
+@pytest.mark.parametrize("first", ["prompt", "evict"])
+def test_first_call_of_a_context_is_captured(first):
+    m = Model([600, 600], kvc=1, seed=318, track=True)
+    graph = torch.cuda.CUDAGraph()
+    if first == "prompt":
+        tensors, out = [dev(x) for x in m.inputs(40)], torch.zeros(2, 40, m.nq * 256, device="cuda")
+        with torch.cuda.graph(graph):
+            m.ctx.gqa_prefill_q4(0, [0], [40], *tensors, out[0])
+        graph.replay()
+        m.ctx.gqa_prefill_q4(0, [1], [40], *tensors, out[1])
+        torch.cuda.synchronize()
+        assert torch.equal(*out)
+    else:
+        kept = torch.full((1,), -7, dtype=torch.int32, device="cuda")
+        m.ctx.gqa_decode_q4(0, [0], *[dev(x) for x in m.inputs(1)], torch.empty(1, m.nq * 256, device="cuda"))
+        with torch.cuda.graph(graph):
+            m.ctx.kv_evict_q4(0, [0], [1], [0], kept=kept)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert kept.item() == 0
+    m.done()
