@@ -58,6 +58,12 @@ void free_cache(dz_ctx* ctx) {
     ctx->q4 = ctx->q4_track = false;
     ctx->q4_frag = nullptr;
     ctx->q4_sc = nullptr;
+    // graphs that hold the scratch hold these caches too: nothing can replay them any more
+    if (ctx->q4_scratch) cudaFree(ctx->q4_scratch);
+    for (void* p : ctx->q4_retired) cudaFree(p);
+    ctx->q4_scratch = nullptr;
+    ctx->q4_scratch_bytes = 0;
+    ctx->q4_retired.clear();
     ctx->n_seqs = 0;
     ctx->caps.clear();
     for (auto& sn : ctx->snaps) sn.valid = false;
@@ -265,8 +271,6 @@ dz_status dz_ctx_destroy(dz_ctx* ctx) {
         free_q1_maps(ctx);
         if (ctx->mlp) cudaFree(ctx->mlp);
         if (ctx->d_err) cudaFree(ctx->d_err);
-        if (ctx->q4_scratch) cudaFree(ctx->q4_scratch);
-        for (void* p : ctx->q4_retired) cudaFree(p);
         if (ctx->snap_mem) cudaFree(ctx->snap_mem);
         for (auto& e : ctx->pf_ev)
             if (e) cudaEventDestroy(e);

@@ -157,7 +157,7 @@ struct dz_ctx {
     cudaEvent_t pf_ev[dz::PF_MAX_SEGMENTS + 1] = {};
     // 4-bit KV caches (dz_cache_create_q4): the decode kernels' q operand, the scores of tracked
     // caches, and scratch of prompts and evictions.  A buffer that is outgrown stays allocated
-    // until the context goes: a captured graph may hold it.
+    // until the caches go: a captured graph may hold it.
     bool q4 = false, q4_track = false;
     dz::RopeAxes axes{};
     uint32_t* q4_frag = nullptr;  // [min(n_seqs, MAXB)][kvc][Q4_FRAG_WORDS]

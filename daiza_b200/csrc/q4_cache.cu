@@ -24,7 +24,7 @@ void rope_axes_set(RopeAxes& a, const int32_t sections[3], bool interleaved, dou
 }
 
 // An allocation is no work of the stream: it may be made while a graph is captured, on this thread or another
-// (the buffer stays until the context goes, so the graph may hold it).
+// (the buffer stays until the caches go, so the graph may hold it).
 static cudaError_t alloc_uncaptured(void** p, size_t bytes) {
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
     cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);

@@ -157,3 +157,19 @@ def test_first_call_of_a_context_is_captured(first):
         torch.cuda.synchronize()
         assert kept.item() == 0
     m.done()
+
+
+def test_scratch_goes_with_the_caches():
+    """The prompt behind 20000 rows takes 80 MB of scratch; smaller caches in the same context give it back."""
+    m = Model([20000], kvc=4, seed=317)
+    zeros = torch.zeros(20000 - 8, 4, 256, device="cuda")
+    m.ctx.kv_import(0, 0, zeros, zeros)
+    qg, k, v = (dev(x) for x in m.inputs(8))
+    m.ctx.gqa_prefill_q4(0, [0], [8], qg, k, v, torch.empty(8, m.nq * 256, device="cuda"))
+    m.ctx.cache_create_q4([16])
+    torch.cuda.synchronize()
+    small = torch.cuda.mem_get_info()[0]
+    m.ctx.cache_create_q4([16])
+    m.ctx.close()
+    torch.cuda.synchronize()
+    assert torch.cuda.mem_get_info()[0] - small <= 32 << 20
