@@ -257,6 +257,7 @@ dz_status guarded(dz_ctx* ctx, F&& body) {
     try {
         return body();
     } catch (const std::exception&) {
+        ctx->err.assign("out of memory");   // short enough to need none
         return DZ_ENOMEM;
     }
 }

@@ -60,9 +60,9 @@ _arrays = {}                                     # ctypes array types by (type, 
 def _ints(name, values, ctype, count=None):
     """ctypes array of whole numbers (a number, list or array); DZ_EINVAL if they do not fit or are not `count`.
     A list goes straight into the array: the numpy route costs as much as a small launch."""
-    v = values if type(values) is list or type(values) is tuple else np.atleast_1d(values).tolist()
-    n = len(v)
     try:
+        v = values if type(values) is list or type(values) is tuple else np.atleast_1d(values).tolist()
+        n = len(v)
         if count is not None and n != count:
             raise ValueError(f"{count} numbers wanted, {n} given")
         top = 1 << 31 if ctype is C.c_int32 else 1 << 63
@@ -82,6 +82,14 @@ def _ids(seq_ids):
 
 def _per_seq(name, values, ids):
     return _ints(name, values, C.c_int64, len(ids))
+
+
+def _positions(pos, B):
+    try:
+        flat = [p for row in pos for p in row]
+    except TypeError as e:
+        raise _ffi.DzError(_ffi.DZ_EINVAL, f"pos is no [{B}][3]: {e}") from None
+    return _ints("pos", flat, C.c_int32, 3 * B)
 
 
 def _total(counts):
@@ -176,7 +184,9 @@ class Context:
 
     def _lens(self, layer, ids):
         out = _ints("lens", [0] * len(ids), C.c_int64)
-        self._chk(self.lib.dz_kv_lens(self.h, layer, len(ids), ids, out))
+        st = self.lib.dz_kv_lens(self.h, layer, len(ids), ids, out)
+        if st != _ffi.DZ_OK:                     # the call takes a const context: it leaves no message there
+            raise _ffi.DzError(st, f"no KV lengths of layer {layer}, seq_ids {list(ids)}")
         return out
 
     def kv_truncate(self, layer, seq, new_len):
@@ -357,7 +367,7 @@ class Context:
         ids, f = _ids(seq_ids), torch.float32
         B, p3 = len(ids), None
         if pos is not None:
-            p3 = _ints("pos", [p for row in pos for p in row], C.c_int32, 3 * B)
+            p3 = _positions(pos, B)
         self._chk(self.lib.dz_gqa_decode_q4(
             self.h, layer, B, ids, p3,
             self._tensor("q_gate", q_gate, f, B * self.nq * QG_ROW), self._tensor("k", k, f, B * self.kvc * HD),

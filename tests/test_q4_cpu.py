@@ -142,3 +142,32 @@ def test_tensors_of_another_gpu_are_refused():
     with pytest.raises(DzError) as e:
         ctx._tensor("x", there, torch.float32, 4)
     assert e.value.status == DZ_EINVAL and "cuda:0" in str(e.value)
+
+
+def test_what_is_no_list_of_numbers_is_refused():
+    pytest.importorskip("torch")
+    from daiza_b200 import engine
+    from daiza_b200._ffi import DZ_EINVAL, DzError
+
+    class OnAGpu:                                    # what numpy does with a CUDA tensor
+        def __array__(self, *a, **kw):
+            raise TypeError("cannot convert a CUDA tensor to numpy")
+
+    for call in (lambda: engine._ids(OnAGpu()), lambda: engine._positions([1, 2, 3], 1),
+                 lambda: engine._positions(7, 1), lambda: engine._positions([[1, 2], [3, 4]], 1),
+                 lambda: engine._positions([[1, 2, 1 << 31]], 1)):
+        with pytest.raises(DzError) as e:
+            call()
+        assert e.value.status == DZ_EINVAL
+    assert list(engine._positions(np.array([[1, 2, 3]], np.int32), 1)) == [1, 2, 3]
+
+
+def test_refused_lengths_say_what_was_asked_for():
+    """dz_kv_lens has no place for a message, and the last one of the context is of another call."""
+    pytest.importorskip("torch")
+    from daiza_b200 import _ffi, engine
+    ctx = engine.Context.__new__(engine.Context)
+    ctx.lib, ctx.h = _ffi.lib(), None
+    with pytest.raises(_ffi.DzError) as e:
+        ctx.kv_lens(5, [7, 9])
+    assert e.value.status == _ffi.DZ_EINVAL and "layer 5" in str(e.value) and "[7, 9]" in str(e.value)
