@@ -232,6 +232,13 @@ constexpr int NTHREADS = 512;
 __host__ __device__ constexpr uint32_t S_COL(int st) { return 128u * (uint32_t)st; }
 constexpr uint32_t O_COL = 256;
 constexpr float OUT_SCALE = 8.0f;
+// The matrix instruction adds to its f32 accumulator with truncation: 2e-7 of the sum an instruction of 16 keys, all one
+// way (131072 keys of like values came out 8.4e-4 short).  So O starts anew every STRETCH blocks of keys, and what it
+// held is added up, rounded to nearest, in memory: 5e-5 short at any length, a fifth of what P's rounding does.  1024
+// tokens behind 65000 take 1470 us so, 1405 without (1450 with 128 blocks).  A launch without a sequence that long (LONG =
+// false) has none of it in its code: packed prompts of 1-1500 took 248.7 us with it, 243.2 without.
+constexpr int STRETCH = 64;
+constexpr int64_t PART_BYTES = (int64_t)BM * HD * sizeof(float);   // a CTA's sums, [dim][row]
 constexpr float RESCALE_THRESHOLD = 8.0f;        // log2 units: P stays below 2^8, far inside f16
 
 struct alignas(1024) Smem {
@@ -401,11 +408,11 @@ struct Packed {
     }
 };
 
-template <typename T>
+template <typename T, bool LONG>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
     q4_pf_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Packed map, int kvc,
-                      const T* __restrict__ q_gate, T* __restrict__ out, int* err) {
+                      const T* __restrict__ q_gate, T* __restrict__ out, float* __restrict__ part, int* err) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     // dynamic shared memory is only 16-byte aligned: round up to 1 KB (the same place in both CTAs)
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
@@ -550,7 +557,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
 #pragma unroll
                         for (int s2 = 0; s2 < 2; ++s2)         // A = P columns of 16 keys
                             mma_ts(go, tmem + O_COL, tmem + S_COL(st) + 8 * (2 * kg + s2), vd + (uint32_t)(s2 * 16 * 128 / 16),
-                                   ID_PV, (j > 0 || kg > 0 || s2 > 0) ? 1u : 0u);
+                                   ID_PV, ((LONG ? j % STRETCH : j) > 0 || kg > 0 || s2 > 0) ? 1u : 0u);
                         commit(go, v_empty + 8 * v_slot);
                         if (++v_slot == NV) {
                             v_slot = 0;
@@ -617,10 +624,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
         const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t p_bar[2] = {peer_addr(&sm.p_full[0], 0), peer_addr(&sm.p_full[1], 0)};
         uint32_t g = 0;                                                // blocks so far
+        if (LONG) part += (int64_t)blockIdx.x * (BM * HD) + 128 * hf * BM + r;       // this thread's sums of earlier stretches
         while (next_tile()) {
             const int64_t qpos = tl.base + tl.q0 + r;                      // absolute position of this query row
             float m_run = -INFINITY, l_run = 0.0f;                         // m identical in both halves; l partial per half
-            for (int j = 0; j < nblk; ++j, ++g) {
+            float m_part = 0.0f;                                           // m_run when the sums in memory were written
+            for (int j0 = 0, j1; j0 < nblk; j0 = j1) {                     // a stretch of blocks
+            j1 = LONG ? min(nblk, j0 + STRETCH) : nblk;
+            for (int j = j0; j < j1; ++j, ++g) {
                 const int st = g & 1;
                 // a wait given up (the rest is skipped then, and nothing is stored) leaves no named barrier out
                 wait(&sm.s_full[st], (g >> 1) & 1, err, ok);
@@ -665,7 +676,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
                     // where it did not: TMEM is read and written by whole warps)
                     const float f = grown ? ex2(m_run - m_new) : 1.0f;
                     l_run *= f;
-                    if (j > 0) {
+                    if (j > j0) {
                         wait(&sm.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, err, ok);
                         __syncwarp();
                         fence_after_sync();
@@ -715,6 +726,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
                 __syncwarp();
                 if (lane == 0) arrive_at(p_bar[st]);
             }
+            if (LONG && j1 < nblk) {                                       // a stretch ends: O to the sums in memory
+                wait(&sm.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, err, ok);
+                __syncwarp();
+                fence_after_sync();
+                const float f = ex2(m_part - m_run);
+#pragma unroll 1
+                for (int c = 0; c < 128; c += 32) {
+                    float o[32];
+                    tmem_ld32(tmem + lane_off + O_COL + 128 * hf + c, o);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        float* sum = part + (c + i) * BM;
+                        *sum = j0 > 0 ? fmaf(*sum, f, o[i]) : o[i];
+                    }
+                }
+                m_part = m_run;
+                fence_before_sync();
+            }
+            }
             // O / l of this thread's row, dims [128 hf, 128 hf + 128), to the output warps
             sm.red_l[hf][r] = l_run;
             named_bar_sync(1, 256);
@@ -723,6 +753,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
             wait(&sm.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, err, ok);
             __syncwarp();
             fence_after_sync();
+            if (LONG && nblk > STRETCH) {                                  // and the sums in memory, into TMEM
+                const float f = ex2(m_part - m_run);
+#pragma unroll 1
+                for (int c = 0; c < 128; c += 32) {
+                    float o[32];
+                    uint32_t ob[32];
+                    tmem_ld32(tmem + lane_off + O_COL + 128 * hf + c, o);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) ob[i] = __float_as_uint(fmaf(part[(c + i) * BM], f, o[i]));
+                    tmem_st32(tmem + lane_off + O_COL + 128 * hf + c, ob);
+                }
+            }
 #pragma unroll
             for (int c0 = 0; c0 < 128; c0 += 32) {
                 float o[32];
@@ -762,11 +804,20 @@ static bool make_map(CUtensorMap* m, const void* base, int64_t d1, int64_t d2, i
 }  // namespace q4
 
 cudaError_t q4_prefill_setup() {
-    const cudaError_t e = cudaFuncSetAttribute(q4::attn::q4_pf_attn_kernel<float>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, q4::attn::SMEM_BYTES);
-    return e != cudaSuccess ? e
-                            : cudaFuncSetAttribute(q4::attn::q4_pf_attn_kernel<__nv_bfloat16>,
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, q4::attn::SMEM_BYTES);
+    using B = __nv_bfloat16;
+    cudaError_t e = cudaSuccess;
+    for (auto kernel : {(const void*)q4::attn::q4_pf_attn_kernel<float, false>, (const void*)q4::attn::q4_pf_attn_kernel<float, true>,
+                        (const void*)q4::attn::q4_pf_attn_kernel<B, false>, (const void*)q4::attn::q4_pf_attn_kernel<B, true>})
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, q4::attn::SMEM_BYTES);
+    return e;
+}
+
+// The attention CTAs' sums in memory, where a sequence has more than a stretch of keys.
+static int64_t part_bytes(const dz_ctx* ctx, const q4::Prompt& d) {
+    int longest = 0;
+    for (int s = 0; s < d.n; ++s) longest = std::max(longest, d.key0[s + 1] - d.key0[s]);
+    return longest > q4::attn::STRETCH * q4::attn::BN ? ctx->n_sm * q4::attn::PART_BYTES : 0;
 }
 
 template <typename T>
@@ -779,6 +830,7 @@ static cudaError_t launch_group(dz_ctx* ctx, int layer, const q4::Prompt& d, con
     cudaError_t e;
     __half* qf = static_cast<__half*>(ctx->q4_scratch);
     __half *kf = qf + qn, *vf = kf + kn;
+    float* part = reinterpret_cast<float*>(vf + kn);           // behind them where a sequence needs it (part_bytes)
     CUtensorMap mq, mk, mv;
     using namespace q4;
     if (!attn::make_map(&mq, qf, tokens, nq, attn::BM) || !attn::make_map(&mk, kf, keys, kvc, attn::BN / 2) ||
@@ -827,7 +879,8 @@ static cudaError_t launch_group(dz_ctx* ctx, int layer, const q4::Prompt& d, con
         lc.stream = st;
         lc.attrs = at;
         lc.numAttrs = 1;
-        e = cudaLaunchKernelEx(&lc, attn::q4_pf_attn_kernel<T>, mq, mk, mv, map, kvc, q_gate, out, ctx->d_err);
+        auto kernel = part_bytes(ctx, d) > 0 ? attn::q4_pf_attn_kernel<T, true> : attn::q4_pf_attn_kernel<T, false>;
+        e = cudaLaunchKernelEx(&lc, kernel, mq, mk, mv, map, kvc, q_gate, out, part, ctx->d_err);
         if (e != cudaSuccess) return e;
         *n_launch += 1;
     }
@@ -871,7 +924,10 @@ static cudaError_t launch_prompts(dz_ctx* ctx, int layer, int n, const int32_t* 
     const int kvc = ctx->cfg.kv_head_count, nq = GRP * kvc;
     q4::Prompt d;
     int64_t most = 0;
-    for (int i = 0; i < n;) most = std::max(most, next_group(L, kvc, i, n, seq_ids, lens, d));
+    for (int i = 0; i < n;) {
+        const int64_t bytes = next_group(L, kvc, i, n, seq_ids, lens, d);
+        most = std::max(most, bytes + part_bytes(ctx, d));
+    }
     cudaError_t e = ensure_q4_scratch(ctx, most);
     if (e != cudaSuccess) return e;
     for (int i = 0; i < n;) {

@@ -118,3 +118,27 @@ def test_prompt_whose_maxima_move(dtype):
     # a score of 21 is the sum of 256 rounded products of one sign: its error 21 * 2^-12.3 / 16 = 2.6e-4 rms, as a normalised row's
     assert (got - want).norm() <= (1.5 * NORM_TOL + step / 3 ** 0.5) * want.norm()
     m.done()
+
+
+@pytest.mark.parametrize("base,T,dtype", [(20000, 130, "float32"), (131000, 3, "float32"), (131000, 140, "bfloat16")])
+def test_prompt_behind_long_cached_rows(base, T, dtype):
+    """Values around 1, which add up in one direction: the matrix instruction truncates, up to 4 * 2^-23 of the sum at each
+    of its additions of 16 keys; over a stretch of 8192 keys, along which the sum grows from 0, that is at most
+    512 / 2 * 4 * 2^-23 = 1.2e-4 of it, whatever the length."""
+    dt = getattr(torch, dtype)
+    m = Model([base + T], kvc=1, seed=302)
+    torch.manual_seed(302)
+    m.ctx.kv_import(0, 0, torch.randn(base, 1, 256, device="cuda"), 1 + 0.1 * torch.randn(base, 1, 256, device="cuda"))
+    qg, k, v = (dev(x, dt) for x in m.inputs(T))
+    v = (1 + 0.1 * v.float()).to(dt)
+    out = torch.empty(T, m.nq * 256, device="cuda", dtype=dt)
+    m.ctx.gqa_prefill_q4(0, [0], [T], qg, k, v, out)
+    want, _ = attention(m, 0, qg, at(base, T))
+    got = out.double().reshape(want.shape)
+    bias = (got / want - 1).mean().item()
+    assert abs(bias) <= 1.2e-4, f"{bias:.2e}"
+    step = 2.0 ** -8 / 3 ** 0.5 if dtype == "bfloat16" else 0.0
+    top, err = held(m, 0)[1].abs().max(), (got - want).abs()
+    assert (err <= MAX_TOL * top + (2.0 ** -8 * want.abs() if step else 0.0)).all(), err.max()
+    assert err.norm() <= (NORM_TOL + step) * want.norm()
+    m.done()
