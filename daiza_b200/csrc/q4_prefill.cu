@@ -209,9 +209,10 @@ __global__ void __launch_bounds__(32 * PREP_WARPS, 2)
 //   warp 9     (first CTA) issues S = Q K^T (N = 128, K = 256) into one of two TMEM buffers
 //              and O += P V (N = 256, K = 128, P from TMEM)
 //   warp 10    TMA of this CTA's 128 dims of each V block (slots of 32 keys)
-//   warps 12-15  outputs: O / l from shared memory (f16: P was rounded to f16 already, and the
-//              sum over many keys is off by more; times 8, which keeps |V| <= 7 * 896 in range
-//              and small values' bits), times the gate's sigmoid, in whole rows
+//   warps 12-15  outputs: O / l from shared memory, times the gate's sigmoid, in whole rows.  bf16
+//              outputs pass as f16 (2^-11, an eighth of what bf16 rounds; times 8, which keeps |V| <=
+//              7 * 896 in range and small values' bits), f32 ones as f32, one half of the dims
+//              after the other
 // A cluster takes several query tiles in turn; while the outputs of one leave, the next one's
 // queries are fetched and its first blocks worked on.  (A cluster per tile, the softmax warps
 // writing the outputs: packed prompts of 1-1500 took 378 us, all of the call, instead of 240:
@@ -245,8 +246,8 @@ struct alignas(1024) Smem {
     uint16_t q[4][BM][64];                       // 4 boxes of 64 dims, 16 KB each
     uint16_t k[NK][BN / 2][64];
     uint16_t v[NV][2][32][64];
-    uint4 out[BM][HD / 8];                       // O / l as f16, 16-byte words of a row in swizzled order
-    uint64_t q_full, q_empty, out_full, out_empty;
+    uint4 out[BM][32];                           // O / l, 16-byte words of a row in swizzled order: 256 dims as f16, or 128 as f32
+    uint64_t q_full, q_empty, out_full[2], out_empty[2];   // out: of either half of the dims (f32), [0] of both (bf16)
     uint64_t k_full[NK], k_empty[NK], v_full[NV], v_empty[NV];
     uint64_t s_full[2], p_full[2], pv_done[2];
     float red_max[2][2][BM];                     // [block parity][key half][row] partial row maxima
@@ -374,9 +375,18 @@ __device__ __forceinline__ float2 gate2(uint32_t ab, float x, float y) {
     unpack2(mul2(pack2(o.x, o.y), pack2(g, h)), out.x, out.y);
     return out;
 }
-__device__ __forceinline__ void store8(float* p, float4 a, float4 b) {
-    reinterpret_cast<float4*>(p)[0] = a;
-    reinterpret_cast<float4*>(p)[1] = b;
+// four f32 values times the gates' sigmoids
+__device__ __forceinline__ float4 gate4(uint4 o, float4 x) {
+    const float v[4] = {__uint_as_float(o.x), __uint_as_float(o.y), __uint_as_float(o.z), __uint_as_float(o.w)};
+    const float g[4] = {x.x, x.y, x.z, x.w};
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float r;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(-LOG2E * g[i])));
+        y[i] = v[i] * r;
+    }
+    return make_float4(y[0], y[1], y[2], y[3]);
 }
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
@@ -416,6 +426,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     // dynamic shared memory is only 16-byte aligned: round up to 1 KB (the same place in both CTAs)
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+    // registers by warpgroup (with 56 / 104 / 176 the f32 kernel spills: packed prompts took 218 us instead of 183)
+    constexpr int REGS_LOAD = sizeof(T) == 4 ? 72 : 56, REGS_OUT = 104, REGS_SOFTMAX = sizeof(T) == 4 ? 168 : 176;
+    static_assert(REGS_LOAD + REGS_OUT + 2 * REGS_SOFTMAX <= 65536 / BM, "a warpgroup each of the first two, two of softmax");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int nq = GRP * kvc, pairs = nq / 2, rank = blockIdx.x & 1;
     // the cluster's tiles, heaviest first: in rounds over all clusters, there and back
@@ -436,8 +449,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
     if (tid == 0) {
         mbar_init(&sm.q_full, 1);
         mbar_init(&sm.q_empty, 1);
-        mbar_init(&sm.out_full, 8);                                    // the softmax warps of this CTA
-        mbar_init(&sm.out_empty, 4);                                   // the output warps
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sm.out_full[i], sizeof(T) == 4 ? 4 : 8);        // the softmax warps of this CTA (f32: of one half)
+            mbar_init(&sm.out_empty[i], 4);                            // the output warps
+        }
         for (int i = 0; i < NK; ++i) {
             mbar_init(&sm.k_full[i], 1);
             mbar_init(&sm.k_empty[i], 1);
@@ -462,7 +477,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
     bool ok = true;
 
     if (warp >= 8 && warp < 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_LOAD));
     if (warp == 8) {
         // ---------------- TMA of Q and K ----------------
         if (lane == 0) {
@@ -572,52 +587,59 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
         }
     }
     } else if (warp >= 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OUT));
         // ---------------- output: O / l * sigmoid(gate), 32 rows a warp ----------------
-        // a lane has 8 dims of a row; gates are fetched to L2 at the tile's start, to registers
-        // AHEAD rows ahead
-        constexpr int AHEAD = 8;
+        // a lane has 8 dims of a row (f32: 4 of one half); gates are fetched to L2 at the tile's start, to
+        // registers AHEAD rows ahead
+        constexpr int AHEAD = 8, HALVES = sizeof(T) / 2, DIMS = 8 / HALVES;
         const int r0 = 32 * (warp - 12);
         while (next_tile()) {
             const int rows = (int)max((int64_t)0, min((int64_t)32, tl.T - tl.q0 - r0));   // that exist
             const int64_t first = (tl.row + r0) * nq + qh;             // (row, head) of the first
-            const T* gates = q_gate + first * QG_ROW + HD + 8 * lane;
-            T* to = out + first * HD + 8 * lane;
             for (int i = lane; i < rows * (HD * (int)sizeof(T) / 128); i += 32) {
                 constexpr int LINES = HD * (int)sizeof(T) / 128;       // 128-byte lines of a row's gates
                 asm volatile("prefetch.global.L2 [%0];" ::"l"(
                     q_gate + (first + (int64_t)(i / LINES) * nq) * QG_ROW + HD + (i % LINES) * (128 / (int)sizeof(T))));
             }
-            decltype(load4(q_gate)) g0[AHEAD], g1[AHEAD];
-            auto load_gates = [&](int i) {
-                const T* p = gates + min(i, rows - 1) * (nq * QG_ROW);
-                g0[i % AHEAD] = load4(p);
-                g1[i % AHEAD] = load4(p + 4);
-            };
-            if (rows > 0) {
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i) load_gates(i);
-            }
-            wait(&sm.out_full, (round - 1) & 1, err, ok);
 #pragma unroll 1
-            for (int i0 = 0; ok && i0 < rows; i0 += AHEAD) {
+            for (int half = 0; half < HALVES; ++half) {
+                const T* gates = q_gate + first * QG_ROW + HD + 128 * half + DIMS * lane;
+                T* to = out + first * HD + 128 * half + DIMS * lane;
+                decltype(load4(q_gate)) g0[AHEAD], g1[AHEAD];          // (g1: bf16 only)
+                auto load_gates = [&](int i) {
+                    const T* p = gates + min(i, rows - 1) * (nq * QG_ROW);
+                    g0[i % AHEAD] = load4(p);
+                    if (HALVES == 1) g1[i % AHEAD] = load4(p + 4);
+                };
+                if (rows > 0) {
 #pragma unroll
-                for (int k = 0; k < AHEAD; ++k) {
-                    const int i = i0 + k;
-                    const uint4 h = sm.out[r0 + i][lane ^ (i & 7)];
-                    const float4 w0 = as_f32(g0[k]), w1 = as_f32(g1[k]);
-                    load_gates(i + AHEAD);
-                    const float2 a = gate2(h.x, w0.x, w0.y), b = gate2(h.y, w0.z, w0.w);
-                    const float2 c = gate2(h.z, w1.x, w1.y), e = gate2(h.w, w1.z, w1.w);
-                    if (i < rows)
-                        store8(to + i * (nq * HD), make_float4(a.x, a.y, b.x, b.y), make_float4(c.x, c.y, e.x, e.y));
+                    for (int i = 0; i < AHEAD; ++i) load_gates(i);
                 }
+                wait(&sm.out_full[half], (round - 1) & 1, err, ok);
+#pragma unroll 1
+                for (int i0 = 0; ok && i0 < rows; i0 += AHEAD) {
+#pragma unroll
+                    for (int k = 0; k < AHEAD; ++k) {
+                        const int i = i0 + k;
+                        const uint4 h = sm.out[r0 + i][lane ^ (i & 7)];
+                        const float4 w0 = as_f32(g0[k]), w1 = HALVES == 1 ? as_f32(g1[k]) : w0;
+                        load_gates(i + AHEAD);
+                        if constexpr (HALVES == 1) {
+                            const float2 a = gate2(h.x, w0.x, w0.y), b = gate2(h.y, w0.z, w0.w);
+                            const float2 c = gate2(h.z, w1.x, w1.y), e = gate2(h.w, w1.z, w1.w);
+                            if (i < rows)
+                                store8(to + i * (nq * HD), make_float4(a.x, a.y, b.x, b.y), make_float4(c.x, c.y, e.x, e.y));
+                        } else if (i < rows) {
+                            *reinterpret_cast<float4*>(to + i * (nq * HD)) = gate4(h, w0);
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.out_empty[half]);
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.out_empty);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
         // ---------------- softmax: 8 warps, thread = (query row, key half) ----------------
         const int r = 32 * (warp & 3) + lane;                          // TMEM lane = query row
         const int hf = warp >> 2;                                      // keys [64 hf, 64 hf + 64) of a block
@@ -628,7 +650,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
         while (next_tile()) {
             const int64_t qpos = tl.base + tl.q0 + r;                      // absolute position of this query row
             float m_run = -INFINITY, l_run = 0.0f;                         // m identical in both halves; l partial per half
-            float m_part = 0.0f;                                           // m_run when the sums in memory were written
+            float m_part = -INFINITY;                                      // m_run when the sums in memory were written
             for (int j0 = 0, j1; j0 < nblk; j0 = j1) {                     // a stretch of blocks
             j1 = LONG ? min(nblk, j0 + STRETCH) : nblk;
             for (int j = j0; j < j1; ++j, ++g) {
@@ -732,13 +754,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
                 fence_after_sync();
                 const float f = ex2(m_part - m_run);
 #pragma unroll 1
-                for (int c = 0; c < 128; c += 32) {
-                    float o[32];
-                    tmem_ld32(tmem + lane_off + O_COL + 128 * hf + c, o);
+                for (int c = 0; c < 128; c += 16) {                        // (by 32 the f32 kernel took a quarter longer)
+                    uint32_t o[16];
+                    tmem_ld16_async(tmem + lane_off + O_COL + 128 * hf + c, o);
+                    tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
+                    for (int i = 0; i < 16; ++i) {
                         float* sum = part + (c + i) * BM;
-                        *sum = j0 > 0 ? fmaf(*sum, f, o[i]) : o[i];
+                        *sum = fmaf(j0 > 0 ? *sum : 0.0f, f, __uint_as_float(o[i]));
                     }
                 }
                 m_part = m_run;
@@ -748,35 +771,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
             // O / l of this thread's row, dims [128 hf, 128 hf + 128), to the output warps
             sm.red_l[hf][r] = l_run;
             named_bar_sync(1, 256);
-            const float inv_l = OUT_SCALE / (l_run + sm.red_l[hf ^ 1][r]);
-            if (round > 1) wait(&sm.out_empty, round & 1, err, ok);
+            constexpr bool F32 = sizeof(T) == 4;
+            const float inv_l = (F32 ? 1.0f : OUT_SCALE) / (l_run + sm.red_l[hf ^ 1][r]);
+            // the place is free: from the last tile's rows, or (f32) their second half, or this tile's first
+            if (round > 1 && !(F32 && hf == 1)) wait(&sm.out_empty[F32], round & 1, err, ok);
+            if (F32 && hf == 1) wait(&sm.out_empty[0], (round - 1) & 1, err, ok);
             wait(&sm.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, err, ok);
             __syncwarp();
             fence_after_sync();
             if (LONG && nblk > STRETCH) {                                  // and the sums in memory, into TMEM
                 const float f = ex2(m_part - m_run);
 #pragma unroll 1
-                for (int c = 0; c < 128; c += 32) {
-                    float o[32];
-                    uint32_t ob[32];
-                    tmem_ld32(tmem + lane_off + O_COL + 128 * hf + c, o);
+                for (int c = 0; c < 128; c += 16) {
+                    uint32_t o[16];
+                    tmem_ld16_async(tmem + lane_off + O_COL + 128 * hf + c, o);
+                    tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) ob[i] = __float_as_uint(fmaf(part[(c + i) * BM], f, o[i]));
-                    tmem_st32(tmem + lane_off + O_COL + 128 * hf + c, ob);
+                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(fmaf(part[(c + i) * BM], f, __uint_as_float(o[i])));
+                    tmem_st16(tmem + lane_off + O_COL + 128 * hf + c, o);
                 }
             }
 #pragma unroll
             for (int c0 = 0; c0 < 128; c0 += 32) {
                 float o[32];
                 tmem_ld32(tmem + lane_off + O_COL + 128 * hf + c0, o);
+                if constexpr (F32) {
 #pragma unroll
-                for (int i = 0; i < 32; i += 8)
-                    sm.out[r][((128 * hf + c0 + i) / 8) ^ (r & 7)] =
-                        make_uint4(pack_f16(o[i] * inv_l, o[i + 1] * inv_l), pack_f16(o[i + 2] * inv_l, o[i + 3] * inv_l),
-                                   pack_f16(o[i + 4] * inv_l, o[i + 5] * inv_l), pack_f16(o[i + 6] * inv_l, o[i + 7] * inv_l));
+                    for (int i = 0; i < 32; i += 4)
+                        sm.out[r][((c0 + i) / 4) ^ (r & 7)] =
+                            make_uint4(__float_as_uint(o[i] * inv_l), __float_as_uint(o[i + 1] * inv_l),
+                                       __float_as_uint(o[i + 2] * inv_l), __float_as_uint(o[i + 3] * inv_l));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8)
+                        sm.out[r][((128 * hf + c0 + i) / 8) ^ (r & 7)] =
+                            make_uint4(pack_f16(o[i] * inv_l, o[i + 1] * inv_l), pack_f16(o[i + 2] * inv_l, o[i + 3] * inv_l),
+                                       pack_f16(o[i + 4] * inv_l, o[i + 5] * inv_l), pack_f16(o[i + 6] * inv_l, o[i + 7] * inv_l));
+                }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.out_full);
+            if (lane == 0) mbar_arrive(&sm.out_full[F32 ? hf : 0]);
         }
     }
     // neither CTA leaves, or frees TMEM, while the other's products or arrivals may touch it; after

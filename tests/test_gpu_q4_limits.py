@@ -65,6 +65,22 @@ def test_queries_of_any_size(size):
     m.done()
 
 
+@pytest.mark.parametrize("T,base", [(1, 4), (100, 0), (150, 333)])
+def test_prompt_f32_outputs_keep_their_bits(T, base):
+    """Zero queries: every P is the same power of two and outputs are plain means, so nothing but the sums' truncation
+    (1 + 483 / 16 additions, 4 * 2^-23 each of a sum that grows: 7.4e-6) and a few f32 roundings stand between."""
+    m = Model([base + T], kvc=1, seed=312)
+    k, v = m.normal(base, 1, 256), 1 + 0.1 * m.normal(base, 1, 256)
+    if base:
+        m.ctx.kv_import(0, 0, k, v)
+        m.refs[0] = R.Cache(1, k, v)
+    q, k, v = m.inputs(T)
+    q[..., :256] = 0
+    (got, want), = prompt(m, [0], [T], inputs=(q, k, 1 + np.float32(0.1) * v))
+    assert np.abs(got - want).max() <= 1e-5 * np.abs(m.refs[0].v).max()
+    m.done()
+
+
 def test_prompt_groups_of_sequences():
     """Five sequences of 120000 cached rows: the f16 rows of four fill the scratch of one group."""
     n, lens = 120000, [3, 1, 40, 2, 130]

@@ -142,3 +142,29 @@ def test_prompt_behind_long_cached_rows(base, T, dtype):
     assert (err <= MAX_TOL * top + (2.0 ** -8 * want.abs() if step else 0.0)).all(), err.max()
     assert err.norm() <= (NORM_TOL + step) * want.norm()
     m.done()
+
+
+def test_prompt_behind_long_rows_of_very_low_scores():
+    """All scores of a head far below 0 (log2 units -160 to -190), and rising from stretch to stretch in others."""
+    base, T = 25000, 40
+    m = Model([base + T], kvc=1, seed=304)
+    torch.manual_seed(304)
+    qg, k, v = m.inputs(T)
+    pos = np.zeros((T, 3), np.int64)
+    qg[:] = qg[:1]
+    q = R.turn(qg[:1, :, :256], m.qn, pos[:1])[0] / 16
+    u = q[0] / (q[0] @ q[0])
+    old = dev(-120 * u).repeat(base, 1, 1) + 0.1 * torch.randn(base, 1, 256, device="cuda")
+    w = q[3] - (q[3] @ q[0]) / (q[0] @ q[0]) * q[0]
+    old += torch.arange(base, device="cuda")[:, None, None] / base * dev(40 * w / (w @ w))
+    k[:] = 0
+    m.kn[:] = 0                                       # the new keys' scores are 0: heads of low scores see them alone
+    m.ctx.set_attn_params(0, m.qn, m.kn)
+    m.ctx.kv_import(0, 0, old, torch.randn(base, 1, 256, device="cuda"))
+    out = torch.empty(T, m.nq * 256, device="cuda")
+    m.ctx.gqa_prefill_q4(0, [0], [T], dev(qg), dev(k), dev(v), out, pos=dev(pos, torch.int32))
+    want, _ = attention(m, 0, qg, pos)
+    got, top = out.double().reshape(want.shape), held(m, 0)[1].abs().max()
+    # scores of up to 120: Q's rounding, 2^-12.3 / 16 of their size for keys along the query, 1.4e-3, 4 sigma in a probability
+    assert (got - want).abs().max() <= (MAX_TOL + 4 * 120 * 2.0 ** -12.3 / 16) * top
+    m.done()
