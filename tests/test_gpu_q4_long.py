@@ -168,3 +168,27 @@ def test_prompt_behind_long_rows_of_very_low_scores():
     # scores of up to 120: Q's rounding, 2^-12.3 / 16 of their size for keys along the query, 1.4e-3, 4 sigma in a probability
     assert (got - want).abs().max() <= (MAX_TOL + 4 * 120 * 2.0 ** -12.3 / 16) * top
     m.done()
+
+
+def test_prompt_long_tail_behind_one_heavy_key():
+    """One key 25 to 26 log2 units above 200000 others, whose weights together are about 0.4 %."""
+    base, T = 200000, 2
+    m = Model([base + T], kvc=1, seed=303)
+    qg, k, v = m.inputs(T)
+    pos = np.zeros((T, 3), np.int64)
+    qg[:] = qg[:1, :1]
+    q = R.turn(qg[:1, :1, :256], m.qn, pos[:1])[0, 0] / 16
+    old = torch.zeros(base, 1, 256, device="cuda")
+    heavy = R.hold(25.5 * np.log(2.0) * q / (q @ q))
+    assert 25.1 < heavy @ q / np.log(2.0) < 25.9
+    old[0, 0] = dev(heavy)
+    values = torch.ones(base, 1, 256, device="cuda")
+    values[0] = 0
+    m.ctx.kv_import(0, 0, old, values)
+    out = torch.empty(T, m.nq * 256, device="cuda")
+    m.ctx.gqa_prefill_q4(0, [0], [T], dev(qg), dev(k), dev(v), out, pos=dev(pos, torch.int32))
+    want, _ = attention(m, 0, qg, pos)
+    got = out.double().reshape(want.shape)
+    # P of the tail is 2^-18.5 or so, with f16's steps of 2^-24 there: within 2 %
+    assert ((got - want).abs() <= 0.02 * want.abs() + 1e-5).all(), ((got - want).abs() / want.abs()).max()
+    m.done()
