@@ -324,6 +324,7 @@ dz_status dz_layer_set_attn_params(dz_ctx* ctx, int layer, const float* q_norm, 
     dz_status st;
     if ((st = upload(ctx, &L.q_norm, q_norm, HD)) != DZ_OK) return st;
     if ((st = upload(ctx, &L.k_norm, k_norm, HD)) != DZ_OK) return st;
+    L.q_up = query_scale(q_norm);
     L.params_set = true;
     return DZ_OK;
 }

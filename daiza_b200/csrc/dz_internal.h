@@ -80,6 +80,7 @@ struct LayerState {
     bool is_attn = false;
     bool params_set = false;
     float* q_norm = nullptr;   // [256]
+    float q_up = 1.0f;         // query_scale of q_norm
     float* k_norm = nullptr;   // [256]
     float* conv_w = nullptr;   // [4][10240]
     float* ssm_a = nullptr;    // [48]
@@ -326,6 +327,7 @@ dz_status q4_import(dz_ctx* ctx, int layer, int seq, const float* k, const float
 dz_status q4_export(dz_ctx* ctx, int layer, int seq, float* k, float* v);
 // grows ctx->q4_scratch to at least `bytes` (the old buffer is kept: see above)
 cudaError_t ensure_q4_scratch(dz_ctx* ctx, size_t bytes);
+float query_scale(const float* q_norm);
 void rope_axes_set(RopeAxes& a, const int32_t sections[3], bool interleaved, double base);
 // a KV length went down: snapshots remember the lowest (dz_attn.cu)
 void kv_lowered(dz_ctx* ctx, int layer, int seq, int64_t new_len);

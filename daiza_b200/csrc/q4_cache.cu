@@ -23,6 +23,17 @@ void rope_axes_set(RopeAxes& a, const int32_t sections[3], bool interleaved, dou
     }
 }
 
+// The power of two that brings the largest q that these norm weights allow, 16 |w| sqrt(2) / 16 log2 e = 2.05 |w| for a row
+// of one value and its rotation, to 2^14 .. 2^15: f16 then holds every query, small weights' too.
+float query_scale(const float* q_norm) {
+    float top = 0.0f;
+    for (int i = 0; i < HD; ++i)
+        if (std::isfinite(q_norm[i])) top = std::max(top, std::fabs(q_norm[i]));
+    int e = 0;
+    std::frexp(2.05 * top, &e);
+    return top > 0.0f ? std::ldexp(1.0f, std::min(std::max(15 - e, -100), 100)) : 1.0f;
+}
+
 // An allocation is no work of the stream: it may be made while a graph is captured, on this thread or another
 // (the buffer stays until the caches go, so the graph may hold it).
 static cudaError_t alloc_uncaptured(void** p, size_t bytes) {

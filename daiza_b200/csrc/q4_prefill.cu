@@ -7,7 +7,8 @@
 // decode call per token.
 //
 // Two kernels:
-//   1. q4_pf_prep : Q normed, rotated, scaled, as f16 [head][token][256]; K (normed, rotated,
+//   1. q4_pf_prep : Q normed, rotated, scaled (by a power of two, too, that keeps it inside f16
+//                   whatever the norm weights: q_up), as f16 [head][token][256]; K (normed, rotated,
 //                   f64) and V quantised into the sequences' tiles; and every held row, old
 //                   and new, as f16 [kv head][key][256] -- exact -- each sequence padded with
 //                   zeros to whole blocks of 128 keys, so that a block never meets another
@@ -79,7 +80,7 @@ __global__ void __launch_bounds__(32 * PREP_WARPS, 2)
                       const Q4Slot* __restrict__ slots, const int32_t* __restrict__ pos, const float* __restrict__ q_norm,
                       const float* __restrict__ k_norm, const T* __restrict__ q_gate, const T* __restrict__ k,
                       const T* __restrict__ v, __half* __restrict__ qf, __half* __restrict__ kf, __half* __restrict__ vf,
-                      int key_heads, int q_heads, bool track, float eps) {
+                      int key_heads, int q_heads, bool track, float eps, float q_up) {
     __shared__ TileMerge merge;
     __shared__ double2 cs[PREP_WARPS][ROPE / 2];
     __shared__ float2 csf[PREP_WARPS][ROPE / 2];
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(32 * PREP_WARPS, 2)
     float w[8];
     load_split(q_norm, lane, w);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] *= 0.0625f * LOG2E;   // scores in log2 units
+    for (int e = 0; e < 8; ++e) w[e] *= 0.0625f * LOG2E * q_up;   // scores in log2 units, times q_up
     auto store_q = [&](int h, const float (&x)[8]) {
         __half* out = qf + ((size_t)h * tokens + row) * HD;
         *reinterpret_cast<uint2*>(out + split_dim(lane, 0)) = make_uint2(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]));
@@ -425,7 +426,7 @@ template <typename T, bool LONG>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
     q4_pf_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Packed map, int kvc,
-                      const T* __restrict__ q_gate, T* __restrict__ out, float* __restrict__ part, int* err) {
+                      const T* __restrict__ q_gate, T* __restrict__ out, float* __restrict__ part, float q_down, int* err) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     // dynamic shared memory is only 16-byte aligned: round up to 1 KB (the same place in both CTAs)
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
@@ -693,7 +694,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
                 }
                 sm.red_max[st][hf][r] = mx;
                 named_bar_sync(1, 256);                                    // also: every S read of this block is done
-                mx = fmaxf(mx, sm.red_max[st][hf ^ 1][r]);
+                mx = fmaxf(mx, sm.red_max[st][hf ^ 1][r]) * q_down;
                 const float m_new = fmaxf(m_run, mx);
                 const bool grown = m_new > m_run + RESCALE_THRESHOLD;
                 if (__any_sync(0xffffffffu, grown)) {
@@ -719,14 +720,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
                 }
                 uint32_t pk[32];
                 {
-                    const uint64_t mm = pack2(m_run - P_LOG2, m_run - P_LOG2);
+                    const uint64_t down = pack2(q_down, q_down), off = pack2(P_LOG2 - m_run, P_LOG2 - m_run);
                     uint64_t acc0 = pack2(0.0f, 0.0f), acc1 = acc0;
 #pragma unroll
                     for (int c = 0; c < 64; c += 4) {
                         float x0, x1, p2, p3;
-                        unpack2(sub2(pack2(s[c], s[c + 1]), mm), x0, x1);
+                        unpack2(fma2(pack2(s[c], s[c + 1]), down, off), x0, x1);
                         const float p0 = ex2(x0), p1 = ex2(x1);
-                        const uint64_t x23 = sub2(pack2(s[c + 2], s[c + 3]), mm);
+                        const uint64_t x23 = fma2(pack2(s[c + 2], s[c + 3]), down, off);
                         if (c % 8 == 0) {                                  // a quarter of them off the special-function unit
                             ex2_poly(x23, p2, p3);
                         } else {
@@ -902,7 +903,7 @@ static cudaError_t launch_group(dz_ctx* ctx, int layer, const q4::Prompt& d, con
                            (q_tasks + PREP_WARPS - 1) / PREP_WARPS;
     q4_pf_prep_kernel<T><<<(unsigned)blocks, 32 * PREP_WARPS, 0, st>>>(
         d, ctx->axes, kvc, L.d_q4, pos, L.q_norm, L.k_norm, q_gate, k, v, qf, kf, vf, key_heads, q_heads, ctx->q4_track,
-        ctx->cfg.rms_eps);
+        ctx->cfg.rms_eps, L.q_up);
     *n_launch += 1;
     if (map.first[d.n] > 0) {
         const unsigned clusters = (unsigned)std::min((int64_t)map.first[d.n] * nq / 2, (int64_t)ctx->n_sm / 2);
@@ -917,7 +918,7 @@ static cudaError_t launch_group(dz_ctx* ctx, int layer, const q4::Prompt& d, con
         lc.attrs = at;
         lc.numAttrs = 1;
         auto kernel = part_bytes(ctx, d) > 0 ? attn::q4_pf_attn_kernel<T, true> : attn::q4_pf_attn_kernel<T, false>;
-        e = cudaLaunchKernelEx(&lc, kernel, mq, mk, mv, map, kvc, q_gate, out, part, ctx->d_err);
+        e = cudaLaunchKernelEx(&lc, kernel, mq, mk, mv, map, kvc, q_gate, out, part, 1.0f / L.q_up, ctx->d_err);
         if (e != cudaSuccess) return e;
         *n_launch += 1;
     }

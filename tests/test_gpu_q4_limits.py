@@ -81,6 +81,32 @@ def test_prompt_f32_outputs_keep_their_bits(T, base):
     m.done()
 
 
+@pytest.mark.parametrize("up", [1e5, 1e4, 1e-2, 1e-4])
+def test_prompt_norm_weights_of_any_size(up):
+    """Queries large or small, keys the other way round: the same scores, and the same tolerance."""
+    m = Model([300], kvc=1, seed=313)
+    m.qn *= np.float32(up)
+    m.kn /= np.float32(up)
+    m.ctx.set_attn_params(0, m.qn, m.kn)
+    m.check_decode([0])
+    m.check_decode([0])
+    check(m, [0], [250])
+    m.done()
+
+
+@pytest.mark.parametrize("weight", [3e6, 1e30])
+def test_prompt_one_large_norm_weight(weight):
+    """A query dim beyond f16 that no key answers."""
+    m = Model([300], kvc=1, seed=319)
+    m.qn[100], m.kn[100] = weight, 0
+    if weight > 1e20:                                # what else there is lies too far below for f16: no score at all
+        m.qn[:100] = m.qn[101:] = 0
+    m.ctx.set_attn_params(0, m.qn, m.kn)
+    m.check_decode([0])
+    check(m, [0], [250])
+    m.done()
+
+
 def test_prompt_groups_of_sequences():
     """Five sequences of 120000 cached rows: the f16 rows of four fill the scratch of one group."""
     n, lens = 120000, [3, 1, 40, 2, 130]
