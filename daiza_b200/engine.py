@@ -341,12 +341,13 @@ class Context:
         return _tensor(name, t, dtype, numel, int(self.device))
 
     def _on(self, stream):
-        """Handle of `stream`, or of the context's device's current one (the raw handle: making a Stream object of it
-        takes 1.3 us)."""
+        """Handle of `stream`, or of the context's device's current one (straight, where this torch has the call for it:
+        making a Stream object takes 1.3 us)."""
         if stream is not None:
             return stream.cuda_stream
         import torch
-        return torch._C._cuda_getCurrentRawStream(int(self.device))
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        return raw(int(self.device)) if raw else torch.cuda.current_stream(int(self.device)).cuda_stream
 
     def qk_mrope(self, layer, pos, q_gate, k, q_out, k_out, stream=None):
         """QK-RMSNorm, rotation by pos [T][3] (int32) and q's 1/16; q_gate [T][6*kvc][512] and k [T][kvc][256] f32 or

@@ -171,3 +171,20 @@ def test_refused_lengths_say_what_was_asked_for():
     with pytest.raises(_ffi.DzError) as e:
         ctx.kv_lens(5, [7, 9])
     assert e.value.status == _ffi.DZ_EINVAL and "layer 5" in str(e.value) and "[7, 9]" in str(e.value)
+
+
+def test_current_stream_without_torchs_private_call(monkeypatch):
+    torch = pytest.importorskip("torch")
+    from daiza_b200 import engine
+    ctx = engine.Context.__new__(engine.Context)
+    ctx.device, ctx.h = 3, None
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 100 + device, raising=False)
+    assert ctx._on(None) == 103
+    monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream")
+
+    class Stream:
+        def __init__(self, device):
+            self.cuda_stream = 200 + device
+
+    monkeypatch.setattr(torch.cuda, "current_stream", Stream)
+    assert ctx._on(None) == 203 and ctx._on(Stream(7)) == 207
