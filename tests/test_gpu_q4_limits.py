@@ -215,3 +215,30 @@ def test_scratch_goes_with_the_caches():
     m.ctx.close()
     torch.cuda.synchronize()
     assert torch.cuda.mem_get_info()[0] - small <= 32 << 20
+
+
+def test_rows_and_weights_of_more_sequences_than_one_launch_takes():
+    n = [1 + s % 19 for s in range(300)]
+    m = Model(n, kvc=2, seed=320, track=True)
+    for s in range(300):
+        m.fill(s, n[s])
+    ids = [int(i) for i in m.rng.permutation(300)]
+    first, count = [n[s] // 3 for s in ids], [n[s] - n[s] // 3 for s in ids]
+    k, v = (torch.full((sum(count), 2, 256), -7.0, device="cuda") for _ in "kv")
+    m.ctx.kv_rows_q4(0, ids, first, count, k, v)
+    for got, name in ((k, "k"), (v, "v")):
+        assert np.array_equal(got.cpu().numpy(), np.concatenate([getattr(m.refs[s], name)[a:] for s, a in zip(ids, first)]))
+    new = [np.abs(m.normal(2, n[s])) for s in ids]
+    m.ctx.kv_set_weights_q4(0, ids, dev(np.concatenate([w.ravel() for w in new])))
+    for w, got in zip(new, m.weights(ids)):
+        assert np.array_equal(w, got)
+    m.done()
+
+
+def test_positions_of_more_prompts_than_one_launch_takes():
+    lens = [s % 4 for s in range(300)]
+    m = Model([8] * 300, kvc=1, seed=321, interleaved=True)
+    pos = m.rng.integers(0, 1 << 20, (sum(lens), 3))
+    check(m, list(range(299, -1, -1)), lens[::-1], pos=pos)
+    m.check_decode(list(range(300)), pos=[[7, 8, s] for s in range(300)])
+    m.done()

@@ -192,3 +192,56 @@ def test_prompt_long_tail_behind_one_heavy_key():
     # P of the tail is 2^-18.5 or so, with f16's steps of 2^-24 there: within 2 %
     assert ((got - want).abs() <= 0.02 * want.abs() + 1e-5).all(), ((got - want).abs() / want.abs()).max()
     m.done()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_long_and_short_prompts_packed_split_and_replayed(dtype):
+    """A prompt behind 9001 rows among short ones: in one call, as two contexts that share the query tiles, and in a graph
+    that is replayed."""
+    import daiza_b200 as dz
+    dt, bases, lens = getattr(torch, dtype), [0, 9001, 300], [140, 300, 5]
+    caps = [a + b for a, b in zip(bases, lens)]
+    m = Model(caps, kvc=1, seed=305, track=True)
+    torch.manual_seed(305)
+    old = [torch.randn(2, n, 1, 256, device="cuda") for n in bases]
+    qg, k, v = (dev(x, dt) for x in m.inputs(sum(lens)))
+
+    def load(ctx):
+        for s, n in enumerate(bases):
+            ctx.kv_import(0, s, old[s][0], old[s][1])
+
+    def run(ctx, out):
+        ctx.gqa_prefill_q4(0, [0, 1, 2], lens, qg, k, v, out)
+
+    load(m.ctx)
+    whole = torch.empty(sum(lens), m.nq * 256, device="cuda", dtype=dt)
+    run(m.ctx, whole)
+    a, step = 0, 2.0 ** -8 if dtype == "bfloat16" else 0.0
+    for s, n in enumerate(lens):
+        want, _ = attention(m, s, qg[a:a + n], at(bases[s], n))
+        got = whole[a:a + n].double().reshape(want.shape)
+        assert ((got - want).abs() <= MAX_TOL * held(m, s)[1].abs().max() + step * want.abs()).all(), s
+        assert (got - want).norm() <= (NORM_TOL + step / 3 ** 0.5) * want.norm(), s
+        a += n
+    halves = torch.full_like(whole, -7.0)
+    for i in range(2):
+        c = dz.Context(0, dz.default_config(n_layers=1, full_attention_interval=1, kv_heads=(0, 1), qtile_split=(i, 2)))
+        c.set_attn_params(0, m.qn, m.kn)
+        c.cache_create_q4(caps)
+        load(c)
+        run(c, halves)
+        torch.cuda.synchronize()
+        c.close()
+    assert torch.equal(halves, whole)
+    for s, n in enumerate(bases):
+        m.ctx.kv_truncate(0, s, n)
+    again = torch.empty_like(whole)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(m.ctx, again)
+    for _ in range(2):
+        again.fill_(-7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(again, whole)
+    m.done()
