@@ -184,7 +184,7 @@ __device__ __forceinline__ void store_split(__nv_bfloat16* row, int lane, const 
 
 // A warp per token and share of its heads: grid (ceil(T / 8), shares).  Several rows are
 // in flight per warp: reading one at a time held the pass at 4.3 TB/s.  32768 bf16 tokens
-// (0.94 GB): 161 us, 5.9 TB/s, 0.89 of a plain copy's rate (7 rows: 164 us, 14: 221).
+// (0.94 GB): 160.4 us, 5.9 TB/s, 0.89 of a plain copy's rate (7 rows: 164 us, 14: 221); 12000 f32 (0.69 GB): 112 us, 6.1.
 constexpr int MROPE_ROWS = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) qk_mrope_kernel(const __grid_constant__ RopeAxes axes, int kvc, int64_t n_tokens,

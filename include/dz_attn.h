@@ -299,11 +299,12 @@ dz_status dz_gqa_decode_q4(dz_ctx* ctx, int layer, int B, const int32_t* seq_ids
  * positions, or NULL for the cache slot on every axis.  Causal within each sequence,
  * over its cached rows and the new ones as held: the result is that of one
  * dz_gqa_decode_q4 per token, except that queries and probabilities are rounded to f16
- * for the matrix products (K and V are exact there; 2e-4 to 4e-4 of an output, at any
- * length), whose f32 sums are truncated (up to 6e-5).  f32 in and out, or bf16 in and out
+ * for the matrix products (K and V are exact there; 3e-4 of an output, at any length),
+ * whose f32 sums are truncated (up to 5e-5).  f32 in and out, or bf16 in and out
  * (rounded once more, from f16).
  * All tensors 16-byte aligned.  Tracked caches: new rows start with weight 0; prompts
- * add no weights.  Scratch grows with the largest prompt (12 KB per new token and 4 KB
+ * add no weights, so before a first decode call an eviction has ties alone and keeps
+ * the earliest entries (and the recent ones): set weights, or decode first.  Scratch grows with the largest prompt (12 KB per new token and 4 KB
  * per key with 4 kv heads; beyond 2 GB a call takes its sequences in groups), within a
  * graph's capture too: outgrown scratch stays for captured graphs until the caches are
  * made anew or the context is destroyed. */
