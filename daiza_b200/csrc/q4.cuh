@@ -263,7 +263,8 @@ __device__ __forceinline__ bool norm_rotate_split(float (&x)[8], const float (&w
     scale_rotate_split(x, fmaf(fmaf(-v * g, g, 1.0f), 0.5f * g, g), w, cs, lane);   // one Newton step: to the last bit or so
     return !out_of_range(v);
 }
-__device__ __forceinline__ void norm_rotate_far(float (&x)[8], const float (&w)[8], const float2 (&cs)[4], float eps, int lane) {
+__device__ __forceinline__ void norm_rotate_far(float (&x)[8], const float (&w)[8], const float2 (&cs)[4], float eps,
+                                                int lane) {
     float ss = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);

@@ -31,7 +31,7 @@ float query_scale(const float* q_norm) {
         if (std::isfinite(q_norm[i])) top = std::max(top, std::fabs(q_norm[i]));
     int e = 0;
     std::frexp(2.05 * top, &e);
-    return top > 0.0f ? std::ldexp(1.0f, std::min(std::max(15 - e, -100), 100)) : 1.0f;
+    return top > 0.0f ? std::ldexp(1.0f, std::min(std::max(15 - e, -120), 120)) : 1.0f;
 }
 
 // An allocation is no work of the stream: it may be made while a graph is captured, on this thread or another

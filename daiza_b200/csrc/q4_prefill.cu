@@ -250,7 +250,7 @@ struct alignas(1024) Smem {
     uint16_t q[4][BM][64];                       // 4 boxes of 64 dims, 16 KB each
     uint16_t k[NK][BN / 2][64];
     uint16_t v[NV][2][32][64];
-    uint4 out[BM][32];                           // O / l, 16-byte words of a row in swizzled order: 256 dims as f16, or 128 as f32
+    uint4 out[BM][32];                           // O / l, a row's 16-byte words swizzled: 256 dims as f16, or 128 as f32
     uint64_t q_full, q_empty, out_full[2], out_empty[2];   // out: of either half of the dims (f32), [0] of both (bf16)
     uint64_t k_full[NK], k_empty[NK], v_full[NV], v_empty[NV];
     uint64_t s_full[2], p_full[2], pv_done[2];
@@ -651,7 +651,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NTHREADS, 1)
         const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t p_bar[2] = {peer_addr(&sm.p_full[0], 0), peer_addr(&sm.p_full[1], 0)};
         uint32_t g = 0;                                                // blocks so far
-        if (LONG) part += (int64_t)blockIdx.x * (BM * HD) + 128 * hf * BM + r;       // this thread's sums of earlier stretches
+        if (LONG) part += (int64_t)blockIdx.x * (BM * HD) + 128 * hf * BM + r;       // this thread's sums
         while (next_tile()) {
             const int64_t qpos = tl.base + tl.q0 + r;                      // absolute position of this query row
             float m_run = -INFINITY, l_run = 0.0f;                         // m identical in both halves; l partial per half
@@ -845,10 +845,11 @@ static bool make_map(CUtensorMap* m, const void* base, int64_t d1, int64_t d2, i
 cudaError_t q4_prefill_setup() {
     using B = __nv_bfloat16;
     cudaError_t e = cudaSuccess;
-    for (auto kernel : {(const void*)q4::attn::q4_pf_attn_kernel<float, false>, (const void*)q4::attn::q4_pf_attn_kernel<float, true>,
-                        (const void*)q4::attn::q4_pf_attn_kernel<B, false>, (const void*)q4::attn::q4_pf_attn_kernel<B, true>})
+    using namespace q4::attn;
+    for (auto kernel : {(const void*)q4_pf_attn_kernel<float, false>, (const void*)q4_pf_attn_kernel<float, true>,
+                        (const void*)q4_pf_attn_kernel<B, false>, (const void*)q4_pf_attn_kernel<B, true>})
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, q4::attn::SMEM_BYTES);
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
     return e;
 }
 

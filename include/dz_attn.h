@@ -304,10 +304,11 @@ dz_status dz_gqa_decode_q4(dz_ctx* ctx, int layer, int B, const int32_t* seq_ids
  * (rounded once more, from f16).
  * All tensors 16-byte aligned.  Tracked caches: new rows start with weight 0; prompts
  * add no weights, so before a first decode call an eviction has ties alone and keeps
- * the earliest entries (and the recent ones): set weights, or decode first.  Scratch grows with the largest prompt (12 KB per new token and 4 KB
- * per key with 4 kv heads; beyond 2 GB a call takes its sequences in groups), within a
- * graph's capture too: outgrown scratch stays for captured graphs until the caches are
- * made anew or the context is destroyed. */
+ * the earliest entries (and the recent ones): set weights, or decode first.
+ * All or nothing: a call that fails (DZ_ENOMEM) leaves every length.  Scratch grows with
+ * the largest prompt (12 KB per new token and 4 KB per key with 4 kv heads; beyond 2 GB a
+ * call takes its sequences in groups), within a graph's capture too: outgrown scratch
+ * stays for captured graphs until the caches are made anew or the context is destroyed. */
 dz_status dz_gqa_prefill_q4(dz_ctx* ctx, int layer, int n_seqs, const int32_t* seq_ids, const int64_t* T,
                             const int32_t* pos, const float* q_gate, const float* k, const float* v, float* out,
                             void* stream);

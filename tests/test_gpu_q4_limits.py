@@ -94,7 +94,7 @@ def test_prompt_norm_weights_of_any_size(up):
     m.done()
 
 
-@pytest.mark.parametrize("weight", [3e6, 1e30])
+@pytest.mark.parametrize("weight", [3e6, 1e30, 1e37])
 def test_prompt_one_large_norm_weight(weight):
     """A query dim beyond f16 that no key answers."""
     m = Model([300], kvc=1, seed=319)
