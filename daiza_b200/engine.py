@@ -46,12 +46,12 @@ def _stream(stream):
 
 def _tensor(name, t, dtype, numel, device=None):
     """Address of a contiguous CUDA tensor (on that device) that a 4-bit cache call takes; DZ_EINVAL otherwise."""
-    if not (t.is_cuda and t.dtype == dtype and t.is_contiguous() and t.numel() == numel and
-            (device is None or t.get_device() == device)):
-        where = "CUDA" if device is None else f"cuda:{device}"
-        raise _ffi.DzError(_ffi.DZ_EINVAL, f"{name} must be a contiguous {where} {dtype} tensor of {numel} values, got "
-                                           f"{tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
-    return t.data_ptr()
+    if (t.get_device() == device or device is None and t.is_cuda) and t.dtype == dtype and t.is_contiguous() and \
+            t.numel() == numel:
+        return t.data_ptr()
+    where = "CUDA" if device is None else f"cuda:{device}"
+    raise _ffi.DzError(_ffi.DZ_EINVAL, f"{name} must be a contiguous {where} {dtype} tensor of {numel} values, got "
+                                       f"{tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
 
 
 _arrays = {}                                     # ctypes array types by (type, length)
@@ -126,6 +126,7 @@ class Context:
             raise _ffi.DzError(st, f"dz_ctx_create(device={device}) failed")
         self.h = h
         self.device = device
+        self.index = int(device)                     # what its tensors' get_device() gives
         self.kvc = self.cfg.kv_head_count
         self.vc = self.cfg.v_head_count
         self.nq = GRP * self.kvc
@@ -337,9 +338,6 @@ class Context:
         s = _ints("sections", sections, C.c_int32, 3)
         self._chk(self.lib.dz_set_rope_axes(self.h, s, int(bool(interleaved))))
 
-    def _tensor(self, name, t, dtype, numel):
-        return _tensor(name, t, dtype, numel, int(self.device))
-
     def _on(self, stream):
         """Handle of `stream`, or of the context's device's current one (straight, where this torch has the call for it:
         making a Stream object takes 1.3 us)."""
@@ -347,7 +345,7 @@ class Context:
             return stream.cuda_stream
         import torch
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        return raw(int(self.device)) if raw else torch.cuda.current_stream(int(self.device)).cuda_stream
+        return raw(self.index) if raw else torch.cuda.current_stream(self.index).cuda_stream
 
     def qk_mrope(self, layer, pos, q_gate, k, q_out, k_out, stream=None):
         """QK-RMSNorm, rotation by pos [T][3] (int32) and q's 1/16; q_gate [T][6*kvc][512] and k [T][kvc][256] f32 or
@@ -356,11 +354,11 @@ class Context:
         T = k.numel() // (self.kvc * HD)
         dt = torch.bfloat16 if k.dtype == torch.bfloat16 else torch.float32
         fn = self.lib.dz_qk_mrope_bf16 if dt == torch.bfloat16 else self.lib.dz_qk_mrope
-        self._chk(fn(self.h, layer, T, self._tensor("pos", pos, torch.int32, 3 * T),
-                     self._tensor("q_gate", q_gate, dt, T * self.nq * QG_ROW),
-                     self._tensor("k", k, dt, T * self.kvc * HD),
-                     self._tensor("q_out", q_out, dt, T * self.nq * HD),
-                     self._tensor("k_out", k_out, dt, T * self.kvc * HD), self._on(stream)))
+        self._chk(fn(self.h, layer, T, _tensor("pos", pos, torch.int32, 3 * T, self.index),
+                     _tensor("q_gate", q_gate, dt, T * self.nq * QG_ROW, self.index),
+                     _tensor("k", k, dt, T * self.kvc * HD, self.index),
+                     _tensor("q_out", q_out, dt, T * self.nq * HD, self.index),
+                     _tensor("k_out", k_out, dt, T * self.kvc * HD, self.index), self._on(stream)))
 
     def gqa_decode_q4(self, layer, seq_ids, q_gate, k, v, out, stream=None, pos=None):
         """gqa_decode on 4-bit caches; pos: [B][3] rotary positions (host), default the cache lengths."""
@@ -371,9 +369,9 @@ class Context:
             p3 = _positions(pos, B)
         self._chk(self.lib.dz_gqa_decode_q4(
             self.h, layer, B, ids, p3,
-            self._tensor("q_gate", q_gate, f, B * self.nq * QG_ROW), self._tensor("k", k, f, B * self.kvc * HD),
-            self._tensor("v", v, f, B * self.kvc * HD), self._tensor("out", out, f, B * self.nq * HD),
-            self._on(stream)))
+            _tensor("q_gate", q_gate, f, B * self.nq * QG_ROW, self.index),
+            _tensor("k", k, f, B * self.kvc * HD, self.index), _tensor("v", v, f, B * self.kvc * HD, self.index),
+            _tensor("out", out, f, B * self.nq * HD, self.index), self._on(stream)))
 
     def gqa_prefill_q4(self, layer, seq_ids, lens, q_gate, k, v, out, stream=None, pos=None):
         """lens[i] new tokens of each sequence, packed: q_gate [sum][6*kvc][512], k and v [sum][kvc][256], out
@@ -385,11 +383,11 @@ class Context:
         dt = torch.bfloat16 if k.dtype == torch.bfloat16 else torch.float32
         fn = self.lib.dz_gqa_prefill_q4_bf16 if dt == torch.bfloat16 else self.lib.dz_gqa_prefill_q4
         self._chk(fn(self.h, layer, len(ids), ids, n,
-                     None if pos is None else self._tensor("pos", pos, torch.int32, 3 * T),
-                     self._tensor("q_gate", q_gate, dt, T * self.nq * QG_ROW),
-                     self._tensor("k", k, dt, T * self.kvc * HD),
-                     self._tensor("v", v, dt, T * self.kvc * HD), self._tensor("out", out, dt, T * self.nq * HD),
-                     self._on(stream)))
+                     None if pos is None else _tensor("pos", pos, torch.int32, 3 * T, self.index),
+                     _tensor("q_gate", q_gate, dt, T * self.nq * QG_ROW, self.index),
+                     _tensor("k", k, dt, T * self.kvc * HD, self.index),
+                     _tensor("v", v, dt, T * self.kvc * HD, self.index),
+                     _tensor("out", out, dt, T * self.nq * HD, self.index), self._on(stream)))
 
     def kv_rows_q4(self, layer, seq_ids, first, count, k, v, stream=None):
         """Held rows [first, first + count) of each sequence as f32 [sum count][kvc][256]."""
@@ -398,8 +396,8 @@ class Context:
         a, n = _per_seq("first", first, ids), _per_seq("count", count, ids)
         total = _total(n) * self.kvc * HD
         self._chk(self.lib.dz_kv_rows_q4(self.h, layer, len(ids), ids, a, n,
-                                         self._tensor("k", k, torch.float32, total),
-                                         self._tensor("v", v, torch.float32, total), self._on(stream)))
+                                         _tensor("k", k, torch.float32, total, self.index),
+                                         _tensor("v", v, torch.float32, total, self.index), self._on(stream)))
 
     def _weights_numel(self, layer, ids):
         return self.kvc * sum(self._lens(layer, ids))
@@ -410,14 +408,14 @@ class Context:
         ids = _ids(seq_ids)
         self._chk(self.lib.dz_kv_weights_q4(
             self.h, layer, len(ids), ids,
-            self._tensor("out", out, torch.float32, self._weights_numel(layer, ids)), self._on(stream)))
+            _tensor("out", out, torch.float32, self._weights_numel(layer, ids), self.index), self._on(stream)))
 
     def kv_set_weights_q4(self, layer, seq_ids, weights, stream=None):
         import torch
         ids = _ids(seq_ids)
         self._chk(self.lib.dz_kv_set_weights_q4(
             self.h, layer, len(ids), ids,
-            self._tensor("weights", weights, torch.float32, self._weights_numel(layer, ids)), self._on(stream)))
+            _tensor("weights", weights, torch.float32, self._weights_numel(layer, ids), self.index), self._on(stream)))
 
     def kv_evict_q4(self, layer, seq_ids, keep, recent, kept=None, into=None, stream=None):
         """Keeps the last recent[b] and the heaviest other entries, keep[b] in all, per kv head; in place, or into the
@@ -429,7 +427,7 @@ class Context:
         out = None
         if kept is not None:
             n = sum(max(0, min(a, b)) for a, b in zip(k, self._lens(layer, ids)))
-            out = self._tensor("kept", kept, torch.int32, n * self.kvc)
+            out = _tensor("kept", kept, torch.int32, n * self.kvc, self.index)
         self._chk(self.lib.dz_kv_evict_q4(self.h, layer, len(ids), ids, to,
                                           k, r, out, self._on(stream)))
 

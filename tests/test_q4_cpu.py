@@ -108,21 +108,21 @@ def test_host_tensors_wrong_types_and_sizes_are_refused():
     assert list(engine._per_seq("count", (4, 5), engine._ids([0, 1]))) == [4, 5]
 
 
-class OfAnotherGpu:
-    """What the checks ask of a tensor, for one that lies on cuda:1."""
-    is_cuda, shape, device = True, (4,), "cuda:1"
+class OnGpu:
+    """What the checks ask of a tensor, for one that lies on another GPU."""
+    is_cuda, shape = True, (256,)
 
-    def __init__(self, torch):
-        self.dtype = torch.float32
+    def __init__(self, torch, index):
+        self.dtype, self.index, self.device = torch.float32, index, f"cuda:{index}"
 
     def get_device(self):
-        return 1
+        return self.index
 
     def is_contiguous(self):
         return True
 
     def numel(self):
-        return 4
+        return 256
 
     def stride(self):
         return (1,)
@@ -135,13 +135,24 @@ def test_tensors_of_another_gpu_are_refused():
     torch = pytest.importorskip("torch")
     from daiza_b200 import engine
     from daiza_b200._ffi import DZ_EINVAL, DzError
-    there = OfAnotherGpu(torch)
-    assert engine._tensor("x", there, torch.float32, 4, 1) == 4096
+    here, there = OnGpu(torch, 0), OnGpu(torch, 1)
+    assert engine._tensor("x", here, torch.float32, 256, 0) == 4096
+
+    class Lib:
+        called = 0
+
+        def dz_kv_rows_q4(self, *a):
+            self.called += 1
+            return 0
+
     ctx = engine.Context.__new__(engine.Context)     # a context of cuda:0, as far as its checks go
-    ctx.device, ctx.h = 0, None
-    with pytest.raises(DzError) as e:
-        ctx._tensor("x", there, torch.float32, 4)
-    assert e.value.status == DZ_EINVAL and "cuda:0" in str(e.value)
+    ctx.index, ctx.h, ctx.kvc, ctx.lib, ctx._on = 0, None, 1, Lib(), lambda stream: None
+    ctx.kv_rows_q4(0, [0], [0], [1], here, here)
+    for pair in ((here, there), (there, here)):
+        with pytest.raises(DzError) as e:
+            ctx.kv_rows_q4(0, [0], [0], [1], *pair)
+        assert e.value.status == DZ_EINVAL and "cuda:0" in str(e.value)
+    assert ctx.lib.called == 1
 
 
 def test_what_is_no_list_of_numbers_is_refused():
@@ -177,7 +188,7 @@ def test_current_stream_without_torchs_private_call(monkeypatch):
     torch = pytest.importorskip("torch")
     from daiza_b200 import engine
     ctx = engine.Context.__new__(engine.Context)
-    ctx.device, ctx.h = 3, None
+    ctx.index, ctx.h = 3, None
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 100 + device, raising=False)
     assert ctx._on(None) == 103
     monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream")
